@@ -41,9 +41,10 @@ extern "C" {
  * mirror call); 105 round 5 - ttsmi_dense_chain_* and the chain tail of ttsmi_dense_block; 106 the backward chain
  * (ttsmi_dense_chain_bwd*, chain_bw, relu_bits_layout); 107 round 6 - ttsmi_dense_chain_bwd_nparts,
  * ttsmi_dense_block_bwd_chained, ttsmi_ft_train_step; the opt-in one-pass attention backward
- * (ttsmi_attention_bwd_fused*, attn_fused_ws) removed - it never beat the two kernels inside the step.  Bindings check it at load time (transformertts_amd/_lib.py) so that a stale build is
+ * (ttsmi_attention_bwd_fused*, attn_fused_ws) removed - it never beat the two kernels inside the step.  110: the sequence operators
+ * (ttsmi_rotary, ttsmi_packed_attention_*, ttsmi_kv_cache_*, ttsmi_paged_attention).  Bindings check it at load time (transformertts_amd/_lib.py) so that a stale build is
  * refused instead of being called with shifted arguments. */
-#define TTSMI_VERSION 109
+#define TTSMI_VERSION 110
 
 enum {
     TTSMI_OK = 0,
@@ -58,7 +59,8 @@ enum {
 /* TTSMI_BF16X3 (the fp32 GEMM entry points: ttsmi_linear_* / ttsmi_conv1d_*): fp32 tensors as TTSMI_F32, every product as THREE
  * bf16 MFMAs on hi / lo splits of both operands (a_hi b_hi + a_hi b_lo + a_lo b_hi, fp32 accumulate): ~2^-16 per product instead
  * of bf16's 2^-8, at ~4 x the exact-fp32 kernels' rate - the GEMM family of the host mirror's precision='bf16x3'. */
-enum { TTSMI_F32 = 0, TTSMI_BF16 = 1, TTSMI_BF16_IO = 2, TTSMI_BF16X3 = 3 };
+/* TTSMI_E4M3 (pages of the key / value cache only): 8-bit values with a power-of-two scale per row, see ttsmi_kv_cache_write. */
+enum { TTSMI_F32 = 0, TTSMI_BF16 = 1, TTSMI_BF16_IO = 2, TTSMI_BF16X3 = 3, TTSMI_E4M3 = 4 };
 
 typedef void* ttsmi_stream_t; /* hipStream_t */
 
@@ -795,6 +797,75 @@ int ttsmi_ft_train_step(const ttsmi_ft_step* step, int phase);
 int ttsmi_add2_f32(const float* a, const float* b, float* out, int64_t n, ttsmi_stream_t stream);
 /* dst[m, 0 .. C) = src[m, 0 .. C), dst[m, C .. Cp) = 0: the zero-padded gradient a Conv1D dgrad with Cout % 8 != 0 reads */
 int ttsmi_pad_cols_f32(const float* src, int C, float* dst, int Cp, int M, ttsmi_stream_t stream);
+
+/* ---------------------------------------------------------------------------------------------
+ * Sequence operators: rotary positions, attention over packed sequences (causal or not, grouped heads), the paged key /
+ * value cache and attention of new tokens over it.  The reference has none of them (its attention is padded, bidirectional
+ * and without state, model/layers.py:105-195).
+ *
+ * Tensors of tokens are [tokens, heads, dh], the last dimension contiguous, with element strides (row, head) of their own -
+ * e.g. the three parts of one fused projection.  dtype is TTSMI_F32 or TTSMI_BF16_IO (fp32 or bf16 tensors).  The attention
+ * and cache entry points need dh a multiple of 8 up to 192 and rows and heads on 16-byte boundaries; H % Hkv == 0, query head
+ * h reads key head h / (H / Hkv).
+ * starts [B + 1] int32 (DEVICE): sequence b owns the packed tokens starts[b] .. starts[b + 1]; starts[0] = 0, ascending; a
+ *   sequence may be empty.  Tokens behind starts[B] belong to no sequence: outputs there are left as they were, or, with
+ *   zero_rest != 0, set to zero.  starts that do not ascend or reach outside give wrong rows, but no access out of range.
+ * Lengths are read on the device only: a captured call replays on other lengths (same B and token count).
+ * ------------------------------------------------------------------------------------------- */
+/* The first rot elements of every head turned by position: pair (2i, 2i + 1) (interleaved != 0) or (i, i + rot / 2) of a
+ * token at positions[t] by the angle positions[t] * freqs[i] (freqs: rot / 2 doubles, radians per position; the angle is
+ * reduced in 64 bits), times scale; inverse != 0 turns back (the gradient).  Elements from rot on are copied.  q and k in
+ * one launch; either may be absent (heads 0).  In place (output = input, same strides) is allowed.  dh even, rot even and at
+ * most 512; no other alignment is needed. */
+int ttsmi_rotary(const void* q, int64_t q_row, int64_t q_head, void* qo, int64_t qo_row, int64_t qo_head, int H, const void* k,
+                 int64_t k_row, int64_t k_head, void* ko, int64_t ko_row, int64_t ko_head, int Hkv, const int32_t* positions,
+                 const double* freqs, int tokens, int dh, int rot, int interleaved, float scale, int inverse, int dtype,
+                 ttsmi_stream_t stream);
+/* out = softmax(scale q k^T) v within each sequence, causal != 0: over the keys up to the query's own.  scale > 0.  The sums
+ * are held in fp32; bf16: the probabilities are rounded to bf16 for the product with v.  lse [Hkv, tokens, H / Hkv] fp32
+ * (natural log; may be NULL) is what the backward reads.  A masked score never reaches the softmax, whatever k holds; a NaN
+ * or infinity in a VALUE row reaches every row of its own sequence whose 32-row block shares a 32-key block with it (0 times
+ * NaN), and no other sequence. */
+int ttsmi_packed_attention_fwd(const void* q, int64_t q_row, int64_t q_head, const void* k, int64_t k_row, int64_t k_head,
+                               const void* v, int64_t v_row, int64_t v_head, const int32_t* starts, int B, int tokens, int H,
+                               int Hkv, int dh, float scale, int causal, void* out, int64_t o_row, int64_t o_head, float* lse,
+                               int zero_rest, int dtype, ttsmi_stream_t stream);
+/* Gradients of q, k and v (summed over the query heads of a group); deterministic.  out and lse are the forward's. */
+size_t ttsmi_packed_attention_bwd_ws_bytes(int tokens, int H);
+int ttsmi_packed_attention_bwd(const void* q, int64_t q_row, int64_t q_head, const void* k, int64_t k_row, int64_t k_head,
+                               const void* v, int64_t v_row, int64_t v_head, const void* out, int64_t o_row, int64_t o_head,
+                               const void* dout, int64_t d_row, int64_t d_head, const float* lse, const int32_t* starts, int B,
+                               int tokens, int H, int Hkv, int dh, float scale, int causal, void* dq, int64_t dq_row,
+                               int64_t dq_head, void* dk, int64_t dk_row, int64_t dk_head, void* dv, int64_t dv_row,
+                               int64_t dv_head, int zero_rest, void* ws, size_t ws_bytes, int dtype, ttsmi_stream_t stream);
+/* The paged cache: k_pages / v_pages [n_pages, Hkv, page_size, dh], page_size a power of two up to 1024; cache_dtype = dtype
+ * (rows as they are) or TTSMI_E4M3 (bytes, with k_exp / v_exp [n_pages, Hkv, page_size]: row = e4m3 value * 2^(exp - 127)).
+ * table [B, table_width] int32: page of the positions p * page_size ... of sequence b.  lens [B] int32: cached length of
+ * sequence b INCLUDING its starts[b + 1] - starts[b] new tokens, which are the last ones.  A page number outside
+ * [0, n_pages) is never written and reads as zeros; a new token without a position (lens too small) is not written.
+ * A page may stand in several tables for reading; a call that writes one row twice leaves either.
+ * e4m3: the smallest power-of-two scale that brings the row's largest finite magnitude to 448 at most, each value rounded to
+ * nearest even; NaN and infinity become NaN. */
+int ttsmi_kv_cache_write(const void* k, int64_t k_row, int64_t k_head, const void* v, int64_t v_row, int64_t v_head, void* k_pages,
+                         void* v_pages, uint8_t* k_exp, uint8_t* v_exp, int cache_dtype, int n_pages, int page_size,
+                         const int32_t* table, int table_width, const int32_t* starts, const int32_t* lens, int B, int tokens,
+                         int Hkv, int dh, int dtype, ttsmi_stream_t stream);
+/* The last starts[b + 1] - starts[b] cached tokens of every sequence back into packed rows (all of them where starts holds the
+ * cumulative lens); rows before position 0 read as zeros. */
+int ttsmi_kv_cache_read(const void* k_pages, const void* v_pages, const uint8_t* k_exp, const uint8_t* v_exp, int cache_dtype,
+                        int n_pages, int page_size, const int32_t* table, int table_width, const int32_t* starts,
+                        const int32_t* lens, int B, int tokens, int Hkv, int dh, void* k, int64_t k_row, int64_t k_head, void* v,
+                        int64_t v_row, int64_t v_head, int zero_rest, int dtype, ttsmi_stream_t stream);
+/* Attention of the packed new tokens over the cache (their own keys and values written before): token i of sequence b, n of
+ * them, is at position lens[b] - n + i and sees the keys up to it.  A token that sees none gets zeros.  max_len: the longest
+ * cached length expected - it sets how finely the keys are split over workgroups, never the result's correctness; the same
+ * value goes into the workspace query. */
+size_t ttsmi_paged_attention_ws_bytes(int B, int tokens, int H, int Hkv, int dh, int max_len);
+int ttsmi_paged_attention(const void* q, int64_t q_row, int64_t q_head, const void* k_pages, const void* v_pages,
+                          const uint8_t* k_exp, const uint8_t* v_exp, int cache_dtype, int n_pages, int page_size,
+                          const int32_t* table, int table_width, const int32_t* starts, const int32_t* lens, int B, int tokens,
+                          int H, int Hkv, int dh, float scale, int max_len, void* out, int64_t o_row, int64_t o_head,
+                          int zero_rest, void* ws, size_t ws_bytes, int dtype, ttsmi_stream_t stream);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,590 @@
+"""-m gpu tests of the sequence operators (rotary positions, attention over packed sequences, the paged key / value cache and
+attention over it) against plain 64-bit CPU restatements.
+
+Tolerances are bounds, element by element, from the sizes of the terms of each sum (in 64 bits) and the roundings that the
+operators make: U = 2^-23 for an fp32 operation (twice the half step, for the matrix unit's accumulation), H = 2^-8 (bf16) for
+each rounding of a probability, a score gradient or an output, 0 for fp32 tensors."""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+DEV = 'cuda:0'
+U = 2.0 ** -23
+HALF = {torch.float32: 2.0 ** -24, torch.bfloat16: 2.0 ** -8}
+
+
+def _ops():
+    from transformertts_amd import ops
+    return ops
+
+
+def _randn(shape, seed, dtype=torch.float32, scale=1.0):
+    return (torch.randn(shape, generator=torch.Generator().manual_seed(seed)) * scale).to(dtype)
+
+
+def _starts(lens):
+    return torch.tensor([0] + torch.tensor(lens).cumsum(0).tolist() if lens else [0], dtype=torch.int32)
+
+
+def _within(got, want, bound, what):
+    got = got.detach().double().cpu()
+    assert got.shape == want.shape, (what, got.shape, want.shape)
+    bad = ~((got - want).abs() <= bound)
+    assert not bad.any(), f'{what}: {int(bad.sum())} of {bad.numel()} off, worst {float((got - want).abs()[bad].max())} where {float(bound[bad].min())} is allowed'
+
+
+# ------------------------------------------------------------------------------------------------------------------ oracle
+def attention_oracle(q, k, v, first, causal, scale, dtype, dout=None):
+    """q [n, H, dh] at positions first .. over k, v [t, Hkv, dh] in 64 bits: ([out, dq, dk, dv], [bound of each])."""
+    n, H, dh = q.shape
+    t, Hkv = k.shape[:2]
+    q, k, v = q.double(), k.double(), v.double()
+    Hb = HALF[dtype] if dtype == torch.bfloat16 else 0.0
+    seen = torch.ones(n, t, dtype=torch.bool)
+    if causal:
+        seen = torch.arange(t)[None] <= first + torch.arange(n)[:, None]
+    out, bout = torch.zeros(n, H, dh).double(), torch.zeros(n, H, dh).double()
+    grads = [torch.zeros_like(x) for x in (q, k, v)]
+    bounds = [torch.zeros_like(x) for x in (q, k, v)]
+    for h in range(H):
+        g = h // (H // Hkv)
+        s = (q[:, h] @ k[:, g].T * scale).masked_fill(~seen, -math.inf)
+        some = seen.any(1, keepdim=True)
+        p = torch.where(seen, torch.softmax(torch.where(some, s, torch.zeros_like(s)), -1), torch.zeros_like(s))
+        # relative error of a probability: twice the score's (its own and the normaliser's), exp2 and the sums
+        mag = (q[:, h].abs() @ k[:, g].abs().T * scale)
+        es = (dh + 8) * U * (mag * seen).amax(1, keepdim=True) if t else torch.zeros(n, 1).double()
+        ep = 2 * es + (t + 16) * U
+        o = p @ v[:, g]
+        out[:, h] = o
+        bo = (ep + Hb) * (p @ v[:, g].abs())
+        bout[:, h] = bo + HALF[dtype] * (o.abs() + bo) + 1e-30
+        if dout is None:
+            continue
+        d = dout[:, h].double()
+        dp, delta = d @ v[:, g].T, (d * o).sum(1, keepdim=True)
+        ds = p * (dp - delta)
+        e_dp = (dh + 8) * U * (d.abs() @ v[:, g].abs().T)
+        e_delta = (d.abs() * bout[:, h]).sum(1, keepdim=True) + (dh + 8) * U * (d.abs() * o.abs()).sum(1, keepdim=True)
+        e_ds = p * ((ep + 4 * U) * (dp - delta).abs() + e_dp + e_delta)
+        e_ds = e_ds + Hb * (ds.abs() + e_ds)
+        rows = n * (H // Hkv)
+        grads[0][:, h] = scale * ds @ k[:, g]
+        bounds[0][:, h] += scale * (e_ds + (t + 8) * U * ds.abs()) @ k[:, g].abs()
+        grads[1][:, g] += scale * ds.T @ q[:, h]
+        bounds[1][:, g] += scale * (e_ds + (rows + 8) * U * ds.abs()).T @ q[:, h].abs()
+        grads[2][:, g] += p.T @ d
+        bounds[2][:, g] += ((ep + Hb + (rows + 8) * U) * p).T @ d.abs()
+    bounds = [b + HALF[dtype] * (x.abs() + b) + 1e-30 for x, b in zip(grads, bounds)]
+    return [out] + grads, [bout] + bounds
+
+
+def packed_oracle(q, k, v, lens, causal, scale, dout=None):
+    parts, at = [], 0
+    for n in lens:
+        x = [None if y is None else y[at:at + n] for y in (q, k, v, dout)]
+        parts.append(attention_oracle(x[0], x[1], x[2], 0, causal, scale, q.dtype, x[3]))
+        at += n
+    return [[torch.cat(c) for c in zip(*(p[i] for p in parts))] for i in (0, 1)]
+
+
+def _grads(out, xs, d):
+    return [out] + list(torch.autograd.grad(out, xs, d))
+
+
+# --------------------------------------------------------------------------------------------------------------- attention
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize('lens,H,Hkv,dh,causal', [
+    ([1], 1, 1, 8, True), ([2], 4, 2, 64, True), ([61], 2, 2, 192, True), ([33], 3, 1, 40, False), ([5, 0, 130, 1, 64], 4, 2, 64, True),
+    ([5, 0, 130, 1, 64], 4, 4, 64, False), ([0, 0, 7], 2, 1, 128, True), ([257, 128, 31], 8, 2, 128, True), ([200, 90], 6, 3, 96, False),
+    ([300], 4, 1, 192, True), ([129, 127], 16, 2, 80, True), ([3] * 70 + [0, 65], 2, 2, 32, True), ([515], 12, 4, 16, True)])
+def test_packed_attention(lens, H, Hkv, dh, causal, dtype):
+    ops = _ops()
+    M = sum(lens)
+    q, k, v, d = (_randn((M, h, dh), i, dtype, s) for i, (h, s) in enumerate([(H, 1.5), (Hkv, 1.5), (Hkv, 1.0), (H, 1.0)]))
+    want, bound = packed_oracle(q, k, v, lens, causal, dh ** -0.5, d)
+    xs = [x.to(DEV).requires_grad_() for x in (q, k, v)]
+    got = _grads(ops.packed_attention(*xs, _starts(lens).to(DEV), causal=causal), xs, d.to(DEV))
+    for name, g, w, b in zip(('out', 'dq', 'dk', 'dv'), got, want, bound):
+        assert g.dtype == dtype
+        _within(g, w, b, name)
+    with torch.no_grad():                                               # the form without lse: the same bits
+        assert torch.equal(ops.packed_attention(*xs, _starts(lens).to(DEV), causal=causal), got[0])
+
+
+def test_packed_attention_scale_and_peaked_scores():
+    """Scores of some hundreds: the running maximum carries them, forward and backward stay finite and right."""
+    ops = _ops()
+    lens, H, dh = [190, 66], 2, 64
+    q, k, v, d = (_randn((256, H, dh), i, torch.float32, 4.0) for i in range(4))
+    want, bound = packed_oracle(q, k, v, lens, True, 0.7, d)
+    xs = [x.to(DEV).requires_grad_() for x in (q, k, v)]
+    got = _grads(ops.packed_attention(*xs, _starts(lens).to(DEV), scale=0.7), xs, d.to(DEV))
+    for name, g, w, b in zip(('out', 'dq', 'dk', 'dv'), got, want, bound):
+        _within(g, w, b, name)
+
+
+def test_packed_attention_gradient_against_differences():
+    """Directional derivatives of the 64-bit definition, by central differences (their own error: h^2 and 2^-52 / h)."""
+    ops = _ops()
+    lens, H, Hkv, dh = [37, 1, 20], 4, 2, 24
+    M = sum(lens)
+    x = [_randn((M, h, dh), i) for i, h in enumerate((H, Hkv, Hkv))]
+    d, dirs = _randn((M, H, dh), 7), [_randn(t.shape, 10 + i).double() for i, t in enumerate(x)]
+    xs = [t.to(DEV).requires_grad_() for t in x]
+    got = _grads(ops.packed_attention(*xs, _starts(lens).to(DEV)), xs, d.to(DEV))[1:]
+    bounds = packed_oracle(*x, lens, True, dh ** -0.5, d)[1][1:]
+    for i in range(3):
+        f = []
+        for h in (1e-4, -1e-4):
+            y = [t.double() + (h * dirs[i] if j == i else 0) for j, t in enumerate(x)]
+            outs, at = [], 0
+            for n in lens:
+                a, b, c = (t[at:at + n].transpose(0, 1) for t in y)
+                b, c = (t.repeat_interleave(H // Hkv, 0) for t in (b, c))
+                w = (a @ b.transpose(1, 2) * dh ** -0.5).masked_fill(~torch.ones(n, n, dtype=torch.bool).tril(), -math.inf)
+                outs.append((torch.softmax(w, -1) @ c).transpose(0, 1))
+                at += n
+            f.append(float((torch.cat(outs) * d.double()).sum()))
+        slope = (f[0] - f[1]) / 2e-4
+        mine = float((got[i].double().cpu() * dirs[i]).sum())
+        assert abs(mine - slope) <= float((bounds[i] * dirs[i].abs()).sum()) + 1e-5 * abs(slope) + 1e-5, (i, mine, slope)
+
+
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float32])
+def test_packed_attention_views_and_orders(dtype):
+    """The parts of one fused projection, rows off 16-byte boundaries, a transposed layout, an expanded gradient: the same
+    bits as contiguous copies."""
+    ops = _ops()
+    lens, H, Hkv, dh = [70, 130], 4, 2, 64
+    M, st = 200, _starts([70, 130]).to(DEV)
+    x = _randn((M, H + 2 * Hkv, dh), 1, dtype).to(DEV)
+    q, k, v = torch.split(x, [H, Hkv, Hkv], dim=1)
+    want = None
+    odd = torch.empty(M * Hkv * dh + 1, dtype=dtype, device=DEV)[1:].view(M, Hkv, dh)
+    odd.copy_(k)
+    across = torch.empty((H, M, dh), dtype=dtype, device=DEV).transpose(0, 1)
+    across.copy_(q)
+    deep = torch.empty((M, Hkv, dh, 2), dtype=dtype, device=DEV)[..., 0]
+    deep.copy_(v)
+    ones = torch.ones((), dtype=dtype, device=DEV).expand(M, H, dh)
+    for a, b, c, d in ((q.contiguous(), k.contiguous(), v.contiguous(), ones.contiguous()), (q, k, v, ones), (across, odd, deep, ones)):
+        a, b, c = (t.detach().requires_grad_() for t in (a, b, c))
+        got = _grads(ops.packed_attention(a, b, c, st), (a, b, c), d)
+        want = want or got
+        assert all(torch.equal(g, w) for g, w in zip(got, want))
+
+
+def test_packed_attention_rows_behind_the_last_sequence():
+    """Zero outputs and gradients behind starts[-1], whatever stands there; the C entry leaves them as they were unless told."""
+    from transformertts_amd import _lib
+    ops = _ops()
+    H, Hkv, dh, M, used = 4, 2, 64, 700, 133
+    st = torch.tensor([0, 100, used], dtype=torch.int32, device=DEV)
+    q, k, v, d = (_randn((M, h, dh), i).to(DEV) for i, h in enumerate((H, Hkv, Hkv, H)))
+    clean = [t[:used].clone().requires_grad_() for t in (q, k, v)]
+    want = _grads(ops.packed_attention(*clean, st), clean, d[:used].clone())
+    for t in (q, k, v, d):
+        t[used:] = float('nan')
+    xs = [t.requires_grad_() for t in (q, k, v)]
+    got = _grads(ops.packed_attention(*xs, st), xs, d)
+    for g, w in zip(got, want):
+        assert torch.equal(g[:used], w) and not g[used:].any()
+    out = torch.full((M, H, dh), 7.0, device=DEV)
+    args = [a for t in (q, k, v) for a in (t.data_ptr(), t.stride(0), t.stride(1))]
+    assert _lib.lib().ttsmi_packed_attention_fwd(*args, st.data_ptr(), 2, M, H, Hkv, dh, dh ** -0.5, 1, out.data_ptr(), H * dh, dh, None, 0,
+                                                 _lib.TTSMI_F32, torch.cuda.current_stream().cuda_stream) == 0
+    assert torch.equal(out[:used], want[0]) and bool((out[used:] == 7).all())
+    none = ops.packed_attention(*(t.detach() for t in xs), torch.zeros(1, dtype=torch.int32, device=DEV))
+    assert none.shape == (M, H, dh) and not none.any()
+    empty = [t.detach()[:0].requires_grad_() for t in xs]
+    got = _grads(ops.packed_attention(*empty, torch.zeros(3, dtype=torch.int32, device=DEV)), empty, d[:0])
+    assert [tuple(g.shape) for g in got] == [(0, H, dh), (0, H, dh), (0, Hkv, dh), (0, Hkv, dh)]
+
+
+def test_packed_attention_nan_stays_in_its_sequence():
+    ops = _ops()
+    lens, H, dh = [50, 64, 90], 2, 64
+    st = _starts(lens).to(DEV)
+    x = [_randn((204, H, dh), i, torch.bfloat16).to(DEV) for i in range(4)]
+    clean = [t.clone().requires_grad_() for t in x[:3]]
+    want = _grads(ops.packed_attention(*clean, st), clean, x[3])
+    for t in x[:3]:
+        t[60:100] = float('nan')
+        t[101] = float('inf')
+    bad = [t.requires_grad_() for t in x[:3]]
+    got = _grads(ops.packed_attention(*bad, st), bad, x[3])
+    for g, w in zip(got, want):
+        assert torch.equal(g[:50], w[:50]) and torch.equal(g[114:], w[114:])
+    # a NaN key that a causal query does not see does not reach it either
+    k = clean[1].detach().clone()
+    k[40:50] = float('nan')
+    assert torch.equal(ops.packed_attention(clean[0].detach(), k, clean[2].detach(), st)[:40], want[0][:40])
+
+
+def test_packed_attention_graph_replays_on_other_lengths():
+    """Forward and backward captured once, replayed with other lengths and inputs, eager work in between; two captured graphs
+    side by side keep their own workspaces."""
+    ops = _ops()
+    H, Hkv, dh, M = 4, 2, 64, 384
+    def eager(x, d, st):
+        y = [t.detach().clone().requires_grad_() for t in x]
+        return [g.clone() for g in _grads(ops.packed_attention(*y, st), y, d)]
+    graphs = []
+    for n in range(2):
+        x = [_randn((M, h, dh), 5 * n + i, torch.bfloat16).to(DEV).requires_grad_() for i, h in enumerate((H, Hkv, Hkv))]
+        d, st = _randn((M, H, dh), 9 + n, torch.bfloat16).to(DEV), torch.zeros(4, dtype=torch.int32, device=DEV)
+        side = torch.cuda.Stream()
+        with torch.cuda.stream(side):
+            st.copy_(_starts([100, 200, 84]))
+            g0 = _grads(ops.packed_attention(*x, st), x, d)
+        torch.cuda.synchronize()
+        del g0
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            res = _grads(ops.packed_attention(*x, st), x, d)
+        graphs.append((graph, x, d, st, res))
+    for lens in ([100, 200, 84], [1, 0, 383], [384, 0, 0], [10, 20, 30]):
+        for n, (graph, x, d, st, res) in enumerate(graphs):
+            with torch.no_grad():
+                for i, t in enumerate(x):
+                    t.copy_(_randn(t.shape, sum(lens) + 3 * i + n, torch.bfloat16))
+            st.copy_(_starts(lens))
+        for graph, *_ in graphs:
+            graph.replay()
+        torch.cuda.synchronize()
+        for graph, x, d, st, res in graphs:
+            assert all(torch.equal(a, b) for a, b in zip(res, eager(x, d, st))), lens
+
+
+def test_packed_attention_on_another_stream_and_twice():
+    ops = _ops()
+    st = _starts([300, 212]).to(DEV)
+    x = [_randn((512, 4, 128), i, torch.bfloat16).to(DEV) for i in range(4)]
+    def go():
+        y = [t.clone().requires_grad_() for t in x[:3]]
+        return _grads(ops.packed_attention(*y, st), y, x[3])
+    want = go()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = go()
+    again = go()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) and torch.equal(a, c) for a, b, c in zip(want, got, again))
+
+
+# ------------------------------------------------------------------------------------------------------------------ rotary
+def rotary_oracle(x, positions, freqs, interleaved, scale, sign=1):
+    n = 2 * len(freqs)
+    y = x.double().clone()
+    ang = positions.double()[:, None, None] * freqs.double()
+    c, s = torch.cos(ang) * scale, torch.sin(ang) * scale * sign
+    ia, ib = (slice(0, n, 2), slice(1, n, 2)) if interleaved else (slice(0, n // 2), slice(n // 2, n))
+    a, b = x[..., ia].double(), x[..., ib].double()
+    y[..., ia], y[..., ib] = a * c - b * s, b * c + a * s
+    mag = torch.zeros_like(y)
+    mag[..., ia], mag[..., ib] = (a.abs() + b.abs()) * scale, (a.abs() + b.abs()) * scale
+    # the cosine and the sine of an angle reduced in 64 bits, each off by a few fp32 steps of 1; the two products and the sum
+    return y, 12 * U * mag + HALF[x.dtype] * (y.abs() + 12 * U * mag)
+
+
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize('interleaved', [False, True])
+@pytest.mark.parametrize('M,H,Hkv,dh,pairs', [(1, 1, 1, 2, 1), (16, 4, 4, 64, 16), (37, 6, 2, 80, 10), (5, 32, 8, 128, 64), (9, 3, 1, 192, 96),
+                                              (3, 2, 1, 26, 5), (130, 5, 5, 66, 33), (4, 1, 1, 512, 256), (6, 2, 2, 64, 0)])
+def test_rotary(M, H, Hkv, dh, pairs, interleaved, dtype):
+    from transformertts_amd.model.transformer_utils import rotary_frequencies
+    ops = _ops()
+    f = torch.from_numpy(rotary_frequencies(2 * pairs)) if pairs else torch.zeros(0, dtype=torch.float64)
+    pos = torch.randint(0, 1 << 20, (M,), generator=torch.Generator().manual_seed(M), dtype=torch.int32)
+    pos[0] = 2 ** 31 - 1
+    q, k, dq, dk = (_randn((M, h, dh), i, dtype) for i, h in enumerate((H, Hkv, H, Hkv)))
+    xs = [t.to(DEV).requires_grad_() for t in (q, k)]
+    out = ops.rotary(*xs, pos.to(DEV), f.to(DEV), interleaved=interleaved, scale=1.25)
+    got = list(out) + list(torch.autograd.grad(out, xs, [dq.to(DEV), dk.to(DEV)]))
+    for g, x, sign in zip(got, (q, k, dq, dk), (1, 1, -1, -1)):
+        _within(g, *rotary_oracle(x, pos, f, interleaved, 1.25, sign), 'rotary')
+    if pairs == 0:
+        assert torch.equal(got[0].cpu(), q)
+    with torch.no_grad():
+        alone = ops.rotary(xs[0], None, pos.to(DEV), f.to(DEV), interleaved=interleaved, scale=1.25)
+        assert torch.equal(alone[0], out[0]) and alone[1] is None
+        here = [x.detach().clone() for x in xs]
+        back = ops.rotary(*here, pos.to(DEV), f.to(DEV), interleaved=interleaved, scale=1.25, inplace=True)
+        assert back[0] is here[0] and all(torch.equal(a, b) for a, b in zip(here, out))
+
+
+def test_rotary_views_and_one_sided_gradient():
+    ops = _ops()
+    x = _randn((50, 10, 64), 3).to(DEV)
+    q, k = x[:, :6], x[:, 6:8]
+    f, pos = torch.rand(32, dtype=torch.float64, device=DEV), torch.arange(50, dtype=torch.int32, device=DEV)
+    want = ops.rotary(q.contiguous(), k.contiguous(), pos, f)
+    assert all(torch.equal(a, b) for a, b in zip(want, ops.rotary(q, k, pos, f)))
+    flat = torch.empty(50 * 6 * 64 + 1, device=DEV)[1:].view(50, 6, 64).copy_(q)                  # off every wide boundary
+    assert torch.equal(ops.rotary(flat, None, pos, f)[0], want[0])
+    other = x.clone()
+    ops.rotary(other[:, :6], other[:, 6:8], pos, f, inplace=True)
+    assert torch.equal(other[:, :6], want[0]) and torch.equal(other[:, 6:8], want[1]) and torch.equal(other[:, 8:], x[:, 8:])
+    kk = k.detach().clone().requires_grad_()
+    d = _randn((50, 2, 64), 4).to(DEV)
+    g, = torch.autograd.grad(ops.rotary(q, kk, pos, f)[1], kk, d)
+    _within(g, *rotary_oracle(d.cpu(), pos.cpu(), f.cpu(), False, 1.0, -1), 'dk')
+
+
+# ------------------------------------------------------------------------------------------------------------------- cache
+class Paged:
+    """A cache and its table on the CPU (64-bit values of what it stands for) and on the GPU."""
+
+    def __init__(self, lens, page, heads, dh, dtype, stored, seed=0, spare=3, fill=float('nan')):
+        ops = _ops()
+        counts = [-(-n // page) for n in lens]
+        pages = sum(counts) + spare
+        order = torch.randperm(pages, generator=torch.Generator().manual_seed(seed)).to(torch.int32)
+        self.table = torch.full((len(lens), max(counts + [1]) + 1), -1, dtype=torch.int32)
+        at = 0
+        for b, c in enumerate(counts):
+            self.table[b, :c] = order[at:at + c]
+            at += c
+        self.cache = ops.KVCache.zeros(pages, page, heads, dh, stored, DEV)
+        if stored == torch.float8_e4m3fn:                               # rows that nobody wrote: NaN
+            self.cache.k.view(torch.uint8).fill_(0x7f)
+            self.cache.v.view(torch.uint8).fill_(0x7f)
+        else:
+            self.cache.k.fill_(fill)
+            self.cache.v.fill_(fill)
+        self.lens, self.k, self.v = lens, [], []
+        starts = _starts(lens).to(DEV)
+        k, v = (_randn((sum(lens), heads, dh), seed + i, dtype) for i in (1, 2))
+        ops.kv_cache_write(self.cache, k.to(DEV), v.to(DEV), self.table.to(DEV), starts, torch.tensor(lens, dtype=torch.int32).to(DEV))
+        if stored == torch.float8_e4m3fn:
+            k, v = (quantised_oracle(x)[0] for x in (k, v))
+        self.k, self.v = torch.split(k, lens), torch.split(v, lens)
+        self.args = (self.table.to(DEV), None, torch.tensor(lens, dtype=torch.int32).to(DEV))
+
+
+def quantised_oracle(x):
+    """(values that the e4m3 rows stand for, biased exponents): the smallest power-of-two scale with |row| <= 448 scale, every
+    value to the nearest multiple of its step (2^-3 of its power of two, at least 2^-9), ties to even."""
+    x = x.double()
+    top = torch.where(torch.isfinite(x), x, torch.zeros_like(x)).abs().amax(-1, keepdim=True)
+    m, e = torch.frexp(top)
+    e = torch.where(top > 0, (e - 9 + (m > 0.875)).clamp(min=-126), torch.zeros_like(e))
+    y = torch.ldexp(x, -e)
+    _, ye = torch.frexp(y)
+    step = torch.ldexp(torch.ones_like(y), (ye - 1).clamp(min=-6) - 3)
+    return torch.where(torch.isfinite(x), torch.round(y / step) * step * torch.ldexp(torch.ones_like(top), e), torch.full_like(x, float('nan'))), (e + 127).squeeze(-1)
+
+
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize('quantise', [False, True])
+@pytest.mark.parametrize('lens,page,heads,dh', [([1], 1, 1, 8), ([5, 0, 70], 16, 2, 64), ([129, 1, 64], 64, 3, 128), ([40], 8, 4, 192), ([33, 2], 1024, 1, 24),
+                                                ([2] * 130, 2, 1, 32)])
+def test_cache_write_and_read(lens, page, heads, dh, quantise, dtype):
+    ops = _ops()
+    stored = torch.float8_e4m3fn if quantise else dtype
+    p = Paged(lens, page, heads, dh, dtype, stored)
+    table, _, ln = p.args
+    for out_type in {dtype, torch.float32} if quantise else {dtype}:
+        k, v = ops.kv_cache_read(p.cache, table, ln, _starts(lens).to(DEV), sum(lens), dtype=out_type)
+        for g, w in ((k, p.k), (v, p.v)):
+            assert torch.equal(g.double().cpu(), torch.cat(w).double())             # exact: one rounding, and none on the way back
+    # only the rows written differ from what was there
+    if not quantise:
+        assert int(torch.isfinite(p.cache.k).sum()) == sum(lens) * heads * dh
+    # the last tokens only, into a longer tensor whose rest stays
+    n = [min(x, 3) for x in lens]
+    out = [torch.full((sum(n) + 5, heads, dh), 9.0, dtype=dtype, device=DEV) for _ in 'kv']
+    ops.kv_cache_read(p.cache, table, ln, _starts(n).to(DEV), sum(n) + 5, out=tuple(out))
+    for g, w in zip(out, (p.k, p.v)):
+        assert torch.equal(g[:sum(n)].double().cpu(), torch.cat([x[len(x) - m:] for x, m in zip(w, n)]).double()) and bool((g[sum(n):] == 9).all())
+    fresh = ops.kv_cache_read(p.cache, table, ln, _starts(n).to(DEV), sum(n) + 5, dtype=dtype)[0]
+    assert torch.equal(fresh[:sum(n)], out[0][:sum(n)]) and not fresh[sum(n):].any()
+
+
+def test_cache_quantised_rows_at_their_borders():
+    """Zeros, one value, values at and next to 448 2^e, halfway cases, tiny and huge rows, NaN and infinity."""
+    ops = _ops()
+    rows = [[0.0] * 8, [448.0] + [1.0] * 7, [449.0, 17.0, 18.0, 19.0, 0.5, -0.5, 464.0, 3.0], [3.5, 0.001, -0.002, 2.0 ** -9, 2.0 ** -10, 3 * 2.0 ** -10, 0.0, -0.0],
+            [1e-38] * 8, [2.0 ** -126, 2.0 ** -130, 0, 0, 0, 0, 0, 1e-40], [3.4e38, -1e37, 1.0, 0, 0, 0, 0, 0], [float('nan'), 2.0, 1.0, 0, 0, 0, 0, 0],
+            [float('inf'), -float('inf'), 5.0, 100.0, 0, 0, 0, 0], [1.0625, 1.1875, 1.3125, -1.0625, 448.0, 432.0, 440.0, 424.0]]
+    x = torch.tensor(rows).view(-1, 1, 8)
+    n = len(rows)
+    cache = ops.KVCache.zeros(1, 16, 1, 8, torch.float8_e4m3fn, DEV)
+    table, st, ln = (torch.tensor(t, dtype=torch.int32, device=DEV) for t in ([[0]], [0, n], [n]))
+    ops.kv_cache_write(cache, x.to(DEV), -x.to(DEV), table, st, ln)
+    want, e = quantised_oracle(x)
+    k, v = ops.kv_cache_read(cache, table, ln, st, n, dtype=torch.float32)
+    assert torch.equal(torch.nan_to_num(k.cpu().double(), nan=1e300), torch.nan_to_num(want.float().double(), nan=1e300))
+    assert torch.equal(torch.nan_to_num(v.cpu().double(), nan=1e300), torch.nan_to_num((-want).float().double(), nan=1e300))
+    assert torch.equal(cache.k_exp[0, 0, :n].cpu().long(), e.view(-1).long())
+
+
+def test_cache_bad_pages_and_positions():
+    """Page numbers outside the cache and tokens without a position: nothing is written, zeros are read, no row of another page
+    changes."""
+    ops = _ops()
+    for dtype in (torch.bfloat16, torch.float8_e4m3fn):
+        cache = ops.KVCache.zeros(4, 8, 2, 32, dtype, DEV)
+        raw = lambda t: t.view(torch.uint8) if dtype == torch.float8_e4m3fn else t
+        raw(cache.k).fill_(1)
+        before = raw(cache.k).clone()
+        table = torch.tensor([[4, 1], [-1, 2 ** 31 - 1], [-2 ** 31, 3]], dtype=torch.int32, device=DEV)
+        st, ln = (torch.tensor(t, dtype=torch.int32, device=DEV) for t in ([0, 10, 20, 24], [10, 40, 2]))
+        k = _randn((24, 2, 32), 1, torch.bfloat16).to(DEV)
+        ops.kv_cache_write(cache, k, k, table, st, ln)
+        # sequence 0: positions 8, 9 lie in page 1; sequence 1: positions 30 .. 39 past the table; sequence 2: 2 tokens too many
+        changed = (raw(cache.k) != before).flatten(2).any(-1).any(-1) if False else (raw(cache.k) != before).view(4, 2, 8, 32).any(-1).any(1)
+        assert changed.nonzero().tolist() == [[1, 0], [1, 1]]
+        back = ops.kv_cache_read(cache, table, ln, st, 24, dtype=torch.bfloat16)[0]
+        assert not back[:8].any() and not back[10:].any() and bool(back[8:10].any())
+
+
+def test_cache_offsets_past_32_bits():
+    """More than 2^32 bytes of pages: the last page is written, read and attended to."""
+    ops = _ops()
+    page, heads, dh = 64, 8, 128
+    pages = (1 << 32) // (page * heads * dh) + 40
+    cache = ops.KVCache(*(torch.empty((pages, heads, page, dh), dtype=torch.uint8, device=DEV).view(torch.float8_e4m3fn) for _ in 'kv'),
+                        *(torch.full((pages, heads, page), 127, dtype=torch.uint8, device=DEV) for _ in 'kv'))
+    n = 100
+    table, st, ln = (torch.tensor(t, dtype=torch.int32, device=DEV) for t in ([[pages - 1, pages - 30]], [0, n], [n]))
+    k, v, q = (_randn((n, h, dh), i, torch.bfloat16) for i, h in enumerate((heads, heads, 16)))
+    ops.kv_cache_write(cache, k.to(DEV), v.to(DEV), table, st, ln)
+    back = ops.kv_cache_read(cache, table, ln, st, n)
+    kq, vq = quantised_oracle(k)[0], quantised_oracle(v)[0]
+    assert torch.equal(back[0].double().cpu(), kq) and torch.equal(back[1].double().cpu(), vq)
+    want, bound = attention_oracle(q, kq, vq, 0, True, dh ** -0.5, torch.bfloat16)
+    _within(ops.paged_attention(q.to(DEV), cache, table, st, ln), want[0], bound[0], 'out')
+
+
+# --------------------------------------------------------------------------------------------------------- paged attention
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize('quantise', [False, True])
+@pytest.mark.parametrize('new,lens,page,H,Hkv,dh', [
+    ([1], [1], 16, 1, 1, 8), ([1] * 5, [1, 700, 64, 65, 1023], 16, 8, 2, 128), ([1, 1], [5000, 3], 64, 4, 4, 64), ([1, 1, 1], [300, 17, 90], 8, 32, 2, 64),
+    ([70, 1, 200], [300, 513, 200], 32, 4, 2, 64), ([129], [129], 1, 2, 1, 192), ([3, 0, 40], [1000, 20, 1040], 128, 6, 3, 80), ([17] * 9, [17 + 31 * i for i in range(9)], 16, 16, 2, 128),
+    ([2, 3, 1, 4], [2000, 999, 640, 641], 64, 8, 1, 192)])
+def test_paged_attention(new, lens, page, H, Hkv, dh, quantise, dtype):
+    ops = _ops()
+    p = Paged(lens, page, Hkv, dh, dtype, torch.float8_e4m3fn if quantise else dtype)
+    q = _randn((sum(new), H, dh), 9, dtype, 1.5)
+    table, _, ln = p.args
+    st = _starts(new).to(DEV)
+    got = ops.paged_attention(q.to(DEV), p.cache, table, st, ln)
+    at = 0
+    want, bound = [], []
+    for b, n in enumerate(new):
+        w, e = attention_oracle(q[at:at + n], p.k[b], p.v[b], lens[b] - n, True, dh ** -0.5, dtype)
+        want.append(w[0])
+        bound.append(e[0])
+        at += n
+    want, bound = torch.cat(want), torch.cat(bound)
+    _within(got, want, bound, 'out')
+    # other splits of the keys (from none to many): within the same bound, and the same bits every time
+    for max_len in (1, 300, 1 << 20):
+        other = ops.paged_attention(q.to(DEV), p.cache, table, st, ln, max_len=max_len)
+        _within(other, want, bound, f'max_len {max_len}')
+        assert torch.equal(other, ops.paged_attention(q.to(DEV), p.cache, table, st, ln, max_len=max_len))
+
+
+def test_paged_attention_rows_that_see_nothing_and_bad_pages():
+    ops = _ops()
+    p = Paged([40, 6], 8, 2, 64, torch.float32, torch.float32)
+    table, _, _ = p.args
+    q = _randn((9, 4, 64), 1).to(DEV)
+    st, ln = (torch.tensor(t, dtype=torch.int32, device=DEV) for t in ([0, 5, 7], [3, 0]))
+    for max_len in (1, 1 << 16):
+        got = ops.paged_attention(q, p.cache, table, st, ln, max_len=max_len)
+        # sequence 0 has 3 cached tokens and 5 queries: the first two stand before position 0; sequence 1 is empty; two rows behind
+        assert not got[:2].any() and not got[5:].any()
+        want, bound = attention_oracle(q[2:5].cpu(), p.k[0][:3], p.v[0][:3], 0, True, 0.125, torch.float32)
+        _within(got[2:5], want[0], bound[0], 'out')
+        out = torch.full_like(q, 5.0)
+        back = ops.paged_attention(q, p.cache, table, st, ln, max_len=max_len, out=out)
+        assert back is out and torch.equal(out[:7], got[:7]) and bool((out[7:] == 5).all())
+    bad = table.clone()
+    bad[0, 1] = 10 ** 6                                        # positions 8 .. 15 read as zeros
+    st, ln = (torch.tensor(t, dtype=torch.int32, device=DEV) for t in ([0, 1, 2], [40, 6]))
+    k, v = p.k[0].clone(), p.v[0].clone()
+    k[8:16], v[8:16] = 0, 0
+    want, bound = attention_oracle(q[:1].cpu(), k, v, 39, True, 0.125, torch.float32)
+    _within(ops.paged_attention(q[:2].contiguous(), p.cache, bad, st, ln)[:1], want[0], bound[0], 'out')
+    # lens past what the table holds: the positions without a page read as zeros as well
+    short = table[:, :2].contiguous()
+    k, v = p.k[0].clone(), p.v[0].clone()
+    k[16:], v[16:] = 0, 0
+    want, bound = attention_oracle(q[:1].cpu(), k, v, 39, True, 0.125, torch.float32)
+    _within(ops.paged_attention(q[:2].contiguous(), p.cache, short, st, ln)[:1], want[0], bound[0], 'out')
+
+
+def test_paged_attention_graph_replay_decodes_on():
+    """One captured decoding step - rotary, cache write, attention - replayed as the sequences grow, against the eager calls."""
+    ops = _ops()
+    H, Hkv, dh, B = 8, 2, 64, 3
+    f = torch.rand(32, dtype=torch.float64, device=DEV)
+    def world():
+        p = Paged([30, 1, 77], 16, Hkv, dh, torch.bfloat16, torch.float8_e4m3fn, spare=30)
+        table = torch.arange(B * 10, dtype=torch.int32, device=DEV).view(B, 10)
+        fresh = ops.KVCache.zeros(B * 10, 16, Hkv, dh, torch.float8_e4m3fn, DEV)
+        k, v = ops.kv_cache_read(p.cache, p.args[0], p.args[2], _starts(p.lens).to(DEV), 108)
+        ops.kv_cache_write(fresh, k, v, table, _starts(p.lens).to(DEV), p.args[2])
+        return fresh, table, p.args[2].clone(), _starts([1] * B).to(DEV)
+    x = [torch.zeros((B, h, dh), dtype=torch.bfloat16, device=DEV) for h in (H, Hkv, Hkv)]
+    def step(cache, table, ln, st):
+        ln += 1
+        q, k = ops.rotary(x[0], x[1], ln - 1, f)
+        ops.kv_cache_write(cache, k, x[2], table, st, ln)
+        return ops.paged_attention(q, cache, table, st, ln, max_len=160)
+    a, b = world(), world()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        step(*world())
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        res = step(*a)
+    for i in range(6):
+        for j, t in enumerate(x):
+            t.copy_(_randn(t.shape, 40 + 3 * i + j, torch.bfloat16))
+        graph.replay()
+        want = step(*b)
+        torch.cuda.synchronize()
+        assert torch.equal(res, want) and torch.equal(a[0].k_exp, b[0].k_exp), i
+
+
+# ----------------------------------------------------------------------------------------------------------------- together
+@pytest.mark.parametrize('stored', [torch.bfloat16, torch.float8_e4m3fn])
+def test_prompt_then_chunks_then_single_tokens(stored):
+    """The operators as they are used together: rotary positions, the prompts through packed attention while their keys and
+    values go into the cache, then a chunk, then single tokens over the cache - against the 64-bit definition on the whole
+    sequences (from the turned and stored values that the operators return)."""
+    from transformertts_amd.model.transformer_utils import rotary_frequencies
+    ops = _ops()
+    H, Hkv, dh, page, dtype = 8, 2, 64, 16, torch.bfloat16
+    f = torch.from_numpy(rotary_frequencies(dh, scaling='bands', factor=8.0)).to(DEV)
+    B, steps = 3, [[50, 7, 129], [40, 1, 3], [1, 1, 1], [1, 1, 1]]
+    cache = ops.KVCache.zeros(60, page, Hkv, dh, stored, DEV)
+    table = torch.randperm(60, generator=torch.Generator().manual_seed(1)).to(torch.int32)[:B * 20].view(B, 20).to(DEV)
+    lens = [0] * B
+    seen_q = [[] for _ in range(B)]
+    for i, new in enumerate(steps):
+        M, st = sum(new), _starts(new).to(DEV)
+        lens = [a + b for a, b in zip(lens, new)]
+        ln = torch.tensor(lens, dtype=torch.int32, device=DEV)
+        q, k, v = (t.to(DEV) for t in torch.split(_randn((M, H + 2 * Hkv, dh), 20 + i, dtype), [H, Hkv, Hkv], 1))
+        pos = torch.cat([torch.arange(a - n, a) for a, n in zip(lens, new)]).to(torch.int32).to(DEV)
+        q, k = ops.rotary(q, k, pos, f)
+        ops.kv_cache_write(cache, k, v, table, st, ln)
+        out = ops.packed_attention(q, k, v, st) if i == 0 else ops.paged_attention(q, cache, table, st, ln)
+        kk, vv = ops.kv_cache_read(cache, table, ln, _starts(lens).to(DEV), sum(lens), dtype=dtype)
+        at, base = 0, 0
+        for b, n in enumerate(new):
+            # (the prompt is attended to as it is, before it is quantised)
+            K, V = (t[base:base + lens[b]].cpu() for t in (kk, vv)) if i else (t[at:at + n].cpu() for t in (k, v))
+            want, bound = attention_oracle(q[at:at + n].cpu(), K, V, lens[b] - n, True, dh ** -0.5, dtype)
+            _within(out[at:at + n], want[0], bound[0], f'step {i}, sequence {b}')
+            at, base = at + n, base + lens[b]

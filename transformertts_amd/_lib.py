@@ -21,7 +21,7 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 # version this binding was written for (EXPECTED_VERSION, checked in lib()).
 _override = os.environ.get('TTSMI_LIB') if os.environ.get('TTSMI_ALLOW_LIB_OVERRIDE') == '1' else None
 LIB_PATH = _override or os.path.join(_HERE, 'lib', 'libttsmi.so')
-EXPECTED_VERSION = 109            # include/ttsmi.h: TTSMI_VERSION
+EXPECTED_VERSION = 110            # include/ttsmi.h: TTSMI_VERSION
 
 P = c_void_p          # every device pointer
 I = c_int
@@ -138,6 +138,16 @@ SIGNATURES = {
     'ttsmi_ft_train_step': (I, [P, I]),
     'ttsmi_add2_f32': (I, [P, P, P, L, S]),
     'ttsmi_pad_cols_f32': (I, [P, I, P, I, I, S]),
+    'ttsmi_rotary': (I, [P, L, L, P, L, L, I, P, L, L, P, L, L, I, P, P, I, I, I, I, F, I, I, S]),
+    'ttsmi_packed_attention_fwd': (I, [P, L, L, P, L, L, P, L, L, P, I, I, I, I, I, F, I, P, L, L, P, I, I, S]),
+    'ttsmi_packed_attention_bwd_ws_bytes': (c_size_t, [I, I]),
+    'ttsmi_packed_attention_bwd': (I, [P, L, L, P, L, L, P, L, L, P, L, L, P, L, L, P, P, I, I, I, I, I, F, I, P, L,
+        L, P, L, L, P, L, L, I, P, c_size_t, I, S]),
+    'ttsmi_kv_cache_write': (I, [P, L, L, P, L, L, P, P, P, P, I, I, I, P, I, P, P, I, I, I, I, I, S]),
+    'ttsmi_kv_cache_read': (I, [P, P, P, P, I, I, I, P, I, P, P, I, I, I, I, P, L, L, P, L, L, I, I, S]),
+    'ttsmi_paged_attention_ws_bytes': (c_size_t, [I, I, I, I, I, I]),
+    'ttsmi_paged_attention': (I, [P, L, L, P, P, P, P, I, I, I, P, I, P, P, I, I, I, I, I, F, I, P, L, L, I, P,
+        c_size_t, I, S]),
 }
 
 
@@ -211,7 +221,7 @@ class FtStep(ctypes.Structure):
     _fields_ = _ft_step_fields()
 
 
-TTSMI_F32, TTSMI_BF16, TTSMI_BF16_IO, TTSMI_BF16X3 = 0, 1, 2, 3
+TTSMI_F32, TTSMI_BF16, TTSMI_BF16_IO, TTSMI_BF16X3, TTSMI_E4M3 = 0, 1, 2, 3, 4
 LAUNCH_OBSERVER = ctypes.CFUNCTYPE(None, c_int, c_char_p, ctypes.c_double, ctypes.c_double, c_void_p)
 
 _lib = None

@@ -16,8 +16,13 @@ LIBDIR = os.path.join(HERE, 'lib')
 OBJDIR = os.path.join(HERE, 'build')
 LIB = os.path.join(LIBDIR, 'libttsmi.so')
 SOURCES = ['api.cpp', 'gemm.hip', 'gemm_bf16.hip', 'attention.hip', 'attention_bf16.hip', 'layernorm.hip',
-           'elementwise.hip', 'lenreg.hip', 'stft_mel.hip', 'dense_block.hip', 'rowgemm.hip', 'gemm_k256.hip', 'chain.hip', 'train_step.hip', 'griffinlim.hip', 'nnls.hip', 'collective.cpp']
+           'elementwise.hip', 'lenreg.hip', 'stft_mel.hip', 'dense_block.hip', 'rowgemm.hip', 'gemm_k256.hip', 'chain.hip', 'train_step.hip', 'griffinlim.hip', 'nnls.hip', 'collective.cpp',
+           'rotary.hip', 'kvcache.hip', 'seq_attention.hip', 'seq_attention_bwd.hip']
 FLAGS = ['--offload-arch=gfx950', '-O3', '-std=c++17', '-fPIC', '-Wno-unused-result']
+# Without packed fp32 arithmetic (v_pk_add / mul / fma_f32), some of whose forms have given wrong results on this card with no
+# error: the sources that do not write it by hand and whose measured kernels were not built with it.
+UNPACKED = {'rotary.hip', 'kvcache.hip', 'seq_attention.hip', 'seq_attention_bwd.hip'}
+UNPACKED_FLAGS = ['-Xclang', '-target-feature', '-Xclang', '-packed-fp32-ops']
 # measurement builds only, e.g. TTSMI_EXTRA_HIPCC_FLAGS=-DTTSMI_ABLATION_BUILD (stage-ablation knobs, csrc/common.h)
 FLAGS += os.environ.get('TTSMI_EXTRA_HIPCC_FLAGS', '').split()
 
@@ -34,7 +39,7 @@ def _digest(paths) -> str:
     for p in paths:
         with open(p, 'rb') as f:
             h.update(f.read())
-    h.update(' '.join(FLAGS).encode())
+    h.update(' '.join(FLAGS + UNPACKED_FLAGS + sorted(UNPACKED)).encode())
     return h.hexdigest()
 
 
@@ -69,7 +74,7 @@ def build(force: bool = False, verbose: bool = True) -> str:
 
     def compile_one(job):
         sp, obj, stamp, dig = job
-        cmd = [hipcc] + FLAGS + ['-x', 'hip', '-c', sp, '-o', obj]
+        cmd = [hipcc] + FLAGS + (UNPACKED_FLAGS if os.path.basename(sp) in UNPACKED else []) + ['-x', 'hip', '-c', sp, '-o', obj]
         r = subprocess.run(cmd, capture_output=True, text=True)
         if r.returncode != 0:
             raise RuntimeError(f'hipcc failed for {sp}:\n{r.stdout}\n{r.stderr}')

@@ -1,0 +1,342 @@
+// Backward of attention over packed sequences, in two passes that recompute the probabilities from lse (no [rows, keys] tensor,
+// no atomics: every gradient element is summed by one workgroup in a fixed order).
+//
+//   delta_i = do_i . o_i     p_ij = exp(s_ij - lse_i)     ds_ij = p_ij (do_i . v_j - delta_i)
+//   dq_i = scale sum_j ds_ij k_j      dk_j = scale sum_i ds_ij q_i      dv_j = sum_i p_ij do_i      (i: every query head of the group)
+//
+// delta:  one pass over do and o.
+// dQ:     as the forward - 128 rows a workgroup, 32 a wave, S^T and dP^T per key tile, dQ^T += K^T dS^T.
+// dK, dV: 128 keys of one key head a workgroup, 32 a wave; the row tiles of every query head of the group pass through LDS, the
+//         wave forms S and dP with a key per lane, so that P and dS are the B operands of dV^T += dO^T P and dK^T += Q^T dS.
+#include "seq_common.h"
+
+struct SeqBwdP {
+    const void* q; long q_row, q_head;
+    const void* k; long k_row, k_head;
+    const void* v; long v_row, v_head;
+    const void* o; long o_row, o_head;
+    const void* d; long d_row, d_head;                    // gradient of the output
+    void* dq; long dq_row, dq_head;
+    void* dk; long dk_row, dk_head;
+    void* dv; long dv_row, dv_head;
+    const float* lse; float* delta;                       // [Hkv][tokens G]
+    const int* starts;
+    int B, tokens, Hkv, G, dh, causal, zero_rest;
+    float scale, c1;
+};
+
+// delta and nothing else: a wave a row of (token, head), 16 bytes a lane
+template <typename T>
+__global__ __launch_bounds__(256) void seq_delta_kernel(SeqBwdP p) {
+    const int H = p.Hkv * p.G;
+    constexpr int LPR = 32;                                // lanes per row: 32 x 8 elements cover 192
+    const long row = (long)blockIdx.x * (256 / LPR) + threadIdx.x / LPR;
+    if (row >= (long)p.tokens * H) return;
+    const int tok = (int)(row / H), head = (int)(row - (long)tok * H), c = (threadIdx.x % LPR) * 8;
+    float s = 0.f;
+    if (c < p.dh) {
+        const typename SeqT<T>::frag a = *reinterpret_cast<const typename SeqT<T>::frag*>((const T*)p.o + (long)tok * p.o_row + (long)head * p.o_head + c);
+        const typename SeqT<T>::frag b = *reinterpret_cast<const typename SeqT<T>::frag*>((const T*)p.d + (long)tok * p.d_row + (long)head * p.d_head + c);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) s += (float)a[e] * (float)b[e];
+    }
+#pragma unroll
+    for (int o = LPR / 2; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
+    if (c == 0) p.delta[(long)(head / p.G) * p.tokens * p.G + (long)tok * p.G + head % p.G] = s;
+}
+
+// four accumulator registers -> four consecutive elements of a gradient row
+template <typename T>
+__device__ __forceinline__ void seq_store4(T* dst, const f32x16& a, int g, float f) {
+    if constexpr (sizeof(T) == 2) {
+        bf16x4 h;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) h[e] = (__bf16)(a[4 * g + e] * f);
+        *reinterpret_cast<bf16x4*>(dst) = h;
+    } else {
+        *reinterpret_cast<float4*>(dst) = make_float4(a[4 * g] * f, a[4 * g + 1] * f, a[4 * g + 2] * f, a[4 * g + 3] * f);
+    }
+}
+
+template <typename T, int DHP>
+__global__ __launch_bounds__(256, (DHP <= 128 && sizeof(T) == 2) ? 2 : 1) void seq_attn_dq_kernel(SeqBwdP p) {
+    using I = SeqImg<T, DHP>;
+    using frag = typename SeqT<T>::frag;
+    constexpr int KT = SeqT<T>::KT, NKB = KT / 32, NS = DHP / 16, NCB = DHP / 32, EPC = 16 / (int)sizeof(T);
+    constexpr int ITEMS = KT * I::CH / 256;
+    __shared__ __attribute__((aligned(16))) unsigned char Ks[KT * I::ROWB], Vs[KT * I::ROWB];
+    const int tid = threadIdx.x, lane = tid & 63, l31 = lane & 31, hh = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int hk = blockIdx.x % p.Hkv, unit = blockIdx.x / p.Hkv;
+    const SeqTile st = find_tile(p.starts, p.B, p.tokens, p.G, 128, unit);
+    if (st.seq < 0) {
+        if (p.zero_rest) seq_zero_rest<T>((T*)p.dq, p.dq_row, p.dq_head, p.starts, p.B, p.tokens, p.G, 128, hk * p.G, p.dh, st.tile);
+        return;
+    }
+    const int tile = st.ntile - 1 - st.tile, rows = st.n * p.G, len = st.n;
+    const int r = tile * 128 + wave * 32 + l31;
+    const bool rok = r < rows;
+    const int tok = r / p.G, head = hk * p.G + r - tok * p.G;
+    const int lim = !rok ? 0 : p.causal ? min(tok + 1, len) : len;
+    const int last = min(tile * 128 + 127, rows - 1) / p.G;
+    const int kend = p.causal ? min(last + 1, len) : len;
+    const int wrow = tile * 128 + wave * 32;
+    const int wend = wrow >= rows ? 0 : p.causal ? min(kend, min(wrow + 31, rows - 1) / p.G + 1) : kend;
+    const int wfull = wrow + 31 < rows ? (p.causal ? wrow / p.G + 1 : len) : 0;
+    const long slot = (long)hk * p.tokens * p.G + (long)st.s0 * p.G + r;
+
+    frag qf[NS], df[NS];
+    {
+        const T* qr = (const T*)p.q + (long)(st.s0 + tok) * p.q_row + (long)head * p.q_head;
+        const T* dr = (const T*)p.d + (long)(st.s0 + tok) * p.d_row + (long)head * p.d_head;
+#pragma unroll
+        for (int s = 0; s < NS; ++s) {
+            const bool ok = rok && 16 * s + 8 * hh < p.dh;
+            qf[s] = seq_load8<T>(qr, 16 * s + 8 * hh, ok);
+            df[s] = seq_load8<T>(dr, 16 * s + 8 * hh, ok);
+        }
+    }
+    const float lse2 = rok ? p.lse[slot] * SEQ_LOG2E : 0.f, delta = rok ? p.delta[slot] : 0.f;
+    f32x16 acc[NCB];
+#pragma unroll
+    for (int cb = 0; cb < NCB; ++cb)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc[cb][i] = 0.f;
+    uint4 rk[ITEMS], rv[ITEMS];
+    auto fetch = [&](int k0) {
+#pragma unroll
+        for (int i = 0; i < ITEMS; ++i) {
+            const int id = tid + 256 * i, row = id / I::CH, ch = id - row * I::CH, key = k0 + row;
+            rk[i] = rv[i] = make_uint4(0u, 0u, 0u, 0u);
+            if (key < kend && ch * EPC < p.dh) {
+                rk[i] = *reinterpret_cast<const uint4*>((const T*)p.k + (long)(st.s0 + key) * p.k_row + (long)hk * p.k_head + ch * EPC);
+                rv[i] = *reinterpret_cast<const uint4*>((const T*)p.v + (long)(st.s0 + key) * p.v_row + (long)hk * p.v_head + ch * EPC);
+            }
+        }
+    };
+    fetch(0);
+    for (int k0 = 0; k0 < kend; k0 += KT) {
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < ITEMS; ++i) {
+            const int id = tid + 256 * i, row = id / I::CH, ch = id - row * I::CH;
+            *reinterpret_cast<uint4*>(Ks + I::at(row, ch)) = rk[i];
+            *reinterpret_cast<uint4*>(Vs + I::at(row, ch)) = rv[i];
+        }
+        __syncthreads();
+        if (k0 + KT < kend) fetch(k0 + KT);
+        if (k0 >= wend) continue;
+        const bool edge = k0 + KT > wfull;
+#pragma unroll
+        for (int kb = 0; kb < NKB; ++kb) {
+            if (k0 + kb * 32 >= wend) break;
+            f32x16 s, dp;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s[i] = dp[i] = 0.f;
+#pragma unroll
+            for (int t = 0; t < NS; ++t) {
+                s = seq_mma(seq_frag<T, DHP>(Ks, kb * 32 + l31, t, hh), qf[t], s);
+                dp = seq_mma(seq_frag<T, DHP>(Vs, kb * 32 + l31, t, hh), df[t], dp);
+            }
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s[i] = __builtin_amdgcn_exp2f(s[i] * p.c1 - lse2) * (dp[i] - delta);
+            if (edge) {
+                const int seen = lim - k0 - kb * 32;
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    if (seq_rowmap(i, hh) >= seen) s[i] = 0.f;
+            }
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                frag f;
+                seq_to_frag(s, t, f);
+#pragma unroll
+                for (int cb = 0; cb < NCB; ++cb) acc[cb] = seq_mma(seq_frag_t<T, DHP>(Ks, kb * 32, t, cb, lane), f, acc[cb]);
+            }
+        }
+    }
+    if (!rok) return;
+    T* dst = (T*)p.dq + (long)(st.s0 + tok) * p.dq_row + (long)head * p.dq_head;
+#pragma unroll
+    for (int cb = 0; cb < NCB; ++cb)
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+            if (cb * 32 + 8 * g + 4 * hh < p.dh) seq_store4<T>(dst + cb * 32 + 8 * g + 4 * hh, acc[cb], g, p.scale);
+}
+
+template <typename T, int DHP>
+__global__ __launch_bounds__(256, 1) void seq_attn_dkv_kernel(SeqBwdP p) {
+    using I = SeqImg<T, DHP>;
+    using frag = typename SeqT<T>::frag;
+    constexpr int KT = SeqT<T>::KT, NKB = KT / 32, NS = DHP / 16, NCB = DHP / 32, EPC = 16 / (int)sizeof(T);
+    constexpr int ITEMS = KT * I::CH / 256;
+    __shared__ __attribute__((aligned(16))) unsigned char Qs[KT * I::ROWB], Ds[KT * I::ROWB];
+    __shared__ __attribute__((aligned(16))) float Ls[2 * KT];                    // lse (log2 units) and delta of the staged rows
+    const int tid = threadIdx.x, lane = tid & 63, l31 = lane & 31, hh = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int hk = blockIdx.x % p.Hkv, unit = blockIdx.x / p.Hkv;
+    const SeqTile st = find_tile(p.starts, p.B, p.tokens, 1, 128, unit);         // causal: the first keys have the most rows
+    if (st.seq < 0) {
+        if (p.zero_rest) {
+            seq_zero_rest<T>((T*)p.dk, p.dk_row, p.dk_head, p.starts, p.B, p.tokens, 1, 128, hk, p.dh, st.tile);
+            seq_zero_rest<T>((T*)p.dv, p.dv_row, p.dv_head, p.starts, p.B, p.tokens, 1, 128, hk, p.dh, st.tile);
+        }
+        return;
+    }
+    const int key0 = st.tile * 128, key = key0 + wave * 32 + l31, rows = st.n * p.G;
+    const bool kok = key < st.n;
+    const bool live = key0 + wave * 32 < st.n;
+    frag kf[NS], vf[NS];
+    {
+        const T* kr = (const T*)p.k + (long)(st.s0 + key) * p.k_row + (long)hk * p.k_head;
+        const T* vr = (const T*)p.v + (long)(st.s0 + key) * p.v_row + (long)hk * p.v_head;
+#pragma unroll
+        for (int s = 0; s < NS; ++s) {
+            const bool ok = kok && 16 * s + 8 * hh < p.dh;
+            kf[s] = seq_load8<T>(kr, 16 * s + 8 * hh, ok);
+            vf[s] = seq_load8<T>(vr, 16 * s + 8 * hh, ok);
+        }
+    }
+    f32x16 dk[NCB], dv[NCB];
+#pragma unroll
+    for (int cb = 0; cb < NCB; ++cb)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) dk[cb][i] = dv[cb][i] = 0.f;
+    const int first = p.causal ? key0 * p.G : 0;                                  // rows before see none of these keys
+    const int wfirst = p.causal ? (key0 + wave * 32) * p.G : 0;
+    const int wfull = p.causal ? (key0 + wave * 32 + 31) * p.G : 0;               // from here on rows see every key of the wave
+    const int low = p.causal ? key * p.G : 0;                                     // this lane's key: rows >= low see it
+    const long slot0 = (long)hk * p.tokens * p.G + (long)st.s0 * p.G;
+    uint4 rq[ITEMS], rd[ITEMS];
+    float rl = 0.f;
+    auto fetch = [&](int r0) {
+#pragma unroll
+        for (int i = 0; i < ITEMS; ++i) {
+            const int id = tid + 256 * i, row = id / I::CH, ch = id - row * I::CH, r = r0 + row;
+            rq[i] = rd[i] = make_uint4(0u, 0u, 0u, 0u);
+            if (r < rows && ch * EPC < p.dh) {
+                const int tok = r / p.G, head = hk * p.G + r - tok * p.G;
+                rq[i] = *reinterpret_cast<const uint4*>((const T*)p.q + (long)(st.s0 + tok) * p.q_row + (long)head * p.q_head + ch * EPC);
+                rd[i] = *reinterpret_cast<const uint4*>((const T*)p.d + (long)(st.s0 + tok) * p.d_row + (long)head * p.d_head + ch * EPC);
+            }
+        }
+        if (tid < 2 * KT) {
+            const int r = r0 + (tid & (KT - 1));
+            rl = r >= rows ? 0.f : tid < KT ? p.lse[slot0 + r] * SEQ_LOG2E : p.delta[slot0 + r];
+        }
+    };
+    const int r_begin = first / KT * KT;
+    fetch(r_begin);
+    for (int r0 = r_begin; r0 < rows; r0 += KT) {
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < ITEMS; ++i) {
+            const int id = tid + 256 * i, row = id / I::CH, ch = id - row * I::CH;
+            *reinterpret_cast<uint4*>(Qs + I::at(row, ch)) = rq[i];
+            *reinterpret_cast<uint4*>(Ds + I::at(row, ch)) = rd[i];
+        }
+        if (tid < 2 * KT) Ls[tid] = rl;
+        __syncthreads();
+        if (r0 + KT < rows) fetch(r0 + KT);
+        if (!live || r0 + KT <= wfirst) continue;
+        const bool edge = r0 < wfull || r0 + KT > rows;
+#pragma unroll
+        for (int kb = 0; kb < NKB; ++kb) {
+            if (r0 + kb * 32 >= rows || r0 + kb * 32 + 32 <= wfirst) continue;
+            f32x16 s, dp;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s[i] = dp[i] = 0.f;
+#pragma unroll
+            for (int t = 0; t < NS; ++t) {
+                s = seq_mma(seq_frag<T, DHP>(Qs, kb * 32 + l31, t, hh), kf[t], s);
+                dp = seq_mma(seq_frag<T, DHP>(Ds, kb * 32 + l31, t, hh), vf[t], dp);
+            }
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const float4 ls = *reinterpret_cast<const float4*>(Ls + kb * 32 + 8 * g + 4 * hh);
+                const float4 dl = *reinterpret_cast<const float4*>(Ls + KT + kb * 32 + 8 * g + 4 * hh);
+                const float le[4] = {ls.x, ls.y, ls.z, ls.w}, de[4] = {dl.x, dl.y, dl.z, dl.w};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    s[4 * g + e] = __builtin_amdgcn_exp2f(s[4 * g + e] * p.c1 - le[e]);
+                    dp[4 * g + e] = s[4 * g + e] * (dp[4 * g + e] - de[e]);
+                }
+            }
+            if (edge) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const int r = r0 + kb * 32 + seq_rowmap(i, hh);
+                    if (r < low || r >= rows) s[i] = dp[i] = 0.f;
+                }
+            }
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                frag f, g;
+                seq_to_frag(s, t, f);
+                seq_to_frag(dp, t, g);
+#pragma unroll
+                for (int cb = 0; cb < NCB; ++cb) {
+                    dv[cb] = seq_mma(seq_frag_t<T, DHP>(Ds, kb * 32, t, cb, lane), f, dv[cb]);
+                    dk[cb] = seq_mma(seq_frag_t<T, DHP>(Qs, kb * 32, t, cb, lane), g, dk[cb]);
+                }
+            }
+        }
+    }
+    if (!kok) return;
+    T* dkr = (T*)p.dk + (long)(st.s0 + key) * p.dk_row + (long)hk * p.dk_head;
+    T* dvr = (T*)p.dv + (long)(st.s0 + key) * p.dv_row + (long)hk * p.dv_head;
+#pragma unroll
+    for (int cb = 0; cb < NCB; ++cb)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            const int c = cb * 32 + 8 * g + 4 * hh;
+            if (c >= p.dh) continue;
+            seq_store4<T>(dkr + c, dk[cb], g, p.scale);
+            seq_store4<T>(dvr + c, dv[cb], g, 1.f);
+        }
+}
+
+template <typename T, int DHP>
+static void seq_bwd_launch(const SeqBwdP& p, hipStream_t st) {
+    const long rows = (long)p.tokens * p.Hkv * p.G;
+    hipLaunchKernelGGL((seq_delta_kernel<T>), dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, st, p);
+    hipLaunchKernelGGL((seq_attn_dkv_kernel<T, DHP>), dim3((unsigned)(seq_units(p.tokens, p.B, 1, 128) * p.Hkv)), dim3(256), 0, st, p);
+    hipLaunchKernelGGL((seq_attn_dq_kernel<T, DHP>), dim3((unsigned)(seq_units(p.tokens, p.B, p.G, 128) * p.Hkv)), dim3(256), 0, st, p);
+}
+template <typename T>
+static int seq_bwd_route(const SeqBwdP& p, hipStream_t st) {
+    if (p.dh <= 64) seq_bwd_launch<T, 64>(p, st);
+    else if (p.dh <= 128) seq_bwd_launch<T, 128>(p, st);
+    else seq_bwd_launch<T, 192>(p, st);
+    TTSMI_CHECK_LAUNCH("packed_attention_bwd");
+    return TTSMI_OK;
+}
+
+extern "C" size_t ttsmi_packed_attention_bwd_ws_bytes(int tokens, int H) {
+    return tokens <= 0 || H <= 0 ? 0 : (size_t)tokens * H * sizeof(float);
+}
+extern "C" int ttsmi_packed_attention_bwd(const void* q, int64_t q_row, int64_t q_head, const void* k, int64_t k_row, int64_t k_head,
+                                          const void* v, int64_t v_row, int64_t v_head, const void* out, int64_t o_row, int64_t o_head,
+                                          const void* dout, int64_t d_row, int64_t d_head, const float* lse, const int32_t* starts,
+                                          int B, int tokens, int H, int Hkv, int dh, float scale, int causal, void* dq, int64_t dq_row,
+                                          int64_t dq_head, void* dk, int64_t dk_row, int64_t dk_head, void* dv, int64_t dv_row,
+                                          int64_t dv_head, int zero_rest, void* ws, size_t ws_bytes, int dtype, ttsmi_stream_t stream) {
+    SEQ_CHECK_COMMON("packed_attention_bwd");
+    if (tokens == 0) return TTSMI_OK;
+    TTSMI_CHECK_ARG(starts && lse, "packed_attention_bwd: null starts or lse");
+    TTSMI_CHECK_ARG(seq_strides_ok(q, q_row, q_head, dtype) && seq_strides_ok(k, k_row, k_head, dtype) && seq_strides_ok(v, v_row, v_head, dtype) &&
+                        seq_strides_ok(out, o_row, o_head, dtype) && seq_strides_ok(dout, d_row, d_head, dtype) &&
+                        seq_strides_ok(dq, dq_row, dq_head, dtype) && seq_strides_ok(dk, dk_row, dk_head, dtype) &&
+                        seq_strides_ok(dv, dv_row, dv_head, dtype), "packed_attention_bwd: a tensor is null or its rows or heads are not 16-byte aligned");
+    if (!ws || ws_bytes < ttsmi_packed_attention_bwd_ws_bytes(tokens, H)) {
+        ttsmi_set_error("packed_attention_bwd: workspace of %zu bytes, %zu needed", ws_bytes, ttsmi_packed_attention_bwd_ws_bytes(tokens, H));
+        return TTSMI_ERR_WORKSPACE;
+    }
+    SeqBwdP p = {};
+    p.q = q; p.q_row = q_row; p.q_head = q_head; p.k = k; p.k_row = k_row; p.k_head = k_head; p.v = v; p.v_row = v_row; p.v_head = v_head;
+    p.o = out; p.o_row = o_row; p.o_head = o_head; p.d = dout; p.d_row = d_row; p.d_head = d_head;
+    p.dq = dq; p.dq_row = dq_row; p.dq_head = dq_head; p.dk = dk; p.dk_row = dk_row; p.dk_head = dk_head; p.dv = dv; p.dv_row = dv_row; p.dv_head = dv_head;
+    p.lse = lse; p.delta = (float*)ws; p.starts = starts; p.B = B; p.tokens = tokens; p.Hkv = Hkv; p.G = H / Hkv; p.dh = dh;
+    p.causal = causal != 0; p.zero_rest = zero_rest != 0; p.scale = scale; p.c1 = scale * SEQ_LOG2E;
+    return dtype == TTSMI_F32 ? seq_bwd_route<float>(p, (hipStream_t)stream) : seq_bwd_route<__bf16>(p, (hipStream_t)stream);
+}

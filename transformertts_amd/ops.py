@@ -2134,3 +2134,341 @@ class PlannedDenseStackFn(torch.autograd.Function):
             pl._defer_ln()
         bottom = plans[0]
         return bottom.t['dh'][:bottom.M].detach(), None, None
+
+
+# =================================================================================================
+# sequence operators: rotary positions, attention over packed sequences, the paged key / value cache (include/ttsmi.h)
+# =================================================================================================
+# Tensors of tokens are [tokens, heads, dh], fp32 or bf16, views with strides of their own among them (the parts of one fused
+# projection); `starts` [B + 1] int32 holds the sequences' first tokens and their end, on the device: nothing is copied to the
+# host, so every call can be captured and replayed on other lengths.
+_SEQ_DTYPES = {torch.float32: TTSMI_F32, torch.bfloat16: _lib.TTSMI_BF16_IO}
+
+
+def _need(ok, message):
+    if not ok:
+        raise _lib.TtsmiError(message)
+
+
+class _Here:
+    def __enter__(self):
+        return self
+
+    def __exit__(self, *exc):
+        return False
+
+
+class _OnDevice:
+    """Another GPU than the current one: launches inside go to that GPU's current stream."""
+
+    def __init__(self, device):
+        self.device = torch.cuda.device(device)
+
+    def __enter__(self):
+        self.device.__enter__()
+        self.pin = pin_stream(None)
+        self.pin.__enter__()
+        return self
+
+    def __exit__(self, *exc):
+        self.pin.__exit__(*exc)
+        return self.device.__exit__(*exc)
+
+
+_HERE_GUARD = _Here()
+
+
+def _device_of(t):
+    return _HERE_GUARD if t.device.index == torch.cuda.current_device() else _OnDevice(t.device)
+
+
+def _seq_check(name, t, like=None, heads=None):
+    _need(isinstance(t, torch.Tensor) and t.dim() == 3, f'{name}: a tensor of [tokens, heads, dh]')
+    _need_gpu(t)
+    _need(t.dtype in _SEQ_DTYPES, f'{name}: {t.dtype} (float32 or bfloat16)')
+    if like is not None:
+        _need(t.dtype == like.dtype and t.device == like.device and t.shape[2] == like.shape[2],
+              f'{name}: {tuple(t.shape)} {t.dtype} on {t.device} beside {tuple(like.shape)} {like.dtype} on {like.device}')
+
+
+def _ints_check(name, t, device, dim=1):
+    _need(isinstance(t, torch.Tensor) and t.dtype == torch.int32 and t.dim() == dim and t.device == device,
+          f'{name}: {dim}-d int32 on {device}')
+    return _c(t)
+
+
+def _strided(t, aligned=True):
+    """t, or a contiguous copy of it where its last dimension is not contiguous or (aligned) its rows or heads do not lie on
+    16-byte boundaries."""
+    st, size = t.stride(), t.element_size()
+    if st[2] == 1 or t.shape[2] == 1:
+        n = 16 // size
+        if not aligned or (t.data_ptr() % 16 == 0 and (t.shape[0] < 2 or st[0] % n == 0) and (t.shape[1] < 2 or st[1] % n == 0)):
+            return t
+    c = t.contiguous()
+    # (a tensor that counts as contiguous where it is - one off a 16-byte boundary - comes back as itself)
+    return c.clone() if aligned and c.data_ptr() % 16 else c
+
+
+def _rs(t):
+    """(pointer, row stride, head stride); the stride of a dimension of one is never used and passed as 0."""
+    st = t.stride()
+    return t.data_ptr(), st[0] if t.shape[0] > 1 else 0, st[1] if t.shape[1] > 1 else 0
+
+
+def _scale_of(scale, dh):
+    scale = dh ** -0.5 if scale is None else float(scale)
+    _need(0.0 < scale < float('inf'), f'scale {scale}: positive and finite')
+    return scale
+
+
+# ---- rotary positions ----------------------------------------------------------------------------------------------
+def _rotary(q, k, qo, ko, positions, freqs, interleaved, scale, inverse):
+    none = (None, 0, 0)
+    check(_lib.lib().ttsmi_rotary(*_rs(q), *_rs(qo), q.shape[1], *(none if k is None else _rs(k)), *(none if k is None else _rs(ko)),
+                                  0 if k is None else k.shape[1], positions.data_ptr(), freqs.data_ptr(), q.shape[0], q.shape[2],
+                                  2 * freqs.numel(), int(interleaved), scale, int(inverse), _SEQ_DTYPES[q.dtype], _stream()), 'rotary')
+
+
+class RotaryFn(torch.autograd.Function):
+    """Queries and keys turned by their positions; the gradients are turned back (ttsmi_rotary)."""
+
+    @staticmethod
+    def forward(ctx, q, k, positions, freqs, interleaved, scale):
+        ctx.stream_h = _stream()
+        ctx.save_for_backward(positions, freqs)
+        ctx.cfg = (interleaved, scale)
+        ctx.set_materialize_grads(False)
+        qo = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        ko = None if k is None else torch.empty(k.shape, dtype=k.dtype, device=k.device)
+        _rotary(q, k, qo, ko, positions, freqs, interleaved, scale, False)
+        return qo, ko
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dq, dk):
+        positions, freqs = ctx.saved_tensors
+        grads = [None, None]
+        some = [(i, _strided(g, aligned=False)) for i, g in enumerate((dq, dk)) if g is not None and ctx.needs_input_grad[i]]
+        if some:
+            with _device_of(positions), pin_stream(ctx.stream_h):
+                for i, g in some:
+                    grads[i] = torch.empty(g.shape, dtype=g.dtype, device=g.device)
+                (a, ga), (b, gb) = some[0], some[1] if len(some) > 1 else (None, None)
+                _rotary(ga, gb, grads[a], None if b is None else grads[b], positions, freqs, *ctx.cfg, True)
+        return grads[0], grads[1], None, None, None, None
+
+
+def rotary(q, k, positions, freqs, interleaved=False, scale=1.0, inplace=False):
+    """The first 2 * len(freqs) elements of every head of q [tokens, H, dh] and k [tokens, Hkv, dh] (or None) turned by
+    positions [tokens] int32 times freqs (float64 radians per position, model.transformer_utils.rotary_frequencies), pairs
+    (2 i, 2 i + 1) if interleaved and (i, i + len(freqs)) otherwise, times scale; the rest passes through.  -> (q, k).
+    inplace: q and k themselves, without gradients."""
+    _seq_check('rotary: q', q)
+    _need(freqs.dtype == torch.float64 and freqs.dim() == 1 and freqs.device == q.device, f'rotary: freqs: 1-d float64 on {q.device}')
+    _need(2 * freqs.numel() <= q.shape[2] and q.shape[2] % 2 == 0 and freqs.numel() <= 256,
+          f'rotary: {freqs.numel()} pairs in a head of {q.shape[2]} elements (even; at most 256 pairs)')
+    positions = _ints_check('rotary: positions', positions, q.device)
+    _need(positions.numel() == q.shape[0], f'rotary: {positions.numel()} positions for {q.shape[0]} tokens')
+    if k is not None:
+        _seq_check('rotary: k', k, q)
+        _need(k.shape[0] == q.shape[0], f'rotary: {q.shape[0]} queries and {k.shape[0]} keys')
+    freqs, scale = _c(freqs), float(scale)
+    grad = torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad))
+    with _device_of(q):
+        if inplace:
+            _need(not grad, 'rotary: in place on a tensor that wants a gradient')
+            _need(q.stride(2) == 1 and (k is None or k.stride(2) == 1), 'rotary: in place needs a contiguous last dimension')
+            _rotary(q, k, q, k, positions, freqs, interleaved, scale, False)
+            return q, k
+        q, k = _strided(q, aligned=False), None if k is None else _strided(k, aligned=False)
+        if grad:
+            return RotaryFn.apply(q, k, positions, freqs, bool(interleaved), scale)
+        qo = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        ko = None if k is None else torch.empty(k.shape, dtype=k.dtype, device=k.device)
+        _rotary(q, k, qo, ko, positions, freqs, interleaved, scale, False)
+        return qo, ko
+
+
+# ---- attention over packed sequences --------------------------------------------------------------------------------
+def _packed_fwd(q, k, v, starts, scale, causal, want_lse):
+    M, H, dh = q.shape
+    Hkv = k.shape[1]
+    out = torch.empty((M, H, dh), dtype=q.dtype, device=q.device)
+    lse = torch.empty((Hkv, M, H // Hkv), dtype=torch.float32, device=q.device) if want_lse else None
+    check(_lib.lib().ttsmi_packed_attention_fwd(*_rs(q), *_rs(k), *_rs(v), starts.data_ptr(), starts.numel() - 1, M, H, Hkv, dh, scale,
+                                                int(causal), *_rs(out), _p(lse), 1, _SEQ_DTYPES[q.dtype], _stream()),
+          'packed_attention_fwd')
+    return out, lse
+
+
+class PackedAttentionFn(torch.autograd.Function):
+    """softmax(scale q k^T) v within packed sequences, grouped heads (ttsmi_packed_attention_fwd / _bwd).  Returns (out, lse)."""
+
+    @staticmethod
+    def forward(ctx, q, k, v, starts, scale, causal):
+        ctx.stream_h = _stream()
+        out, lse = _packed_fwd(q, k, v, starts, scale, causal, True)
+        ctx.save_for_backward(q, k, v, out, lse, starts)
+        ctx.cfg = (scale, causal)
+        ctx.mark_non_differentiable(lse)
+        ctx.set_materialize_grads(False)
+        return out, lse
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dout, _dlse):
+        if dout is None:
+            return (None,) * 6
+        q, k, v, out, lse, starts = ctx.saved_tensors
+        scale, causal = ctx.cfg
+        M, H, dh = q.shape
+        l = _lib.lib()
+        with _device_of(q), pin_stream(ctx.stream_h):
+            dout = _strided(dout)
+            dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
+            ws = _ws(l.ttsmi_packed_attention_bwd_ws_bytes(M, H), q.device)
+            check(l.ttsmi_packed_attention_bwd(*_rs(q), *_rs(k), *_rs(v), *_rs(out), *_rs(dout), lse.data_ptr(), starts.data_ptr(),
+                                               starts.numel() - 1, M, H, k.shape[1], dh, scale, int(causal), *_rs(dq), *_rs(dk),
+                                               *_rs(dv), 1, ws.data_ptr(), ws.numel(), _SEQ_DTYPES[q.dtype], _stream()),
+                  'packed_attention_bwd')
+        return dq, dk, dv, None, None, None
+
+
+def packed_attention(q, k, v, starts, causal=True, scale=None):
+    """Attention within each of the packed sequences: q [tokens, H, dh], k and v [tokens, Hkv, dh], H a multiple of Hkv (query
+    head h reads key head h // (H // Hkv)), dh a multiple of 8 up to 192; sequence b is tokens starts[b] .. starts[b + 1], over
+    the keys up to the query's own if causal and over all of them otherwise; scale defaults to dh ** -0.5.  Tokens behind
+    starts[-1] get zeros, and zero gradients.  -> [tokens, H, dh].  Tensors whose rows or heads do not lie on 16-byte
+    boundaries are copied first."""
+    _seq_check('packed_attention: q', q)
+    _seq_check('packed_attention: k', k, q)
+    _seq_check('packed_attention: v', v, q)
+    _need(k.shape == v.shape and k.shape[0] == q.shape[0] and k.shape[1] > 0 and q.shape[1] % k.shape[1] == 0,
+          f'packed_attention: q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}')
+    _need(q.shape[2] % 8 == 0 and 0 < q.shape[2] <= 192, f'packed_attention: head size {q.shape[2]} (a multiple of 8 up to 192)')
+    starts = _ints_check('packed_attention: starts', starts, q.device)
+    _need(starts.numel() > 0, 'packed_attention: starts holds the end of the last sequence at least')
+    scale = _scale_of(scale, q.shape[2])
+    with _device_of(q):
+        q, k, v = _strided(q), _strided(k), _strided(v)
+        if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+            return PackedAttentionFn.apply(q, k, v, starts, scale, bool(causal))[0]
+        return _packed_fwd(q, k, v, starts, scale, causal, False)[0]
+
+
+# ---- the paged key / value cache --------------------------------------------------------------------------------------
+_CACHE_DTYPES = {torch.float32: TTSMI_F32, torch.bfloat16: _lib.TTSMI_BF16_IO, torch.float8_e4m3fn: _lib.TTSMI_E4M3}
+
+
+class KVCache:
+    """The pages of a key / value cache: k and v [pages, Hkv, page size, dh] of float32, bfloat16 or float8_e4m3fn, the page size
+    a power of two up to 1024; float8_e4m3fn pages with k_exp and v_exp [pages, Hkv, page size] uint8, the biased exponent of
+    each row's power-of-two scale (value = e4m3 * 2 ** (exp - 127)).  It holds the tensors it is given; which pages belong to
+    which sequence is the caller's (`table`)."""
+    __slots__ = ('k', 'v', 'k_exp', 'v_exp', 'args', 'heads', 'dh', 'page_size', 'dtype', 'device')
+
+    def __init__(self, k, v, k_exp=None, v_exp=None):
+        _need(k.dim() == 4 and k.shape == v.shape and k.dtype == v.dtype and k.device == v.device and k.dtype in _CACHE_DTYPES,
+              f'KVCache: pages {tuple(k.shape)} {k.dtype} and {tuple(v.shape)} {v.dtype}')
+        n, self.heads, self.page_size, self.dh = k.shape
+        _need(0 < self.page_size <= 1024 and self.page_size & (self.page_size - 1) == 0 and self.heads > 0,
+              f'KVCache: pages of {self.page_size} rows (a power of two up to 1024)')
+        _need(self.dh % 8 == 0 and 0 < self.dh <= 192, f'KVCache: head size {self.dh} (a multiple of 8 up to 192)')
+        quantised = k.dtype == torch.float8_e4m3fn
+        _need((k_exp is not None and v_exp is not None) == quantised, 'KVCache: float8_e4m3fn pages, and only they, have exponents')
+        for t in (k_exp, v_exp) if quantised else ():
+            _need(t.shape == k.shape[:3] and t.dtype == torch.uint8 and t.device == k.device and t.is_contiguous(),
+                  f'KVCache: exponents {tuple(t.shape)} {t.dtype} of pages {tuple(k.shape)}')
+        _need_gpu(k)
+        _need(k.is_contiguous() and v.is_contiguous() and (k.data_ptr() | v.data_ptr()) % 16 == 0, 'KVCache: contiguous, 16-byte aligned pages')
+        self.k, self.v, self.k_exp, self.v_exp, self.dtype, self.device = k, v, k_exp, v_exp, k.dtype, k.device
+        self.args = (k.data_ptr(), v.data_ptr(), _p(k_exp), _p(v_exp), _CACHE_DTYPES[k.dtype], n, self.page_size)
+
+    @classmethod
+    def zeros(cls, pages, page_size, heads, dh, dtype=torch.bfloat16, device='cuda'):
+        shape, exp = (pages, heads, page_size, dh), None
+        if dtype == torch.float8_e4m3fn:
+            exp = [torch.full(shape[:3], 127, dtype=torch.uint8, device=device) for _ in 'kv']
+            pages = [torch.zeros(shape, dtype=torch.uint8, device=device).view(dtype) for _ in 'kv']
+        else:
+            pages = [torch.zeros(shape, dtype=dtype, device=device) for _ in 'kv']
+        return cls(*pages, *(exp or ()))
+
+
+def _paged_check(name, cache, table, starts, lens):
+    _need(isinstance(cache, KVCache), f'{name}: a KVCache')
+    table, starts = _ints_check(f'{name}: table', table, cache.device, 2), _ints_check(f'{name}: starts', starts, cache.device)
+    lens = _ints_check(f'{name}: lens', lens, cache.device)
+    _need(starts.numel() == lens.numel() + 1 and table.shape[0] == lens.numel(),
+          f'{name}: {starts.numel()} starts, {lens.numel()} lens, table {tuple(table.shape)}')
+    return table, starts, lens
+
+
+def _kv_check(name, cache, k, v):
+    _seq_check(f'{name}: k', k)
+    _seq_check(f'{name}: v', v, k)
+    _need(k.shape == v.shape and k.shape[1] == cache.heads and k.shape[2] == cache.dh and k.device == cache.device,
+          f'{name}: k {tuple(k.shape)}, v {tuple(v.shape)} on {k.device}; pages {tuple(cache.k.shape)} on {cache.device}')
+    _need(cache.dtype in (k.dtype, torch.float8_e4m3fn), f'{name}: {k.dtype} beside pages of {cache.dtype}')
+
+
+def kv_cache_write(cache, k, v, table, starts, lens):
+    """The packed new tokens' keys and values [tokens, Hkv, dh] into their pages, quantised if the pages are float8_e4m3fn.
+    table [B, n] int32: the pages of every sequence in order; starts [B + 1] int32: its new tokens; lens [B] int32: its cached
+    length with them, which are the last ones.  A page number outside the cache, or a token without a position, is not written."""
+    table, starts, lens = _paged_check('kv_cache_write', cache, table, starts, lens)
+    _kv_check('kv_cache_write', cache, k, v)
+    with _device_of(k):
+        k, v = _strided(k), _strided(v)
+        check(_lib.lib().ttsmi_kv_cache_write(*_rs(k), *_rs(v), *cache.args, table.data_ptr(), table.shape[1], starts.data_ptr(),
+                                              lens.data_ptr(), lens.numel(), k.shape[0], cache.heads, cache.dh, _SEQ_DTYPES[k.dtype],
+                                              _stream()), 'kv_cache_write')
+
+
+def kv_cache_read(cache, table, lens, starts, tokens, dtype=None, out=None):
+    """The last starts[b + 1] - starts[b] cached tokens of every sequence (all of them where starts holds the cumulative lens)
+    in packed order -> (k, v) [tokens, Hkv, dh].  dtype: the pages' own, or either for float8_e4m3fn pages (default bfloat16).
+    Rows behind starts[-1] are zeros; with out = (k, v) they are left as they were."""
+    table, starts, lens = _paged_check('kv_cache_read', cache, table, starts, lens)
+    if out is None:
+        dtype = dtype or (torch.bfloat16 if cache.dtype == torch.float8_e4m3fn else cache.dtype)
+        k, v = (torch.empty((int(tokens), cache.heads, cache.dh), dtype=dtype, device=cache.device) for _ in 'kv')
+    else:
+        k, v = out
+        _need(k.shape[0] == tokens and _strided(k) is k and _strided(v) is v, f'kv_cache_read: out of {tokens} tokens on 16-byte boundaries')
+    _kv_check('kv_cache_read', cache, k, v)
+    with _device_of(k):
+        check(_lib.lib().ttsmi_kv_cache_read(*cache.args, table.data_ptr(), table.shape[1], starts.data_ptr(), lens.data_ptr(), lens.numel(),
+                                             k.shape[0], cache.heads, cache.dh, *_rs(k), *_rs(v), int(out is None), _SEQ_DTYPES[k.dtype],
+                                             _stream()), 'kv_cache_read')
+    return k, v
+
+
+def paged_attention(q, cache, table, starts, lens, scale=None, max_len=None, out=None):
+    """Attention of packed new tokens q [tokens, H, dh] over the cache, their own keys and values in it already
+    (kv_cache_write): token i of the n new ones of sequence b is at position lens[b] - n + i and sees the keys up to it; a
+    token that sees none gets zeros.  max_len: the longest length expected (default: what the table holds) - it only sets how
+    finely the keys are split.  Without gradients.  Rows behind starts[-1] are zeros; in `out` they are left as they were."""
+    _seq_check('paged_attention: q', q)
+    table, starts, lens = _paged_check('paged_attention', cache, table, starts, lens)
+    M, H, dh = q.shape
+    _need(dh == cache.dh and H % cache.heads == 0 and H > 0 and q.device == cache.device and cache.dtype in (q.dtype, torch.float8_e4m3fn),
+          f'paged_attention: q {tuple(q.shape)} {q.dtype} on {q.device}; pages {tuple(cache.k.shape)} {cache.dtype} on {cache.device}')
+    _need(not (torch.is_grad_enabled() and q.requires_grad), 'paged_attention: has no gradient')
+    scale = _scale_of(scale, dh)
+    max_len = int(table.shape[1] * cache.page_size if max_len is None else max_len)
+    given = out is not None
+    if given:
+        _need(out.shape == q.shape and out.dtype == q.dtype and out.device == q.device and _strided(out) is out,
+              f'paged_attention: out {tuple(out.shape)} {out.dtype} for q {tuple(q.shape)} {q.dtype}, on 16-byte boundaries')
+    l = _lib.lib()
+    with _device_of(q):
+        q = _strided(q)
+        out = out if given else torch.empty((M, H, dh), dtype=q.dtype, device=q.device)
+        need = l.ttsmi_paged_attention_ws_bytes(lens.numel(), M, H, cache.heads, dh, max_len)
+        ws = _ws(need, q.device) if need else None
+        check(l.ttsmi_paged_attention(*_rs(q), *cache.args, table.data_ptr(), table.shape[1], starts.data_ptr(), lens.data_ptr(),
+                                      lens.numel(), M, H, cache.heads, dh, scale, max_len, *_rs(out), int(not given), _p(ws),
+                                      0 if ws is None else ws.numel(), _SEQ_DTYPES[q.dtype], _stream()), 'paged_attention')
+    return out
