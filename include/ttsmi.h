@@ -831,7 +831,7 @@ int ttsmi_packed_attention_fwd(const void* q, int64_t q_row, int64_t q_head, con
                                int Hkv, int dh, float scale, int causal, void* out, int64_t o_row, int64_t o_head, float* lse,
                                int zero_rest, int dtype, ttsmi_stream_t stream);
 /* Gradients of q, k and v (summed over the query heads of a group); deterministic.  out and lse are the forward's. */
-size_t ttsmi_packed_attention_bwd_ws_bytes(int tokens, int H);
+size_t ttsmi_packed_attention_bwd_ws_bytes(int B, int tokens, int H, int Hkv, int dh);
 int ttsmi_packed_attention_bwd(const void* q, int64_t q_row, int64_t q_head, const void* k, int64_t k_row, int64_t k_head,
                                const void* v, int64_t v_row, int64_t v_head, const void* out, int64_t o_row, int64_t o_head,
                                const void* dout, int64_t d_row, int64_t d_head, const float* lse, const int32_t* starts, int B,
@@ -857,14 +857,13 @@ int ttsmi_kv_cache_read(const void* k_pages, const void* v_pages, const uint8_t*
                         const int32_t* lens, int B, int tokens, int Hkv, int dh, void* k, int64_t k_row, int64_t k_head, void* v,
                         int64_t v_row, int64_t v_head, int zero_rest, int dtype, ttsmi_stream_t stream);
 /* Attention of the packed new tokens over the cache (their own keys and values written before): token i of sequence b, n of
- * them, is at position lens[b] - n + i and sees the keys up to it.  A token that sees none gets zeros.  max_len: the longest
- * cached length expected - it sets how finely the keys are split over workgroups, never the result's correctness; the same
- * value goes into the workspace query. */
-size_t ttsmi_paged_attention_ws_bytes(int B, int tokens, int H, int Hkv, int dh, int max_len);
+ * them, is at position lens[b] - n + i and sees the keys up to it.  A token that sees none gets zeros.  The keys are split over
+ * workgroups by the lengths found on the device; the sums of the splits pass through ws. */
+size_t ttsmi_paged_attention_ws_bytes(int B, int tokens, int H, int Hkv, int dh, int cache_dtype);
 int ttsmi_paged_attention(const void* q, int64_t q_row, int64_t q_head, const void* k_pages, const void* v_pages,
                           const uint8_t* k_exp, const uint8_t* v_exp, int cache_dtype, int n_pages, int page_size,
                           const int32_t* table, int table_width, const int32_t* starts, const int32_t* lens, int B, int tokens,
-                          int H, int Hkv, int dh, float scale, int max_len, void* out, int64_t o_row, int64_t o_head,
+                          int H, int Hkv, int dh, float scale, void* out, int64_t o_row, int64_t o_head,
                           int zero_rest, void* ws, size_t ws_bytes, int dtype, ttsmi_stream_t stream);
 
 #ifdef __cplusplus

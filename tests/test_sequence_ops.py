@@ -20,7 +20,7 @@ F32, BF16, E4M3 = 0, 2, 4
 def _packed(lib, bwd=False, **over):
     a = dict(q=ONE, q_row=256, q_head=64, k=ONE, k_row=128, k_head=64, v=ONE, v_row=128, v_head=64, out=ONE, o_row=256, o_head=64, dout=ONE,
              d_row=256, d_head=64, lse=ONE, starts=ONE, B=2, tokens=10, H=4, Hkv=2, dh=64, scale=0.125, causal=1, dq=ONE, dq_row=256, dq_head=64,
-             dk=ONE, dk_row=128, dk_head=64, dv=ONE, dv_row=128, dv_head=64, zero_rest=1, ws=ONE, ws_bytes=1 << 20, dtype=BF16)
+             dk=ONE, dk_row=128, dk_head=64, dv=ONE, dv_row=128, dv_head=64, zero_rest=1, ws=ONE, ws_bytes=1 << 30, dtype=BF16)
     a.update(over)
     fwd = 'q q_row q_head k k_row k_head v v_row v_head starts B tokens H Hkv dh scale causal out o_row o_head lse zero_rest dtype'
     back = ('q q_row q_head k k_row k_head v v_row v_head out o_row o_head dout d_row d_head lse starts B tokens H Hkv dh scale causal dq dq_row '
@@ -43,16 +43,16 @@ def test_packed_attention_refuses(lib, over, code, word, bwd):
 
 def test_packed_attention_bwd_refuses_and_empty_calls_pass(lib):
     for over, code, word in ((dict(lse=None), -1, b'lse'), (dict(dq=ODD), -1, b'aligned'), (dict(dk=None), -1, b'null'), (dict(dv_row=4), -1, b'aligned'),
-                             (dict(ws=None), -4, b'workspace'), (dict(ws_bytes=10 * 4 * 4 - 1), -4, b'workspace')):
+                             (dict(ws=None), -4, b'workspace'), (dict(ws_bytes=10 * 4 * 4 - 1), -4, b'workspace'), (dict(ws=ODD), -4, b'workspace')):
         rc, err = _packed(lib, True, **over)
         assert rc == code and word in err, (over, rc, err)
     assert _packed(lib, tokens=0, q=None)[0] == 0 and _packed(lib, True, tokens=0, ws=None)[0] == 0
-    assert lib.ttsmi_packed_attention_bwd_ws_bytes(10, 4) >= 160 and lib.ttsmi_packed_attention_bwd_ws_bytes(0, 4) == 0
+    assert lib.ttsmi_packed_attention_bwd_ws_bytes(2, 10, 4, 2, 64) >= 160 and lib.ttsmi_packed_attention_bwd_ws_bytes(2, 0, 4, 2, 64) == 0
 
 
 def _cache_args(order, **over):
     a = dict(k=ONE, k_row=128, k_head=64, v=ONE, v_row=128, v_head=64, q=ONE, q_row=256, q_head=64, out=ONE, o_row=256, o_head=64, kp=ONE, vp=ONE, ke=ONE, ve=ONE,
-             cache=E4M3, pages=8, page=16, table=ONE, width=4, starts=ONE, lens=ONE, B=2, tokens=10, H=4, Hkv=2, dh=64, scale=0.125, max_len=1 << 16, zero_rest=1,
+             cache=E4M3, pages=8, page=16, table=ONE, width=4, starts=ONE, lens=ONE, B=2, tokens=10, H=4, Hkv=2, dh=64, scale=0.125, zero_rest=1,
              ws=ONE, ws_bytes=1 << 30, dtype=BF16)
     a.update(over)
     return [a[n] for n in order.split()] + [None]
@@ -61,7 +61,7 @@ def _cache_args(order, **over):
 _ORDERS = {
     'ttsmi_kv_cache_write': 'k k_row k_head v v_row v_head kp vp ke ve cache pages page table width starts lens B tokens Hkv dh dtype',
     'ttsmi_kv_cache_read': 'kp vp ke ve cache pages page table width starts lens B tokens Hkv dh k k_row k_head v v_row v_head zero_rest dtype',
-    'ttsmi_paged_attention': 'q q_row q_head kp vp ke ve cache pages page table width starts lens B tokens H Hkv dh scale max_len out o_row o_head zero_rest ws ws_bytes dtype'}
+    'ttsmi_paged_attention': 'q q_row q_head kp vp ke ve cache pages page table width starts lens B tokens H Hkv dh scale out o_row o_head zero_rest ws ws_bytes dtype'}
 
 
 @pytest.mark.parametrize('name', sorted(_ORDERS))
@@ -81,13 +81,13 @@ def test_cache_entries_refuse(lib, name, over, word):
 
 
 def test_paged_attention_workspace(lib):
-    need = lib.ttsmi_paged_attention_ws_bytes(2, 10, 4, 2, 64, 1 << 16)
+    need = lib.ttsmi_paged_attention_ws_bytes(2, 10, 4, 2, 64, E4M3)
     assert need >= 2 * 10 * 4 * 66 * 4                                       # a few rows over a long cache are split
     order = _ORDERS['ttsmi_paged_attention']
     for over in (dict(ws=None), dict(ws_bytes=need - 1), dict(ws=ODD)):
         assert lib.ttsmi_paged_attention(*_cache_args(order, **over)) == -4 and b'workspace' in lib.ttsmi_last_error()
-    assert lib.ttsmi_paged_attention_ws_bytes(2, 10, 4, 2, 64, 1) == 0       # one short key range is not
-    assert lib.ttsmi_paged_attention_ws_bytes(0, 0, 4, 2, 64, 1 << 16) == 0 and lib.ttsmi_paged_attention_ws_bytes(1, 1, 4, 0, 64, 99) == 0
+    assert lib.ttsmi_paged_attention_ws_bytes(1, 1 << 16, 32, 8, 128, BF16) == 0          # tiles that fill the card are not
+    assert lib.ttsmi_paged_attention_ws_bytes(0, 0, 4, 2, 64, BF16) == 0 and lib.ttsmi_paged_attention_ws_bytes(1, 1, 4, 0, 64, BF16) == 0
     for over in (dict(scale=0.0), dict(H=3), dict(out=None)):
         assert lib.ttsmi_paged_attention(*_cache_args(order, **over)) == -1
 

@@ -151,13 +151,9 @@ static int kv_launch(const KvP& p, bool write, hipStream_t st) {
     TTSMI_CHECK_ARG(dtype == TTSMI_F32 || dtype == TTSMI_BF16_IO, who ": dtype %d (TTSMI_F32 or TTSMI_BF16_IO)", dtype);                \
     TTSMI_CHECK_ARG(B >= 0 && tokens >= 0 && Hkv > 0, who ": sequences %d, tokens %d, key heads %d", B, tokens, Hkv);              \
     TTSMI_CHECK_ARG(dh > 0 && dh <= 192 && dh % 8 == 0, who ": head size %d (a multiple of 8 up to 192)", dh);                     \
-    TTSMI_CHECK_ARG(n_pages >= 0 && page_size > 0 && page_size <= 1024 && (page_size & (page_size - 1)) == 0 && table_width >= 0,  \
-                    who ": %d pages of %d rows (a power of two up to 1024)", n_pages, page_size);                                 \
-    if (tokens == 0) return TTSMI_OK;                                                                                   \
-    TTSMI_CHECK_ARG(starts && (B == 0 || (lens && (table || table_width == 0))), who ": null starts, lens or table");                           \
-    TTSMI_CHECK_ARG(n_pages == 0 || (k_pages && v_pages && (((uintptr_t)k_pages | (uintptr_t)v_pages) & 15) == 0),                 \
-                    who ": pages null or not 16-byte aligned");                                                                   \
-    TTSMI_CHECK_ARG(cache_dtype != TTSMI_E4M3 || n_pages == 0 || (k_exp && v_exp), who ": an e4m3 cache needs its exponents");      \
+    SEQ_CHECK_PAGES(who);                                                                                                         \
+    if (tokens == 0) return TTSMI_OK;                                                                                             \
+    SEQ_CHECK_CACHE(who);                                                                                                         \
     TTSMI_CHECK_ARG(seq_strides_ok(k, k_row, k_head, dtype) && seq_strides_ok(v, v_row, v_head, dtype),                           \
                     who ": a tensor is null or its rows or heads are not 16-byte aligned");                                       \
     KvP p = {};                                                                                                                   \

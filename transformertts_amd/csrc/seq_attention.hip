@@ -6,21 +6,9 @@
 // sequence and key head (seq_common.h: rows are (token, query head of the group) pairs), 32 rows a wave.  The wave forms the
 // TRANSPOSED score tile S^T = K Q^T, so that a lane holds one row's scores for 16 keys: the softmax is in-lane plus one exchange
 // of the two half-waves, and the accumulator registers, rounded, ARE the B operand of O^T += V^T P^T.
-// Keys can be split over workgroups (grid y): each writes its normaliser and unnormalised sum, a second launch joins them.
+// Over a cache the keys can be split over workgroups (find_unit): each leaves its maximum, sum and unnormalised output, and a second
+// launch joins them (paged_attention.hip).
 #include "seq_common.h"
-
-struct SeqFwdP {
-    const void* q; long q_row, q_head;                    // element strides
-    const void* k; long k_row, k_head;
-    const void* v; long v_row, v_head;
-    void* o; long o_row, o_head;
-    float* lse;                                           // [Hkv][tokens G] natural log, or null
-    const int* starts; const int* lens;                   // lens: paged only (tokens in the cache, the new ones among them)
-    SeqPages pg;
-    int B, tokens, Hkv, G, dh, causal, nsplit, zero_rest;
-    float c1;                                             // scale log2(e)
-    float* part_o; float* part_ml;                        // splits: [nsplit][Hkv tokens G][dh], [nsplit][Hkv tokens G][2]
-};
 
 // CT: the cache's element type for PAGED (T, or uint8_t = e4m3)
 template <typename T, typename CT, int DHP, bool PAGED>
@@ -34,12 +22,17 @@ __global__ __launch_bounds__(256, (DHP <= 128 && sizeof(T) == 2) ? 2 : 1) void s
     const int tid = threadIdx.x, lane = tid & 63, l31 = lane & 31, hh = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int hk = blockIdx.x % p.Hkv, unit = blockIdx.x / p.Hkv;       // bid % 8 = XCD: the tiles of a key head share few L2s
-    const SeqTile st = find_tile(p.starts, p.B, p.tokens, p.G, 128, unit);
+    SeqUnit un;
+    if constexpr (PAGED) {
+        if (p.slots > 0) un = find_unit(p.starts, p.lens, 1, p.B, p.tokens, p.G, 128, p.slots, KT, SEQ_TILE_LEAST, unit, false);
+    }
+    const bool splits = PAGED && p.slots > 0;
+    const SeqTile st = splits ? un.t : find_tile(p.starts, p.B, p.tokens, p.G, 128, unit);
     if (st.seq < 0) {
-        if (p.zero_rest && p.nsplit == 1) seq_zero_rest<T>((T*)p.o, p.o_row, p.o_head, p.starts, p.B, p.tokens, p.G, 128, hk * p.G, p.dh, st.tile);
+        if (p.zero_rest) seq_zero_rest<T>((T*)p.o, p.o_row, p.o_head, p.starts, p.B, p.tokens, p.G, 128, hk * p.G, p.dh, st.tile);
         return;
     }
-    const int tile = st.ntile - 1 - st.tile;              // causal: the tiles with the most keys first
+    const int tile = splits ? st.tile : st.ntile - 1 - st.tile;              // causal: the tiles with the most keys first
     const int rows = st.n * p.G;
     int len = st.n, off = 0;
     if (PAGED) {
@@ -54,10 +47,10 @@ __global__ __launch_bounds__(256, (DHP <= 128 && sizeof(T) == 2) ? 2 : 1) void s
     // the same for the workgroup's last row, and for this wave's: no key behind is fetched / multiplied
     const int last = min(tile * 128 + 127, rows - 1) / p.G;
     int kend = p.causal ? min(max(off + last + 1, 0), len) : len, kbeg = 0;
-    if (p.nsplit > 1) {
-        const int per = ((kend + KT - 1) / KT + p.nsplit - 1) / p.nsplit * KT;
-        kbeg = min((int)blockIdx.y * per, kend);
-        kend = min(kbeg + per, kend);
+    const bool part = splits && un.nsplit > 1;
+    if (part) {
+        kbeg = min(un.split * un.per, kend);
+        kend = min(kbeg + un.per, kend);
     }
     const int wrow = tile * 128 + wave * 32;
     const int wlast = min(wrow + 31, rows - 1) / p.G;
@@ -78,28 +71,36 @@ __global__ __launch_bounds__(256, (DHP <= 128 && sizeof(T) == 2) ? 2 : 1) void s
     float m = -INFINITY, l = 0.f;
 
     // ---- tile staging: global -> registers (a tile ahead) -> LDS; rows past the last key are zeros ----
+    // PAGED: the page rows of a tile are looked up one tile earlier still, so that no load waits for another
     uint4 rk[ITEMS], rv[ITEMS];
+    long at[PAGED ? ITEMS : 1];
+    auto look = [&](int k0) {
+        if constexpr (PAGED) {
+#pragma unroll
+            for (int i = 0; i < ITEMS; ++i) {
+                const int key = k0 + (tid + 256 * i) / I::CH;
+                at[i] = key < kend ? p.pg.row(st.seq, hk, key) : -1;
+            }
+        }
+    };
     auto fetch = [&](int k0) {
 #pragma unroll
         for (int i = 0; i < ITEMS; ++i) {
             const int id = tid + 256 * i, row = id / I::CH, ch = id - row * I::CH, key = k0 + row;
             rk[i] = rv[i] = make_uint4(0u, 0u, 0u, 0u);
-            if (key < kend && ch * EPC < p.dh) {
-                if constexpr (PAGED) {
-                    const long at = p.pg.row(st.seq, hk, key);
-                    if (at >= 0) {
-                        if constexpr (sizeof(CT) == 1) {
-                            rk[i] = seq_dequant_chunk<T>((const uint8_t*)p.pg.k + at * p.dh + ch * EPC, seq_scale_of(p.pg.ke[at]));
-                            rv[i] = seq_dequant_chunk<T>((const uint8_t*)p.pg.v + at * p.dh + ch * EPC, seq_scale_of(p.pg.ve[at]));
-                        } else {
-                            rk[i] = *reinterpret_cast<const uint4*>((const T*)p.pg.k + at * p.dh + ch * EPC);
-                            rv[i] = *reinterpret_cast<const uint4*>((const T*)p.pg.v + at * p.dh + ch * EPC);
-                        }
+            if constexpr (PAGED) {
+                if (at[i] >= 0 && ch * EPC < p.dh) {
+                    if constexpr (sizeof(CT) == 1) {
+                        rk[i] = seq_dequant_chunk<T>((const uint8_t*)p.pg.k + at[i] * p.dh + ch * EPC, seq_scale_of(p.pg.ke[at[i]]));
+                        rv[i] = seq_dequant_chunk<T>((const uint8_t*)p.pg.v + at[i] * p.dh + ch * EPC, seq_scale_of(p.pg.ve[at[i]]));
+                    } else {
+                        rk[i] = *reinterpret_cast<const uint4*>((const T*)p.pg.k + at[i] * p.dh + ch * EPC);
+                        rv[i] = *reinterpret_cast<const uint4*>((const T*)p.pg.v + at[i] * p.dh + ch * EPC);
                     }
-                } else {
-                    rk[i] = *reinterpret_cast<const uint4*>((const T*)p.k + (long)(st.s0 + key) * p.k_row + (long)hk * p.k_head + ch * EPC);
-                    rv[i] = *reinterpret_cast<const uint4*>((const T*)p.v + (long)(st.s0 + key) * p.v_row + (long)hk * p.v_head + ch * EPC);
                 }
+            } else if (key < kend && ch * EPC < p.dh) {
+                rk[i] = *reinterpret_cast<const uint4*>((const T*)p.k + (long)(st.s0 + key) * p.k_row + (long)hk * p.k_head + ch * EPC);
+                rv[i] = *reinterpret_cast<const uint4*>((const T*)p.v + (long)(st.s0 + key) * p.v_row + (long)hk * p.v_head + ch * EPC);
             }
         }
     };
@@ -112,12 +113,19 @@ __global__ __launch_bounds__(256, (DHP <= 128 && sizeof(T) == 2) ? 2 : 1) void s
         }
     };
 
-    if (kbeg < kend) fetch(kbeg);
+    if (kbeg < kend) {
+        look(kbeg);
+        fetch(kbeg);
+        look(kbeg + KT);
+    }
     for (int k0 = kbeg; k0 < kend; k0 += KT) {
         __syncthreads();
         stash();
         __syncthreads();
-        if (k0 + KT < kend) fetch(k0 + KT);
+        if (k0 + KT < kend) {
+            fetch(k0 + KT);
+            look(k0 + 2 * KT);
+        }
         if (k0 >= wend) continue;
         f32x16 s[NKB];
 #pragma unroll
@@ -170,8 +178,8 @@ __global__ __launch_bounds__(256, (DHP <= 128 && sizeof(T) == 2) ? 2 : 1) void s
     l = seq_half_sum(l);
     if (!rok) return;
     const long slot = (long)hk * p.tokens * p.G + (long)st.s0 * p.G + r;
-    if (p.nsplit > 1) {
-        const long ps = (long)blockIdx.y * p.Hkv * p.tokens * p.G + slot;
+    if (part) {
+        const long ps = ((un.first + un.split) * p.Hkv + hk) * 128 + wave * 32 + l31;
         if (hh == 0) *reinterpret_cast<float2*>(p.part_ml + 2 * ps) = make_float2(m, l);
         if (l > 0.f || !(l == l)) {
 #pragma unroll
@@ -204,56 +212,23 @@ __global__ __launch_bounds__(256, (DHP <= 128 && sizeof(T) == 2) ? 2 : 1) void s
         }
 }
 
-// joins the splits of one row: o = sum_z 2^(m_z - m) o_z / sum_z 2^(m_z - m) l_z.  One wave a row, 4 rows a workgroup.  Rows that
-// belong to no sequence have no partial sums: they are recognised by `starts` and left alone.
-template <typename T>
-__global__ __launch_bounds__(256) void seq_attn_join_kernel(SeqFwdP p) {
-    const int lane = threadIdx.x & 63;
-    const long nrow = (long)p.Hkv * p.tokens * p.G, slot = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (slot >= nrow) return;
-    const int hk = (int)(slot / ((long)p.tokens * p.G));
-    const long rr = slot - (long)hk * p.tokens * p.G;
-    const int tok = (int)(rr / p.G), head = hk * p.G + (int)(rr - (long)tok * p.G);
-    T* orow = (T*)p.o + (long)tok * p.o_row + (long)head * p.o_head;
-    if (tok < p.starts[0]) return;
-    if (tok >= p.starts[p.B]) {
-        if (p.zero_rest)
-            for (int c = lane; c < p.dh; c += 64) orow[c] = (T)0.f;
-        return;
-    }
-    float m = -INFINITY;
-    for (int z = 0; z < p.nsplit; ++z) m = fmaxf(m, p.part_ml[2 * (z * nrow + slot)]);
-    float l = 0.f, acc[3] = {0.f, 0.f, 0.f};
-    for (int z = 0; z < p.nsplit; ++z) {
-        const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + 2 * (z * nrow + slot));
-        if (ml.y == 0.f) continue;
-        const float w = __builtin_amdgcn_exp2f(ml.x - m);
-        l += w * ml.y;
-#pragma unroll
-        for (int i = 0; i < 3; ++i)
-            if (lane + 64 * i < p.dh) acc[i] += w * p.part_o[(z * nrow + slot) * p.dh + lane + 64 * i];
-    }
-    const float inv = l == 0.f ? 0.f : 1.f / l;
-#pragma unroll
-    for (int i = 0; i < 3; ++i)
-        if (lane + 64 * i < p.dh) orow[lane + 64 * i] = (T)(acc[i] * inv);
-}
-
 // ---- launches -----------------------------------------------------------------------------------------
 
 template <typename T, typename CT, bool PAGED>
 static int seq_fwd_launch(const SeqFwdP& p, hipStream_t st) {
-    const long grid = seq_units(p.tokens, p.B, p.G, 128) * p.Hkv;
-    const dim3 g((unsigned)grid, (unsigned)p.nsplit);
+    const long units = p.slots > 0 ? seq_split_units(p.tokens, p.B, p.G, 128, p.slots) : seq_units(p.tokens, p.B, p.G, 128);
+    const dim3 g((unsigned)(units * p.Hkv));
     if (p.dh <= 64) hipLaunchKernelGGL((seq_attn_fwd_kernel<T, CT, 64, PAGED>), g, dim3(256), 0, st, p);
     else if (p.dh <= 128) hipLaunchKernelGGL((seq_attn_fwd_kernel<T, CT, 128, PAGED>), g, dim3(256), 0, st, p);
     else hipLaunchKernelGGL((seq_attn_fwd_kernel<T, CT, 192, PAGED>), g, dim3(256), 0, st, p);
-    if (p.nsplit > 1) {
-        const long nrow = (long)p.Hkv * p.tokens * p.G;
-        hipLaunchKernelGGL((seq_attn_join_kernel<T>), dim3((unsigned)((nrow + 3) / 4)), dim3(256), 0, st, p);
-    }
     TTSMI_CHECK_LAUNCH("seq_attention");
     return TTSMI_OK;
+}
+// the tile form of the paged attention (paged_attention.hip)
+int seq_paged_tiles(const SeqFwdP& p, int dtype, int cache_dtype, hipStream_t st) {
+    if (dtype == TTSMI_F32)
+        return cache_dtype == TTSMI_E4M3 ? seq_fwd_launch<float, uint8_t, true>(p, st) : seq_fwd_launch<float, float, true>(p, st);
+    return cache_dtype == TTSMI_E4M3 ? seq_fwd_launch<__bf16, uint8_t, true>(p, st) : seq_fwd_launch<__bf16, __bf16, true>(p, st);
 }
 
 extern "C" int ttsmi_packed_attention_fwd(const void* q, int64_t q_row, int64_t q_head, const void* k, int64_t k_row, int64_t k_head,
@@ -268,57 +243,6 @@ extern "C" int ttsmi_packed_attention_fwd(const void* q, int64_t q_row, int64_t 
     SeqFwdP p = {};
     p.q = q; p.q_row = q_row; p.q_head = q_head; p.k = k; p.k_row = k_row; p.k_head = k_head; p.v = v; p.v_row = v_row; p.v_head = v_head;
     p.o = out; p.zero_rest = zero_rest != 0; p.o_row = o_row; p.o_head = o_head; p.lse = lse; p.starts = starts;
-    p.B = B; p.tokens = tokens; p.Hkv = Hkv; p.G = H / Hkv; p.dh = dh; p.causal = causal != 0; p.nsplit = 1; p.c1 = scale * SEQ_LOG2E;
+    p.B = B; p.tokens = tokens; p.Hkv = Hkv; p.G = H / Hkv; p.dh = dh; p.causal = causal != 0; p.c1 = scale * SEQ_LOG2E;
     return dtype == TTSMI_F32 ? seq_fwd_launch<float, float, false>(p, (hipStream_t)stream) : seq_fwd_launch<__bf16, __bf16, false>(p, (hipStream_t)stream);
-}
-
-// How many workgroups share the keys of one tile: with fewer tiles than the card has workgroup slots (256 compute units, two
-// workgroups each) the keys are split until they are filled, each split at least 256 keys long.  max_len is the longest sequence
-// that the caller expects; the kernel divides every sequence's own length, so a longer one is only divided less finely.
-static int paged_splits(int B, int tokens, int Hkv, int G, int max_len) {
-    const long tiles = seq_units(tokens, B, G, 128) * Hkv;
-    long n = (512 + tiles - 1) / tiles;
-    const long most = (max_len + 255) / 256;
-    n = n < most ? n : most;
-    return (int)(n < 1 ? 1 : n > 64 ? 64 : n);
-}
-extern "C" size_t ttsmi_paged_attention_ws_bytes(int B, int tokens, int H, int Hkv, int dh, int max_len) {
-    if (B <= 0 || tokens <= 0 || H <= 0 || Hkv <= 0 || dh <= 0) return 0;
-    const int n = paged_splits(B, tokens, Hkv, H / Hkv, max_len);
-    return n < 2 ? 0 : (size_t)n * tokens * H * (dh + 2) * sizeof(float);
-}
-extern "C" int ttsmi_paged_attention(const void* q, int64_t q_row, int64_t q_head, const void* k_pages, const void* v_pages,
-                                     const uint8_t* k_exp, const uint8_t* v_exp, int cache_dtype, int n_pages, int page_size,
-                                     const int32_t* table, int table_width, const int32_t* starts, const int32_t* lens, int B,
-                                     int tokens, int H, int Hkv, int dh, float scale, int max_len, void* out, int64_t o_row,
-                                     int64_t o_head, int zero_rest, void* ws, size_t ws_bytes, int dtype, ttsmi_stream_t stream) {
-    SEQ_CHECK_COMMON("paged_attention");
-    TTSMI_CHECK_ARG(cache_dtype == dtype || cache_dtype == TTSMI_E4M3, "paged_attention: cache dtype %d with tensors of dtype %d", cache_dtype, dtype);
-    TTSMI_CHECK_ARG(n_pages >= 0 && page_size > 0 && page_size <= 1024 && (page_size & (page_size - 1)) == 0 && table_width >= 0,
-                    "paged_attention: %d pages of %d rows (a power of two up to 1024)", n_pages, page_size);
-    if (tokens == 0) return TTSMI_OK;
-    TTSMI_CHECK_ARG(starts && (B == 0 || (lens && (table || table_width == 0))), "paged_attention: null starts, lens or table");
-    TTSMI_CHECK_ARG(n_pages == 0 || (k_pages && v_pages && (((uintptr_t)k_pages | (uintptr_t)v_pages) & 15) == 0), "paged_attention: pages null or not 16-byte aligned");
-    TTSMI_CHECK_ARG(cache_dtype != TTSMI_E4M3 || n_pages == 0 || (k_exp && v_exp), "paged_attention: an e4m3 cache needs its exponents");
-    TTSMI_CHECK_ARG(seq_strides_ok(q, q_row, q_head, dtype) && seq_strides_ok(out, o_row, o_head, dtype),
-                    "paged_attention: a tensor is null or its rows or heads are not 16-byte aligned");
-    SeqFwdP p = {};
-    p.q = q; p.q_row = q_row; p.q_head = q_head; p.o = out; p.zero_rest = zero_rest != 0; p.o_row = o_row; p.o_head = o_head; p.starts = starts; p.lens = lens;
-    p.pg.k = k_pages; p.pg.v = v_pages; p.pg.ke = k_exp; p.pg.ve = v_exp; p.pg.table = table; p.pg.table_width = table_width;
-    p.pg.n_pages = n_pages; p.pg.shift = __builtin_ctz(page_size); p.pg.heads = Hkv; p.pg.dh = dh;
-    p.B = B; p.tokens = tokens; p.Hkv = Hkv; p.G = H / Hkv; p.dh = dh; p.causal = 1; p.c1 = scale * SEQ_LOG2E;
-    p.nsplit = paged_splits(B, tokens, Hkv, p.G, max_len);
-    if (p.nsplit > 1) {
-        const size_t need = ttsmi_paged_attention_ws_bytes(B, tokens, H, Hkv, dh, max_len);
-        if (!ws || ws_bytes < need || ((uintptr_t)ws & 15)) {
-            ttsmi_set_error("paged_attention: workspace of %zu bytes, %zu (16-byte aligned) needed", ws_bytes, need);
-            return TTSMI_ERR_WORKSPACE;
-        }
-        p.part_o = (float*)ws;
-        p.part_ml = (float*)ws + (size_t)p.nsplit * tokens * H * dh;
-    }
-    hipStream_t st = (hipStream_t)stream;
-    if (dtype == TTSMI_F32)
-        return cache_dtype == TTSMI_E4M3 ? seq_fwd_launch<float, uint8_t, true>(p, st) : seq_fwd_launch<float, float, true>(p, st);
-    return cache_dtype == TTSMI_E4M3 ? seq_fwd_launch<__bf16, uint8_t, true>(p, st) : seq_fwd_launch<__bf16, __bf16, true>(p, st);
 }

@@ -23,7 +23,11 @@ struct SeqBwdP {
     const int* starts;
     int B, tokens, Hkv, G, dh, causal, zero_rest;
     float scale, c1;
+    // row splits of the dK / dV pass (slots > 0): sums of unit u, key head hk at [(u Hkv + hk)][dK, dV][128 keys][dh], fp32
+    int slots; float* part;
 };
+// rows of a split at least: eight tiles of work against the traffic of its partial sums (bf16); the fp32 products are slower
+template <typename T> struct SeqLeast { static constexpr int ROWS = sizeof(T) == 2 ? 512 : 128; };
 
 // delta and nothing else: a wave a row of (token, head), 16 bytes a lane
 template <typename T>
@@ -175,7 +179,9 @@ __global__ __launch_bounds__(256, 1) void seq_attn_dkv_kernel(SeqBwdP p) {
     const int tid = threadIdx.x, lane = tid & 63, l31 = lane & 31, hh = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int hk = blockIdx.x % p.Hkv, unit = blockIdx.x / p.Hkv;
-    const SeqTile st = find_tile(p.starts, p.B, p.tokens, 1, 128, unit);         // causal: the first keys have the most rows
+    SeqUnit un;
+    if (p.slots > 0) un = find_unit(p.starts, nullptr, p.G, p.B, p.tokens, 1, 128, p.slots, KT, SeqLeast<T>::ROWS, unit, false);
+    const SeqTile st = p.slots > 0 ? un.t : find_tile(p.starts, p.B, p.tokens, 1, 128, unit);   // causal: the first keys have the most rows
     if (st.seq < 0) {
         if (p.zero_rest) {
             seq_zero_rest<T>((T*)p.dk, p.dk_row, p.dk_head, p.starts, p.B, p.tokens, 1, 128, hk, p.dh, st.tile);
@@ -183,7 +189,16 @@ __global__ __launch_bounds__(256, 1) void seq_attn_dkv_kernel(SeqBwdP p) {
         }
         return;
     }
-    const int key0 = st.tile * 128, key = key0 + wave * 32 + l31, rows = st.n * p.G;
+    const int key0 = st.tile * 128, key = key0 + wave * 32 + l31;
+    const int first = p.causal ? key0 * p.G : 0;                                  // rows before see none of these keys
+    int rows = st.n * p.G, r_begin = first / KT * KT;
+    bool part = false;
+    if (p.slots > 0 && un.nsplit > 1) {
+        if ((un.split + 1) * (long)un.per <= first) return;                       // a split in front of the first row: nothing
+        part = first / un.per < un.nsplit - 1;                                    // more than one split has rows
+        r_begin = max(r_begin, un.split * un.per);
+        rows = (int)min((long)rows, (un.split + 1) * (long)un.per);
+    }
     const bool kok = key < st.n;
     const bool live = key0 + wave * 32 < st.n;
     frag kf[NS], vf[NS];
@@ -202,7 +217,6 @@ __global__ __launch_bounds__(256, 1) void seq_attn_dkv_kernel(SeqBwdP p) {
     for (int cb = 0; cb < NCB; ++cb)
 #pragma unroll
         for (int i = 0; i < 16; ++i) dk[cb][i] = dv[cb][i] = 0.f;
-    const int first = p.causal ? key0 * p.G : 0;                                  // rows before see none of these keys
     const int wfirst = p.causal ? (key0 + wave * 32) * p.G : 0;
     const int wfull = p.causal ? (key0 + wave * 32 + 31) * p.G : 0;               // from here on rows see every key of the wave
     const int low = p.causal ? key * p.G : 0;                                     // this lane's key: rows >= low see it
@@ -225,7 +239,6 @@ __global__ __launch_bounds__(256, 1) void seq_attn_dkv_kernel(SeqBwdP p) {
             rl = r >= rows ? 0.f : tid < KT ? p.lse[slot0 + r] * SEQ_LOG2E : p.delta[slot0 + r];
         }
     };
-    const int r_begin = first / KT * KT;
     fetch(r_begin);
     for (int r0 = r_begin; r0 < rows; r0 += KT) {
         __syncthreads();
@@ -283,6 +296,19 @@ __global__ __launch_bounds__(256, 1) void seq_attn_dkv_kernel(SeqBwdP p) {
         }
     }
     if (!kok) return;
+    if (part) {
+        float* dst = p.part + (((un.first + un.split) * p.Hkv + hk) * 2 * 128 + wave * 32 + l31) * p.dh;
+#pragma unroll
+        for (int cb = 0; cb < NCB; ++cb)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const int c = cb * 32 + 8 * g + 4 * hh;
+                if (c >= p.dh) continue;
+                seq_store4<float>(dst + c, dk[cb], g, 1.f);
+                seq_store4<float>(dst + 128 * p.dh + c, dv[cb], g, 1.f);
+            }
+        return;
+    }
     T* dkr = (T*)p.dk + (long)(st.s0 + key) * p.dk_row + (long)hk * p.dk_head;
     T* dvr = (T*)p.dv + (long)(st.s0 + key) * p.dv_row + (long)hk * p.dv_head;
 #pragma unroll
@@ -296,11 +322,44 @@ __global__ __launch_bounds__(256, 1) void seq_attn_dkv_kernel(SeqBwdP p) {
         }
 }
 
+// the sums of a key tile's splits, in their order: 16 keys a workgroup (grid y), four elements a thread
+template <typename T>
+__global__ __launch_bounds__(256) void seq_dkv_join_kernel(SeqBwdP p) {
+    const int hk = blockIdx.x % p.Hkv;
+    const SeqUnit un = find_unit(p.starts, nullptr, p.G, p.B, p.tokens, 1, 128, p.slots, SeqT<T>::KT, SeqLeast<T>::ROWS, blockIdx.x / p.Hkv, true);
+    if (un.t.seq < 0) return;
+    const int key0 = un.t.tile * 128, z0 = (p.causal ? key0 * p.G : 0) / un.per;
+    if (un.nsplit - z0 < 2) return;
+    const int per = p.dh / 4, keys = min(16, un.t.n - key0 - 16 * (int)blockIdx.y);
+    const long step = 2L * 128 * p.dh * p.Hkv;
+    for (int i = threadIdx.x; i < 2 * keys * per; i += 256) {
+        const int which = i >= keys * per, j = i - which * keys * per, row = 16 * blockIdx.y + j / per, c = (j % per) * 4;
+        const float* src = p.part + (((un.first + z0) * p.Hkv + hk) * 2 * 128 + which * 128 + row) * p.dh + c;
+        float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+        for (int z = z0; z < un.nsplit; ++z, src += step) {
+            const float4 b = *reinterpret_cast<const float4*>(src);
+            a.x += b.x; a.y += b.y; a.z += b.z; a.w += b.w;
+        }
+        const long tok = un.t.s0 + key0 + row;
+        T* dst = which ? (T*)p.dv + tok * p.dv_row + (long)hk * p.dv_head + c : (T*)p.dk + tok * p.dk_row + (long)hk * p.dk_head + c;
+        const float f = which ? 1.f : p.scale;
+        dst[0] = (T)(a.x * f); dst[1] = (T)(a.y * f); dst[2] = (T)(a.z * f); dst[3] = (T)(a.w * f);
+    }
+}
+
+// Row splits a key head: two workgroups a compute unit in all; none where the key tiles alone are that many.
+static int seq_bwd_slots(int tokens, int Hkv) {
+    const int fill = 512 / Hkv < 1 ? 1 : 512 / Hkv;
+    return tokens / 128 >= fill ? 0 : fill;
+}
+
 template <typename T, int DHP>
 static void seq_bwd_launch(const SeqBwdP& p, hipStream_t st) {
     const long rows = (long)p.tokens * p.Hkv * p.G;
     hipLaunchKernelGGL((seq_delta_kernel<T>), dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, st, p);
-    hipLaunchKernelGGL((seq_attn_dkv_kernel<T, DHP>), dim3((unsigned)(seq_units(p.tokens, p.B, 1, 128) * p.Hkv)), dim3(256), 0, st, p);
+    hipLaunchKernelGGL((seq_attn_dkv_kernel<T, DHP>), dim3((unsigned)((p.slots > 0 ? seq_split_units(p.tokens, p.B, 1, 128, p.slots) : seq_units(p.tokens, p.B, 1, 128)) * p.Hkv)), dim3(256), 0, st, p);
+    if (p.slots > 0) hipLaunchKernelGGL((seq_dkv_join_kernel<T>), dim3((unsigned)(seq_units(p.tokens, p.B, 1, 128) * p.Hkv), 8), dim3(256), 0, st, p);
     hipLaunchKernelGGL((seq_attn_dq_kernel<T, DHP>), dim3((unsigned)(seq_units(p.tokens, p.B, p.G, 128) * p.Hkv)), dim3(256), 0, st, p);
 }
 template <typename T>
@@ -312,8 +371,11 @@ static int seq_bwd_route(const SeqBwdP& p, hipStream_t st) {
     return TTSMI_OK;
 }
 
-extern "C" size_t ttsmi_packed_attention_bwd_ws_bytes(int tokens, int H) {
-    return tokens <= 0 || H <= 0 ? 0 : (size_t)tokens * H * sizeof(float);
+static size_t seq_delta_bytes(int tokens, int H) { return ((size_t)tokens * H * sizeof(float) + 255) / 256 * 256; }
+extern "C" size_t ttsmi_packed_attention_bwd_ws_bytes(int B, int tokens, int H, int Hkv, int dh) {
+    if (B < 0 || tokens <= 0 || H <= 0 || Hkv <= 0 || dh <= 0) return 0;
+    const int slots = seq_bwd_slots(tokens, Hkv);
+    return seq_delta_bytes(tokens, H) + (slots ? (size_t)seq_split_units(tokens, B, 1, 128, slots) * Hkv * 2 * 128 * dh * sizeof(float) : 0);
 }
 extern "C" int ttsmi_packed_attention_bwd(const void* q, int64_t q_row, int64_t q_head, const void* k, int64_t k_row, int64_t k_head,
                                           const void* v, int64_t v_row, int64_t v_head, const void* out, int64_t o_row, int64_t o_head,
@@ -328,8 +390,9 @@ extern "C" int ttsmi_packed_attention_bwd(const void* q, int64_t q_row, int64_t 
                         seq_strides_ok(out, o_row, o_head, dtype) && seq_strides_ok(dout, d_row, d_head, dtype) &&
                         seq_strides_ok(dq, dq_row, dq_head, dtype) && seq_strides_ok(dk, dk_row, dk_head, dtype) &&
                         seq_strides_ok(dv, dv_row, dv_head, dtype), "packed_attention_bwd: a tensor is null or its rows or heads are not 16-byte aligned");
-    if (!ws || ws_bytes < ttsmi_packed_attention_bwd_ws_bytes(tokens, H)) {
-        ttsmi_set_error("packed_attention_bwd: workspace of %zu bytes, %zu needed", ws_bytes, ttsmi_packed_attention_bwd_ws_bytes(tokens, H));
+    const size_t need = ttsmi_packed_attention_bwd_ws_bytes(B, tokens, H, Hkv, dh);
+    if (!ws || ws_bytes < need || ((uintptr_t)ws & 15)) {
+        ttsmi_set_error("packed_attention_bwd: workspace of %zu bytes, %zu (16-byte aligned) needed", ws_bytes, need);
         return TTSMI_ERR_WORKSPACE;
     }
     SeqBwdP p = {};
@@ -338,5 +401,7 @@ extern "C" int ttsmi_packed_attention_bwd(const void* q, int64_t q_row, int64_t 
     p.dq = dq; p.dq_row = dq_row; p.dq_head = dq_head; p.dk = dk; p.dk_row = dk_row; p.dk_head = dk_head; p.dv = dv; p.dv_row = dv_row; p.dv_head = dv_head;
     p.lse = lse; p.delta = (float*)ws; p.starts = starts; p.B = B; p.tokens = tokens; p.Hkv = Hkv; p.G = H / Hkv; p.dh = dh;
     p.causal = causal != 0; p.zero_rest = zero_rest != 0; p.scale = scale; p.c1 = scale * SEQ_LOG2E;
+    p.slots = seq_bwd_slots(tokens, Hkv);
+    p.part = (float*)((char*)ws + seq_delta_bytes(tokens, H));
     return dtype == TTSMI_F32 ? seq_bwd_route<float>(p, (hipStream_t)stream) : seq_bwd_route<__bf16>(p, (hipStream_t)stream);
 }

@@ -121,6 +121,76 @@ __device__ __forceinline__ void seq_zero_rest(T* dst, long row, long head, const
     }
 }
 
+// ---- key splits: units of (sequence, row tile, key range) ---------------------------------------------
+// With few row tiles the keys are split over workgroups.  One split length for the whole call, chosen on the device so that all
+// splits together number about `slots` a key head: long sequences get many, short ones one, and no workgroup has more than
+// one split's keys - the batch is even whatever its lengths.  Units of a sequence: its row tiles, each with its splits in turn.
+struct SeqUnit {
+    SeqTile t;
+    int len;                      // keys of the sequence
+    int split, nsplit, per;       // key range [split per, (split + 1) per)
+    long first;                   // unit number of the tile's first split
+};
+static inline __host__ __device__ long seq_split_units(long tokens, int B, int G, int R, int slots) { return tokens * G / R + B + 1 + slots; }
+// Tiles: R rows of G a token.  Keys: lens, or `own` times the sequence's tokens where lens is null (the backward's splits of the
+// rows that a key tile meets).  by_tile: `unit` counts tiles instead (the join).
+__device__ __forceinline__ SeqUnit find_unit(const int* starts, const int* lens, int own, int B, int tokens, int G, int R, int slots,
+                                             int quantum, int least, int unit, bool by_tile) {
+    const int lane = threadIdx.x & 63;
+    long total = 0;
+    int s0 = 0, n = 0, len = 0, tiles = 0;
+    auto look = [&](int b) {
+        s0 = n = len = 0;
+        if (b < B) {
+            s0 = min(max(starts[b], 0), tokens);
+            n = min(max(starts[b + 1], s0), tokens) - s0;
+            len = lens ? max(lens[b], 0) : n * own;
+        }
+        tiles = (int)(((long)n * G + R - 1) / R);
+    };
+    for (int b0 = 0; b0 < B; b0 += 64) {
+        look(b0 + lane);
+        total += (long)tiles * len;
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) total += __shfl_xor(total, o, 64);
+    const long even = (total + slots - 1) / slots;
+    const int per = (int)min((max(even, (long)least) + quantum - 1) / quantum * quantum, (long)0x7fffff00);
+    SeqUnit u;
+    u.t.seq = -1; u.t.tile = u.t.ntile = u.t.s0 = u.t.n = 0;
+    u.len = u.split = 0; u.nsplit = 1; u.per = per; u.first = 0;
+    long before = 0;
+    for (int b0 = 0; b0 < B; b0 += 64) {
+        if (B > 64) look(b0 + lane);                               // (the only 64 are still in registers)
+        const int splits = max((len + per - 1) / per, 1), units = tiles * splits, counted = by_tile ? tiles : units;
+        int upto = counted, all = units;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const int v = __shfl_up(upto, o, 64), w = __shfl_up(all, o, 64);
+            if (lane >= o) { upto += v; all += w; }
+        }
+        const uint64_t hit = __ballot(upto > unit);
+        if (hit) {
+            const int at = __builtin_amdgcn_readfirstlane(__builtin_ctzll(hit));
+            const int rem = unit - (__builtin_amdgcn_readlane(upto, at) - __builtin_amdgcn_readlane(counted, at));
+            u.t.seq = b0 + at;
+            u.t.ntile = __builtin_amdgcn_readlane(tiles, at);
+            u.t.s0 = __builtin_amdgcn_readlane(s0, at);
+            u.t.n = __builtin_amdgcn_readlane(n, at);
+            u.len = __builtin_amdgcn_readlane(len, at);
+            u.nsplit = __builtin_amdgcn_readlane(splits, at);
+            u.t.tile = by_tile ? rem : rem / u.nsplit;
+            u.split = by_tile ? 0 : rem - u.t.tile * u.nsplit;
+            u.first = before + __builtin_amdgcn_readlane(all, at) - __builtin_amdgcn_readlane(units, at) + (long)u.t.tile * u.nsplit;
+            return u;
+        }
+        unit -= __builtin_amdgcn_readlane(upto, 63);
+        before += __builtin_amdgcn_readlane(all, 63);
+    }
+    u.t.tile = unit;
+    return u;
+}
+
 // ---- the paged cache ---------------------------------------------------------------------------------
 // pages [n_pages][Hkv][2^shift][dh] of bf16, fp32 or e4m3 bytes; e4m3: exp [n_pages][Hkv][2^shift], the biased exponent of the
 // row's power-of-two scale.  A page number outside [0, n_pages) reads as zeros and is never written.
@@ -140,6 +210,23 @@ struct SeqPages {
 };
 // 2^(e - 127) of a stored exponent byte (0 and 255 are not written by the cache kernels)
 __device__ __forceinline__ float seq_scale_of(uint32_t e) { return __builtin_bit_cast(float, e << 23); }
+
+// ---- what a forward launch takes ----
+#define SEQ_TILE_LEAST 256           // keys of a split, tile form: at least four tiles
+struct SeqFwdP {
+    const void* q; long q_row, q_head;                    // element strides
+    const void* k; long k_row, k_head;
+    const void* v; long v_row, v_head;
+    void* o; long o_row, o_head;
+    float* lse;                                           // [Hkv][tokens G] natural log, or null
+    const int* starts; const int* lens;                   // lens: paged only (tokens in the cache, the new ones among them)
+    SeqPages pg;
+    int B, tokens, Hkv, G, dh, causal, zero_rest;
+    float c1;                                             // scale log2(e)
+    // key splits (slots > 0): partial sums of unit u, key head hk at [(u Hkv + hk)][R rows][dh], their maximum and sum at [..][R][2]
+    int slots; float* part_o; float* part_ml;
+};
+
 
 // ---- 16-byte chunks of an LDS tile image ----------------------------------------------------------
 // A tile image is [rows][DHP] with the 16-byte chunks of a row permuted by the row number, so that the 32 rows of a fragment
@@ -228,3 +315,15 @@ static inline bool seq_strides_ok(const void* ptr, int64_t row, int64_t head, in
     TTSMI_CHECK_ARG(dh > 0 && dh <= 192 && dh % 8 == 0, who ": head size %d (a multiple of 8 up to 192)", dh);             \
     TTSMI_CHECK_ARG(scale > 0.f && scale < INFINITY, who ": scale must be positive and finite");                          \
     TTSMI_CHECK_ARG((long)tokens * H + 128L * B * Hkv < (1L << 31), who ": tokens * heads too large");
+#define SEQ_CHECK_PAGES(who)                                                                                                      \
+    TTSMI_CHECK_ARG(n_pages >= 0 && page_size > 0 && page_size <= 1024 && (page_size & (page_size - 1)) == 0 && table_width >= 0 &&  \
+                        (long)n_pages * Hkv < (1L << 31), who ": %d pages of %d rows (a power of two up to 1024)", n_pages, page_size)
+#define SEQ_CHECK_CACHE(who)                                                                                                      \
+    do {                                                                                                                          \
+        TTSMI_CHECK_ARG(starts && (B == 0 || (lens && (table || table_width == 0))), who ": null starts, lens or table");         \
+        TTSMI_CHECK_ARG(n_pages == 0 || (k_pages && v_pages && (((uintptr_t)k_pages | (uintptr_t)v_pages) & 15) == 0),             \
+                        who ": pages null or not 16-byte aligned");                                                               \
+        TTSMI_CHECK_ARG(cache_dtype != TTSMI_E4M3 || n_pages == 0 || (k_exp && v_exp), who ": an e4m3 cache needs its exponents");  \
+    } while (0)
+
+int seq_paged_tiles(const SeqFwdP& p, int dtype, int cache_dtype, hipStream_t st);

@@ -2327,7 +2327,7 @@ class PackedAttentionFn(torch.autograd.Function):
         with _device_of(q), pin_stream(ctx.stream_h):
             dout = _strided(dout)
             dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
-            ws = _ws(l.ttsmi_packed_attention_bwd_ws_bytes(M, H), q.device)
+            ws = _ws(l.ttsmi_packed_attention_bwd_ws_bytes(starts.numel() - 1, M, H, k.shape[1], dh), q.device)
             check(l.ttsmi_packed_attention_bwd(*_rs(q), *_rs(k), *_rs(v), *_rs(out), *_rs(dout), lse.data_ptr(), starts.data_ptr(),
                                                starts.numel() - 1, M, H, k.shape[1], dh, scale, int(causal), *_rs(dq), *_rs(dk),
                                                *_rs(dv), 1, ws.data_ptr(), ws.numel(), _SEQ_DTYPES[q.dtype], _stream()),
@@ -2445,11 +2445,10 @@ def kv_cache_read(cache, table, lens, starts, tokens, dtype=None, out=None):
     return k, v
 
 
-def paged_attention(q, cache, table, starts, lens, scale=None, max_len=None, out=None):
+def paged_attention(q, cache, table, starts, lens, scale=None, out=None):
     """Attention of packed new tokens q [tokens, H, dh] over the cache, their own keys and values in it already
     (kv_cache_write): token i of the n new ones of sequence b is at position lens[b] - n + i and sees the keys up to it; a
-    token that sees none gets zeros.  max_len: the longest length expected (default: what the table holds) - it only sets how
-    finely the keys are split.  Without gradients.  Rows behind starts[-1] are zeros; in `out` they are left as they were."""
+    token that sees none gets zeros.  Without gradients.  Rows behind starts[-1] are zeros; in `out` they are left as they were."""
     _seq_check('paged_attention: q', q)
     table, starts, lens = _paged_check('paged_attention', cache, table, starts, lens)
     M, H, dh = q.shape
@@ -2457,7 +2456,6 @@ def paged_attention(q, cache, table, starts, lens, scale=None, max_len=None, out
           f'paged_attention: q {tuple(q.shape)} {q.dtype} on {q.device}; pages {tuple(cache.k.shape)} {cache.dtype} on {cache.device}')
     _need(not (torch.is_grad_enabled() and q.requires_grad), 'paged_attention: has no gradient')
     scale = _scale_of(scale, dh)
-    max_len = int(table.shape[1] * cache.page_size if max_len is None else max_len)
     given = out is not None
     if given:
         _need(out.shape == q.shape and out.dtype == q.dtype and out.device == q.device and _strided(out) is out,
@@ -2466,9 +2464,9 @@ def paged_attention(q, cache, table, starts, lens, scale=None, max_len=None, out
     with _device_of(q):
         q = _strided(q)
         out = out if given else torch.empty((M, H, dh), dtype=q.dtype, device=q.device)
-        need = l.ttsmi_paged_attention_ws_bytes(lens.numel(), M, H, cache.heads, dh, max_len)
+        need = l.ttsmi_paged_attention_ws_bytes(lens.numel(), M, H, cache.heads, dh, _CACHE_DTYPES[cache.dtype])
         ws = _ws(need, q.device) if need else None
         check(l.ttsmi_paged_attention(*_rs(q), *cache.args, table.data_ptr(), table.shape[1], starts.data_ptr(), lens.data_ptr(),
-                                      lens.numel(), M, H, cache.heads, dh, scale, max_len, *_rs(out), int(not given), _p(ws),
+                                      lens.numel(), M, H, cache.heads, dh, scale, *_rs(out), int(not given), _p(ws),
                                       0 if ws is None else ws.numel(), _SEQ_DTYPES[q.dtype], _stream()), 'paged_attention')
     return out
