@@ -831,7 +831,7 @@ int ttsmi_packed_attention_fwd(const void* q, int64_t q_row, int64_t q_head, con
                                int Hkv, int dh, float scale, int causal, void* out, int64_t o_row, int64_t o_head, float* lse,
                                int zero_rest, int dtype, ttsmi_stream_t stream);
 /* Gradients of q, k and v (summed over the query heads of a group); deterministic.  out and lse are the forward's. */
-size_t ttsmi_packed_attention_bwd_ws_bytes(int B, int tokens, int H, int Hkv, int dh);
+size_t ttsmi_packed_attention_bwd_ws_bytes(int B, int tokens, int H, int Hkv, int dh, int causal);
 int ttsmi_packed_attention_bwd(const void* q, int64_t q_row, int64_t q_head, const void* k, int64_t k_row, int64_t k_head,
                                const void* v, int64_t v_row, int64_t v_head, const void* out, int64_t o_row, int64_t o_head,
                                const void* dout, int64_t d_row, int64_t d_head, const float* lse, const int32_t* starts, int B,

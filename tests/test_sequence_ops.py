@@ -47,7 +47,7 @@ def test_packed_attention_bwd_refuses_and_empty_calls_pass(lib):
         rc, err = _packed(lib, True, **over)
         assert rc == code and word in err, (over, rc, err)
     assert _packed(lib, tokens=0, q=None)[0] == 0 and _packed(lib, True, tokens=0, ws=None)[0] == 0
-    assert lib.ttsmi_packed_attention_bwd_ws_bytes(2, 10, 4, 2, 64) >= 160 and lib.ttsmi_packed_attention_bwd_ws_bytes(2, 0, 4, 2, 64) == 0
+    assert lib.ttsmi_packed_attention_bwd_ws_bytes(2, 10, 4, 2, 64, 1) >= 160 and lib.ttsmi_packed_attention_bwd_ws_bytes(2, 0, 4, 2, 64, 1) == 0
 
 
 def _cache_args(order, **over):

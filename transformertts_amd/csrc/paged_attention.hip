@@ -13,21 +13,10 @@
 // transposing 8-bit LDS read, and the value scales multiply the probabilities instead (both exact: powers of two).
 #include "seq_common.h"
 
-__device__ __forceinline__ void pg_dma16(const void* src, unsigned lds) {
-    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(lds) : "memory", "m0");
-}
-__device__ __forceinline__ void pg_dma4(const void* src, unsigned lds) {
-    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(src), "s"(lds) : "memory", "m0");
-}
-__device__ __forceinline__ void pg_dma1(const void* src, unsigned lds) {       // a byte a lane, stored as a dword
-    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_ubyte %0, off" ::"v"(src), "s"(lds) : "memory", "m0");
-}
 template <int N> __device__ __forceinline__ void pg_wait() {
     static_assert(N >= 0 && N < 64, "the counter has six bits");
     asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
 }
-__device__ __forceinline__ unsigned pg_lds(const void* p) { return (unsigned)(size_t)(__attribute__((address_space(3))) const void*)p; }
-
 // 8 e4m3 bytes times a power of two
 typedef __bf16 pg_bf16x2 __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ void pg_cvt8(uint2 w, float scale, bf16x8& f) {
@@ -60,7 +49,9 @@ __global__ __launch_bounds__((64 * PgCfg<CT, DHP>::NW), 1) void paged_rows_kerne
     using C = PgCfg<CT, DHP>;
     using frag = typename SeqT<T>::frag;
     constexpr bool Q8 = sizeof(CT) == 1;
-    constexpr int NW = C::NW, NBUF = C::NBUF, ROWB = C::ROWB, CH = ROWB / 16, MASK = CH % 16 == 0 ? 15 : CH % 8 == 0 ? 7 : 3;
+    constexpr int NW = C::NW, NBUF = C::NBUF, ROWB = C::ROWB, CH = ROWB / 16;
+    using I = SeqImg<CT, DHP>;
+    using A = SeqLane<T, DHP>;
     constexpr int NI = 32 * CH / 64, PER = 2 * NI + 1 + (Q8 ? 1 : 0), NS = DHP / 16, NCB = DHP / 32;
     constexpr int STAGES = NW * NBUF * C::BLOCK, SIDE = NW * NBUF * 256;
     constexpr int JOIN = NW * 32 * (DHP + 4) * 4;
@@ -110,7 +101,7 @@ __global__ __launch_bounds__((64 * PgCfg<CT, DHP>::NW), 1) void paged_rows_kerne
         const int pmask = (1 << p.pg.shift) - 1, rowb = p.dh * (int)sizeof(CT);
         const uint32_t pageb = (uint32_t)rowb << p.pg.shift;
         auto key_of = [&](int x) { return min(kbeg + (x * NW + wave) * 32 + l31, kend - 1); };
-        auto ask_ids = [&](int x, int st) { pg_dma4(trow + min(key_of(x) >> p.pg.shift, p.pg.table_width - 1), pg_lds(ids + st * 64)); };
+        auto ask_ids = [&](int x, int st) { seq_dma4(trow + min(key_of(x) >> p.pg.shift, p.pg.table_width - 1), seq_lds(ids + st * 64)); };
         uint32_t bad[NBUF];
         // block x into stage st: its page numbers have landed there
         auto request = [&](int x, int st) {
@@ -123,13 +114,13 @@ __global__ __launch_bounds__((64 * PgCfg<CT, DHP>::NW), 1) void paged_rows_kerne
             unsigned char* const img = mine + st * C::BLOCK;
 #pragma unroll
             for (int i = 0; i < NI; ++i) {
-                const int id16 = i * 64 + lane, row = id16 / CH, phys = id16 - row * CH, ch = (phys ^ (row & MASK)) * 16;
+                const int id16 = i * 64 + lane, row = id16 / CH, phys = id16 - row * CH, ch = (phys ^ I::swz(row)) * 16;
                 const int rkey = min(kbeg + (x * NW + wave) * 32 + row, kend - 1) & pmask;
                 const uint64_t src = (uint64_t)(uint32_t)__shfl((int)head_page, row, 64) * pageb + (uint32_t)(rkey * rowb + (ch < rowb ? ch : 0));
-                pg_dma16((const char*)p.pg.k + src, pg_lds(img + i * 1024));
-                pg_dma16((const char*)p.pg.v + src, pg_lds(img + 32 * ROWB + i * 1024));
+                seq_dma16((const char*)p.pg.k + src, seq_lds(img + i * 1024));
+                seq_dma16((const char*)p.pg.v + src, seq_lds(img + 32 * ROWB + i * 1024));
             }
-            if constexpr (Q8) pg_dma1((hh ? p.pg.ve : p.pg.ke) + (((uint64_t)head_page << p.pg.shift) + (uint32_t)(key & pmask)), pg_lds(exps + st * 64));
+            if constexpr (Q8) seq_dma1((hh ? p.pg.ve : p.pg.ke) + (((uint64_t)head_page << p.pg.shift) + (uint32_t)(key & pmask)), seq_lds(exps + st * 64));
             ask_ids(x + NBUF, st);
         };
 #pragma unroll
@@ -157,15 +148,15 @@ __global__ __launch_bounds__((64 * PgCfg<CT, DHP>::NW), 1) void paged_rows_kerne
 #pragma unroll
                 for (int t = 0; t < NS; ++t) {
                     frag f;
-                    pg_cvt8(*reinterpret_cast<const uint2*>(Ks + l31 * ROWB + ((t ^ (l31 & MASK)) << 4) + 8 * hh), ks, f);
+                    pg_cvt8(*reinterpret_cast<const uint2*>(Ks + I::at(l31, t) + 8 * hh), ks, f);
                     s = seq_mma(f, qf[t], s);
                 }
             } else {
 #pragma unroll
-                for (int t = 0; t < NS; ++t) s = seq_mma(seq_frag<T, DHP>(Ks, l31, t, hh), qf[t], s);
+                for (int t = 0; t < NS; ++t) s = seq_mma(A::row(A::rows(Ks, lane), 0, t), qf[t], s);
             }
             if (k0 + 32 > full || k0 + 32 > kend) {
-                const int seen = min(lim, kend) - k0;
+                const int seen = seq_rare(min(lim, kend) - k0);
 #pragma unroll
                 for (int i = 0; i < 16; ++i)
                     if (seq_rowmap(i, hh) >= seen) s[i] = -INFINITY;
@@ -208,12 +199,12 @@ __global__ __launch_bounds__((64 * PgCfg<CT, DHP>::NW), 1) void paged_rows_kerne
                         typedef int pg_v2i __attribute__((ext_vector_type(2)));
                         typedef __attribute__((address_space(3))) pg_v2i* lds_ptr;
                         const int j = lane & 15, e = j >> 1, row = 16 * t + 8 * (e >> 2) + 4 * hh + (e & 3), ch = cb * 2 + ((lane >> 4) & 1);
-                        const pg_v2i w = __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_ptr)(Vs + row * ROWB + ((ch ^ (row & MASK)) << 4) + 8 * (j & 1)));
+                        const pg_v2i w = __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_ptr)(Vs + I::at(row, ch) + 8 * (j & 1)));
                         frag f;
                         pg_cvt8(make_uint2((uint32_t)w[0], (uint32_t)w[1]), 1.f, f);
                         o[cb] = seq_mma(f, pf, o[cb]);
                     } else {
-                        o[cb] = seq_mma(seq_frag_t<T, DHP>(Vs, 0, t, cb, lane), pf, o[cb]);
+                        o[cb] = seq_mma(A::col(A::cols(Vs, lane), 0, t, cb), pf, o[cb]);
                     }
                 }
             }
@@ -255,7 +246,7 @@ __global__ __launch_bounds__((64 * PgCfg<CT, DHP>::NW), 1) void paged_rows_kerne
     if (wave == 0 && hh == 0) *reinterpret_cast<float2*>(fin + 2 * l31) = make_float2(M, L);
     __syncthreads();
     const int per = p.dh / 4, live = min(32, rows - un.t.tile * 32);
-    const long ubase = ((un.first + un.split) * p.Hkv + hk) * 32;
+    const long ubase = ((un.first + (long)un.split * un.t.ntile) * p.Hkv + hk) * 32;
     for (int i = threadIdx.x; i < live * per; i += 64 * NW) {
         const int row = i / per, c = (i - row * per) * 4;
         float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -298,7 +289,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PgJoinP j) {
     for (int row = blockIdx.y * 4 + wave; row < live; row += 4 * gridDim.y) {
         float m = -INFINITY, l = 0.f;
         float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-        const long step = (long)p.Hkv * j.R, base = (un.first * p.Hkv + hk) * j.R + row;
+        const long step = (long)p.Hkv * j.R * un.t.ntile, base = (un.first * p.Hkv + hk) * j.R + row;
         for (int z0 = 0; z0 < un.nsplit; z0 += 64) {
             float2 ml = make_float2(-INFINITY, 0.f);
             if (z0 + lane < un.nsplit) ml = *reinterpret_cast<const float2*>(p.part_ml + (base + (z0 + lane) * step) * 2);

@@ -16,8 +16,10 @@ __global__ __launch_bounds__(256, (DHP <= 128 && sizeof(T) == 2) ? 2 : 1) void s
     using I = SeqImg<T, DHP>;
     using frag = typename SeqT<T>::frag;
     constexpr int KT = SeqT<T>::KT, NKB = KT / 32, NS = DHP / 16, NCB = DHP / 32, EPC = 16 / (int)sizeof(T);
-    constexpr int ITEMS = KT * I::CH / 256;               // 16-byte chunks per thread and tile image
-    __shared__ __attribute__((aligned(16))) unsigned char Ks[KT * I::ROWB], Vs[KT * I::ROWB];
+    using D = SeqDma<T, DHP, KT>;
+    constexpr bool Q8 = PAGED && sizeof(CT) == 1;
+    constexpr int IMG = KT * I::ROWB, ITEMS = D::NI;      // 16-byte pieces a lane and tile image
+    __shared__ __attribute__((aligned(1024))) unsigned char sm[4 * IMG];         // two stages of a K and a V tile
 
     const int tid = threadIdx.x, lane = tid & 63, l31 = lane & 31, hh = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -63,6 +65,8 @@ __global__ __launch_bounds__(256, (DHP <= 128 && sizeof(T) == 2) ? 2 : 1) void s
 #pragma unroll
         for (int s = 0; s < NS; ++s) qf[s] = seq_load8<T>(qr, 16 * s + 8 * hh, rok && 16 * s + 8 * hh < p.dh);
     }
+#pragma unroll
+    for (int s = 0; s < NS; ++s) asm volatile("" : "+v"(qf[s]));          // waited for in front of the first DMA
     f32x16 o[NCB];
 #pragma unroll
     for (int cb = 0; cb < NCB; ++cb)
@@ -70,73 +74,139 @@ __global__ __launch_bounds__(256, (DHP <= 128 && sizeof(T) == 2) ? 2 : 1) void s
         for (int i = 0; i < 16; ++i) o[cb][i] = 0.f;
     float m = -INFINITY, l = 0.f;
 
-    // ---- tile staging: global -> registers (a tile ahead) -> LDS; rows past the last key are zeros ----
-    // PAGED: the page rows of a tile are looked up one tile earlier still, so that no load waits for another
-    uint4 rk[ITEMS], rv[ITEMS];
-    long at[PAGED ? ITEMS : 1];
+    // ---- tile staging, two stages, one barrier a tile ----
+    // Rows of this type: LDS-DMA; a row past the last key repeats it (its score is masked).  A paged tile's rows are looked up a
+    // tile earlier, so that no load waits for another; rows of a page that is not there are cleared when they have landed.
+    // e4m3 rows: through registers, converted on the way.
+    uint32_t ko[ITEMS], vo[ITEMS];
+    if constexpr (!PAGED) {
+#pragma unroll
+        for (int i = 0; i < ITEMS; ++i) {
+            ko[i] = D::row(i, wave, lane) * (uint32_t)(p.k_row * (long)sizeof(T)) + D::piece(i, wave, lane, p.dh);
+            vo[i] = D::row(i, wave, lane) * (uint32_t)(p.v_row * (long)sizeof(T)) + D::piece(i, wave, lane, p.dh);
+        }
+    }
+    int pid[PAGED ? ITEMS : 1];                           // page numbers of the next tile's rows, as they come
+    uint32_t gone = 0, gone_next = 0;                     // bit i: item i's row of the tile has no page
+    uint2 wk[Q8 ? ITEMS : 1], wv[Q8 ? ITEMS : 1];
+    uint32_t ek[Q8 ? ITEMS : 1], ev[Q8 ? ITEMS : 1];
     auto look = [&](int k0) {
         if constexpr (PAGED) {
+            const int* const trow = p.pg.table + (long)st.seq * p.pg.table_width;
 #pragma unroll
             for (int i = 0; i < ITEMS; ++i) {
-                const int key = k0 + (tid + 256 * i) / I::CH;
-                at[i] = key < kend ? p.pg.row(st.seq, hk, key) : -1;
+                const int at = min(k0 + D::row(i, wave, lane), kend - 1) >> p.pg.shift;
+                pid[i] = at < p.pg.table_width ? trow[at] : -1;
             }
         }
     };
-    auto fetch = [&](int k0) {
+    auto fetch = [&](int k0, int buf) {
+        unsigned char* const img = sm + buf * 2 * IMG;
+        long at[PAGED ? ITEMS : 1];
+        if constexpr (PAGED) {
 #pragma unroll
-        for (int i = 0; i < ITEMS; ++i) {
-            const int id = tid + 256 * i, row = id / I::CH, ch = id - row * I::CH, key = k0 + row;
-            rk[i] = rv[i] = make_uint4(0u, 0u, 0u, 0u);
-            if constexpr (PAGED) {
-                if (at[i] >= 0 && ch * EPC < p.dh) {
-                    if constexpr (sizeof(CT) == 1) {
-                        rk[i] = seq_dequant_chunk<T>((const uint8_t*)p.pg.k + at[i] * p.dh + ch * EPC, seq_scale_of(p.pg.ke[at[i]]));
-                        rv[i] = seq_dequant_chunk<T>((const uint8_t*)p.pg.v + at[i] * p.dh + ch * EPC, seq_scale_of(p.pg.ve[at[i]]));
-                    } else {
-                        rk[i] = *reinterpret_cast<const uint4*>((const T*)p.pg.k + at[i] * p.dh + ch * EPC);
-                        rv[i] = *reinterpret_cast<const uint4*>((const T*)p.pg.v + at[i] * p.dh + ch * EPC);
-                    }
+            for (int i = 0; i < ITEMS; ++i) asm volatile("" : "+v"(pid[i]));                  // all of them, in front of the first load below
+            gone_next = 0;
+#pragma unroll
+            for (int i = 0; i < ITEMS; ++i) {
+                const int key = min(k0 + D::row(i, wave, lane), kend - 1);
+                const bool ok = (unsigned)pid[i] < (unsigned)p.pg.n_pages;
+                if (!ok) gone_next |= 1u << i;
+                at[i] = (((long)(ok ? pid[i] : 0) * p.pg.heads + hk) << p.pg.shift) + (key & ((1 << p.pg.shift) - 1));
+            }
+        }
+        if constexpr (Q8) {
+#pragma unroll
+            for (int i = 0; i < ITEMS; ++i) {
+                const int c = (int)D::piece(i, wave, lane, p.dh) / (int)sizeof(T);
+                wk[i] = wv[i] = make_uint2(0u, 0u);
+                ek[i] = ev[i] = 127;
+                if ((gone_next >> i) & 1) continue;
+                const uint8_t* const a = (const uint8_t*)p.pg.k + at[i] * p.dh + c;
+                const uint8_t* const b = (const uint8_t*)p.pg.v + at[i] * p.dh + c;
+                if constexpr (sizeof(T) == 2) {
+                    wk[i] = *reinterpret_cast<const uint2*>(a);
+                    wv[i] = *reinterpret_cast<const uint2*>(b);
+                } else {
+                    wk[i].x = *reinterpret_cast<const uint32_t*>(a);
+                    wv[i].x = *reinterpret_cast<const uint32_t*>(b);
                 }
-            } else if (key < kend && ch * EPC < p.dh) {
-                rk[i] = *reinterpret_cast<const uint4*>((const T*)p.k + (long)(st.s0 + key) * p.k_row + (long)hk * p.k_head + ch * EPC);
-                rv[i] = *reinterpret_cast<const uint4*>((const T*)p.v + (long)(st.s0 + key) * p.v_row + (long)hk * p.v_head + ch * EPC);
+                ek[i] = p.pg.ke[at[i]];
+                ev[i] = p.pg.ve[at[i]];
+            }
+        } else if constexpr (PAGED) {
+#pragma unroll
+            for (int i = 0; i < ITEMS; ++i) {
+                const long src = at[i] * (p.dh * (long)sizeof(T)) + D::piece(i, wave, lane, p.dh);
+                seq_dma16((const char*)p.pg.k + src, seq_lds(img + (wave + 4 * i) * 1024));
+                seq_dma16((const char*)p.pg.v + src, seq_lds(img + IMG + (wave + 4 * i) * 1024));
+            }
+        } else {
+            const char* const kb = (const char*)p.k + ((long)(st.s0 + k0) * p.k_row + (long)hk * p.k_head) * (long)sizeof(T);
+            const char* const vb = (const char*)p.v + ((long)(st.s0 + k0) * p.v_row + (long)hk * p.v_head) * (long)sizeof(T);
+            if (k0 + KT <= kend) {
+#pragma unroll
+                for (int i = 0; i < ITEMS; ++i) {
+                    seq_dma16(kb, ko[i], seq_lds(img + (wave + 4 * i) * 1024));
+                    seq_dma16(vb, vo[i], seq_lds(img + IMG + (wave + 4 * i) * 1024));
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < ITEMS; ++i) {
+                    const uint32_t row = min(D::row(i, wave, lane), kend - 1 - k0), c = D::piece(i, wave, lane, p.dh);
+                    seq_dma16(kb, row * (uint32_t)(p.k_row * (long)sizeof(T)) + c, seq_lds(img + (wave + 4 * i) * 1024));
+                    seq_dma16(vb, row * (uint32_t)(p.v_row * (long)sizeof(T)) + c, seq_lds(img + IMG + (wave + 4 * i) * 1024));
+                }
             }
         }
     };
-    auto stash = [&]() {
+    auto land = [&](int buf) {                            // the wave's share of a tile is complete in LDS
+        unsigned char* const img = sm + buf * 2 * IMG;
+        if constexpr (Q8) {
 #pragma unroll
-        for (int i = 0; i < ITEMS; ++i) {
-            const int id = tid + 256 * i, row = id / I::CH, ch = id - row * I::CH;
-            *reinterpret_cast<uint4*>(Ks + I::at(row, ch)) = rk[i];
-            *reinterpret_cast<uint4*>(Vs + I::at(row, ch)) = rv[i];
+            for (int i = 0; i < ITEMS; ++i) {
+                *reinterpret_cast<uint4*>(img + (wave + 4 * i) * 1024 + lane * 16) = seq_dequant_chunk<T>(wk[i], seq_scale_of(ek[i]));
+                *reinterpret_cast<uint4*>(img + IMG + (wave + 4 * i) * 1024 + lane * 16) = seq_dequant_chunk<T>(wv[i], seq_scale_of(ev[i]));
+            }
+        } else if constexpr (PAGED) {
+            gone = gone_next;
+            if (__ballot(gone != 0)) {
+                asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+#pragma unroll
+                for (int i = 0; i < ITEMS; ++i)
+                    if ((gone >> i) & 1)
+                        *reinterpret_cast<uint4*>(img + (wave + 4 * i) * 1024 + lane * 16) = *reinterpret_cast<uint4*>(img + IMG + (wave + 4 * i) * 1024 + lane * 16) = make_uint4(0u, 0u, 0u, 0u);
+            }
         }
+        seq_dma_barrier();
     };
 
     if (kbeg < kend) {
         look(kbeg);
-        fetch(kbeg);
-        look(kbeg + KT);
+        fetch(kbeg, 0);
+        if (kbeg + KT < kend) look(kbeg + KT);
     }
-    for (int k0 = kbeg; k0 < kend; k0 += KT) {
-        __syncthreads();
-        stash();
-        __syncthreads();
+    using A = SeqLane<T, DHP>;
+    const uint32_t kbase = A::rows(sm, lane), vbase = A::cols(sm + IMG, lane);
+    int buf = 0;
+    for (int k0 = kbeg; k0 < kend; k0 += KT, buf ^= 1) {
+        land(buf);
         if (k0 + KT < kend) {
-            fetch(k0 + KT);
+            fetch(k0 + KT, buf ^ 1);
             look(k0 + 2 * KT);
         }
         if (k0 >= wend) continue;
+        const uint32_t ka = kbase + buf * 2 * IMG, va = vbase + buf * 2 * IMG;
         f32x16 s[NKB];
 #pragma unroll
         for (int kb = 0; kb < NKB; ++kb) {
 #pragma unroll
             for (int i = 0; i < 16; ++i) s[kb][i] = 0.f;
 #pragma unroll
-            for (int t = 0; t < NS; ++t) s[kb] = seq_mma(seq_frag<T, DHP>(Ks, kb * 32 + l31, t, hh), qf[t], s[kb]);
+            for (int t = 0; t < NS; ++t) s[kb] = seq_mma(A::row(ka, kb * 32, t), qf[t], s[kb]);
         }
         if (k0 + KT > wfull || k0 + KT > kend) {
-            const int seen = min(lim, kend) - k0;
+            const int seen = seq_rare(min(lim, kend) - k0);
 #pragma unroll
             for (int kb = 0; kb < NKB; ++kb)
 #pragma unroll
@@ -149,9 +219,16 @@ __global__ __launch_bounds__(256, (DHP <= 128 && sizeof(T) == 2) ? 2 : 1) void s
 #pragma unroll
             for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[kb][i]);
         mx = seq_half_max(mx) * p.c1;
-        const float mn = fmaxf(m, mx), ms = mn == -INFINITY ? 0.f : mn;      // a row that has seen no key yet keeps p = 0
-        const float a = __builtin_amdgcn_exp2f(m - ms);
-        m = mn;
+        if (__ballot(mx > m)) {                           // a new maximum is rare behind the first tiles
+            const float mn = fmaxf(m, mx), a = __builtin_amdgcn_exp2f(m - (mn == -INFINITY ? 0.f : mn));
+            m = mn;
+            l *= a;
+#pragma unroll
+            for (int cb = 0; cb < NCB; ++cb)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) o[cb][i] *= a;
+        }
+        const float ms = m == -INFINITY ? 0.f : m;        // a row that has seen no key yet keeps p = 0
         float sum = 0.f;
 #pragma unroll
         for (int kb = 0; kb < NKB; ++kb)
@@ -160,11 +237,7 @@ __global__ __launch_bounds__(256, (DHP <= 128 && sizeof(T) == 2) ? 2 : 1) void s
                 s[kb][i] = __builtin_amdgcn_exp2f(s[kb][i] * p.c1 - ms);
                 sum += s[kb][i];
             }
-        l = l * a + sum;                                                     // (this half-wave's keys; joined at the end)
-#pragma unroll
-        for (int cb = 0; cb < NCB; ++cb)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) o[cb][i] *= a;
+        l += sum;                                         // (this half-wave's keys; joined at the end)
 #pragma unroll
         for (int kb = 0; kb < NKB; ++kb)
 #pragma unroll
@@ -172,14 +245,14 @@ __global__ __launch_bounds__(256, (DHP <= 128 && sizeof(T) == 2) ? 2 : 1) void s
                 frag pf;
                 seq_to_frag(s[kb], t, pf);
 #pragma unroll
-                for (int cb = 0; cb < NCB; ++cb) o[cb] = seq_mma(seq_frag_t<T, DHP>(Vs, kb * 32, t, cb, lane), pf, o[cb]);
+                for (int cb = 0; cb < NCB; ++cb) o[cb] = seq_mma(A::col(va, kb * 32, t, cb), pf, o[cb]);
             }
     }
     l = seq_half_sum(l);
     if (!rok) return;
     const long slot = (long)hk * p.tokens * p.G + (long)st.s0 * p.G + r;
     if (part) {
-        const long ps = ((un.first + un.split) * p.Hkv + hk) * 128 + wave * 32 + l31;
+        const long ps = ((un.first + (long)un.split * un.t.ntile) * p.Hkv + hk) * 128 + wave * 32 + l31;
         if (hh == 0) *reinterpret_cast<float2*>(p.part_ml + 2 * ps) = make_float2(m, l);
         if (l > 0.f || !(l == l)) {
 #pragma unroll

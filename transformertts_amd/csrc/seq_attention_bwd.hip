@@ -4,8 +4,8 @@
 //   delta_i = do_i . o_i     p_ij = exp(s_ij - lse_i)     ds_ij = p_ij (do_i . v_j - delta_i)
 //   dq_i = scale sum_j ds_ij k_j      dk_j = scale sum_i ds_ij q_i      dv_j = sum_i p_ij do_i      (i: every query head of the group)
 //
-// delta:  one pass over do and o.
-// dQ:     as the forward - 128 rows a workgroup, 32 a wave, S^T and dP^T per key tile, dQ^T += K^T dS^T.
+// dQ:     as the forward - 128 rows a workgroup, 32 a wave, S^T and dP^T per key tile, dQ^T += K^T dS^T.  It also forms delta and
+//         lse in log2 units, once, for the second pass.
 // dK, dV: 128 keys of one key head a workgroup, 32 a wave; the row tiles of every query head of the group pass through LDS, the
 //         wave forms S and dP with a key per lane, so that P and dS are the B operands of dV^T += dO^T P and dK^T += Q^T dS.
 #include "seq_common.h"
@@ -19,7 +19,7 @@ struct SeqBwdP {
     void* dq; long dq_row, dq_head;
     void* dk; long dk_row, dk_head;
     void* dv; long dv_row, dv_head;
-    const float* lse; float* delta;                       // [Hkv][tokens G]
+    const float* lse; float* lse2; float* delta;          // [Hkv][tokens G]; lse2: in log2 units
     const int* starts;
     int B, tokens, Hkv, G, dh, causal, zero_rest;
     float scale, c1;
@@ -28,26 +28,6 @@ struct SeqBwdP {
 };
 // rows of a split at least: eight tiles of work against the traffic of its partial sums (bf16); the fp32 products are slower
 template <typename T> struct SeqLeast { static constexpr int ROWS = sizeof(T) == 2 ? 512 : 128; };
-
-// delta and nothing else: a wave a row of (token, head), 16 bytes a lane
-template <typename T>
-__global__ __launch_bounds__(256) void seq_delta_kernel(SeqBwdP p) {
-    const int H = p.Hkv * p.G;
-    constexpr int LPR = 32;                                // lanes per row: 32 x 8 elements cover 192
-    const long row = (long)blockIdx.x * (256 / LPR) + threadIdx.x / LPR;
-    if (row >= (long)p.tokens * H) return;
-    const int tok = (int)(row / H), head = (int)(row - (long)tok * H), c = (threadIdx.x % LPR) * 8;
-    float s = 0.f;
-    if (c < p.dh) {
-        const typename SeqT<T>::frag a = *reinterpret_cast<const typename SeqT<T>::frag*>((const T*)p.o + (long)tok * p.o_row + (long)head * p.o_head + c);
-        const typename SeqT<T>::frag b = *reinterpret_cast<const typename SeqT<T>::frag*>((const T*)p.d + (long)tok * p.d_row + (long)head * p.d_head + c);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) s += (float)a[e] * (float)b[e];
-    }
-#pragma unroll
-    for (int o = LPR / 2; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
-    if (c == 0) p.delta[(long)(head / p.G) * p.tokens * p.G + (long)tok * p.G + head % p.G] = s;
-}
 
 // four accumulator registers -> four consecutive elements of a gradient row
 template <typename T>
@@ -66,9 +46,10 @@ template <typename T, int DHP>
 __global__ __launch_bounds__(256, (DHP <= 128 && sizeof(T) == 2) ? 2 : 1) void seq_attn_dq_kernel(SeqBwdP p) {
     using I = SeqImg<T, DHP>;
     using frag = typename SeqT<T>::frag;
-    constexpr int KT = SeqT<T>::KT, NKB = KT / 32, NS = DHP / 16, NCB = DHP / 32, EPC = 16 / (int)sizeof(T);
-    constexpr int ITEMS = KT * I::CH / 256;
-    __shared__ __attribute__((aligned(16))) unsigned char Ks[KT * I::ROWB], Vs[KT * I::ROWB];
+    constexpr int KT = SeqT<T>::KT, NKB = KT / 32, NS = DHP / 16, NCB = DHP / 32;
+    using D = SeqDma<T, DHP, KT>;
+    constexpr int IMG = KT * I::ROWB, ITEMS = D::NI;
+    __shared__ __attribute__((aligned(1024))) unsigned char sm[4 * IMG];             // two stages of a K and a V tile
     const int tid = threadIdx.x, lane = tid & 63, l31 = lane & 31, hh = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int hk = blockIdx.x % p.Hkv, unit = blockIdx.x / p.Hkv;
@@ -100,36 +81,58 @@ __global__ __launch_bounds__(256, (DHP <= 128 && sizeof(T) == 2) ? 2 : 1) void s
             df[s] = seq_load8<T>(dr, 16 * s + 8 * hh, ok);
         }
     }
-    const float lse2 = rok ? p.lse[slot] * SEQ_LOG2E : 0.f, delta = rok ? p.delta[slot] : 0.f;
+    float lse2 = 0.f, delta = 0.f;
+    if (rok) {                                                         // delta and lse2 of this row, left for the dK / dV pass too
+        const T* orow = (const T*)p.o + (long)(st.s0 + tok) * p.o_row + (long)head * p.o_head;
+        lse2 = p.lse[slot] * SEQ_LOG2E;
+#pragma unroll
+        for (int s = 0; s < NS; ++s) {
+            const frag f = seq_load8<T>(orow, 16 * s + 8 * hh, 16 * s + 8 * hh < p.dh);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) delta += (float)f[e] * (float)df[s][e];
+        }
+    }
+    delta = seq_half_sum(delta);
+    if (rok && hh == 0) {
+        p.delta[slot] = delta;
+        p.lse2[slot] = lse2;
+    }
     f32x16 acc[NCB];
 #pragma unroll
     for (int cb = 0; cb < NCB; ++cb)
 #pragma unroll
         for (int i = 0; i < 16; ++i) acc[cb][i] = 0.f;
-    uint4 rk[ITEMS], rv[ITEMS];
-    auto fetch = [&](int k0) {
+#pragma unroll
+    for (int s = 0; s < NS; ++s) asm volatile("" : "+v"(qf[s]), "+v"(df[s]));
+    asm volatile("" : "+v"(lse2), "+v"(delta));                        // everything loaded in front of the first DMA
+    uint32_t ko[ITEMS], vo[ITEMS];
+    const uint32_t krb = (uint32_t)(p.k_row * (long)sizeof(T)), vrb = (uint32_t)(p.v_row * (long)sizeof(T));
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i) {
+        ko[i] = D::row(i, wave, lane) * krb + D::piece(i, wave, lane, p.dh);
+        vo[i] = D::row(i, wave, lane) * vrb + D::piece(i, wave, lane, p.dh);
+    }
+    auto fetch = [&](int k0, int buf) {                                // a row past the last key repeats it (its score is masked)
+        unsigned char* const img = sm + buf * 2 * IMG;
+        const char* const kb = (const char*)p.k + ((long)(st.s0 + k0) * p.k_row + (long)hk * p.k_head) * (long)sizeof(T);
+        const char* const vb = (const char*)p.v + ((long)(st.s0 + k0) * p.v_row + (long)hk * p.v_head) * (long)sizeof(T);
+        const bool whole = k0 + KT <= kend;
 #pragma unroll
         for (int i = 0; i < ITEMS; ++i) {
-            const int id = tid + 256 * i, row = id / I::CH, ch = id - row * I::CH, key = k0 + row;
-            rk[i] = rv[i] = make_uint4(0u, 0u, 0u, 0u);
-            if (key < kend && ch * EPC < p.dh) {
-                rk[i] = *reinterpret_cast<const uint4*>((const T*)p.k + (long)(st.s0 + key) * p.k_row + (long)hk * p.k_head + ch * EPC);
-                rv[i] = *reinterpret_cast<const uint4*>((const T*)p.v + (long)(st.s0 + key) * p.v_row + (long)hk * p.v_head + ch * EPC);
-            }
+            const uint32_t row = min(D::row(i, wave, lane), kend - 1 - k0), c = D::piece(i, wave, lane, p.dh);
+            seq_dma16(kb, whole ? ko[i] : row * krb + c, seq_lds(img + (wave + 4 * i) * 1024));
+            seq_dma16(vb, whole ? vo[i] : row * vrb + c, seq_lds(img + IMG + (wave + 4 * i) * 1024));
         }
     };
-    fetch(0);
-    for (int k0 = 0; k0 < kend; k0 += KT) {
-        __syncthreads();
-#pragma unroll
-        for (int i = 0; i < ITEMS; ++i) {
-            const int id = tid + 256 * i, row = id / I::CH, ch = id - row * I::CH;
-            *reinterpret_cast<uint4*>(Ks + I::at(row, ch)) = rk[i];
-            *reinterpret_cast<uint4*>(Vs + I::at(row, ch)) = rv[i];
-        }
-        __syncthreads();
-        if (k0 + KT < kend) fetch(k0 + KT);
+    fetch(0, 0);
+    using A = SeqLane<T, DHP>;
+    const uint32_t kbase = A::rows(sm, lane), tbase = A::cols(sm, lane);
+    int buf = 0;
+    for (int k0 = 0; k0 < kend; k0 += KT, buf ^= 1) {
+        seq_dma_barrier();
+        if (k0 + KT < kend) fetch(k0 + KT, buf ^ 1);
         if (k0 >= wend) continue;
+        const uint32_t ka = kbase + buf * 2 * IMG, ta = tbase + buf * 2 * IMG;
         const bool edge = k0 + KT > wfull;
 #pragma unroll
         for (int kb = 0; kb < NKB; ++kb) {
@@ -139,13 +142,13 @@ __global__ __launch_bounds__(256, (DHP <= 128 && sizeof(T) == 2) ? 2 : 1) void s
             for (int i = 0; i < 16; ++i) s[i] = dp[i] = 0.f;
 #pragma unroll
             for (int t = 0; t < NS; ++t) {
-                s = seq_mma(seq_frag<T, DHP>(Ks, kb * 32 + l31, t, hh), qf[t], s);
-                dp = seq_mma(seq_frag<T, DHP>(Vs, kb * 32 + l31, t, hh), df[t], dp);
+                s = seq_mma(A::row(ka, kb * 32, t), qf[t], s);
+                dp = seq_mma(A::row(ka + IMG, kb * 32, t), df[t], dp);
             }
 #pragma unroll
             for (int i = 0; i < 16; ++i) s[i] = __builtin_amdgcn_exp2f(s[i] * p.c1 - lse2) * (dp[i] - delta);
             if (edge) {
-                const int seen = lim - k0 - kb * 32;
+                const int seen = seq_rare(lim - k0 - kb * 32);
 #pragma unroll
                 for (int i = 0; i < 16; ++i)
                     if (seq_rowmap(i, hh) >= seen) s[i] = 0.f;
@@ -155,7 +158,7 @@ __global__ __launch_bounds__(256, (DHP <= 128 && sizeof(T) == 2) ? 2 : 1) void s
                 frag f;
                 seq_to_frag(s, t, f);
 #pragma unroll
-                for (int cb = 0; cb < NCB; ++cb) acc[cb] = seq_mma(seq_frag_t<T, DHP>(Ks, kb * 32, t, cb, lane), f, acc[cb]);
+                for (int cb = 0; cb < NCB; ++cb) acc[cb] = seq_mma(A::col(ta, kb * 32, t, cb), f, acc[cb]);
             }
         }
     }
@@ -169,13 +172,13 @@ __global__ __launch_bounds__(256, (DHP <= 128 && sizeof(T) == 2) ? 2 : 1) void s
 }
 
 template <typename T, int DHP>
-__global__ __launch_bounds__(256, 1) void seq_attn_dkv_kernel(SeqBwdP p) {
+__global__ __launch_bounds__(256, (DHP <= 128 && sizeof(T) == 2) ? 2 : 1) void seq_attn_dkv_kernel(SeqBwdP p) {
     using I = SeqImg<T, DHP>;
     using frag = typename SeqT<T>::frag;
-    constexpr int KT = SeqT<T>::KT, NKB = KT / 32, NS = DHP / 16, NCB = DHP / 32, EPC = 16 / (int)sizeof(T);
-    constexpr int ITEMS = KT * I::CH / 256;
-    __shared__ __attribute__((aligned(16))) unsigned char Qs[KT * I::ROWB], Ds[KT * I::ROWB];
-    __shared__ __attribute__((aligned(16))) float Ls[2 * KT];                    // lse (log2 units) and delta of the staged rows
+    constexpr int KT = SeqT<T>::KT, NKB = KT / 32, NS = DHP / 16, NCB = DHP / 32;
+    using D = SeqDma<T, DHP, KT>;
+    constexpr int IMG = KT * I::ROWB, ITEMS = D::NI, STAGE = 2 * IMG + 512;
+    __shared__ __attribute__((aligned(1024))) unsigned char sm[2 * STAGE];           // two stages of a Q and a dO tile, lse2 and delta
     const int tid = threadIdx.x, lane = tid & 63, l31 = lane & 31, hh = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int hk = blockIdx.x % p.Hkv, unit = blockIdx.x / p.Hkv;
@@ -219,55 +222,88 @@ __global__ __launch_bounds__(256, 1) void seq_attn_dkv_kernel(SeqBwdP p) {
         for (int i = 0; i < 16; ++i) dk[cb][i] = dv[cb][i] = 0.f;
     const int wfirst = p.causal ? (key0 + wave * 32) * p.G : 0;
     const int wfull = p.causal ? (key0 + wave * 32 + 31) * p.G : 0;               // from here on rows see every key of the wave
-    const int low = p.causal ? key * p.G : 0;                                     // this lane's key: rows >= low see it
     const long slot0 = (long)hk * p.tokens * p.G + (long)st.s0 * p.G;
-    uint4 rq[ITEMS], rd[ITEMS];
-    float rl = 0.f;
-    auto fetch = [&](int r0) {
 #pragma unroll
-        for (int i = 0; i < ITEMS; ++i) {
-            const int id = tid + 256 * i, row = id / I::CH, ch = id - row * I::CH, r = r0 + row;
-            rq[i] = rd[i] = make_uint4(0u, 0u, 0u, 0u);
-            if (r < rows && ch * EPC < p.dh) {
-                const int tok = r / p.G, head = hk * p.G + r - tok * p.G;
-                rq[i] = *reinterpret_cast<const uint4*>((const T*)p.q + (long)(st.s0 + tok) * p.q_row + (long)head * p.q_head + ch * EPC);
-                rd[i] = *reinterpret_cast<const uint4*>((const T*)p.d + (long)(st.s0 + tok) * p.d_row + (long)head * p.d_head + ch * EPC);
+    for (int s = 0; s < NS; ++s) asm volatile("" : "+v"(kf[s]), "+v"(vf[s]));        // loaded in front of the first DMA
+    const float inv_g = 1.f / (float)p.G;
+    // rows r0 .. r0 + KT into stage buf; a row past the last repeats it (masked).  Row r0 is head `rem` of token `tok`: the small
+    // quotient (rem + row) / G is exact in fp32.  Where G divides the rows of an instruction, the items of a lane lie whole tokens
+    // apart and share one offset.
+    constexpr int RPI = 256 / I::CH;                                                 // image rows between a lane's items
+    const bool even = 256 % I::CH == 0 && RPI % 16 == 0 && RPI % p.G == 0;          // (the permutation repeats after 16 rows)
+    auto fetch = [&](int r0, int buf) {
+        unsigned char* const img = sm + buf * STAGE;
+        const int ln = seq_lane_here();
+        const int tok = __builtin_amdgcn_readfirstlane(r0 / p.G), rem = r0 - tok * p.G;
+        const uint32_t qrb = (uint32_t)(p.q_row * (long)sizeof(T)), qhb = (uint32_t)(p.q_head * (long)sizeof(T));
+        const uint32_t drb = (uint32_t)(p.d_row * (long)sizeof(T)), dhb = (uint32_t)(p.d_head * (long)sizeof(T));
+        const char* const qb = (const char*)p.q + ((long)(st.s0 + tok) * p.q_row + (long)hk * p.G * p.q_head) * (long)sizeof(T);
+        const char* const db = (const char*)p.d + ((long)(st.s0 + tok) * p.d_row + (long)hk * p.G * p.d_head) * (long)sizeof(T);
+        if (even && r0 + KT <= rows) {
+            const int x = rem + D::row(0, wave, ln), t = (int)(((float)x + 0.5f) * inv_g), g = x - t * p.G;
+            const uint32_t c = D::piece(0, wave, ln, p.dh), qo = t * qrb + g * qhb + c, dO = t * drb + g * dhb + c;
+            const long qstep = (long)(RPI / p.G) * qrb, dstep = (long)(RPI / p.G) * drb;
+#pragma unroll
+            for (int i = 0; i < ITEMS; ++i) {
+                seq_dma16(qb + i * qstep, qo, seq_lds(img + (wave + 4 * i) * 1024));
+                seq_dma16(db + i * dstep, dO, seq_lds(img + IMG + (wave + 4 * i) * 1024));
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < ITEMS; ++i) {
+                const int x = rem + min(D::row(i, wave, ln), rows - 1 - r0), t = (int)(((float)x + 0.5f) * inv_g), g = x - t * p.G;
+                const uint32_t c = D::piece(i, wave, ln, p.dh);
+                seq_dma16(qb, t * qrb + g * qhb + c, seq_lds(img + (wave + 4 * i) * 1024));
+                seq_dma16(db, t * drb + g * dhb + c, seq_lds(img + IMG + (wave + 4 * i) * 1024));
             }
         }
-        if (tid < 2 * KT) {
-            const int r = r0 + (tid & (KT - 1));
-            rl = r >= rows ? 0.f : tid < KT ? p.lse[slot0 + r] * SEQ_LOG2E : p.delta[slot0 + r];
-        }
+        const int x = min(r0 + (ln & (KT - 1)), rows - 1);
+        if (wave == 0) seq_dma4(p.lse2 + slot0 + x, seq_lds(img + 2 * IMG));
+        if (wave == 1) seq_dma4(p.delta + slot0 + x, seq_lds(img + 2 * IMG + 256));
     };
-    fetch(r_begin);
-    for (int r0 = r_begin; r0 < rows; r0 += KT) {
-        __syncthreads();
-#pragma unroll
-        for (int i = 0; i < ITEMS; ++i) {
-            const int id = tid + 256 * i, row = id / I::CH, ch = id - row * I::CH;
-            *reinterpret_cast<uint4*>(Qs + I::at(row, ch)) = rq[i];
-            *reinterpret_cast<uint4*>(Ds + I::at(row, ch)) = rd[i];
-        }
-        if (tid < 2 * KT) Ls[tid] = rl;
-        __syncthreads();
-        if (r0 + KT < rows) fetch(r0 + KT);
+    r_begin = __builtin_amdgcn_readfirstlane(r_begin);
+    rows = __builtin_amdgcn_readfirstlane(rows);
+    fetch(r_begin, 0);
+    using A = SeqLane<T, DHP>;
+    const uint32_t rbase = A::rows(sm, lane), tbase = A::cols(sm, lane);
+    int buf = 0;
+    for (int r0 = r_begin; r0 < rows; r0 += KT, buf ^= 1) {
+        seq_dma_barrier();
+        if (r0 + KT < rows) fetch(r0 + KT, buf ^ 1);
+        const uint32_t qa = rbase + buf * STAGE, ta = tbase + buf * STAGE;
+        const float* const Ls = reinterpret_cast<const float*>(sm + buf * STAGE + 2 * IMG) + 4 * hh;
         if (!live || r0 + KT <= wfirst) continue;
         const bool edge = r0 < wfull || r0 + KT > rows;
-#pragma unroll
+#pragma unroll 1
         for (int kb = 0; kb < NKB; ++kb) {
             if (r0 + kb * 32 >= rows || r0 + kb * 32 + 32 <= wfirst) continue;
+            const uint32_t qk = qa + kb * 32 * I::ROWB, tk = ta + kb * 32 * I::ROWB;
             f32x16 s, dp;
 #pragma unroll
             for (int i = 0; i < 16; ++i) s[i] = dp[i] = 0.f;
+            // (operands two steps ahead of their products: with the registers that are left the compiler would read each
+            // one just before its use, an LDS round trip per product)
+            frag fq[2], fd[2];
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                fq[t] = A::row(qk, 0, t);
+                fd[t] = A::row(qk + IMG, 0, t);
+            }
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int t = 0; t < NS; ++t) {
-                s = seq_mma(seq_frag<T, DHP>(Qs, kb * 32 + l31, t, hh), kf[t], s);
-                dp = seq_mma(seq_frag<T, DHP>(Ds, kb * 32 + l31, t, hh), vf[t], dp);
+                s = seq_mma(fq[t & 1], kf[t], s);
+                dp = seq_mma(fd[t & 1], vf[t], dp);
+                if (t + 2 < NS) {
+                    fq[t & 1] = A::row(qk, 0, t + 2);
+                    fd[t & 1] = A::row(qk + IMG, 0, t + 2);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
             }
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
-                const float4 ls = *reinterpret_cast<const float4*>(Ls + kb * 32 + 8 * g + 4 * hh);
-                const float4 dl = *reinterpret_cast<const float4*>(Ls + KT + kb * 32 + 8 * g + 4 * hh);
+                const float4 ls = *reinterpret_cast<const float4*>(Ls + kb * 32 + 8 * g);
+                const float4 dl = *reinterpret_cast<const float4*>(Ls + 64 + kb * 32 + 8 * g);
                 const float le[4] = {ls.x, ls.y, ls.z, ls.w}, de[4] = {dl.x, dl.y, dl.z, dl.w};
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
@@ -276,28 +312,38 @@ __global__ __launch_bounds__(256, 1) void seq_attn_dkv_kernel(SeqBwdP p) {
                 }
             }
             if (edge) {
+                const int ln = seq_lane_here(), base = r0 + kb * 32 + 4 * (ln >> 5);
+                const int from = (p.causal ? (key0 + wave * 32 + (ln & 31)) * p.G : 0) - base, to = rows - base;      // rows >= the key's own see it
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
-                    const int r = r0 + kb * 32 + seq_rowmap(i, hh);
-                    if (r < low || r >= rows) s[i] = dp[i] = 0.f;
+                    const int r = seq_rowmap(i, 0);
+                    if (r < from || r >= to) s[i] = dp[i] = 0.f;
                 }
             }
+            frag pf[2], sf[2];
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
-                frag f, g;
-                seq_to_frag(s, t, f);
-                seq_to_frag(dp, t, g);
+                seq_to_frag(s, t, pf[t]);
+                seq_to_frag(dp, t, sf[t]);
+            }
+            fd[0] = A::col(tk + IMG, 0, 0, 0);
+            fq[0] = A::col(tk, 0, 0, 0);
 #pragma unroll
-                for (int cb = 0; cb < NCB; ++cb) {
-                    dv[cb] = seq_mma(seq_frag_t<T, DHP>(Ds, kb * 32, t, cb, lane), f, dv[cb]);
-                    dk[cb] = seq_mma(seq_frag_t<T, DHP>(Qs, kb * 32, t, cb, lane), g, dk[cb]);
+            for (int x = 0; x < 2 * NCB; ++x) {
+                const int t = x / NCB, cb = x % NCB;
+                if (x + 1 < 2 * NCB) {
+                    fd[(x + 1) & 1] = A::col(tk + IMG, 0, (x + 1) / NCB, (x + 1) % NCB);
+                    fq[(x + 1) & 1] = A::col(tk, 0, (x + 1) / NCB, (x + 1) % NCB);
+                    __builtin_amdgcn_sched_barrier(0);
                 }
+                dv[cb] = seq_mma(fd[x & 1], pf[t], dv[cb]);
+                dk[cb] = seq_mma(fq[x & 1], sf[t], dk[cb]);
             }
         }
     }
     if (!kok) return;
     if (part) {
-        float* dst = p.part + (((un.first + un.split) * p.Hkv + hk) * 2 * 128 + wave * 32 + l31) * p.dh;
+        float* dst = p.part + (((un.first + (long)un.split * un.t.ntile) * p.Hkv + hk) * 2 * 128 + wave * 32 + l31) * p.dh;
 #pragma unroll
         for (int cb = 0; cb < NCB; ++cb)
 #pragma unroll
@@ -331,10 +377,10 @@ __global__ __launch_bounds__(256) void seq_dkv_join_kernel(SeqBwdP p) {
     const int key0 = un.t.tile * 128, z0 = (p.causal ? key0 * p.G : 0) / un.per;
     if (un.nsplit - z0 < 2) return;
     const int per = p.dh / 4, keys = min(16, un.t.n - key0 - 16 * (int)blockIdx.y);
-    const long step = 2L * 128 * p.dh * p.Hkv;
+    const long step = 2L * 128 * p.dh * p.Hkv * un.t.ntile;
     for (int i = threadIdx.x; i < 2 * keys * per; i += 256) {
         const int which = i >= keys * per, j = i - which * keys * per, row = 16 * blockIdx.y + j / per, c = (j % per) * 4;
-        const float* src = p.part + (((un.first + z0) * p.Hkv + hk) * 2 * 128 + which * 128 + row) * p.dh + c;
+        const float* src = p.part + (((un.first + (long)z0 * un.t.ntile) * p.Hkv + hk) * 2 * 128 + which * 128 + row) * p.dh + c;
         float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
         for (int z = z0; z < un.nsplit; ++z, src += step) {
@@ -348,19 +394,19 @@ __global__ __launch_bounds__(256) void seq_dkv_join_kernel(SeqBwdP p) {
     }
 }
 
-// Row splits a key head: two workgroups a compute unit in all; none where the key tiles alone are that many.
-static int seq_bwd_slots(int tokens, int Hkv) {
-    const int fill = 512 / Hkv < 1 ? 1 : 512 / Hkv;
+// Row splits a key head, for all key heads together: enough for two workgroups a compute unit; three times that where causal, whose
+// splits are empty to a half and uneven at the ends (8192 tokens of three sequences, 16 / 2 heads of 128: dK / dV pass 384 us at
+// 1536, 450 us at 1024, 410 us at 2048).  None where the key tiles alone are that many.
+static int seq_bwd_slots(int tokens, int Hkv, int causal) {
+    const int all = causal ? 1536 : 512, fill = all / Hkv < 1 ? 1 : all / Hkv;
     return tokens / 128 >= fill ? 0 : fill;
 }
 
 template <typename T, int DHP>
 static void seq_bwd_launch(const SeqBwdP& p, hipStream_t st) {
-    const long rows = (long)p.tokens * p.Hkv * p.G;
-    hipLaunchKernelGGL((seq_delta_kernel<T>), dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, st, p);
+    hipLaunchKernelGGL((seq_attn_dq_kernel<T, DHP>), dim3((unsigned)(seq_units(p.tokens, p.B, p.G, 128) * p.Hkv)), dim3(256), 0, st, p);
     hipLaunchKernelGGL((seq_attn_dkv_kernel<T, DHP>), dim3((unsigned)((p.slots > 0 ? seq_split_units(p.tokens, p.B, 1, 128, p.slots) : seq_units(p.tokens, p.B, 1, 128)) * p.Hkv)), dim3(256), 0, st, p);
     if (p.slots > 0) hipLaunchKernelGGL((seq_dkv_join_kernel<T>), dim3((unsigned)(seq_units(p.tokens, p.B, 1, 128) * p.Hkv), 8), dim3(256), 0, st, p);
-    hipLaunchKernelGGL((seq_attn_dq_kernel<T, DHP>), dim3((unsigned)(seq_units(p.tokens, p.B, p.G, 128) * p.Hkv)), dim3(256), 0, st, p);
 }
 template <typename T>
 static int seq_bwd_route(const SeqBwdP& p, hipStream_t st) {
@@ -371,10 +417,10 @@ static int seq_bwd_route(const SeqBwdP& p, hipStream_t st) {
     return TTSMI_OK;
 }
 
-static size_t seq_delta_bytes(int tokens, int H) { return ((size_t)tokens * H * sizeof(float) + 255) / 256 * 256; }
-extern "C" size_t ttsmi_packed_attention_bwd_ws_bytes(int B, int tokens, int H, int Hkv, int dh) {
+static size_t seq_delta_bytes(int tokens, int H) { return (2 * (size_t)tokens * H * sizeof(float) + 255) / 256 * 256; }     // delta and lse2
+extern "C" size_t ttsmi_packed_attention_bwd_ws_bytes(int B, int tokens, int H, int Hkv, int dh, int causal) {
     if (B < 0 || tokens <= 0 || H <= 0 || Hkv <= 0 || dh <= 0) return 0;
-    const int slots = seq_bwd_slots(tokens, Hkv);
+    const int slots = seq_bwd_slots(tokens, Hkv, causal);
     return seq_delta_bytes(tokens, H) + (slots ? (size_t)seq_split_units(tokens, B, 1, 128, slots) * Hkv * 2 * 128 * dh * sizeof(float) : 0);
 }
 extern "C" int ttsmi_packed_attention_bwd(const void* q, int64_t q_row, int64_t q_head, const void* k, int64_t k_row, int64_t k_head,
@@ -390,7 +436,7 @@ extern "C" int ttsmi_packed_attention_bwd(const void* q, int64_t q_row, int64_t 
                         seq_strides_ok(out, o_row, o_head, dtype) && seq_strides_ok(dout, d_row, d_head, dtype) &&
                         seq_strides_ok(dq, dq_row, dq_head, dtype) && seq_strides_ok(dk, dk_row, dk_head, dtype) &&
                         seq_strides_ok(dv, dv_row, dv_head, dtype), "packed_attention_bwd: a tensor is null or its rows or heads are not 16-byte aligned");
-    const size_t need = ttsmi_packed_attention_bwd_ws_bytes(B, tokens, H, Hkv, dh);
+    const size_t need = ttsmi_packed_attention_bwd_ws_bytes(B, tokens, H, Hkv, dh, causal);
     if (!ws || ws_bytes < need || ((uintptr_t)ws & 15)) {
         ttsmi_set_error("packed_attention_bwd: workspace of %zu bytes, %zu (16-byte aligned) needed", ws_bytes, need);
         return TTSMI_ERR_WORKSPACE;
@@ -399,9 +445,9 @@ extern "C" int ttsmi_packed_attention_bwd(const void* q, int64_t q_row, int64_t 
     p.q = q; p.q_row = q_row; p.q_head = q_head; p.k = k; p.k_row = k_row; p.k_head = k_head; p.v = v; p.v_row = v_row; p.v_head = v_head;
     p.o = out; p.o_row = o_row; p.o_head = o_head; p.d = dout; p.d_row = d_row; p.d_head = d_head;
     p.dq = dq; p.dq_row = dq_row; p.dq_head = dq_head; p.dk = dk; p.dk_row = dk_row; p.dk_head = dk_head; p.dv = dv; p.dv_row = dv_row; p.dv_head = dv_head;
-    p.lse = lse; p.delta = (float*)ws; p.starts = starts; p.B = B; p.tokens = tokens; p.Hkv = Hkv; p.G = H / Hkv; p.dh = dh;
+    p.lse = lse; p.delta = (float*)ws; p.lse2 = (float*)ws + (size_t)tokens * H; p.starts = starts; p.B = B; p.tokens = tokens; p.Hkv = Hkv; p.G = H / Hkv; p.dh = dh;
     p.causal = causal != 0; p.zero_rest = zero_rest != 0; p.scale = scale; p.c1 = scale * SEQ_LOG2E;
-    p.slots = seq_bwd_slots(tokens, Hkv);
+    p.slots = seq_bwd_slots(tokens, Hkv, causal);
     p.part = (float*)((char*)ws + seq_delta_bytes(tokens, H));
     return dtype == TTSMI_F32 ? seq_bwd_route<float>(p, (hipStream_t)stream) : seq_bwd_route<__bf16>(p, (hipStream_t)stream);
 }

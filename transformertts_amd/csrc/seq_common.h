@@ -124,12 +124,13 @@ __device__ __forceinline__ void seq_zero_rest(T* dst, long row, long head, const
 // ---- key splits: units of (sequence, row tile, key range) ---------------------------------------------
 // With few row tiles the keys are split over workgroups.  One split length for the whole call, chosen on the device so that all
 // splits together number about `slots` a key head: long sequences get many, short ones one, and no workgroup has more than
-// one split's keys - the batch is even whatever its lengths.  Units of a sequence: its row tiles, each with its splits in turn.
+// one split's keys - the batch is even whatever its lengths.  Units of a sequence: the first split of all its tiles, then the second ...:
+// workgroups that run together read the same range, through one L2.
 struct SeqUnit {
     SeqTile t;
     int len;                      // keys of the sequence
     int split, nsplit, per;       // key range [split per, (split + 1) per)
-    long first;                   // unit number of the tile's first split
+    long first;                   // unit number of the tile's first split; its next ones follow at steps of ntile
 };
 static inline __host__ __device__ long seq_split_units(long tokens, int B, int G, int R, int slots) { return tokens * G / R + B + 1 + slots; }
 // Tiles: R rows of G a token.  Keys: lens, or `own` times the sequence's tokens where lens is null (the backward's splits of the
@@ -155,7 +156,7 @@ __device__ __forceinline__ SeqUnit find_unit(const int* starts, const int* lens,
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) total += __shfl_xor(total, o, 64);
     const long even = (total + slots - 1) / slots;
-    const int per = (int)min((max(even, (long)least) + quantum - 1) / quantum * quantum, (long)0x7fffff00);
+    const int per = __builtin_amdgcn_readfirstlane((int)min((max(even, (long)least) + quantum - 1) / quantum * quantum, (long)0x7fffff00));
     SeqUnit u;
     u.t.seq = -1; u.t.tile = u.t.ntile = u.t.s0 = u.t.n = 0;
     u.len = u.split = 0; u.nsplit = 1; u.per = per; u.first = 0;
@@ -179,9 +180,9 @@ __device__ __forceinline__ SeqUnit find_unit(const int* starts, const int* lens,
             u.t.n = __builtin_amdgcn_readlane(n, at);
             u.len = __builtin_amdgcn_readlane(len, at);
             u.nsplit = __builtin_amdgcn_readlane(splits, at);
-            u.t.tile = by_tile ? rem : rem / u.nsplit;
-            u.split = by_tile ? 0 : rem - u.t.tile * u.nsplit;
-            u.first = before + __builtin_amdgcn_readlane(all, at) - __builtin_amdgcn_readlane(units, at) + (long)u.t.tile * u.nsplit;
+            u.split = __builtin_amdgcn_readfirstlane(by_tile ? 0 : rem / u.t.ntile);
+            u.t.tile = by_tile ? rem : rem - u.split * u.t.ntile;
+            u.first = before + __builtin_amdgcn_readlane(all, at) - __builtin_amdgcn_readlane(units, at) + u.t.tile;
             return u;
         }
         unit -= __builtin_amdgcn_readlane(upto, 63);
@@ -229,49 +230,125 @@ struct SeqFwdP {
 
 
 // ---- 16-byte chunks of an LDS tile image ----------------------------------------------------------
-// A tile image is [rows][DHP] with the 16-byte chunks of a row permuted by the row number, so that the 32 rows of a fragment
-// read (same chunk, consecutive rows) and the 4 rows of a transposing read fall into different banks without padding.
+// A tile image is [rows][DHP] with the 16-byte chunks of a row permuted by an exclusive-or with swz(row), so that both ways of
+// reading it touch all 64 banks once: a fragment read (one chunk of 16 consecutive rows at a time) needs swz to take 16 different
+// bank places over 16 rows; a transposing read (4 chunks of 4 consecutive rows; of 8-bit elements 2 chunks of rows 0-3 and 8-11;
+// of fp32 8 chunks of two rows 4 apart) needs the high bits of swz to differ between those rows.  With the plain row number in
+// its place four rows of every transposing read met in the same 16 banks: 60 % of the LDS cycles of the bf16 kernels.
 template <typename T, int DHP> struct SeqImg {
     static constexpr int CH = DHP * (int)sizeof(T) / 16;           // chunks per row
     static constexpr int ROWB = DHP * (int)sizeof(T);
-    static constexpr int MASK = CH % 16 == 0 ? 15 : 7;
-    __device__ static __forceinline__ int at(int row, int chunk) { return row * ROWB + ((chunk ^ (row & MASK)) << 4); }   // byte offset
-};
-template <typename T, int DHP>
-__device__ __forceinline__ typename SeqT<T>::frag seq_frag(const unsigned char* img, int row, int step, int hh) {
-    using I = SeqImg<T, DHP>;
-    if constexpr (sizeof(T) == 2) {
-        return *reinterpret_cast<const bf16x8*>(img + I::at(row, 2 * step + hh));
-    } else {
-        const float4 a = *reinterpret_cast<const float4*>(img + I::at(row, 4 * step + 2 * hh));
-        const float4 b = *reinterpret_cast<const float4*>(img + I::at(row, 4 * step + 2 * hh + 1));
-        f32x8 f = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-        return f;
+    __device__ static __forceinline__ int swz(int row) {
+        if constexpr (sizeof(T) == 4) return (row & 3) | ((row >> 1) & 4) | ((row << 1) & 8);            // row bits 0, 1, 3, 2
+        else if constexpr (CH % 16 == 0) return ((row & 3) << 2) | ((row >> 2) & 3);                     // bits 2, 3, 0, 1
+        else if constexpr (CH % 8 == 0) return ((row << 1) & 4) | ((row >> 2) & 2) | ((row >> 2) & 1);   // bits 2, 3, 1 (bit 0 is a half of the banks)
+        else return ((row >> 2) & 2) | ((row >> 2) & 1);                                                 // bits 2, 3
     }
-}
-// The transposed operand: lane holds column cb 32 + l31 of the image, reduction indices k0 + rowmap(8 t + e, hh), e < 8 - the
-// order in which accumulator registers become the other operand.  bf16: two transposing LDS reads (a 16-lane group fetches
-// [4 rows][16 columns] and lane c gets column c).  fp32: eight 4-byte reads, consecutive lanes on consecutive columns.
+    __device__ static __forceinline__ int at(int row, int chunk) { return row * ROWB + ((chunk ^ swz(row)) << 4); }   // byte offset
+};
 typedef short seq_s16x4 __attribute__((ext_vector_type(4)));
 typedef short seq_s16x8 __attribute__((ext_vector_type(8)));
-template <typename T, int DHP>
-__device__ __forceinline__ typename SeqT<T>::frag seq_frag_t(const unsigned char* img, int k0, int t, int cb, int lane) {
+// Fragment addresses.  The chunk number of a step is a constant, so a lane needs ONE base a tile - its row and first chunk,
+// permuted - and flips the constant's low bits into it: (base ^ lo) + rest, the rest an instruction offset.  (Tables of the
+// permuted addresses cost the dK / dV kernel its registers: reloading spilled ones waited for the tile in flight behind them.)
+template <typename T, int DHP> struct SeqLane {
     using I = SeqImg<T, DHP>;
-    if constexpr (sizeof(T) == 2) {
-        typedef __attribute__((address_space(3))) seq_s16x4* lds_ptr;
-        const int row = k0 + 16 * t + 4 * (lane >> 5) + ((lane & 15) >> 2);
-        const int chunk = cb * 4 + ((lane >> 4) & 1) * 2 + ((lane & 3) >> 1), sub = (lane & 1) * 8;
-        const seq_s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(img + I::at(row, chunk) + sub));
-        const seq_s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(img + I::at(row + 8, chunk) + sub));
-        return __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
-    } else {
-        const int c = cb * 32 + (lane & 31), hh = lane >> 5;
-        f32x8 f;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) f[e] = *reinterpret_cast<const float*>(img + I::at(k0 + seq_rowmap(8 * t + e, hh), c >> 2) + (c & 3) * 4);
-        return f;
+    using frag = typename SeqT<T>::frag;
+    static constexpr int LOW = I::CH % 16 == 0 ? 15 : 7;
+    typedef __attribute__((address_space(3))) const unsigned char* lds;
+    // row operand: lane holds image row row0 + l31
+    __device__ static __forceinline__ uint32_t rows(const unsigned char* img, int lane) {
+        const int r = lane & 31, hh = lane >> 5;
+        return (uint32_t)(size_t)(lds)img + r * I::ROWB + (((sizeof(T) == 2 ? hh : 2 * hh) ^ I::swz(r)) << 4);
     }
+    __device__ static __forceinline__ frag row(uint32_t base, int row0, int step) {
+        const int chunk = (sizeof(T) == 2 ? 2 : 4) * step, rest = row0 * I::ROWB + (chunk & ~LOW) * 16;
+        const uint32_t a = base ^ ((chunk & LOW) << 4);
+        if constexpr (sizeof(T) == 2) {
+            return *(__attribute__((address_space(3))) const bf16x8*)(size_t)(a + rest);
+        } else {
+            typedef float f32x4 __attribute__((ext_vector_type(4)));
+            const f32x4 x = *(__attribute__((address_space(3))) const f32x4*)(size_t)(a + rest);
+            const f32x4 y = *(__attribute__((address_space(3))) const f32x4*)(size_t)((a ^ 16) + rest);
+            f32x8 f = {x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
+            return f;
+        }
+    }
+    // The transposed operand: lane holds column cb 32 + l31 of the image, reduction indices k0 + rowmap(8 t + e, hh), e < 8 - the
+    // order in which accumulator registers become the other operand.  bf16: two transposing LDS reads (a 16-lane group fetches
+    // [4 rows][16 columns] and lane c gets column c).  fp32: eight 4-byte reads, consecutive lanes on consecutive columns.
+    __device__ static __forceinline__ uint32_t cols(const unsigned char* img, int lane) {
+        const int hh = lane >> 5;
+        if constexpr (sizeof(T) == 2) {
+            const int r = 4 * hh + ((lane & 15) >> 2);
+            return (uint32_t)(size_t)(lds)img + r * I::ROWB + (((((lane >> 4) & 1) * 2 + ((lane & 3) >> 1)) ^ I::swz(r)) << 4) + (lane & 1) * 8;
+        } else {
+            return (uint32_t)(size_t)(lds)img + 4 * hh * I::ROWB + ((((lane & 31) >> 2) ^ I::swz(4 * hh)) << 4) + (lane & 3) * 4;
+        }
+    }
+    __device__ static __forceinline__ frag col(uint32_t base, int k0, int t, int cb) {
+        if constexpr (sizeof(T) == 2) {
+            typedef __attribute__((address_space(3))) seq_s16x4* tr;
+            const int chunk = 4 * cb, rest = (k0 + 16 * t) * I::ROWB + (chunk & ~LOW) * 16;
+            const uint32_t a = base ^ ((chunk & LOW) << 4);
+            const seq_s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr)(size_t)(a + rest));
+            const seq_s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr)(size_t)((a ^ (I::swz(8) << 4)) + rest + 8 * I::ROWB));
+            return __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+        } else {
+            f32x8 f;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const int r = (e & 3) + 8 * (e >> 2), chunk = 8 * cb, rest = (k0 + 16 * t + r) * I::ROWB + (chunk & ~LOW) * 16;
+                f[e] = *(__attribute__((address_space(3))) const float*)(size_t)((base ^ (((chunk & LOW) ^ I::swz(r)) << 4)) + rest);
+            }
+            return f;
+        }
+    }
+};
+
+// ---- LDS-DMA staging ---------------------------------------------------------------------------------
+// global_load_lds_dwordx4: 64 lanes x 16 bytes to 1 KB of LDS behind a wave-uniform offset, no registers in between.  Inline asm
+// because the compiler orders every LDS read behind a builtin DMA; the kernels wait themselves (vmcnt, then the barrier).
+__device__ __forceinline__ void seq_dma16(const void* base, uint32_t off, unsigned lds) {          // uniform base + lane offset
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(lds) : "memory", "m0");
 }
+__device__ __forceinline__ void seq_dma16(const void* src, unsigned lds) {
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(lds) : "memory", "m0");
+}
+__device__ __forceinline__ void seq_dma4(const void* src, unsigned lds) {
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(src), "s"(lds) : "memory", "m0");
+}
+__device__ __forceinline__ void seq_dma1(const void* src, unsigned lds) {                           // a byte a lane, stored as a dword
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_ubyte %0, off" ::"v"(src), "s"(lds) : "memory", "m0");
+}
+__device__ __forceinline__ unsigned seq_lds(const void* p) { return (unsigned)(size_t)(__attribute__((address_space(3))) const void*)p; }
+// the lane number, formed where it is used: what is derived from it does not stay in registers around a loop
+__device__ __forceinline__ int seq_lane_here() {
+    int l;
+    asm volatile("v_mbcnt_lo_u32_b32 %0, -1, 0\n\tv_mbcnt_hi_u32_b32 %0, -1, %0" : "=v"(l));
+    return l;
+}
+// a value used inside a rarely taken uniform branch: keeps it a branch (its selects would be done every time)
+__device__ __forceinline__ int seq_rare(int v) {
+    asm volatile("" : "+v"(v));
+    return v;
+}
+// this wave's loads have landed and its LDS reads are done, then everybody's
+__device__ __forceinline__ void seq_dma_barrier() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
+// One wave's share of a tile image of ROWS rows: instructions wave, wave + 4, ... of 1 KB each; item i of lane l is image row
+// row(i), and the 16-byte piece of the source row that belongs there (the swizzle is in the source address).  Pieces past
+// dh repeat the row's first one: they meet zeros of the other operand, or end in columns that are not stored.
+template <typename T, int DHP, int ROWS> struct SeqDma {
+    using I = SeqImg<T, DHP>;
+    static constexpr int NI = ROWS * I::CH / 256;                  // instructions a wave
+    __device__ static __forceinline__ int row(int i, int wave, int lane) { return ((wave + 4 * i) * 64 + lane) / I::CH; }
+    __device__ static __forceinline__ uint32_t piece(int i, int wave, int lane, int dh) {
+        const int id = (wave + 4 * i) * 64 + lane, r = id / I::CH, c = ((id - r * I::CH) ^ I::swz(r)) * 16;
+        return c < dh * (int)sizeof(T) ? c : 0;
+    }
+};
+
 // a fragment straight from global memory: elements [c, c + 8) of a row, zeros past dh (dh is a multiple of 8)
 template <typename T>
 __device__ __forceinline__ typename SeqT<T>::frag seq_load8(const T* row, int c, bool ok) {
@@ -281,11 +358,10 @@ __device__ __forceinline__ typename SeqT<T>::frag seq_load8(const T* row, int c,
     for (int e = 0; e < 8; ++e) f[e] = (T)0.f;
     return f;
 }
-// 16 bytes of tile row data in T from a cache of e4m3 bytes (16 / sizeof(T) elements): exact, the scale is a power of two
+// 16 bytes of tile row data in T from 16 / sizeof(T) e4m3 bytes: exact, the scale is a power of two
 template <typename T>
-__device__ __forceinline__ uint4 seq_dequant_chunk(const uint8_t* src, float scale) {
+__device__ __forceinline__ uint4 seq_dequant_chunk(uint2 w, float scale) {
     if constexpr (sizeof(T) == 2) {
-        const uint2 w = *reinterpret_cast<const uint2*>(src);
         bf16x8 o;
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
@@ -296,8 +372,7 @@ __device__ __forceinline__ uint4 seq_dequant_chunk(const uint8_t* src, float sca
         }
         return __builtin_bit_cast(uint4, o);
     } else {
-        const uint32_t v = *reinterpret_cast<const uint32_t*>(src);
-        const f32x2 a = __builtin_amdgcn_cvt_pk_f32_fp8(v, false), b = __builtin_amdgcn_cvt_pk_f32_fp8(v, true);
+        const f32x2 a = __builtin_amdgcn_cvt_pk_f32_fp8(w.x, false), b = __builtin_amdgcn_cvt_pk_f32_fp8(w.x, true);
         const float4 o = make_float4(a[0] * scale, a[1] * scale, b[0] * scale, b[1] * scale);
         return __builtin_bit_cast(uint4, o);
     }

@@ -2145,9 +2145,18 @@ class PlannedDenseStackFn(torch.autograd.Function):
 _SEQ_DTYPES = {torch.float32: TTSMI_F32, torch.bfloat16: _lib.TTSMI_BF16_IO}
 
 
-def _need(ok, message):
-    if not ok:
-        raise _lib.TtsmiError(message)
+# (a decoding step makes three such calls per layer from the host: the checks build their messages only when they fail, and the
+# stream is looked up by its raw handle - torch.cuda.current_stream() costs more than a launch)
+_raw_stream = torch._C._cuda_getCurrentRawStream
+_current_device = torch._C._cuda_getDevice
+
+
+def _seq_stream(device_index):
+    return _PINNED_STREAM if _PINNED_STREAM is not None else _raw_stream(device_index)
+
+
+def _refuse(message):
+    raise _lib.TtsmiError(message)
 
 
 class _Here:
@@ -2179,21 +2188,23 @@ _HERE_GUARD = _Here()
 
 
 def _device_of(t):
-    return _HERE_GUARD if t.device.index == torch.cuda.current_device() else _OnDevice(t.device)
+    return _HERE_GUARD if t.device.index == _current_device() else _OnDevice(t.device)
 
 
-def _seq_check(name, t, like=None, heads=None):
-    _need(isinstance(t, torch.Tensor) and t.dim() == 3, f'{name}: a tensor of [tokens, heads, dh]')
+def _seq_check(name, t, like=None):
+    if not (isinstance(t, torch.Tensor) and t.dim() == 3):
+        _refuse(f'{name}: a tensor of [tokens, heads, dh]')
     _need_gpu(t)
-    _need(t.dtype in _SEQ_DTYPES, f'{name}: {t.dtype} (float32 or bfloat16)')
+    if not (t.dtype in _SEQ_DTYPES):
+        _refuse(f'{name}: {t.dtype} (float32 or bfloat16)')
     if like is not None:
-        _need(t.dtype == like.dtype and t.device == like.device and t.shape[2] == like.shape[2],
-              f'{name}: {tuple(t.shape)} {t.dtype} on {t.device} beside {tuple(like.shape)} {like.dtype} on {like.device}')
+        if not (t.dtype == like.dtype and t.device == like.device and t.shape[2] == like.shape[2]):
+            _refuse(f'{name}: {tuple(t.shape)} {t.dtype} on {t.device} beside {tuple(like.shape)} {like.dtype} on {like.device}')
 
 
 def _ints_check(name, t, device, dim=1):
-    _need(isinstance(t, torch.Tensor) and t.dtype == torch.int32 and t.dim() == dim and t.device == device,
-          f'{name}: {dim}-d int32 on {device}')
+    if not (isinstance(t, torch.Tensor) and t.dtype == torch.int32 and t.dim() == dim and t.device == device):
+        _refuse(f'{name}: {dim}-d int32 on {device}')
     return _c(t)
 
 
@@ -2218,7 +2229,8 @@ def _rs(t):
 
 def _scale_of(scale, dh):
     scale = dh ** -0.5 if scale is None else float(scale)
-    _need(0.0 < scale < float('inf'), f'scale {scale}: positive and finite')
+    if not (0.0 < scale < float('inf')):
+        _refuse(f'scale {scale}: positive and finite')
     return scale
 
 
@@ -2227,7 +2239,7 @@ def _rotary(q, k, qo, ko, positions, freqs, interleaved, scale, inverse):
     none = (None, 0, 0)
     check(_lib.lib().ttsmi_rotary(*_rs(q), *_rs(qo), q.shape[1], *(none if k is None else _rs(k)), *(none if k is None else _rs(ko)),
                                   0 if k is None else k.shape[1], positions.data_ptr(), freqs.data_ptr(), q.shape[0], q.shape[2],
-                                  2 * freqs.numel(), int(interleaved), scale, int(inverse), _SEQ_DTYPES[q.dtype], _stream()), 'rotary')
+                                  2 * freqs.numel(), int(interleaved), scale, int(inverse), _SEQ_DTYPES[q.dtype], _seq_stream(q.device.index)), 'rotary')
 
 
 class RotaryFn(torch.autograd.Function):
@@ -2235,7 +2247,7 @@ class RotaryFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, q, k, positions, freqs, interleaved, scale):
-        ctx.stream_h = _stream()
+        ctx.stream_h = _seq_stream(q.device.index)
         ctx.save_for_backward(positions, freqs)
         ctx.cfg = (interleaved, scale)
         ctx.set_materialize_grads(False)
@@ -2265,20 +2277,25 @@ def rotary(q, k, positions, freqs, interleaved=False, scale=1.0, inplace=False):
     (2 i, 2 i + 1) if interleaved and (i, i + len(freqs)) otherwise, times scale; the rest passes through.  -> (q, k).
     inplace: q and k themselves, without gradients."""
     _seq_check('rotary: q', q)
-    _need(freqs.dtype == torch.float64 and freqs.dim() == 1 and freqs.device == q.device, f'rotary: freqs: 1-d float64 on {q.device}')
-    _need(2 * freqs.numel() <= q.shape[2] and q.shape[2] % 2 == 0 and freqs.numel() <= 256,
-          f'rotary: {freqs.numel()} pairs in a head of {q.shape[2]} elements (even; at most 256 pairs)')
+    if not (freqs.dtype == torch.float64 and freqs.dim() == 1 and freqs.device == q.device):
+        _refuse(f'rotary: freqs: 1-d float64 on {q.device}')
+    if not (2 * freqs.numel() <= q.shape[2] and q.shape[2] % 2 == 0 and freqs.numel() <= 256):
+        _refuse(f'rotary: {freqs.numel()} pairs in a head of {q.shape[2]} elements (even; at most 256 pairs)')
     positions = _ints_check('rotary: positions', positions, q.device)
-    _need(positions.numel() == q.shape[0], f'rotary: {positions.numel()} positions for {q.shape[0]} tokens')
+    if not (positions.numel() == q.shape[0]):
+        _refuse(f'rotary: {positions.numel()} positions for {q.shape[0]} tokens')
     if k is not None:
         _seq_check('rotary: k', k, q)
-        _need(k.shape[0] == q.shape[0], f'rotary: {q.shape[0]} queries and {k.shape[0]} keys')
+        if not (k.shape[0] == q.shape[0]):
+            _refuse(f'rotary: {q.shape[0]} queries and {k.shape[0]} keys')
     freqs, scale = _c(freqs), float(scale)
     grad = torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad))
     with _device_of(q):
         if inplace:
-            _need(not grad, 'rotary: in place on a tensor that wants a gradient')
-            _need(q.stride(2) == 1 and (k is None or k.stride(2) == 1), 'rotary: in place needs a contiguous last dimension')
+            if not (not grad):
+                _refuse('rotary: in place on a tensor that wants a gradient')
+            if not (q.stride(2) == 1 and (k is None or k.stride(2) == 1)):
+                _refuse('rotary: in place needs a contiguous last dimension')
             _rotary(q, k, q, k, positions, freqs, interleaved, scale, False)
             return q, k
         q, k = _strided(q, aligned=False), None if k is None else _strided(k, aligned=False)
@@ -2297,7 +2314,7 @@ def _packed_fwd(q, k, v, starts, scale, causal, want_lse):
     out = torch.empty((M, H, dh), dtype=q.dtype, device=q.device)
     lse = torch.empty((Hkv, M, H // Hkv), dtype=torch.float32, device=q.device) if want_lse else None
     check(_lib.lib().ttsmi_packed_attention_fwd(*_rs(q), *_rs(k), *_rs(v), starts.data_ptr(), starts.numel() - 1, M, H, Hkv, dh, scale,
-                                                int(causal), *_rs(out), _p(lse), 1, _SEQ_DTYPES[q.dtype], _stream()),
+                                                int(causal), *_rs(out), _p(lse), 1, _SEQ_DTYPES[q.dtype], _seq_stream(q.device.index)),
           'packed_attention_fwd')
     return out, lse
 
@@ -2307,7 +2324,7 @@ class PackedAttentionFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, q, k, v, starts, scale, causal):
-        ctx.stream_h = _stream()
+        ctx.stream_h = _seq_stream(q.device.index)
         out, lse = _packed_fwd(q, k, v, starts, scale, causal, True)
         ctx.save_for_backward(q, k, v, out, lse, starts)
         ctx.cfg = (scale, causal)
@@ -2327,10 +2344,10 @@ class PackedAttentionFn(torch.autograd.Function):
         with _device_of(q), pin_stream(ctx.stream_h):
             dout = _strided(dout)
             dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
-            ws = _ws(l.ttsmi_packed_attention_bwd_ws_bytes(starts.numel() - 1, M, H, k.shape[1], dh), q.device)
+            ws = _ws(l.ttsmi_packed_attention_bwd_ws_bytes(starts.numel() - 1, M, H, k.shape[1], dh, int(causal)), q.device)
             check(l.ttsmi_packed_attention_bwd(*_rs(q), *_rs(k), *_rs(v), *_rs(out), *_rs(dout), lse.data_ptr(), starts.data_ptr(),
                                                starts.numel() - 1, M, H, k.shape[1], dh, scale, int(causal), *_rs(dq), *_rs(dk),
-                                               *_rs(dv), 1, ws.data_ptr(), ws.numel(), _SEQ_DTYPES[q.dtype], _stream()),
+                                               *_rs(dv), 1, ws.data_ptr(), ws.numel(), _SEQ_DTYPES[q.dtype], _seq_stream(q.device.index)),
                   'packed_attention_bwd')
         return dq, dk, dv, None, None, None
 
@@ -2344,11 +2361,13 @@ def packed_attention(q, k, v, starts, causal=True, scale=None):
     _seq_check('packed_attention: q', q)
     _seq_check('packed_attention: k', k, q)
     _seq_check('packed_attention: v', v, q)
-    _need(k.shape == v.shape and k.shape[0] == q.shape[0] and k.shape[1] > 0 and q.shape[1] % k.shape[1] == 0,
-          f'packed_attention: q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}')
-    _need(q.shape[2] % 8 == 0 and 0 < q.shape[2] <= 192, f'packed_attention: head size {q.shape[2]} (a multiple of 8 up to 192)')
+    if not (k.shape == v.shape and k.shape[0] == q.shape[0] and k.shape[1] > 0 and q.shape[1] % k.shape[1] == 0):
+        _refuse(f'packed_attention: q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}')
+    if not (q.shape[2] % 8 == 0 and 0 < q.shape[2] <= 192):
+        _refuse(f'packed_attention: head size {q.shape[2]} (a multiple of 8 up to 192)')
     starts = _ints_check('packed_attention: starts', starts, q.device)
-    _need(starts.numel() > 0, 'packed_attention: starts holds the end of the last sequence at least')
+    if not (starts.numel() > 0):
+        _refuse('packed_attention: starts holds the end of the last sequence at least')
     scale = _scale_of(scale, q.shape[2])
     with _device_of(q):
         q, k, v = _strided(q), _strided(k), _strided(v)
@@ -2369,19 +2388,22 @@ class KVCache:
     __slots__ = ('k', 'v', 'k_exp', 'v_exp', 'args', 'heads', 'dh', 'page_size', 'dtype', 'device')
 
     def __init__(self, k, v, k_exp=None, v_exp=None):
-        _need(k.dim() == 4 and k.shape == v.shape and k.dtype == v.dtype and k.device == v.device and k.dtype in _CACHE_DTYPES,
-              f'KVCache: pages {tuple(k.shape)} {k.dtype} and {tuple(v.shape)} {v.dtype}')
+        if not (k.dim() == 4 and k.shape == v.shape and k.dtype == v.dtype and k.device == v.device and k.dtype in _CACHE_DTYPES):
+            _refuse(f'KVCache: pages {tuple(k.shape)} {k.dtype} and {tuple(v.shape)} {v.dtype}')
         n, self.heads, self.page_size, self.dh = k.shape
-        _need(0 < self.page_size <= 1024 and self.page_size & (self.page_size - 1) == 0 and self.heads > 0,
-              f'KVCache: pages of {self.page_size} rows (a power of two up to 1024)')
-        _need(self.dh % 8 == 0 and 0 < self.dh <= 192, f'KVCache: head size {self.dh} (a multiple of 8 up to 192)')
+        if not (0 < self.page_size <= 1024 and self.page_size & (self.page_size - 1) == 0 and self.heads > 0):
+            _refuse(f'KVCache: pages of {self.page_size} rows (a power of two up to 1024)')
+        if not (self.dh % 8 == 0 and 0 < self.dh <= 192):
+            _refuse(f'KVCache: head size {self.dh} (a multiple of 8 up to 192)')
         quantised = k.dtype == torch.float8_e4m3fn
-        _need((k_exp is not None and v_exp is not None) == quantised, 'KVCache: float8_e4m3fn pages, and only they, have exponents')
+        if not ((k_exp is not None and v_exp is not None) == quantised):
+            _refuse('KVCache: float8_e4m3fn pages, and only they, have exponents')
         for t in (k_exp, v_exp) if quantised else ():
-            _need(t.shape == k.shape[:3] and t.dtype == torch.uint8 and t.device == k.device and t.is_contiguous(),
-                  f'KVCache: exponents {tuple(t.shape)} {t.dtype} of pages {tuple(k.shape)}')
+            if not (t.shape == k.shape[:3] and t.dtype == torch.uint8 and t.device == k.device and t.is_contiguous()):
+                _refuse(f'KVCache: exponents {tuple(t.shape)} {t.dtype} of pages {tuple(k.shape)}')
         _need_gpu(k)
-        _need(k.is_contiguous() and v.is_contiguous() and (k.data_ptr() | v.data_ptr()) % 16 == 0, 'KVCache: contiguous, 16-byte aligned pages')
+        if not (k.is_contiguous() and v.is_contiguous() and (k.data_ptr() | v.data_ptr()) % 16 == 0):
+            _refuse('KVCache: contiguous, 16-byte aligned pages')
         self.k, self.v, self.k_exp, self.v_exp, self.dtype, self.device = k, v, k_exp, v_exp, k.dtype, k.device
         self.args = (k.data_ptr(), v.data_ptr(), _p(k_exp), _p(v_exp), _CACHE_DTYPES[k.dtype], n, self.page_size)
 
@@ -2397,20 +2419,22 @@ class KVCache:
 
 
 def _paged_check(name, cache, table, starts, lens):
-    _need(isinstance(cache, KVCache), f'{name}: a KVCache')
+    if not (isinstance(cache, KVCache)):
+        _refuse(f'{name}: a KVCache')
     table, starts = _ints_check(f'{name}: table', table, cache.device, 2), _ints_check(f'{name}: starts', starts, cache.device)
     lens = _ints_check(f'{name}: lens', lens, cache.device)
-    _need(starts.numel() == lens.numel() + 1 and table.shape[0] == lens.numel(),
-          f'{name}: {starts.numel()} starts, {lens.numel()} lens, table {tuple(table.shape)}')
+    if not (starts.numel() == lens.numel() + 1 and table.shape[0] == lens.numel()):
+        _refuse(f'{name}: {starts.numel()} starts, {lens.numel()} lens, table {tuple(table.shape)}')
     return table, starts, lens
 
 
 def _kv_check(name, cache, k, v):
     _seq_check(f'{name}: k', k)
     _seq_check(f'{name}: v', v, k)
-    _need(k.shape == v.shape and k.shape[1] == cache.heads and k.shape[2] == cache.dh and k.device == cache.device,
-          f'{name}: k {tuple(k.shape)}, v {tuple(v.shape)} on {k.device}; pages {tuple(cache.k.shape)} on {cache.device}')
-    _need(cache.dtype in (k.dtype, torch.float8_e4m3fn), f'{name}: {k.dtype} beside pages of {cache.dtype}')
+    if not (k.shape == v.shape and k.shape[1] == cache.heads and k.shape[2] == cache.dh and k.device == cache.device):
+        _refuse(f'{name}: k {tuple(k.shape)}, v {tuple(v.shape)} on {k.device}; pages {tuple(cache.k.shape)} on {cache.device}')
+    if not (cache.dtype in (k.dtype, torch.float8_e4m3fn)):
+        _refuse(f'{name}: {k.dtype} beside pages of {cache.dtype}')
 
 
 def kv_cache_write(cache, k, v, table, starts, lens):
@@ -2423,7 +2447,7 @@ def kv_cache_write(cache, k, v, table, starts, lens):
         k, v = _strided(k), _strided(v)
         check(_lib.lib().ttsmi_kv_cache_write(*_rs(k), *_rs(v), *cache.args, table.data_ptr(), table.shape[1], starts.data_ptr(),
                                               lens.data_ptr(), lens.numel(), k.shape[0], cache.heads, cache.dh, _SEQ_DTYPES[k.dtype],
-                                              _stream()), 'kv_cache_write')
+                                              _seq_stream(k.device.index)), 'kv_cache_write')
 
 
 def kv_cache_read(cache, table, lens, starts, tokens, dtype=None, out=None):
@@ -2436,12 +2460,13 @@ def kv_cache_read(cache, table, lens, starts, tokens, dtype=None, out=None):
         k, v = (torch.empty((int(tokens), cache.heads, cache.dh), dtype=dtype, device=cache.device) for _ in 'kv')
     else:
         k, v = out
-        _need(k.shape[0] == tokens and _strided(k) is k and _strided(v) is v, f'kv_cache_read: out of {tokens} tokens on 16-byte boundaries')
+        if not (k.shape[0] == tokens and _strided(k) is k and _strided(v) is v):
+            _refuse(f'kv_cache_read: out of {tokens} tokens on 16-byte boundaries')
     _kv_check('kv_cache_read', cache, k, v)
     with _device_of(k):
         check(_lib.lib().ttsmi_kv_cache_read(*cache.args, table.data_ptr(), table.shape[1], starts.data_ptr(), lens.data_ptr(), lens.numel(),
                                              k.shape[0], cache.heads, cache.dh, *_rs(k), *_rs(v), int(out is None), _SEQ_DTYPES[k.dtype],
-                                             _stream()), 'kv_cache_read')
+                                             _seq_stream(k.device.index)), 'kv_cache_read')
     return k, v
 
 
@@ -2452,14 +2477,15 @@ def paged_attention(q, cache, table, starts, lens, scale=None, out=None):
     _seq_check('paged_attention: q', q)
     table, starts, lens = _paged_check('paged_attention', cache, table, starts, lens)
     M, H, dh = q.shape
-    _need(dh == cache.dh and H % cache.heads == 0 and H > 0 and q.device == cache.device and cache.dtype in (q.dtype, torch.float8_e4m3fn),
-          f'paged_attention: q {tuple(q.shape)} {q.dtype} on {q.device}; pages {tuple(cache.k.shape)} {cache.dtype} on {cache.device}')
-    _need(not (torch.is_grad_enabled() and q.requires_grad), 'paged_attention: has no gradient')
+    if not (dh == cache.dh and H % cache.heads == 0 and H > 0 and q.device == cache.device and cache.dtype in (q.dtype, torch.float8_e4m3fn)):
+        _refuse(f'paged_attention: q {tuple(q.shape)} {q.dtype} on {q.device}; pages {tuple(cache.k.shape)} {cache.dtype} on {cache.device}')
+    if not (not (torch.is_grad_enabled() and q.requires_grad)):
+        _refuse('paged_attention: has no gradient')
     scale = _scale_of(scale, dh)
     given = out is not None
     if given:
-        _need(out.shape == q.shape and out.dtype == q.dtype and out.device == q.device and _strided(out) is out,
-              f'paged_attention: out {tuple(out.shape)} {out.dtype} for q {tuple(q.shape)} {q.dtype}, on 16-byte boundaries')
+        if not (out.shape == q.shape and out.dtype == q.dtype and out.device == q.device and _strided(out) is out):
+            _refuse(f'paged_attention: out {tuple(out.shape)} {out.dtype} for q {tuple(q.shape)} {q.dtype}, on 16-byte boundaries')
     l = _lib.lib()
     with _device_of(q):
         q = _strided(q)
@@ -2468,5 +2494,5 @@ def paged_attention(q, cache, table, starts, lens, scale=None, out=None):
         ws = _ws(need, q.device) if need else None
         check(l.ttsmi_paged_attention(*_rs(q), *cache.args, table.data_ptr(), table.shape[1], starts.data_ptr(), lens.data_ptr(),
                                       lens.numel(), M, H, cache.heads, dh, scale, *_rs(out), int(not given), _p(ws),
-                                      0 if ws is None else ws.numel(), _SEQ_DTYPES[q.dtype], _stream()), 'paged_attention')
+                                      0 if ws is None else ws.numel(), _SEQ_DTYPES[q.dtype], _seq_stream(q.device.index)), 'paged_attention')
     return out
