@@ -859,7 +859,7 @@ int ttsmi_kv_cache_read(const void* k_pages, const void* v_pages, const uint8_t*
 /* Attention of the packed new tokens over the cache (their own keys and values written before): token i of sequence b, n of
  * them, is at position lens[b] - n + i and sees the keys up to it.  A token that sees none gets zeros.  The keys are split over
  * workgroups by the lengths found on the device; the sums of the splits pass through ws. */
-size_t ttsmi_paged_attention_ws_bytes(int B, int tokens, int H, int Hkv, int dh, int cache_dtype);
+size_t ttsmi_paged_attention_ws_bytes(int B, int tokens, int H, int Hkv, int dh, int cache_dtype, int dtype);
 int ttsmi_paged_attention(const void* q, int64_t q_row, int64_t q_head, const void* k_pages, const void* v_pages,
                           const uint8_t* k_exp, const uint8_t* v_exp, int cache_dtype, int n_pages, int page_size,
                           const int32_t* table, int table_width, const int32_t* starts, const int32_t* lens, int B, int tokens,

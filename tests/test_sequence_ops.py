@@ -81,13 +81,13 @@ def test_cache_entries_refuse(lib, name, over, word):
 
 
 def test_paged_attention_workspace(lib):
-    need = lib.ttsmi_paged_attention_ws_bytes(2, 10, 4, 2, 64, E4M3)
+    need = lib.ttsmi_paged_attention_ws_bytes(2, 10, 4, 2, 64, E4M3, BF16)
     assert need >= 2 * 10 * 4 * 66 * 4                                       # a few rows over a long cache are split
     order = _ORDERS['ttsmi_paged_attention']
     for over in (dict(ws=None), dict(ws_bytes=need - 1), dict(ws=ODD)):
         assert lib.ttsmi_paged_attention(*_cache_args(order, **over)) == -4 and b'workspace' in lib.ttsmi_last_error()
-    assert lib.ttsmi_paged_attention_ws_bytes(1, 1 << 16, 32, 8, 128, BF16) == 0          # tiles that fill the card are not
-    assert lib.ttsmi_paged_attention_ws_bytes(0, 0, 4, 2, 64, BF16) == 0 and lib.ttsmi_paged_attention_ws_bytes(1, 1, 4, 0, 64, BF16) == 0
+    assert lib.ttsmi_paged_attention_ws_bytes(1, 1 << 16, 32, 8, 128, BF16, BF16) == 0          # tiles that fill the card are not
+    assert lib.ttsmi_paged_attention_ws_bytes(0, 0, 4, 2, 64, BF16, BF16) == 0 and lib.ttsmi_paged_attention_ws_bytes(1, 1, 4, 0, 64, BF16, BF16) == 0
     for over in (dict(scale=0.0), dict(H=3), dict(out=None)):
         assert lib.ttsmi_paged_attention(*_cache_args(order, **over)) == -1
 

@@ -145,7 +145,7 @@ SIGNATURES = {
         L, P, L, L, P, L, L, I, P, c_size_t, I, S]),
     'ttsmi_kv_cache_write': (I, [P, L, L, P, L, L, P, P, P, P, I, I, I, P, I, P, P, I, I, I, I, I, S]),
     'ttsmi_kv_cache_read': (I, [P, P, P, P, I, I, I, P, I, P, P, I, I, I, I, P, L, L, P, L, L, I, I, S]),
-    'ttsmi_paged_attention_ws_bytes': (c_size_t, [I, I, I, I, I, I]),
+    'ttsmi_paged_attention_ws_bytes': (c_size_t, [I, I, I, I, I, I, I]),
     'ttsmi_paged_attention': (I, [P, L, L, P, P, P, P, I, I, I, P, I, P, P, I, I, I, I, I, F, P, L, L, I, P,
         c_size_t, I, S]),
 }

@@ -36,27 +36,29 @@ __device__ __forceinline__ void pg_cvt8(uint2 w, float scale, f32x8& f) {
     }
 }
 
-// waves and stages: as much in flight as the 160 KB of a compute unit hold, at most 63 counted loads
-template <typename CT, int DHP> struct PgCfg {
+// Waves a SIMD (WPS), waves a workgroup and stages: as much in flight as the 160 KB of a compute unit hold, at most 63 counted
+// loads.  The bytes of an e4m3 block are half, so two waves a SIMD have room: one converts and multiplies while the other waits.
+template <typename T, typename CT, int DHP> struct PgCfg {
     static constexpr int ROWB = DHP * (int)sizeof(CT), BLOCK = 2 * 32 * ROWB;          // bytes of a block's keys and values
-    static constexpr int NW = BLOCK <= 16384 ? 4 : BLOCK <= 32768 ? 2 : 1;
-    static constexpr int FIT = 147456 / (NW * BLOCK);
-    static constexpr int NBUF = FIT > 4 ? 4 : BLOCK > 32768 ? 2 : FIT;
+    static constexpr int WPS = sizeof(CT) == 1 && sizeof(T) == 2 && DHP <= 128 ? 2 : 1;
+    static constexpr int NW = BLOCK <= 16384 ? 2 : 1;
+    static constexpr int FIT = 36864 / (WPS * BLOCK), NBUF = FIT > 4 ? 4 : FIT < 2 ? 2 : FIT;
+    static constexpr int STAGES = NW * NBUF * BLOCK, JOIN = NW * 32 * (DHP + 4) * 4, MAIN = STAGES > JOIN ? STAGES : JOIN;
+    static constexpr int SIDE = NW * NBUF * 256 * (sizeof(CT) == 1 ? 2 : 1), LDS = MAIN + SIDE + NW * 256 + 256;
+    static constexpr int BY_LDS = 163840 / LDS, BY_WAVES = 4 * WPS / NW, RESIDENT = BY_LDS < BY_WAVES ? BY_LDS : BY_WAVES;   // workgroups a compute unit
 };
 
 template <typename T, typename CT, int DHP>
-__global__ __launch_bounds__((64 * PgCfg<CT, DHP>::NW), 1) void paged_rows_kernel(SeqFwdP p) {
-    using C = PgCfg<CT, DHP>;
+__global__ __launch_bounds__((64 * PgCfg<T, CT, DHP>::NW), (PgCfg<T, CT, DHP>::WPS)) void paged_rows_kernel(SeqFwdP p) {
+    using C = PgCfg<T, CT, DHP>;
     using frag = typename SeqT<T>::frag;
     constexpr bool Q8 = sizeof(CT) == 1;
     constexpr int NW = C::NW, NBUF = C::NBUF, ROWB = C::ROWB, CH = ROWB / 16;
     using I = SeqImg<CT, DHP>;
     using A = SeqLane<T, DHP>;
     constexpr int NI = 32 * CH / 64, PER = 2 * NI + 1 + (Q8 ? 1 : 0), NS = DHP / 16, NCB = DHP / 32;
-    constexpr int STAGES = NW * NBUF * C::BLOCK, SIDE = NW * NBUF * 256;
-    constexpr int JOIN = NW * 32 * (DHP + 4) * 4;
-    constexpr int MAIN = STAGES > JOIN ? STAGES : JOIN;
-    __shared__ __attribute__((aligned(1024))) unsigned char sm[MAIN + (Q8 ? 2 : 1) * SIDE + NW * 256 + 256];
+    constexpr int MAIN = C::MAIN, SIDE = NW * NBUF * 256;
+    __shared__ __attribute__((aligned(1024))) unsigned char sm[C::LDS];
     const int lane = threadIdx.x & 63, l31 = lane & 31, hh = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     unsigned char* const mine = sm + wave * NBUF * C::BLOCK;
@@ -299,12 +301,19 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PgJoinP j) {
             m = top;
             acc.x *= a; acc.y *= a; acc.z *= a; acc.w *= a;
             const int n = min(64, un.nsplit - z0);
-#pragma unroll 8
-            for (int z = 0; z < n; z += NG) {
-                const float wz = __shfl(w, (z + g) & 63, 64);                               // (0 past the last split)
-                if (c < p.dh && wz != 0.f) {                                                // (an empty split left its rows unwritten)
-                    const float4 b = *reinterpret_cast<const float4*>(p.part_o + (base + (z0 + z + g) * step) * p.dh + c);
-                    acc.x += wz * b.x; acc.y += wz * b.y; acc.z += wz * b.z; acc.w += wz * b.w;
+            // eight loads at a time, of every split: an empty one left its rows unwritten, its values are dropped, not its load
+            for (int z = 0; z < n; z += 8 * NG) {
+                float4 b[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    b[i] = *reinterpret_cast<const float4*>(p.part_o + (base + (z0 + min(z + i * NG + g, n - 1)) * step) * p.dh + (c < p.dh ? c : 0));
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const int at = z + i * NG + g;
+                    const float wz = __shfl(w, at & 63, 64);
+                    const bool live = at < n && wz != 0.f;
+                    acc.x += live ? wz * b[i].x : 0.f; acc.y += live ? wz * b[i].y : 0.f;
+                    acc.z += live ? wz * b[i].z : 0.f; acc.w += live ? wz * b[i].w : 0.f;
                 }
             }
         }
@@ -336,9 +345,18 @@ static bool pg_rows_form(int B, int tokens, int G, int dh, int cache_dtype) {
     const int size = cache_dtype == TTSMI_F32 ? 4 : cache_dtype == TTSMI_E4M3 ? 1 : 2;
     return (long)tokens * G <= 32L * B && dh * size % 16 == 0;
 }
-// Key splits a key head: two workgroups a compute unit for all heads together; none where the tiles alone fill the card.
-static int pg_slots(int B, int tokens, int Hkv, int G, bool rows_form) {
-    const int fill = 512 / Hkv < 1 ? 1 : 512 / Hkv;
+// Key splits a key head: together as many workgroups as the card holds at once; none where the tiles alone fill it.
+template <typename T, typename CT>
+static int pg_resident(int dh) {
+    return 256 * (dh <= 64 ? PgCfg<T, CT, 64>::RESIDENT : dh <= 128 ? PgCfg<T, CT, 128>::RESIDENT : PgCfg<T, CT, 192>::RESIDENT);
+}
+static int pg_slots(int B, int tokens, int Hkv, int G, int dh, bool rows_form, int cache_dtype, int dtype) {
+    int all = 1024;
+    if (rows_form) {
+        if (dtype == TTSMI_F32) all = cache_dtype == TTSMI_E4M3 ? pg_resident<float, uint8_t>(dh) : pg_resident<float, float>(dh);
+        else all = cache_dtype == TTSMI_E4M3 ? pg_resident<__bf16, uint8_t>(dh) : pg_resident<__bf16, __bf16>(dh);
+    }
+    const int fill = all / Hkv < 1 ? 1 : all / Hkv;
     return !rows_form && (long)tokens * G / 128 >= fill ? 0 : fill;
 }
 template <typename T, typename CT>
@@ -346,7 +364,7 @@ static void pg_rows_launch(const SeqFwdP& p, PgJoinP& j, hipStream_t st) {
     const dim3 g((unsigned)(seq_split_units(p.tokens, p.B, p.G, 32, p.slots) * p.Hkv));
 #define PG_GO(D)                                                                                                           \
     do {                                                                                                                   \
-        constexpr int NW = PgCfg<CT, D>::NW;                                                                               \
+        constexpr int NW = PgCfg<T, CT, D>::NW;                                                                               \
         j.quantum = 32 * NW; j.least = 64 * NW;                                                                            \
         hipLaunchKernelGGL((paged_rows_kernel<T, CT, D>), g, dim3(64 * NW), 0, st, p);                                     \
     } while (0)
@@ -356,11 +374,11 @@ static void pg_rows_launch(const SeqFwdP& p, PgJoinP& j, hipStream_t st) {
 #undef PG_GO
 }
 
-extern "C" size_t ttsmi_paged_attention_ws_bytes(int B, int tokens, int H, int Hkv, int dh, int cache_dtype) {
+extern "C" size_t ttsmi_paged_attention_ws_bytes(int B, int tokens, int H, int Hkv, int dh, int cache_dtype, int dtype) {
     if (B < 0 || tokens <= 0 || H <= 0 || Hkv <= 0 || dh <= 0) return 0;
     const int G = H / Hkv;
     const bool rows_form = pg_rows_form(B, tokens, G, dh, cache_dtype);
-    const int slots = pg_slots(B, tokens, Hkv, G, rows_form), R = rows_form ? 32 : 128;
+    const int slots = pg_slots(B, tokens, Hkv, G, dh, rows_form, cache_dtype, dtype), R = rows_form ? 32 : 128;
     return slots == 0 ? 0 : (size_t)seq_split_units(tokens, B, G, R, slots) * Hkv * R * (dh + 2) * sizeof(float);
 }
 extern "C" int ttsmi_paged_attention(const void* q, int64_t q_row, int64_t q_head, const void* k_pages, const void* v_pages,
@@ -380,7 +398,7 @@ extern "C" int ttsmi_paged_attention(const void* q, int64_t q_row, int64_t q_hea
     p.pg.k = k_pages; p.pg.v = v_pages; p.pg.ke = k_exp; p.pg.ve = v_exp; p.pg.table = table; p.pg.table_width = table_width;
     p.pg.n_pages = n_pages; p.pg.shift = __builtin_ctz(page_size); p.pg.heads = Hkv; p.pg.dh = dh;
     p.B = B; p.tokens = tokens; p.Hkv = Hkv; p.G = H / Hkv; p.dh = dh; p.causal = 1; p.c1 = scale * SEQ_LOG2E; p.zero_rest = zero_rest != 0;
-    const size_t need = ttsmi_paged_attention_ws_bytes(B, tokens, H, Hkv, dh, cache_dtype);
+    const size_t need = ttsmi_paged_attention_ws_bytes(B, tokens, H, Hkv, dh, cache_dtype, dtype);
     if (need && (!ws || ws_bytes < need || ((uintptr_t)ws & 15))) {
         ttsmi_set_error("paged_attention: workspace of %zu bytes, %zu (16-byte aligned) needed", ws_bytes, need);
         return TTSMI_ERR_WORKSPACE;
@@ -388,7 +406,7 @@ extern "C" int ttsmi_paged_attention(const void* q, int64_t q_row, int64_t q_hea
     bool rows_form = pg_rows_form(B, tokens, p.G, dh, cache_dtype);
     PgJoinP j = {};
     j.R = rows_form ? 32 : 128; j.quantum = dtype == TTSMI_F32 ? 32 : 64; j.least = SEQ_TILE_LEAST;
-    p.slots = pg_slots(B, tokens, Hkv, p.G, rows_form);
+    p.slots = pg_slots(B, tokens, Hkv, p.G, dh, rows_form, cache_dtype, dtype);
     if (p.slots > 0) {
         p.part_o = (float*)ws;
         p.part_ml = (float*)ws + (size_t)seq_split_units(tokens, B, p.G, j.R, p.slots) * Hkv * j.R * dh;

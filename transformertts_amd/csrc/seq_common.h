@@ -63,6 +63,18 @@ __device__ __forceinline__ float seq_half_sum(float v) {
     return a + b;
 }
 
+// inclusive prefix sum over the wave in eight vector instructions (row shifts, then the row totals carried up); lane 63 has the sum
+__device__ __forceinline__ int seq_scan_add(int v) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);              // row_shr:1, 2, 4, 8 within rows of 16
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);              // row_bcast:15 into rows 1 and 3
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);              // row_bcast:31 into rows 2 and 3
+    return v;
+}
+__device__ __forceinline__ int seq_wave_total(int v) { return __builtin_amdgcn_readlane(seq_scan_add(v), 63); }
+
 // ---- which tile of which sequence ------------------------------------------------------------------
 struct SeqTile {
     int seq, tile, ntile;         // seq < 0: this workgroup has none
@@ -83,12 +95,7 @@ __device__ __forceinline__ SeqTile find_tile(const int* starts, int B, int token
             n = min(max(starts[b + 1], s0), tokens) - s0;
         }
         const int tiles = (int)(((long)n * G + rows_per_tile - 1) / rows_per_tile);
-        int upto = tiles;                                          // inclusive prefix sum over the wave
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const int v = __shfl_up(upto, o, 64);
-            if (lane >= o) upto += v;
-        }
+        const int upto = seq_scan_add(tiles);
         const uint64_t hit = __ballot(upto > unit);
         if (hit) {
             const int at = __builtin_amdgcn_readfirstlane(__builtin_ctzll(hit));
@@ -138,7 +145,7 @@ static inline __host__ __device__ long seq_split_units(long tokens, int B, int G
 __device__ __forceinline__ SeqUnit find_unit(const int* starts, const int* lens, int own, int B, int tokens, int G, int R, int slots,
                                              int quantum, int least, int unit, bool by_tile) {
     const int lane = threadIdx.x & 63;
-    long total = 0;
+    float total = 0.f;
     int s0 = 0, n = 0, len = 0, tiles = 0;
     auto look = [&](int b) {
         s0 = n = len = 0;
@@ -151,25 +158,37 @@ __device__ __forceinline__ SeqUnit find_unit(const int* starts, const int* lens,
     };
     for (int b0 = 0; b0 < B; b0 += 64) {
         look(b0 + lane);
-        total += (long)tiles * len;
+        total += (float)tiles * (float)len;
     }
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) total += __shfl_xor(total, o, 64);
-    const long even = (total + slots - 1) / slots;
-    const int per = __builtin_amdgcn_readfirstlane((int)min((max(even, (long)least) + quantum - 1) / quantum * quantum, (long)0x7fffff00));
+    total = wave_sum_dpp(total) * (1.f + 0x1p-16f);                  // (never short of the true sum: the grid is sized by it)
+    long per_l = max((long)(total / (float)slots) + 1, (long)least);
+    per_l = min((per_l + quantum - 1) / quantum * quantum, 0x7fffff00l / quantum * quantum);
+    int per = __builtin_amdgcn_readfirstlane((int)per_l);
+    if (lens) {
+        // Every sequence's last split is a partial one: lengthen the splits until the units really fit the slots (a few units more
+        // would run alone in a second round), or the sequences' tiles alone are most of them.
+        for (int it = 0; it < 8; ++it) {
+            int units = 0, all = 0;
+            for (int b0 = 0; b0 < B; b0 += 64) {
+                if (B > 64) look(b0 + lane);
+                units += tiles * max((int)(((long)len + per - 1) / per), 1);
+                all += tiles;
+            }
+            units = seq_wave_total(units);
+            all = seq_wave_total(all);
+            if (units <= max(slots, all + all / 2) || per >= 0x3fffff00) break;
+            const int more = (int)min((long)per * (units - slots) / max(units, 1) / 2, 0x3fffff00l);
+            per = __builtin_amdgcn_readfirstlane(per + max(more / quantum, 1) * quantum);
+        }
+    }
     SeqUnit u;
     u.t.seq = -1; u.t.tile = u.t.ntile = u.t.s0 = u.t.n = 0;
     u.len = u.split = 0; u.nsplit = 1; u.per = per; u.first = 0;
     long before = 0;
     for (int b0 = 0; b0 < B; b0 += 64) {
         if (B > 64) look(b0 + lane);                               // (the only 64 are still in registers)
-        const int splits = max((len + per - 1) / per, 1), units = tiles * splits, counted = by_tile ? tiles : units;
-        int upto = counted, all = units;
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const int v = __shfl_up(upto, o, 64), w = __shfl_up(all, o, 64);
-            if (lane >= o) { upto += v; all += w; }
-        }
+        const int splits = max((int)(((long)len + per - 1) / per), 1), units = tiles * splits, counted = by_tile ? tiles : units;
+        const int upto = seq_scan_add(counted), all = by_tile ? seq_scan_add(units) : upto;
         const uint64_t hit = __ballot(upto > unit);
         if (hit) {
             const int at = __builtin_amdgcn_readfirstlane(__builtin_ctzll(hit));

@@ -2257,7 +2257,6 @@ class RotaryFn(torch.autograd.Function):
         return qo, ko
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dq, dk):
         positions, freqs = ctx.saved_tensors
         grads = [None, None]
@@ -2320,7 +2319,7 @@ def _packed_fwd(q, k, v, starts, scale, causal, want_lse):
 
 
 class PackedAttentionFn(torch.autograd.Function):
-    """softmax(scale q k^T) v within packed sequences, grouped heads (ttsmi_packed_attention_fwd / _bwd).  Returns (out, lse)."""
+    """softmax(scale q k^T) v within packed sequences, grouped heads (ttsmi_packed_attention_fwd / _bwd)."""
 
     @staticmethod
     def forward(ctx, q, k, v, starts, scale, causal):
@@ -2328,13 +2327,11 @@ class PackedAttentionFn(torch.autograd.Function):
         out, lse = _packed_fwd(q, k, v, starts, scale, causal, True)
         ctx.save_for_backward(q, k, v, out, lse, starts)
         ctx.cfg = (scale, causal)
-        ctx.mark_non_differentiable(lse)
         ctx.set_materialize_grads(False)
-        return out, lse
+        return out
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dout, _dlse):
+    def backward(ctx, dout):
         if dout is None:
             return (None,) * 6
         q, k, v, out, lse, starts = ctx.saved_tensors
@@ -2343,7 +2340,7 @@ class PackedAttentionFn(torch.autograd.Function):
         l = _lib.lib()
         with _device_of(q), pin_stream(ctx.stream_h):
             dout = _strided(dout)
-            dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
+            dq, dk, dv = torch.empty_like(out), torch.empty(k.shape, dtype=k.dtype, device=k.device), torch.empty(v.shape, dtype=v.dtype, device=v.device)
             ws = _ws(l.ttsmi_packed_attention_bwd_ws_bytes(starts.numel() - 1, M, H, k.shape[1], dh, int(causal)), q.device)
             check(l.ttsmi_packed_attention_bwd(*_rs(q), *_rs(k), *_rs(v), *_rs(out), *_rs(dout), lse.data_ptr(), starts.data_ptr(),
                                                starts.numel() - 1, M, H, k.shape[1], dh, scale, int(causal), *_rs(dq), *_rs(dk),
@@ -2372,7 +2369,7 @@ def packed_attention(q, k, v, starts, causal=True, scale=None):
     with _device_of(q):
         q, k, v = _strided(q), _strided(k), _strided(v)
         if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
-            return PackedAttentionFn.apply(q, k, v, starts, scale, bool(causal))[0]
+            return PackedAttentionFn.apply(q, k, v, starts, scale, bool(causal))
         return _packed_fwd(q, k, v, starts, scale, causal, False)[0]
 
 
@@ -2490,7 +2487,7 @@ def paged_attention(q, cache, table, starts, lens, scale=None, out=None):
     with _device_of(q):
         q = _strided(q)
         out = out if given else torch.empty((M, H, dh), dtype=q.dtype, device=q.device)
-        need = l.ttsmi_paged_attention_ws_bytes(lens.numel(), M, H, cache.heads, dh, _CACHE_DTYPES[cache.dtype])
+        need = l.ttsmi_paged_attention_ws_bytes(lens.numel(), M, H, cache.heads, dh, _CACHE_DTYPES[cache.dtype], _SEQ_DTYPES[q.dtype])
         ws = _ws(need, q.device) if need else None
         check(l.ttsmi_paged_attention(*_rs(q), *cache.args, table.data_ptr(), table.shape[1], starts.data_ptr(), lens.data_ptr(),
                                       lens.numel(), M, H, cache.heads, dh, scale, *_rs(out), int(not given), _p(ws),
