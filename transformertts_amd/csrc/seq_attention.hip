@@ -11,11 +11,12 @@
 #include "seq_common.h"
 
 // CT: the cache's element type for PAGED (T, or uint8_t = e4m3)
-template <typename T, typename CT, int DHP, bool PAGED>
+template <typename T, typename CT, int DHP, bool PAGED, int KS = 1>
 __global__ __launch_bounds__(256, (DHP <= 128 && sizeof(T) == 2) ? 2 : 1) void seq_attn_fwd_kernel(SeqFwdP p) {
     using I = SeqImg<T, DHP>;
     using frag = typename SeqT<T>::frag;
-    constexpr int KT = SeqT<T>::KT, NKB = KT / 32, NS = DHP / 16, NCB = DHP / 32, EPC = 16 / (int)sizeof(T);
+    constexpr int KW = SeqKeys<T, DHP, KS>::KW, KT = KW * KS, NKB = KW / 32, NS = DHP / 16, NCB = DHP / 32;
+    constexpr int ROWS = 128 / KS;
     using D = SeqDma<T, DHP, KT>;
     constexpr bool Q8 = PAGED && sizeof(CT) == 1;
     constexpr int IMG = KT * I::ROWB, ITEMS = D::NI;      // 16-byte pieces a lane and tile image
@@ -29,9 +30,9 @@ __global__ __launch_bounds__(256, (DHP <= 128 && sizeof(T) == 2) ? 2 : 1) void s
         if (p.slots > 0) un = find_unit(p.starts, p.lens, 1, p.B, p.tokens, p.G, 128, p.slots, KT, SEQ_TILE_LEAST, unit, false);
     }
     const bool splits = PAGED && p.slots > 0;
-    const SeqTile st = splits ? un.t : find_tile(p.starts, p.B, p.tokens, p.G, 128, unit);
+    const SeqTile st = splits ? un.t : find_tile(p.starts, p.B, p.tokens, p.G, ROWS, unit);
     if (st.seq < 0) {
-        if (p.zero_rest) seq_zero_rest<T>((T*)p.o, p.o_row, p.o_head, p.starts, p.B, p.tokens, p.G, 128, hk * p.G, p.dh, st.tile);
+        if (p.zero_rest) seq_zero_rest<T>((T*)p.o, p.o_row, p.o_head, p.starts, p.B, p.tokens, p.G, ROWS, hk * p.G, p.dh, st.tile);
         return;
     }
     const int tile = splits ? st.tile : st.ntile - 1 - st.tile;              // causal: the tiles with the most keys first
@@ -42,19 +43,19 @@ __global__ __launch_bounds__(256, (DHP <= 128 && sizeof(T) == 2) ? 2 : 1) void s
         off = len - st.n;                                 // position of the first new token
     }
     // this lane's row and the number of keys it sees
-    const int r = tile * 128 + wave * 32 + l31;
+    const int half = KS == 2 ? wave >> 1 : 0, wrow = tile * ROWS + (KS == 2 ? wave & 1 : wave) * 32;
+    const int r = wrow + l31;
     const bool rok = r < rows;
     const int tok = r / p.G, head = hk * p.G + r - tok * p.G;
     const int lim = !rok ? 0 : p.causal ? min(max(off + tok + 1, 0), len) : len;
     // the same for the workgroup's last row, and for this wave's: no key behind is fetched / multiplied
-    const int last = min(tile * 128 + 127, rows - 1) / p.G;
+    const int last = min(tile * ROWS + ROWS - 1, rows - 1) / p.G;
     int kend = p.causal ? min(max(off + last + 1, 0), len) : len, kbeg = 0;
     const bool part = splits && un.nsplit > 1;
     if (part) {
         kbeg = min(un.split * un.per, kend);
         kend = min(kbeg + un.per, kend);
     }
-    const int wrow = tile * 128 + wave * 32;
     const int wlast = min(wrow + 31, rows - 1) / p.G;
     const int wend = wrow >= rows ? 0 : min(kend, p.causal ? max(off + wlast + 1, 0) : len);
     const int wfull = wrow + 31 < rows ? (p.causal ? off + wrow / p.G + 1 : len) : 0;     // keys that every row of the wave sees
@@ -187,7 +188,7 @@ __global__ __launch_bounds__(256, (DHP <= 128 && sizeof(T) == 2) ? 2 : 1) void s
         if (kbeg + KT < kend) look(kbeg + KT);
     }
     using A = SeqLane<T, DHP>;
-    const uint32_t kbase = A::rows(sm, lane), vbase = A::cols(sm + IMG, lane);
+    const uint32_t kbase = A::rows(sm, lane) + half * KW * I::ROWB, vbase = A::cols(sm + IMG, lane) + half * KW * I::ROWB;
     int buf = 0;
     for (int k0 = kbeg; k0 < kend; k0 += KT, buf ^= 1) {
         land(buf);
@@ -195,7 +196,8 @@ __global__ __launch_bounds__(256, (DHP <= 128 && sizeof(T) == 2) ? 2 : 1) void s
             fetch(k0 + KT, buf ^ 1);
             look(k0 + 2 * KT);
         }
-        if (k0 >= wend) continue;
+        const int kw = k0 + half * KW;                    // this wave's keys of the tile
+        if (kw >= wend) continue;
         const uint32_t ka = kbase + buf * 2 * IMG, va = vbase + buf * 2 * IMG;
         f32x16 s[NKB];
 #pragma unroll
@@ -205,8 +207,8 @@ __global__ __launch_bounds__(256, (DHP <= 128 && sizeof(T) == 2) ? 2 : 1) void s
 #pragma unroll
             for (int t = 0; t < NS; ++t) s[kb] = seq_mma(A::row(ka, kb * 32, t), qf[t], s[kb]);
         }
-        if (k0 + KT > wfull || k0 + KT > kend) {
-            const int seen = seq_rare(min(lim, kend) - k0);
+        if (kw + KW > wfull || kw + KW > kend) {
+            const int seen = seq_rare(min(lim, kend) - kw);
 #pragma unroll
             for (int kb = 0; kb < NKB; ++kb)
 #pragma unroll
@@ -249,6 +251,32 @@ __global__ __launch_bounds__(256, (DHP <= 128 && sizeof(T) == 2) ? 2 : 1) void s
             }
     }
     l = seq_half_sum(l);
+    if constexpr (KS == 2) {                              // the two halves of the keys: the second wave of a row block hands over
+        constexpr int LDO = DHP + 4;
+        float* const mo = reinterpret_cast<float*>(sm) + (wave & 1) * 32 * (LDO + 2) + l31 * (LDO + 2);
+        seq_dma_barrier();
+        if (half == 1) {
+            if (hh == 0) *reinterpret_cast<float2*>(mo + LDO) = make_float2(m, l);
+#pragma unroll
+            for (int cb = 0; cb < NCB; ++cb)
+#pragma unroll
+                for (int g = 0; g < 4; ++g)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e)
+                        *reinterpret_cast<float2*>(mo + cb * 32 + 8 * g + 4 * hh + 2 * e) = make_float2(o[cb][4 * g + 2 * e], o[cb][4 * g + 2 * e + 1]);
+        }
+        __syncthreads();
+        if (half == 1) return;
+        const float2 other = *reinterpret_cast<const float2*>(mo + LDO);
+        const float mn = fmaxf(m, other.x), ms = mn == -INFINITY ? 0.f : mn;
+        const float a = __builtin_amdgcn_exp2f(m - ms), b = __builtin_amdgcn_exp2f(other.x - ms);
+        m = mn;
+        l = l * a + other.y * b;
+#pragma unroll
+        for (int cb = 0; cb < NCB; ++cb)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[cb][i] = o[cb][i] * a + mo[cb * 32 + 8 * (i >> 2) + 4 * hh + (i & 3)] * b;
+    }
     if (!rok) return;
     const long slot = (long)hk * p.tokens * p.G + (long)st.s0 * p.G + r;
     if (part) {
@@ -287,21 +315,39 @@ __global__ __launch_bounds__(256, (DHP <= 128 && sizeof(T) == 2) ? 2 : 1) void s
 
 // ---- launches -----------------------------------------------------------------------------------------
 
-template <typename T, typename CT, bool PAGED>
-static int seq_fwd_launch(const SeqFwdP& p, hipStream_t st) {
+template <typename T, typename CT, int DHP, bool PAGED, int KS>
+static void seq_fwd_go(const SeqFwdP& p, long units, hipStream_t st) {
+    hipLaunchKernelGGL((seq_attn_fwd_kernel<T, CT, DHP, PAGED, KS>), dim3((unsigned)(units * p.Hkv)), dim3(256), 0, st, p);
+}
+template <typename T>
+static int seq_packed_launch(const SeqFwdP& p, hipStream_t st) {
+    const bool two = seq_two_halves(p.tokens, p.B, p.G, p.Hkv, p.dh, sizeof(T) == 4);
+    const long units = seq_units(p.tokens, p.B, p.G, two ? 64 : 128);
+    if (two) {
+        if (p.dh <= 64) seq_fwd_go<T, T, 64, false, 2>(p, units, st);
+        else if (p.dh <= 128) seq_fwd_go<T, T, 128, false, 2>(p, units, st);
+        else if constexpr (sizeof(T) == 2) seq_fwd_go<T, T, 192, false, 2>(p, units, st);
+    } else if (p.dh <= 64) seq_fwd_go<T, T, 64, false, 1>(p, units, st);
+    else if (p.dh <= 128) seq_fwd_go<T, T, 128, false, 1>(p, units, st);
+    else seq_fwd_go<T, T, 192, false, 1>(p, units, st);
+    ttsmi_note_kernel(two ? "seq_attn_fwd_kernel, two halves" : "seq_attn_fwd_kernel");
+    TTSMI_CHECK_LAUNCH("packed_attention_fwd");
+    return TTSMI_OK;
+}
+template <typename T, typename CT>
+static int seq_paged_launch(const SeqFwdP& p, hipStream_t st) {
     const long units = p.slots > 0 ? seq_split_units(p.tokens, p.B, p.G, 128, p.slots) : seq_units(p.tokens, p.B, p.G, 128);
-    const dim3 g((unsigned)(units * p.Hkv));
-    if (p.dh <= 64) hipLaunchKernelGGL((seq_attn_fwd_kernel<T, CT, 64, PAGED>), g, dim3(256), 0, st, p);
-    else if (p.dh <= 128) hipLaunchKernelGGL((seq_attn_fwd_kernel<T, CT, 128, PAGED>), g, dim3(256), 0, st, p);
-    else hipLaunchKernelGGL((seq_attn_fwd_kernel<T, CT, 192, PAGED>), g, dim3(256), 0, st, p);
-    TTSMI_CHECK_LAUNCH("seq_attention");
+    if (p.dh <= 64) seq_fwd_go<T, CT, 64, true, 1>(p, units, st);
+    else if (p.dh <= 128) seq_fwd_go<T, CT, 128, true, 1>(p, units, st);
+    else seq_fwd_go<T, CT, 192, true, 1>(p, units, st);
+    TTSMI_CHECK_LAUNCH("paged_attention");
     return TTSMI_OK;
 }
 // the tile form of the paged attention (paged_attention.hip)
 int seq_paged_tiles(const SeqFwdP& p, int dtype, int cache_dtype, hipStream_t st) {
     if (dtype == TTSMI_F32)
-        return cache_dtype == TTSMI_E4M3 ? seq_fwd_launch<float, uint8_t, true>(p, st) : seq_fwd_launch<float, float, true>(p, st);
-    return cache_dtype == TTSMI_E4M3 ? seq_fwd_launch<__bf16, uint8_t, true>(p, st) : seq_fwd_launch<__bf16, __bf16, true>(p, st);
+        return cache_dtype == TTSMI_E4M3 ? seq_paged_launch<float, uint8_t>(p, st) : seq_paged_launch<float, float>(p, st);
+    return cache_dtype == TTSMI_E4M3 ? seq_paged_launch<__bf16, uint8_t>(p, st) : seq_paged_launch<__bf16, __bf16>(p, st);
 }
 
 extern "C" int ttsmi_packed_attention_fwd(const void* q, int64_t q_row, int64_t q_head, const void* k, int64_t k_row, int64_t k_head,
@@ -317,5 +363,5 @@ extern "C" int ttsmi_packed_attention_fwd(const void* q, int64_t q_row, int64_t 
     p.q = q; p.q_row = q_row; p.q_head = q_head; p.k = k; p.k_row = k_row; p.k_head = k_head; p.v = v; p.v_row = v_row; p.v_head = v_head;
     p.o = out; p.zero_rest = zero_rest != 0; p.o_row = o_row; p.o_head = o_head; p.lse = lse; p.starts = starts;
     p.B = B; p.tokens = tokens; p.Hkv = Hkv; p.G = H / Hkv; p.dh = dh; p.causal = causal != 0; p.c1 = scale * SEQ_LOG2E;
-    return dtype == TTSMI_F32 ? seq_fwd_launch<float, float, false>(p, (hipStream_t)stream) : seq_fwd_launch<__bf16, __bf16, false>(p, (hipStream_t)stream);
+    return dtype == TTSMI_F32 ? seq_packed_launch<float>(p, (hipStream_t)stream) : seq_packed_launch<__bf16>(p, (hipStream_t)stream);
 }

@@ -27,7 +27,7 @@ struct SeqBwdP {
     int slots; float* part;
 };
 // rows of a split at least: eight tiles of work against the traffic of its partial sums (bf16); the fp32 products are slower
-template <typename T> struct SeqLeast { static constexpr int ROWS = sizeof(T) == 2 ? 512 : 128; };
+template <typename T> struct SeqLeast { static constexpr int ROWS = sizeof(T) == 2 ? 512 : 192; };
 
 // four accumulator registers -> four consecutive elements of a gradient row
 template <typename T>
@@ -42,30 +42,30 @@ __device__ __forceinline__ void seq_store4(T* dst, const f32x16& a, int g, float
     }
 }
 
-template <typename T, int DHP>
+template <typename T, int DHP, int KS>
 __global__ __launch_bounds__(256, (DHP <= 128 && sizeof(T) == 2) ? 2 : 1) void seq_attn_dq_kernel(SeqBwdP p) {
     using I = SeqImg<T, DHP>;
     using frag = typename SeqT<T>::frag;
-    constexpr int KT = SeqT<T>::KT, NKB = KT / 32, NS = DHP / 16, NCB = DHP / 32;
+    constexpr int KW = SeqKeys<T, DHP, KS>::KW, KT = KW * KS, NKB = KW / 32, NS = DHP / 16, NCB = DHP / 32, ROWS = 128 / KS;
     using D = SeqDma<T, DHP, KT>;
     constexpr int IMG = KT * I::ROWB, ITEMS = D::NI;
     __shared__ __attribute__((aligned(1024))) unsigned char sm[4 * IMG];             // two stages of a K and a V tile
     const int tid = threadIdx.x, lane = tid & 63, l31 = lane & 31, hh = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int hk = blockIdx.x % p.Hkv, unit = blockIdx.x / p.Hkv;
-    const SeqTile st = find_tile(p.starts, p.B, p.tokens, p.G, 128, unit);
+    const SeqTile st = find_tile(p.starts, p.B, p.tokens, p.G, ROWS, unit);
     if (st.seq < 0) {
-        if (p.zero_rest) seq_zero_rest<T>((T*)p.dq, p.dq_row, p.dq_head, p.starts, p.B, p.tokens, p.G, 128, hk * p.G, p.dh, st.tile);
+        if (p.zero_rest) seq_zero_rest<T>((T*)p.dq, p.dq_row, p.dq_head, p.starts, p.B, p.tokens, p.G, ROWS, hk * p.G, p.dh, st.tile);
         return;
     }
     const int tile = st.ntile - 1 - st.tile, rows = st.n * p.G, len = st.n;
-    const int r = tile * 128 + wave * 32 + l31;
+    const int half = KS == 2 ? wave >> 1 : 0, wrow = tile * ROWS + (KS == 2 ? wave & 1 : wave) * 32;
+    const int r = wrow + l31;
     const bool rok = r < rows;
     const int tok = r / p.G, head = hk * p.G + r - tok * p.G;
     const int lim = !rok ? 0 : p.causal ? min(tok + 1, len) : len;
-    const int last = min(tile * 128 + 127, rows - 1) / p.G;
+    const int last = min(tile * ROWS + ROWS - 1, rows - 1) / p.G;
     const int kend = p.causal ? min(last + 1, len) : len;
-    const int wrow = tile * 128 + wave * 32;
     const int wend = wrow >= rows ? 0 : p.causal ? min(kend, min(wrow + 31, rows - 1) / p.G + 1) : kend;
     const int wfull = wrow + 31 < rows ? (p.causal ? wrow / p.G + 1 : len) : 0;
     const long slot = (long)hk * p.tokens * p.G + (long)st.s0 * p.G + r;
@@ -93,7 +93,7 @@ __global__ __launch_bounds__(256, (DHP <= 128 && sizeof(T) == 2) ? 2 : 1) void s
         }
     }
     delta = seq_half_sum(delta);
-    if (rok && hh == 0) {
+    if (rok && hh == 0 && half == 0) {
         p.delta[slot] = delta;
         p.lse2[slot] = lse2;
     }
@@ -126,17 +126,18 @@ __global__ __launch_bounds__(256, (DHP <= 128 && sizeof(T) == 2) ? 2 : 1) void s
     };
     fetch(0, 0);
     using A = SeqLane<T, DHP>;
-    const uint32_t kbase = A::rows(sm, lane), tbase = A::cols(sm, lane);
+    const uint32_t kbase = A::rows(sm, lane) + half * KW * I::ROWB, tbase = A::cols(sm, lane) + half * KW * I::ROWB;
     int buf = 0;
     for (int k0 = 0; k0 < kend; k0 += KT, buf ^= 1) {
         seq_dma_barrier();
         if (k0 + KT < kend) fetch(k0 + KT, buf ^ 1);
-        if (k0 >= wend) continue;
+        const int kw = k0 + half * KW;                                 // this wave's keys of the tile
+        if (kw >= wend) continue;
         const uint32_t ka = kbase + buf * 2 * IMG, ta = tbase + buf * 2 * IMG;
-        const bool edge = k0 + KT > wfull;
+        const bool edge = kw + KW > wfull;
 #pragma unroll
         for (int kb = 0; kb < NKB; ++kb) {
-            if (k0 + kb * 32 >= wend) break;
+            if (kw + kb * 32 >= wend) break;
             f32x16 s, dp;
 #pragma unroll
             for (int i = 0; i < 16; ++i) s[i] = dp[i] = 0.f;
@@ -148,7 +149,7 @@ __global__ __launch_bounds__(256, (DHP <= 128 && sizeof(T) == 2) ? 2 : 1) void s
 #pragma unroll
             for (int i = 0; i < 16; ++i) s[i] = __builtin_amdgcn_exp2f(s[i] * p.c1 - lse2) * (dp[i] - delta);
             if (edge) {
-                const int seen = seq_rare(lim - k0 - kb * 32);
+                const int seen = seq_rare(lim - kw - kb * 32);
 #pragma unroll
                 for (int i = 0; i < 16; ++i)
                     if (seq_rowmap(i, hh) >= seen) s[i] = 0.f;
@@ -161,6 +162,22 @@ __global__ __launch_bounds__(256, (DHP <= 128 && sizeof(T) == 2) ? 2 : 1) void s
                 for (int cb = 0; cb < NCB; ++cb) acc[cb] = seq_mma(A::col(ta, kb * 32, t, cb), f, acc[cb]);
             }
         }
+    }
+    if constexpr (KS == 2) {
+        float* const mo = reinterpret_cast<float*>(sm) + ((wave & 1) * 32 + l31) * (DHP + 4) + 4 * hh;
+        seq_dma_barrier();
+        if (half == 1) {
+#pragma unroll
+            for (int cb = 0; cb < NCB; ++cb)
+#pragma unroll
+                for (int g = 0; g < 4; ++g) seq_store4<float>(mo + cb * 32 + 8 * g, acc[cb], g, 1.f);
+        }
+        __syncthreads();
+        if (half == 1) return;
+#pragma unroll
+        for (int cb = 0; cb < NCB; ++cb)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) acc[cb][i] += mo[cb * 32 + 8 * (i >> 2) + (i & 3)];
     }
     if (!rok) return;
     T* dst = (T*)p.dq + (long)(st.s0 + tok) * p.dq_row + (long)head * p.dq_head;
@@ -404,7 +421,13 @@ static int seq_bwd_slots(int tokens, int Hkv, int causal) {
 
 template <typename T, int DHP>
 static void seq_bwd_launch(const SeqBwdP& p, hipStream_t st) {
-    hipLaunchKernelGGL((seq_attn_dq_kernel<T, DHP>), dim3((unsigned)(seq_units(p.tokens, p.B, p.G, 128) * p.Hkv)), dim3(256), 0, st, p);
+    // the dQ pass divides its tiles as the forward does
+    const bool two = seq_two_halves(p.tokens, p.B, p.G, p.Hkv, p.dh, sizeof(T) == 4);
+    const dim3 g((unsigned)(seq_units(p.tokens, p.B, p.G, two ? 64 : 128) * p.Hkv));
+    if constexpr (sizeof(T) == 2 || DHP <= 128) {
+        if (two) hipLaunchKernelGGL((seq_attn_dq_kernel<T, DHP, 2>), g, dim3(256), 0, st, p);
+    }
+    if (!two) hipLaunchKernelGGL((seq_attn_dq_kernel<T, DHP, 1>), g, dim3(256), 0, st, p);
     hipLaunchKernelGGL((seq_attn_dkv_kernel<T, DHP>), dim3((unsigned)((p.slots > 0 ? seq_split_units(p.tokens, p.B, 1, 128, p.slots) : seq_units(p.tokens, p.B, 1, 128)) * p.Hkv)), dim3(256), 0, st, p);
     if (p.slots > 0) hipLaunchKernelGGL((seq_dkv_join_kernel<T>), dim3((unsigned)(seq_units(p.tokens, p.B, 1, 128) * p.Hkv), 8), dim3(256), 0, st, p);
 }

@@ -231,6 +231,19 @@ struct SeqPages {
 // 2^(e - 127) of a stored exponent byte (0 and 255 are not written by the cache kernels)
 __device__ __forceinline__ float seq_scale_of(uint32_t e) { return __builtin_bit_cast(float, e << 23); }
 
+// ---- few tiles: two halves of the keys --------------------------------------------------------------
+// With 128 rows a workgroup, 32 a wave, a small batch leaves most of the card idle and its time is one wave's walk over a whole
+// sequence.  Then (KS = 2) a workgroup takes 64 rows, and two waves share a row block: each meets every other KW keys of the tiles,
+// and their sums are joined through LDS at the end.  KW: keys of a wave's step; a stage of KS KW keys has to fit twice.
+template <typename T, int DHP, int KS> struct SeqKeys {
+    static constexpr int KW = KS == 2 && DHP > 128 ? 32 : SeqT<T>::KT;
+};
+// where the tiles of 128 rows are fewer than the compute units (fp32 heads above 128 have no room for it)
+static inline bool seq_two_halves(long tokens, int B, int G, int Hkv, int dh, bool f32) {
+    const long tiles = (tokens * G / 128 + (B + 1) / 2) * Hkv;
+    return tiles < 256 && !(f32 && dh > 128);
+}
+
 // ---- what a forward launch takes ----
 #define SEQ_TILE_LEAST 256           // keys of a split, tile form: at least four tiles
 struct SeqFwdP {
