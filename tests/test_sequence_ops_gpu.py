@@ -114,6 +114,24 @@ def test_packed_attention(lens, H, Hkv, dh, causal, dtype):
         assert torch.equal(ops.packed_attention(*xs, _starts(lens).to(DEV), causal=causal), got[0])
 
 
+@pytest.mark.parametrize('dtype,lens,H,Hkv,dh,causal', [
+    (torch.bfloat16, [1100, 0, 3, 1001], 16, 16, 64, True), (torch.bfloat16, [650, 490], 32, 32, 128, True), (torch.bfloat16, [1030, 65], 32, 32, 192, False),
+    (torch.float32, [900, 350], 32, 32, 64, True), (torch.float32, [700, 450], 32, 32, 128, False), (torch.float32, [600], 64, 64, 184, True),
+    (torch.bfloat16, [1100], 64, 64, 8, False), (torch.float32, [900, 700], 128, 128, 8, True), (torch.bfloat16, [700, 33], 96, 12, 72, True)])
+def test_packed_attention_many_tiles(dtype, lens, H, Hkv, dh, causal):
+    """Batches that fill the card: a wave meets every key of its tiles, and key tiles enough for the dK / dV pass not to split rows."""
+    from transformertts_amd import _lib
+    ops = _ops()
+    M = sum(lens)
+    q, k, v, d = (_randn((M, h, dh), 50 + i, dtype) for i, h in enumerate((H, Hkv, Hkv, H)))
+    want, bound = packed_oracle(q, k, v, lens, causal, dh ** -0.5, d)
+    xs = [x.to(DEV).requires_grad_() for x in (q, k, v)]
+    out = ops.packed_attention(*xs, _starts(lens).to(DEV), causal=causal)
+    assert _lib.lib().ttsmi_last_kernel() == b'seq_attn_fwd_kernel'
+    for name, g, w, b in zip(('out', 'dq', 'dk', 'dv'), _grads(out, xs, d.to(DEV)), want, bound):
+        _within(g, w, b, name)
+
+
 def test_packed_attention_scale_and_peaked_scores():
     """Scores of some hundreds: the running maximum carries them, forward and backward stay finite and right."""
     ops = _ops()
@@ -467,8 +485,10 @@ def test_cache_offsets_past_32_bits():
 @pytest.mark.parametrize('new,lens,page,H,Hkv,dh', [
     ([1], [1], 16, 1, 1, 8), ([1] * 5, [1, 700, 64, 65, 1023], 16, 8, 2, 128), ([1, 1], [5000, 3], 64, 4, 4, 64), ([1, 1, 1], [300, 17, 90], 8, 32, 2, 64),
     ([70, 1, 200], [300, 513, 200], 32, 4, 2, 64), ([129], [129], 1, 2, 1, 192), ([3, 0, 40], [1000, 20, 1040], 128, 6, 3, 80), ([17] * 9, [17 + 31 * i for i in range(9)], 16, 16, 2, 128),
-    ([2, 3, 1, 4], [2000, 999, 640, 641], 64, 8, 1, 192)])
+    ([2, 3, 1, 4], [2000, 999, 640, 641], 64, 8, 1, 192), ([1] * 150, [1 + 7 * i for i in range(150)], 8, 4, 2, 32), ([1], [20000], 64, 2, 1, 64),
+    ([300], [310], 16, 512, 32, 8), ([40, 90], [700, 90], 32, 4, 2, 24)])
 def test_paged_attention(new, lens, page, H, Hkv, dh, quantise, dtype):
+    from transformertts_amd import _lib
     ops = _ops()
     p = Paged(lens, page, Hkv, dh, dtype, torch.float8_e4m3fn if quantise else dtype)
     q = _randn((sum(new), H, dh), 9, dtype, 1.5)
@@ -485,6 +505,8 @@ def test_paged_attention(new, lens, page, H, Hkv, dh, quantise, dtype):
     want, bound = torch.cat(want), torch.cat(bound)
     _within(got, want, bound, 'out')
     assert torch.equal(got, ops.paged_attention(q.to(DEV), p.cache, table, st, ln))
+    rows = sum(new) * (H // Hkv) <= 32 * len(new) and dh * p.cache.k.element_size() % 16 == 0
+    assert _lib.lib().ttsmi_last_kernel() == (b'paged_rows_kernel' if rows else b'seq_attn_fwd_kernel')
 
 
 def test_paged_attention_rows_that_see_nothing_and_bad_pages():

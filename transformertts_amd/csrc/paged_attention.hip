@@ -167,7 +167,7 @@ __global__ __launch_bounds__((64 * PgCfg<T, CT, DHP>::NW), (PgCfg<T, CT, DHP>::W
 #pragma unroll
             for (int i = 1; i < 16; ++i) mx = fmaxf(mx, s[i]);
             mx = seq_half_max(mx) * p.c1;
-            if (__ballot(mx > m)) {                                                         // a new maximum is rare behind the first blocks
+            if (__ballot(mx > m + 8.f)) {                                                   // 8 binary digits of slack, as in the tile kernels
                 const float mn = fmaxf(m, mx), a = __builtin_amdgcn_exp2f(m - (mn == -INFINITY ? 0.f : mn));
                 m = mn;
                 l *= a;
