@@ -2159,14 +2159,6 @@ def _refuse(message):
     raise _lib.TtsmiError(message)
 
 
-class _Here:
-    def __enter__(self):
-        return self
-
-    def __exit__(self, *exc):
-        return False
-
-
 class _OnDevice:
     """Another GPU than the current one: launches inside go to that GPU's current stream."""
 
@@ -2184,47 +2176,37 @@ class _OnDevice:
         return self.device.__exit__(*exc)
 
 
-_HERE_GUARD = _Here()
-
-
-def _device_of(t):
-    return _HERE_GUARD if t.device.index == _current_device() else _OnDevice(t.device)
-
-
 def _seq_check(name, t, like=None):
-    if not (isinstance(t, torch.Tensor) and t.dim() == 3):
+    if not isinstance(t, torch.Tensor) or t.dim() != 3:
         _refuse(f'{name}: a tensor of [tokens, heads, dh]')
-    _need_gpu(t)
-    if not (t.dtype in _SEQ_DTYPES):
+    if not t.is_cuda:
+        _need_gpu(t)
+    if t.dtype not in _SEQ_DTYPES:
         _refuse(f'{name}: {t.dtype} (float32 or bfloat16)')
-    if like is not None:
-        if not (t.dtype == like.dtype and t.device == like.device and t.shape[2] == like.shape[2]):
-            _refuse(f'{name}: {tuple(t.shape)} {t.dtype} on {t.device} beside {tuple(like.shape)} {like.dtype} on {like.device}')
+    if like is not None and (t.dtype != like.dtype or t.get_device() != like.get_device() or t.shape[2] != like.shape[2]):
+        _refuse(f'{name}: {tuple(t.shape)} {t.dtype} on {t.device} beside {tuple(like.shape)} {like.dtype} on {like.device}')
 
 
-def _ints_check(name, t, device, dim=1):
-    if not (isinstance(t, torch.Tensor) and t.dtype == torch.int32 and t.dim() == dim and t.device == device):
-        _refuse(f'{name}: {dim}-d int32 on {device}')
-    return _c(t)
+def _ints_check(name, what, t, index, dim=1):
+    if not isinstance(t, torch.Tensor) or t.dtype != torch.int32 or t.dim() != dim or not t.is_cuda or t.get_device() != index:
+        _refuse(f'{name}: {what}: {dim}-d int32 on cuda:{index}')
+    return t if t.is_contiguous() else t.contiguous()
 
 
 def _strided(t, aligned=True):
     """t, or a contiguous copy of it where its last dimension is not contiguous or (aligned) its rows or heads do not lie on
     16-byte boundaries."""
-    st, size = t.stride(), t.element_size()
-    if st[2] == 1 or t.shape[2] == 1:
-        n = 16 // size
-        if not aligned or (t.data_ptr() % 16 == 0 and (t.shape[0] < 2 or st[0] % n == 0) and (t.shape[1] < 2 or st[1] % n == 0)):
-            return t
-    c = t.contiguous()
-    # (a tensor that counts as contiguous where it is - one off a 16-byte boundary - comes back as itself)
-    return c.clone() if aligned and c.data_ptr() % 16 else c
+    row, head, one = t.stride()
+    if one == 1 and (not aligned or (t.data_ptr() | row * t.element_size() | head * t.element_size()) % 16 == 0):
+        return t
+    c = torch.empty(t.shape, dtype=t.dtype, device=t.device)
+    return c.copy_(t)
 
 
 def _rs(t):
-    """(pointer, row stride, head stride); the stride of a dimension of one is never used and passed as 0."""
-    st = t.stride()
-    return t.data_ptr(), st[0] if t.shape[0] > 1 else 0, st[1] if t.shape[1] > 1 else 0
+    """(pointer, row stride, head stride)"""
+    row, head, _ = t.stride()
+    return t.data_ptr(), row, head
 
 
 def _scale_of(scale, dh):
@@ -2262,7 +2244,7 @@ class RotaryFn(torch.autograd.Function):
         grads = [None, None]
         some = [(i, _strided(g, aligned=False)) for i, g in enumerate((dq, dk)) if g is not None and ctx.needs_input_grad[i]]
         if some:
-            with _device_of(positions), pin_stream(ctx.stream_h):
+            with pin_stream(ctx.stream_h):
                 for i, g in some:
                     grads[i] = torch.empty(g.shape, dtype=g.dtype, device=g.device)
                 (a, ga), (b, gb) = some[0], some[1] if len(some) > 1 else (None, None)
@@ -2276,34 +2258,40 @@ def rotary(q, k, positions, freqs, interleaved=False, scale=1.0, inplace=False):
     (2 i, 2 i + 1) if interleaved and (i, i + len(freqs)) otherwise, times scale; the rest passes through.  -> (q, k).
     inplace: q and k themselves, without gradients."""
     _seq_check('rotary: q', q)
-    if not (freqs.dtype == torch.float64 and freqs.dim() == 1 and freqs.device == q.device):
+    dev = q.get_device()
+    if dev != _current_device():
+        with _OnDevice(q.device):
+            return rotary(q, k, positions, freqs, interleaved, scale, inplace)
+    pairs, M, dh = freqs.numel(), q.shape[0], q.shape[2]
+    if freqs.dtype != torch.float64 or freqs.dim() != 1 or not freqs.is_cuda or freqs.get_device() != dev:
         _refuse(f'rotary: freqs: 1-d float64 on {q.device}')
-    if not (2 * freqs.numel() <= q.shape[2] and q.shape[2] % 2 == 0 and freqs.numel() <= 256):
-        _refuse(f'rotary: {freqs.numel()} pairs in a head of {q.shape[2]} elements (even; at most 256 pairs)')
-    positions = _ints_check('rotary: positions', positions, q.device)
-    if not (positions.numel() == q.shape[0]):
-        _refuse(f'rotary: {positions.numel()} positions for {q.shape[0]} tokens')
+    if 2 * pairs > dh or dh % 2 or pairs > 256:
+        _refuse(f'rotary: {pairs} pairs in a head of {dh} elements (even; at most 256 pairs)')
+    positions = _ints_check('rotary', 'positions', positions, dev)
+    if positions.numel() != M:
+        _refuse(f'rotary: {positions.numel()} positions for {M} tokens')
+    grad = q.requires_grad
     if k is not None:
         _seq_check('rotary: k', k, q)
-        if not (k.shape[0] == q.shape[0]):
-            _refuse(f'rotary: {q.shape[0]} queries and {k.shape[0]} keys')
+        if k.shape[0] != M:
+            _refuse(f'rotary: {M} queries and {k.shape[0]} keys')
+        grad = grad or k.requires_grad
+    grad = grad and torch.is_grad_enabled()
     freqs, scale = _c(freqs), float(scale)
-    grad = torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad))
-    with _device_of(q):
-        if inplace:
-            if not (not grad):
-                _refuse('rotary: in place on a tensor that wants a gradient')
-            if not (q.stride(2) == 1 and (k is None or k.stride(2) == 1)):
-                _refuse('rotary: in place needs a contiguous last dimension')
-            _rotary(q, k, q, k, positions, freqs, interleaved, scale, False)
-            return q, k
-        q, k = _strided(q, aligned=False), None if k is None else _strided(k, aligned=False)
+    if inplace:
         if grad:
-            return RotaryFn.apply(q, k, positions, freqs, bool(interleaved), scale)
-        qo = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        ko = None if k is None else torch.empty(k.shape, dtype=k.dtype, device=k.device)
-        _rotary(q, k, qo, ko, positions, freqs, interleaved, scale, False)
-        return qo, ko
+            _refuse('rotary: in place on a tensor that wants a gradient')
+        if q.stride(2) != 1 or (k is not None and k.stride(2) != 1):
+            _refuse('rotary: in place needs a contiguous last dimension')
+        _rotary(q, k, q, k, positions, freqs, interleaved, scale, False)
+        return q, k
+    q, k = _strided(q, False), None if k is None else _strided(k, False)
+    if grad:
+        return RotaryFn.apply(q, k, positions, freqs, bool(interleaved), scale)
+    qo = q.new_empty(q.shape)
+    ko = None if k is None else k.new_empty(k.shape)
+    _rotary(q, k, qo, ko, positions, freqs, interleaved, scale, False)
+    return qo, ko
 
 
 # ---- attention over packed sequences --------------------------------------------------------------------------------
@@ -2338,7 +2326,7 @@ class PackedAttentionFn(torch.autograd.Function):
         scale, causal = ctx.cfg
         M, H, dh = q.shape
         l = _lib.lib()
-        with _device_of(q), pin_stream(ctx.stream_h):
+        with pin_stream(ctx.stream_h):
             dout = _strided(dout)
             dq, dk, dv = torch.empty_like(out), torch.empty(k.shape, dtype=k.dtype, device=k.device), torch.empty(v.shape, dtype=v.dtype, device=v.device)
             ws = _ws(l.ttsmi_packed_attention_bwd_ws_bytes(starts.numel() - 1, M, H, k.shape[1], dh, int(causal)), q.device)
@@ -2356,21 +2344,26 @@ def packed_attention(q, k, v, starts, causal=True, scale=None):
     starts[-1] get zeros, and zero gradients.  -> [tokens, H, dh].  Tensors whose rows or heads do not lie on 16-byte
     boundaries are copied first."""
     _seq_check('packed_attention: q', q)
+    dev = q.get_device()
+    if dev != _current_device():
+        with _OnDevice(q.device):
+            return packed_attention(q, k, v, starts, causal, scale)
     _seq_check('packed_attention: k', k, q)
     _seq_check('packed_attention: v', v, q)
-    if not (k.shape == v.shape and k.shape[0] == q.shape[0] and k.shape[1] > 0 and q.shape[1] % k.shape[1] == 0):
+    M, H, dh = q.shape
+    Hkv = k.shape[1]
+    if k.shape != v.shape or k.shape[0] != M or Hkv == 0 or H == 0 or H % Hkv:
         _refuse(f'packed_attention: q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}')
-    if not (q.shape[2] % 8 == 0 and 0 < q.shape[2] <= 192):
-        _refuse(f'packed_attention: head size {q.shape[2]} (a multiple of 8 up to 192)')
-    starts = _ints_check('packed_attention: starts', starts, q.device)
-    if not (starts.numel() > 0):
+    if dh % 8 or not 0 < dh <= 192:
+        _refuse(f'packed_attention: head size {dh} (a multiple of 8 up to 192)')
+    starts = _ints_check('packed_attention', 'starts', starts, dev)
+    if starts.numel() == 0:
         _refuse('packed_attention: starts holds the end of the last sequence at least')
-    scale = _scale_of(scale, q.shape[2])
-    with _device_of(q):
-        q, k, v = _strided(q), _strided(k), _strided(v)
-        if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
-            return PackedAttentionFn.apply(q, k, v, starts, scale, bool(causal))
-        return _packed_fwd(q, k, v, starts, scale, causal, False)[0]
+    scale = _scale_of(scale, dh)
+    q, k, v = _strided(q), _strided(k), _strided(v)
+    if (q.requires_grad or k.requires_grad or v.requires_grad) and torch.is_grad_enabled():
+        return PackedAttentionFn.apply(q, k, v, starts, scale, bool(causal))
+    return _packed_fwd(q, k, v, starts, scale, causal, False)[0]
 
 
 # ---- the paged key / value cache --------------------------------------------------------------------------------------
@@ -2382,27 +2375,28 @@ class KVCache:
     a power of two up to 1024; float8_e4m3fn pages with k_exp and v_exp [pages, Hkv, page size] uint8, the biased exponent of
     each row's power-of-two scale (value = e4m3 * 2 ** (exp - 127)).  It holds the tensors it is given; which pages belong to
     which sequence is the caller's (`table`)."""
-    __slots__ = ('k', 'v', 'k_exp', 'v_exp', 'args', 'heads', 'dh', 'page_size', 'dtype', 'device')
+    __slots__ = ('k', 'v', 'k_exp', 'v_exp', 'args', 'heads', 'dh', 'page_size', 'dtype', 'code', 'index')
 
     def __init__(self, k, v, k_exp=None, v_exp=None):
-        if not (k.dim() == 4 and k.shape == v.shape and k.dtype == v.dtype and k.device == v.device and k.dtype in _CACHE_DTYPES):
+        if k.dim() != 4 or k.shape != v.shape or k.dtype != v.dtype or k.device != v.device or k.dtype not in _CACHE_DTYPES:
             _refuse(f'KVCache: pages {tuple(k.shape)} {k.dtype} and {tuple(v.shape)} {v.dtype}')
-        n, self.heads, self.page_size, self.dh = k.shape
-        if not (0 < self.page_size <= 1024 and self.page_size & (self.page_size - 1) == 0 and self.heads > 0):
-            _refuse(f'KVCache: pages of {self.page_size} rows (a power of two up to 1024)')
-        if not (self.dh % 8 == 0 and 0 < self.dh <= 192):
+        n, self.heads, size, self.dh = k.shape
+        if not 0 < size <= 1024 or size & (size - 1) or self.heads == 0:
+            _refuse(f'KVCache: pages of {size} rows (a power of two up to 1024)')
+        if self.dh % 8 or not 0 < self.dh <= 192:
             _refuse(f'KVCache: head size {self.dh} (a multiple of 8 up to 192)')
         quantised = k.dtype == torch.float8_e4m3fn
-        if not ((k_exp is not None and v_exp is not None) == quantised):
+        if (k_exp is None or v_exp is None) if quantised else (k_exp is not None or v_exp is not None):
             _refuse('KVCache: float8_e4m3fn pages, and only they, have exponents')
         for t in (k_exp, v_exp) if quantised else ():
-            if not (t.shape == k.shape[:3] and t.dtype == torch.uint8 and t.device == k.device and t.is_contiguous()):
+            if t.shape != k.shape[:3] or t.dtype != torch.uint8 or t.device != k.device or not t.is_contiguous():
                 _refuse(f'KVCache: exponents {tuple(t.shape)} {t.dtype} of pages {tuple(k.shape)}')
         _need_gpu(k)
-        if not (k.is_contiguous() and v.is_contiguous() and (k.data_ptr() | v.data_ptr()) % 16 == 0):
+        if not k.is_contiguous() or not v.is_contiguous() or (k.data_ptr() | v.data_ptr()) % 16:
             _refuse('KVCache: contiguous, 16-byte aligned pages')
-        self.k, self.v, self.k_exp, self.v_exp, self.dtype, self.device = k, v, k_exp, v_exp, k.dtype, k.device
-        self.args = (k.data_ptr(), v.data_ptr(), _p(k_exp), _p(v_exp), _CACHE_DTYPES[k.dtype], n, self.page_size)
+        self.k, self.v, self.k_exp, self.v_exp, self.dtype, self.page_size = k, v, k_exp, v_exp, k.dtype, size
+        self.index, self.code = k.get_device(), _CACHE_DTYPES[k.dtype]
+        self.args = (k.data_ptr(), v.data_ptr(), _p(k_exp), _p(v_exp), self.code, n, size)
 
     @classmethod
     def zeros(cls, pages, page_size, heads, dh, dtype=torch.bfloat16, device='cuda'):
@@ -2416,11 +2410,11 @@ class KVCache:
 
 
 def _paged_check(name, cache, table, starts, lens):
-    if not (isinstance(cache, KVCache)):
+    if not isinstance(cache, KVCache):
         _refuse(f'{name}: a KVCache')
-    table, starts = _ints_check(f'{name}: table', table, cache.device, 2), _ints_check(f'{name}: starts', starts, cache.device)
-    lens = _ints_check(f'{name}: lens', lens, cache.device)
-    if not (starts.numel() == lens.numel() + 1 and table.shape[0] == lens.numel()):
+    dev = cache.index
+    table, starts, lens = _ints_check(name, 'table', table, dev, 2), _ints_check(name, 'starts', starts, dev), _ints_check(name, 'lens', lens, dev)
+    if starts.numel() != lens.numel() + 1 or table.shape[0] != lens.numel():
         _refuse(f'{name}: {starts.numel()} starts, {lens.numel()} lens, table {tuple(table.shape)}')
     return table, starts, lens
 
@@ -2428,9 +2422,9 @@ def _paged_check(name, cache, table, starts, lens):
 def _kv_check(name, cache, k, v):
     _seq_check(f'{name}: k', k)
     _seq_check(f'{name}: v', v, k)
-    if not (k.shape == v.shape and k.shape[1] == cache.heads and k.shape[2] == cache.dh and k.device == cache.device):
-        _refuse(f'{name}: k {tuple(k.shape)}, v {tuple(v.shape)} on {k.device}; pages {tuple(cache.k.shape)} on {cache.device}')
-    if not (cache.dtype in (k.dtype, torch.float8_e4m3fn)):
+    if k.shape != v.shape or k.shape[1] != cache.heads or k.shape[2] != cache.dh or k.get_device() != cache.index:
+        _refuse(f'{name}: k {tuple(k.shape)}, v {tuple(v.shape)} on {k.device}; pages {tuple(cache.k.shape)} on {cache.k.device}')
+    if cache.dtype != k.dtype and cache.dtype != torch.float8_e4m3fn:
         _refuse(f'{name}: {k.dtype} beside pages of {cache.dtype}')
 
 
@@ -2440,11 +2434,13 @@ def kv_cache_write(cache, k, v, table, starts, lens):
     length with them, which are the last ones.  A page number outside the cache, or a token without a position, is not written."""
     table, starts, lens = _paged_check('kv_cache_write', cache, table, starts, lens)
     _kv_check('kv_cache_write', cache, k, v)
-    with _device_of(k):
-        k, v = _strided(k), _strided(v)
-        check(_lib.lib().ttsmi_kv_cache_write(*_rs(k), *_rs(v), *cache.args, table.data_ptr(), table.shape[1], starts.data_ptr(),
-                                              lens.data_ptr(), lens.numel(), k.shape[0], cache.heads, cache.dh, _SEQ_DTYPES[k.dtype],
-                                              _seq_stream(k.device.index)), 'kv_cache_write')
+    if cache.index != _current_device():
+        with _OnDevice(k.device):
+            return kv_cache_write(cache, k, v, table, starts, lens)
+    k, v = _strided(k), _strided(v)
+    check(_lib.lib().ttsmi_kv_cache_write(*_rs(k), *_rs(v), *cache.args, table.data_ptr(), table.shape[1], starts.data_ptr(), lens.data_ptr(),
+                                          lens.numel(), k.shape[0], cache.heads, cache.dh, _SEQ_DTYPES[k.dtype], _seq_stream(cache.index)),
+          'kv_cache_write')
 
 
 def kv_cache_read(cache, table, lens, starts, tokens, dtype=None, out=None):
@@ -2452,18 +2448,21 @@ def kv_cache_read(cache, table, lens, starts, tokens, dtype=None, out=None):
     in packed order -> (k, v) [tokens, Hkv, dh].  dtype: the pages' own, or either for float8_e4m3fn pages (default bfloat16).
     Rows behind starts[-1] are zeros; with out = (k, v) they are left as they were."""
     table, starts, lens = _paged_check('kv_cache_read', cache, table, starts, lens)
+    if cache.index != _current_device():
+        with _OnDevice(cache.k.device):
+            return kv_cache_read(cache, table, lens, starts, tokens, dtype, out)
     if out is None:
         dtype = dtype or (torch.bfloat16 if cache.dtype == torch.float8_e4m3fn else cache.dtype)
-        k, v = (torch.empty((int(tokens), cache.heads, cache.dh), dtype=dtype, device=cache.device) for _ in 'kv')
+        shape = (int(tokens), cache.heads, cache.dh)
+        k, v = torch.empty(shape, dtype=dtype, device=cache.k.device), torch.empty(shape, dtype=dtype, device=cache.k.device)
     else:
         k, v = out
-        if not (k.shape[0] == tokens and _strided(k) is k and _strided(v) is v):
-            _refuse(f'kv_cache_read: out of {tokens} tokens on 16-byte boundaries')
     _kv_check('kv_cache_read', cache, k, v)
-    with _device_of(k):
-        check(_lib.lib().ttsmi_kv_cache_read(*cache.args, table.data_ptr(), table.shape[1], starts.data_ptr(), lens.data_ptr(), lens.numel(),
-                                             k.shape[0], cache.heads, cache.dh, *_rs(k), *_rs(v), int(out is None), _SEQ_DTYPES[k.dtype],
-                                             _seq_stream(k.device.index)), 'kv_cache_read')
+    if out is not None and (k.shape[0] != tokens or _strided(k) is not k or _strided(v) is not v):
+        _refuse(f'kv_cache_read: out of {tokens} tokens on 16-byte boundaries')
+    check(_lib.lib().ttsmi_kv_cache_read(*cache.args, table.data_ptr(), table.shape[1], starts.data_ptr(), lens.data_ptr(), lens.numel(),
+                                         k.shape[0], cache.heads, cache.dh, *_rs(k), *_rs(v), int(out is None), _SEQ_DTYPES[k.dtype],
+                                         _seq_stream(cache.index)), 'kv_cache_read')
     return k, v
 
 
@@ -2474,22 +2473,26 @@ def paged_attention(q, cache, table, starts, lens, scale=None, out=None):
     _seq_check('paged_attention: q', q)
     table, starts, lens = _paged_check('paged_attention', cache, table, starts, lens)
     M, H, dh = q.shape
-    if not (dh == cache.dh and H % cache.heads == 0 and H > 0 and q.device == cache.device and cache.dtype in (q.dtype, torch.float8_e4m3fn)):
-        _refuse(f'paged_attention: q {tuple(q.shape)} {q.dtype} on {q.device}; pages {tuple(cache.k.shape)} {cache.dtype} on {cache.device}')
-    if not (not (torch.is_grad_enabled() and q.requires_grad)):
+    Hkv = cache.heads
+    if dh != cache.dh or H == 0 or H % Hkv or q.get_device() != cache.index or (cache.dtype != q.dtype and cache.dtype != torch.float8_e4m3fn):
+        _refuse(f'paged_attention: q {tuple(q.shape)} {q.dtype} on {q.device}; pages {tuple(cache.k.shape)} {cache.dtype} on {cache.k.device}')
+    if q.requires_grad and torch.is_grad_enabled():
         _refuse('paged_attention: has no gradient')
+    if cache.index != _current_device():
+        with _OnDevice(q.device):
+            return paged_attention(q, cache, table, starts, lens, scale, out)
     scale = _scale_of(scale, dh)
+    q = _strided(q)
     given = out is not None
-    if given:
-        if not (out.shape == q.shape and out.dtype == q.dtype and out.device == q.device and _strided(out) is out):
-            _refuse(f'paged_attention: out {tuple(out.shape)} {out.dtype} for q {tuple(q.shape)} {q.dtype}, on 16-byte boundaries')
+    if not given:
+        out = torch.empty((M, H, dh), dtype=q.dtype, device=q.device)
+    elif out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or _strided(out) is not out:
+        _refuse(f'paged_attention: out {tuple(out.shape)} {out.dtype} for q {tuple(q.shape)} {q.dtype}, on 16-byte boundaries')
     l = _lib.lib()
-    with _device_of(q):
-        q = _strided(q)
-        out = out if given else torch.empty((M, H, dh), dtype=q.dtype, device=q.device)
-        need = l.ttsmi_paged_attention_ws_bytes(lens.numel(), M, H, cache.heads, dh, _CACHE_DTYPES[cache.dtype], _SEQ_DTYPES[q.dtype])
-        ws = _ws(need, q.device) if need else None
-        check(l.ttsmi_paged_attention(*_rs(q), *cache.args, table.data_ptr(), table.shape[1], starts.data_ptr(), lens.data_ptr(),
-                                      lens.numel(), M, H, cache.heads, dh, scale, *_rs(out), int(not given), _p(ws),
-                                      0 if ws is None else ws.numel(), _SEQ_DTYPES[q.dtype], _seq_stream(q.device.index)), 'paged_attention')
+    dtype = _SEQ_DTYPES[q.dtype]
+    need = l.ttsmi_paged_attention_ws_bytes(lens.numel(), M, H, Hkv, dh, cache.code, dtype)
+    ws = _ws(need, q.device) if need else None
+    check(l.ttsmi_paged_attention(*_rs(q), *cache.args, table.data_ptr(), table.shape[1], starts.data_ptr(), lens.data_ptr(), lens.numel(), M, H,
+                                  Hkv, dh, scale, *_rs(out), int(not given), _p(ws), 0 if ws is None else ws.numel(), dtype,
+                                  _seq_stream(cache.index)), 'paged_attention')
     return out
