@@ -805,11 +805,11 @@ int ttsmi_pad_cols_f32(const float* src, int C, float* dst, int Cp, int M, ttsmi
  *
  * Tensors of tokens are [tokens, heads, dh], the last dimension contiguous, with element strides (row, head) of their own -
  * e.g. the three parts of one fused projection.  dtype is TTSMI_F32 or TTSMI_BF16_IO (fp32 or bf16 tensors).  The attention
- * and cache entry points need dh a multiple of 8 up to 192 and rows and heads on 16-byte boundaries; H % Hkv == 0, query head
- * h reads key head h / (H / Hkv).
- * starts [B + 1] int32 (DEVICE): sequence b owns the packed tokens starts[b] .. starts[b + 1]; starts[0] = 0, ascending; a
- *   sequence may be empty.  Tokens behind starts[B] belong to no sequence: outputs there are left as they were, or, with
- *   zero_rest != 0, set to zero.  starts that do not ascend or reach outside give wrong rows, but no access out of range.
+ * and cache entry points need dh a multiple of 8 up to 192 and rows and heads on 16-byte boundaries (packed attention also
+ * 130 rows and the H / Hkv heads of a group within 4 GiB); H % Hkv == 0, query head h reads key head h / (H / Hkv).
+ * starts [B + 1] int32 (DEVICE): sequence b owns the packed tokens starts[b] .. starts[b + 1]; ascending; a sequence may
+ *   be empty.  Tokens in front of starts[0] and behind starts[B] belong to no sequence: outputs there are left as they were, or,
+ *   with zero_rest != 0, set to zero.  starts that do not ascend or reach outside give wrong rows, but no access out of range.
  * Lengths are read on the device only: a captured call replays on other lengths (same B and token count).
  * ------------------------------------------------------------------------------------------- */
 /* The first rot elements of every head turned by position: pair (2i, 2i + 1) (interleaved != 0) or (i, i + rot / 2) of a
@@ -823,9 +823,10 @@ int ttsmi_rotary(const void* q, int64_t q_row, int64_t q_head, void* qo, int64_t
                  ttsmi_stream_t stream);
 /* out = softmax(scale q k^T) v within each sequence, causal != 0: over the keys up to the query's own.  scale > 0.  The sums
  * are held in fp32; bf16: the probabilities are rounded to bf16 for the product with v.  lse [Hkv, tokens, H / Hkv] fp32
- * (natural log; may be NULL) is what the backward reads.  A masked score never reaches the softmax, whatever k holds; a NaN
- * or infinity in a VALUE row reaches every row of its own sequence whose 32-row block shares a 32-key block with it (0 times
- * NaN), and no other sequence. */
+ * (natural log; may be NULL) is what the backward reads.  A masked score never reaches the softmax, whatever k holds.  A NaN
+ * or infinity in a VALUE row, which the product meets with a zero where it is masked, may reach rows of its own sequence up to
+ * 127 tokens in front of it (in the backward: one in q, k, v or dout, gradient rows up to 127 tokens off); never another
+ * sequence, nor from tokens of none. */
 int ttsmi_packed_attention_fwd(const void* q, int64_t q_row, int64_t q_head, const void* k, int64_t k_row, int64_t k_head,
                                const void* v, int64_t v_row, int64_t v_head, const int32_t* starts, int B, int tokens, int H,
                                int Hkv, int dh, float scale, int causal, void* out, int64_t o_row, int64_t o_head, float* lse,
@@ -842,7 +843,8 @@ int ttsmi_packed_attention_bwd(const void* q, int64_t q_row, int64_t q_head, con
  * (rows as they are) or TTSMI_E4M3 (bytes, with k_exp / v_exp [n_pages, Hkv, page_size]: row = e4m3 value * 2^(exp - 127)).
  * table [B, table_width] int32: page of the positions p * page_size ... of sequence b.  lens [B] int32: cached length of
  * sequence b INCLUDING its starts[b + 1] - starts[b] new tokens, which are the last ones.  A page number outside
- * [0, n_pages) is never written and reads as zeros; a new token without a position (lens too small) is not written.
+ * [0, n_pages) is never written and reads as zeros; a new token without a position (lens too small, or past the table) is not
+ * written.
  * A page may stand in several tables for reading; a call that writes one row twice leaves either.
  * e4m3: the smallest power-of-two scale that brings the row's largest finite magnitude to 448 at most, each value rounded to
  * nearest even; NaN and infinity become NaN. */
@@ -857,8 +859,9 @@ int ttsmi_kv_cache_read(const void* k_pages, const void* v_pages, const uint8_t*
                         const int32_t* lens, int B, int tokens, int Hkv, int dh, void* k, int64_t k_row, int64_t k_head, void* v,
                         int64_t v_row, int64_t v_head, int zero_rest, int dtype, ttsmi_stream_t stream);
 /* Attention of the packed new tokens over the cache (their own keys and values written before): token i of sequence b, n of
- * them, is at position lens[b] - n + i and sees the keys up to it.  A token that sees none gets zeros.  The keys are split over
- * workgroups by the lengths found on the device; the sums of the splits pass through ws. */
+ * them, is at position lens[b] - n + i and sees the keys up to it.  A token that sees none gets zeros; positions past the
+ * table's pages (or 2^30) hold no key.  The keys are split over workgroups by the lengths found on the device; the sums of the
+ * splits pass through ws. */
 size_t ttsmi_paged_attention_ws_bytes(int B, int tokens, int H, int Hkv, int dh, int cache_dtype, int dtype);
 int ttsmi_paged_attention(const void* q, int64_t q_row, int64_t q_head, const void* k_pages, const void* v_pages,
                           const uint8_t* k_exp, const uint8_t* v_exp, int cache_dtype, int n_pages, int page_size,

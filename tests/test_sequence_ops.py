@@ -34,7 +34,8 @@ def _packed(lib, bwd=False, **over):
     (dict(dh=60), -1, b'head size'), (dict(dh=200), -1, b'head size'), (dict(dh=0), -1, b'head size'), (dict(scale=0.0), -1, b'scale'),
     (dict(scale=-1.0), -1, b'scale'), (dict(scale=float('nan')), -1, b'scale'), (dict(scale=float('inf')), -1, b'scale'), (dict(tokens=-1), -1, b'tokens'),
     (dict(B=-1), -1, b'sequences'), (dict(tokens=1 << 30), -1, b'too large'), (dict(starts=None), -1, b'starts'), (dict(q=None), -1, b'null'),
-    (dict(k=ODD), -1, b'aligned'), (dict(v_row=132), -1, b'aligned'), (dict(q_head=60), -1, b'aligned'), (dict(out=None), -1, b'null'), (dict(k_row=-128), -1, b'aligned')])
+    (dict(k=ODD), -1, b'aligned'), (dict(v_row=132), -1, b'aligned'), (dict(q_head=60), -1, b'aligned'), (dict(out=None), -1, b'null'), (dict(k_row=-128), -1, b'aligned'),
+    (dict(k_row=1 << 24), -1, b'too far apart'), (dict(q_head=1 << 30), -1, b'too far apart'), (dict(q_row=1 << 40), -1, b'too far apart')])
 @pytest.mark.parametrize('bwd', [False, True])
 def test_packed_attention_refuses(lib, over, code, word, bwd):
     rc, err = _packed(lib, bwd, **over)

@@ -532,12 +532,123 @@ def test_paged_attention_rows_that_see_nothing_and_bad_pages():
     k[8:16], v[8:16] = 0, 0
     want, bound = attention_oracle(q[:1].cpu(), k, v, 39, True, 0.125, torch.float32)
     _within(ops.paged_attention(q[:2].contiguous(), p.cache, bad, st, ln)[:1], want[0], bound[0], 'out')
-    # lens past what the table holds: the positions without a page read as zeros as well
-    short = table[:, :2].contiguous()
-    k, v = p.k[0].clone(), p.v[0].clone()
-    k[16:], v[16:] = 0, 0
-    want, bound = attention_oracle(q[:1].cpu(), k, v, 39, True, 0.125, torch.float32)
-    _within(ops.paged_attention(q[:2].contiguous(), p.cache, short, st, ln)[:1], want[0], bound[0], 'out')
+    # lens past what the table holds: those positions hold no key, however far they reach
+    want, bound = attention_oracle(q[:1].cpu(), p.k[0][:16], p.v[0][:16], 39, True, 0.125, torch.float32)
+    for length in (40, 2 ** 31 - 1):
+        ln[0] = length
+        _within(ops.paged_attention(q[:2].contiguous(), p.cache, table[:, :2].contiguous(), st, ln)[:1], want[0], bound[0], 'out')
+        wide = q[:1].expand(64, 64, 64).contiguous()           # the form for many rows: 64 new tokens, the last one here
+        many = torch.tensor([0, 64], dtype=torch.int32, device=DEV)
+        got = ops.paged_attention(wide, p.cache, table[:1, :2].contiguous(), many, ln[:1] + (24 if length == 40 else 0))[-1:]
+        _within(got, want[0], bound[0], 'out')
+
+
+@pytest.mark.parametrize('H', [4, 64])
+def test_cache_without_pages_or_table(H):
+    """A cache of no pages, and a table of no columns: nothing is written, zeros are read, and attention gives zeros."""
+    ops = _ops()
+    st, ln = (torch.tensor(t, dtype=torch.int32, device=DEV) for t in ([0, 3, 40], [9, 37]))
+    for dtype in (torch.bfloat16, torch.float8_e4m3fn):
+        for pages, width in ((0, 3), (2, 0)):
+            cache = ops.KVCache.zeros(pages, 8, 2, 64, dtype, DEV)
+            table = torch.zeros((2, width), dtype=torch.int32, device=DEV)
+            k = _randn((40, 2, 64), 1, torch.bfloat16).to(DEV)
+            ops.kv_cache_write(cache, k, k, table, st, ln)
+            assert not any(t.any() for t in ops.kv_cache_read(cache, table, ln, st, 40, dtype=torch.bfloat16))
+            assert not ops.paged_attention(_randn((40, H, 64), 2, torch.bfloat16).to(DEV), cache, table, st, ln).any()
+
+
+def test_paged_attention_missing_page_beside_any_exponents():
+    """A page that is not there reads as zeros, whatever the bytes of the page that stands in for it."""
+    ops = _ops()
+    for H in (4, 64):
+        q = _randn((1, H, 64), 3, torch.bfloat16)
+        p = Paged([40], 8, 2, 64, torch.bfloat16, torch.float8_e4m3fn)
+        table = p.args[0]
+        st, ln = torch.tensor([0, 1], dtype=torch.int32, device=DEV), torch.tensor([40], dtype=torch.int32, device=DEV)
+        table = table.clone()
+        first = table == 0
+        spare = torch.cat([p.cache.k.view(torch.uint8), p.cache.k.view(torch.uint8)[:1]]), torch.cat([p.cache.v.view(torch.uint8), p.cache.v.view(torch.uint8)[:1]])
+        exps = [torch.cat([e, e[:1]]) for e in (p.cache.k_exp, p.cache.v_exp)]
+        table[first] = len(spare[0]) - 1                         # page 0 moves behind the last, and nobody names it any more
+        for e in exps:
+            e[0] = 255
+        cache = ops.KVCache(*(t.view(torch.float8_e4m3fn) for t in spare), *exps)
+        table[0, 1] = -1
+        k, v = p.k[0].clone(), p.v[0].clone()
+        k[8:16], v[8:16] = 0, 0
+        want, bound = attention_oracle(q, k, v, 39, True, 0.125, torch.bfloat16)
+        _within(ops.paged_attention(q.to(DEV), cache, table, st, ln), want[0], bound[0], 'out')
+
+
+def test_tokens_in_front_of_the_first_sequence():
+    """They belong to no sequence: zeros out, zero gradients, nothing of them in the others; in a given output they stay."""
+    ops = _ops()
+    front, lens, M, dh = 150, [40, 133], 400, 64
+    st = _starts(lens).to(DEV) + front
+    for dtype, H, Hkv in ((torch.bfloat16, 4, 2), (torch.float32, 6, 1)):
+        x = [_randn((M, h, dh), i, dtype).to(DEV) for i, h in enumerate((H, Hkv, Hkv, H))]
+        own = slice(front, front + 173)
+        clean = [t[own].clone().requires_grad_() for t in x[:3]]
+        want = _grads(ops.packed_attention(*clean, st - front), clean, x[3][own].clone())
+        for t in x:
+            t[:front], t[front + 173:] = float('nan'), float('nan')
+        xs = [t.requires_grad_() for t in x[:3]]
+        for g, w in zip(_grads(ops.packed_attention(*xs, st), xs, x[3]), want):
+            assert torch.equal(g[own], w) and not g[:front].any() and not g[front + 173:].any()
+    p = Paged([40, 133], 16, 2, 64, torch.bfloat16, torch.bfloat16)
+    table, _, ln = p.args
+    st0 = st - front
+    for t, w in zip(ops.kv_cache_read(p.cache, table, ln, st, M), ops.kv_cache_read(p.cache, table, ln, st0, 173)):
+        assert torch.equal(t[own], w) and not t[:front].any() and not t[front + 173:].any()
+    for H in (4, 64):
+        q = _randn((M, H, 64), 5, torch.bfloat16).to(DEV)
+        got, want = ops.paged_attention(q, p.cache, table, st, ln), ops.paged_attention(q[own].contiguous(), p.cache, table, st0, ln)
+        assert not got[:front].any() and not got[front + 173:].any()
+        # (the keys may be split elsewhere: fp32 sums in another order, then one rounding to bf16, a step at most between them)
+        assert bool(((got[own].float() - want.float()).abs() <= 2.0 ** -7 * want.float().abs() + 2.0 ** -16).all())
+
+
+def test_starts_that_overlap_stay_in_range():
+    """Not a valid call - but every access is bounded by the token count and the workspace, and it ends: the rows are whatever
+    they are, memory on both sides of the outputs stays as it was."""
+    ops = _ops()
+    M, H, Hkv, dh, B = 300, 8, 2, 64, 65
+    st = torch.tensor([(0 if b % 2 == 0 else M) for b in range(B + 1)], dtype=torch.int32, device=DEV)
+    x = [_randn((M, h, dh), i, torch.bfloat16).to(DEV) for i, h in enumerate((H, Hkv, Hkv, H))]
+    _grads(ops.packed_attention(*[t.requires_grad_() for t in x[:3]], st), x[:3], x[3])
+    p = Paged([700] * B, 64, Hkv, dh, torch.bfloat16, torch.bfloat16)
+    table, _, ln = p.args
+    guarded = torch.full((M + 200, H, dh), 3.0, dtype=torch.bfloat16, device=DEV)
+    for new in (40, M):
+        ops.paged_attention(x[0][:new].detach().contiguous(), p.cache, table, st.clamp(max=new), ln, out=guarded[100:100 + new])
+        assert bool((guarded[:100] == 3).all()) and bool((guarded[100 + new:] == 3).all())
+    torch.cuda.synchronize()
+
+
+def test_rows_too_far_apart_and_broadcast_destinations():
+    from transformertts_amd import _lib
+    ops = _ops()
+    st = torch.tensor([0, 3], dtype=torch.int32, device=DEV)
+    q, k, v = (_randn((3, h, 64), i, torch.bfloat16).to(DEV) for i, h in enumerate((4, 2, 2)))
+    far = torch.zeros(2 * (1 << 25) + 256, dtype=torch.bfloat16, device=DEV).as_strided((3, 4, 64), (1 << 25, 64, 1))
+    far.copy_(q)
+    assert torch.equal(ops.packed_attention(far, k, v, st), ops.packed_attention(q, k, v, st))
+    one = q[:1].expand(3, 4, 64)
+    pos, freqs = torch.arange(3, dtype=torch.int32, device=DEV), torch.ones(32, dtype=torch.float64, device=DEV)
+    cache = ops.KVCache.zeros(2, 8, 2, 64, torch.bfloat16, DEV)
+    table, ln = torch.zeros((1, 1), dtype=torch.int32, device=DEV), torch.tensor([3], dtype=torch.int32, device=DEV)
+    for call in (lambda: ops.rotary(one, k, pos, freqs, inplace=True), lambda: ops.rotary(q, k[:, :1].expand(3, 2, 64), pos, freqs, inplace=True),
+                 lambda: ops.paged_attention(q, cache, table, st, ln, out=one), lambda: ops.kv_cache_read(cache, table, ln, st, 3, out=(k, one[:, :2])),
+                 lambda: ops.KVCache(cache.k, cache.k)):
+        with pytest.raises(_lib.TtsmiError):
+            call()
+    w = torch.ones((64, 8), device=DEV, requires_grad=True)
+    x = _randn((3, 2, 64), 7).to(DEV)
+    y = (x @ w).sum()
+    ops.rotary(x, None, pos, freqs, inplace=True)               # what the product saved has changed: its gradient is refused, not wrong
+    with pytest.raises(RuntimeError):
+        y.backward()
 
 
 def test_paged_attention_graph_replay_decodes_on():

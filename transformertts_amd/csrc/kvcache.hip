@@ -93,10 +93,8 @@ __global__ __launch_bounds__(256) void kv_read_kernel(KvP p) {
     if (tok >= p.tokens) return;
     int pos = 0;
     const int seq = kv_find(p, tok, lane, pos);
-    if (seq < 0 && !(p.zero_rest && tok >= p.starts[p.B])) {
-        // (a token that is in a sequence but before its first position - more rows asked for than are cached - reads zeros)
-        if (tok < p.starts[0] || tok >= p.starts[p.B]) return;
-    }
+    // (a token that is in a sequence but before its first position - more rows asked for than are cached - reads zeros)
+    if (seq < 0 && !p.zero_rest && (tok < p.starts[0] || tok >= p.starts[p.B])) return;
     const long at0 = seq < 0 ? -1 : p.pg.row(seq, 0, pos);
     const int c = (lane % LPR) * 8;
     if (c >= p.pg.dh) return;
@@ -154,8 +152,8 @@ static int kv_launch(const KvP& p, bool write, hipStream_t st) {
     SEQ_CHECK_PAGES(who);                                                                                                         \
     if (tokens == 0) return TTSMI_OK;                                                                                             \
     SEQ_CHECK_CACHE(who);                                                                                                         \
-    TTSMI_CHECK_ARG(seq_strides_ok(k, k_row, k_head, dtype) && seq_strides_ok(v, v_row, v_head, dtype),                           \
-                    who ": a tensor is null or its rows or heads are not 16-byte aligned");                                       \
+    TTSMI_CHECK_ARG(seq_strides_ok(k, k_row, k_head, 0, dtype) && seq_strides_ok(v, v_row, v_head, 0, dtype),                         \
+                    who ": a tensor is null or its rows or heads are not 16-byte aligned");                                      \
     KvP p = {};                                                                                                                   \
     p.k = k; p.k_row = k_row; p.k_head = k_head; p.v = v; p.v_row = v_row; p.v_head = v_head;                                      \
     p.pg.k = k_pages; p.pg.v = v_pages; p.pg.ke = k_exp; p.pg.ve = v_exp; p.pg.table = table; p.pg.table_width = table_width;      \

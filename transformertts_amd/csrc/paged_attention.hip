@@ -67,7 +67,7 @@ __global__ __launch_bounds__((64 * PgCfg<T, CT, DHP>::NW), (PgCfg<T, CT, DHP>::W
     float* const mls = reinterpret_cast<float*>(sm + MAIN + (Q8 ? 2 : 1) * SIDE);           // [NW][32][2]
 
     const int hk = blockIdx.x % p.Hkv;
-    const SeqUnit un = find_unit(p.starts, p.lens, 1, p.B, p.tokens, p.G, 32, p.slots, 32 * NW, 64 * NW, blockIdx.x / p.Hkv, false);
+    const SeqUnit un = find_unit(p.starts, p.lens, 1, p.most, p.B, p.tokens, p.G, 32, p.slots, 32 * NW, 64 * NW, blockIdx.x / p.Hkv, false);
     if (un.t.seq < 0) {
         if (p.zero_rest) seq_zero_rest<T>((T*)p.o, p.o_row, p.o_head, p.starts, p.B, p.tokens, p.G, 32, hk * p.G, p.dh, un.t.tile);
         return;
@@ -77,7 +77,7 @@ __global__ __launch_bounds__((64 * PgCfg<T, CT, DHP>::NW), (PgCfg<T, CT, DHP>::W
     const int tok = r / p.G, head = hk * p.G + r - tok * p.G;
     const int lim = rok ? min(max(off + tok + 1, 0), len) : 0;
     const int last = min(un.t.tile * 32 + 31, rows - 1) / p.G;
-    int kend = min(max(off + last + 1, 0), len);
+    int kend = min(min(max(off + last + 1, 0), len), p.most);
     const int kbeg = min(un.split * un.per, kend);
     kend = min(kbeg + un.per, kend);
     const int full = off + un.t.tile * 32 / p.G + 1;                                        // keys that every row of the tile sees
@@ -103,13 +103,13 @@ __global__ __launch_bounds__((64 * PgCfg<T, CT, DHP>::NW), (PgCfg<T, CT, DHP>::W
         const int pmask = (1 << p.pg.shift) - 1, rowb = p.dh * (int)sizeof(CT);
         const uint32_t pageb = (uint32_t)rowb << p.pg.shift;
         auto key_of = [&](int x) { return min(kbeg + (x * NW + wave) * 32 + l31, kend - 1); };
-        auto ask_ids = [&](int x, int st) { seq_dma4(trow + min(key_of(x) >> p.pg.shift, p.pg.table_width - 1), seq_lds(ids + st * 64)); };
+        auto ask_ids = [&](int x, int st) { seq_dma4(trow + (key_of(x) >> p.pg.shift), seq_lds(ids + st * 64)); };
         uint32_t bad[NBUF];
         // block x into stage st: its page numbers have landed there
         auto request = [&](int x, int st) {
             const int key = key_of(x);
             const uint32_t id = ids[st * 64 + lane];
-            const bool wrong = id >= (uint32_t)p.pg.n_pages || (key >> p.pg.shift) >= p.pg.table_width;
+            const bool wrong = id >= (uint32_t)p.pg.n_pages;
             bad[st] = (uint32_t)__ballot(wrong);
             const uint32_t head_page = (wrong ? 0u : id) * (uint32_t)p.pg.heads + (uint32_t)hk;
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");                              // the stage's last readers are done
@@ -141,12 +141,13 @@ __global__ __launch_bounds__((64 * PgCfg<T, CT, DHP>::NW), (PgCfg<T, CT, DHP>::W
                     const int id16 = i * 64 + lane, row = (id16 / CH) & 31;
                     if ((bad[st] >> row) & 1) *reinterpret_cast<uint4*>(Ks + id16 * 16) = make_uint4(0u, 0u, 0u, 0u);
                 }
+                if (Q8 && ((bad[st] >> l31) & 1)) exps[st * 64 + lane] = 127;
             }
             f32x16 s;
 #pragma unroll
             for (int i = 0; i < 16; ++i) s[i] = 0.f;
             if constexpr (Q8) {
-                const float ks = (bad[st] >> l31) & 1 ? 1.f : seq_scale_of(exps[st * 64 + l31]);
+                const float ks = seq_scale_of(exps[st * 64 + l31]);
 #pragma unroll
                 for (int t = 0; t < NS; ++t) {
                     frag f;
@@ -284,8 +285,9 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PgJoinP j) {
     constexpr int NG = 64 / LPR;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int hk = blockIdx.x % p.Hkv;
-    const SeqUnit un = find_unit(p.starts, p.lens, 1, p.B, p.tokens, p.G, j.R, p.slots, j.quantum, j.least, blockIdx.x / p.Hkv, true);
+    const SeqUnit un = find_unit(p.starts, p.lens, 1, p.most, p.B, p.tokens, p.G, j.R, p.slots, j.quantum, j.least, blockIdx.x / p.Hkv, true);
     if (un.t.seq < 0 || un.nsplit < 2) return;
+    if (un.first + (long)(un.nsplit - 1) * un.t.ntile >= seq_split_units(p.tokens, p.B, p.G, j.R, p.slots)) return;      // (`starts` that overlap)
     const int rows = un.t.n * p.G, live = min(j.R, rows - un.t.tile * j.R);
     const int c = (lane % LPR) * 4, g = lane / LPR;
     for (int row = blockIdx.y * 4 + wave; row < live; row += 4 * gridDim.y) {
@@ -391,7 +393,7 @@ extern "C" int ttsmi_paged_attention(const void* q, int64_t q_row, int64_t q_hea
     SEQ_CHECK_PAGES("paged_attention");
     if (tokens == 0) return TTSMI_OK;
     SEQ_CHECK_CACHE("paged_attention");
-    TTSMI_CHECK_ARG(seq_strides_ok(q, q_row, q_head, dtype) && seq_strides_ok(out, o_row, o_head, dtype),
+    TTSMI_CHECK_ARG(seq_strides_ok(q, q_row, q_head, 0, dtype) && seq_strides_ok(out, o_row, o_head, 0, dtype),
                     "paged_attention: a tensor is null or its rows or heads are not 16-byte aligned");
     SeqFwdP p = {};
     p.q = q; p.q_row = q_row; p.q_head = q_head; p.o = out; p.o_row = o_row; p.o_head = o_head; p.starts = starts; p.lens = lens;
@@ -403,7 +405,7 @@ extern "C" int ttsmi_paged_attention(const void* q, int64_t q_row, int64_t q_hea
         ttsmi_set_error("paged_attention: workspace of %zu bytes, %zu (16-byte aligned) needed", ws_bytes, need);
         return TTSMI_ERR_WORKSPACE;
     }
-    bool rows_form = pg_rows_form(B, tokens, p.G, dh, cache_dtype);
+    const bool rows_form = pg_rows_form(B, tokens, p.G, dh, cache_dtype);
     PgJoinP j = {};
     j.R = rows_form ? 32 : 128; j.quantum = dtype == TTSMI_F32 ? 32 : 64; j.least = SEQ_TILE_LEAST;
     p.slots = pg_slots(B, tokens, Hkv, p.G, dh, rows_form, cache_dtype, dtype);
@@ -411,7 +413,8 @@ extern "C" int ttsmi_paged_attention(const void* q, int64_t q_row, int64_t q_hea
         p.part_o = (float*)ws;
         p.part_ml = (float*)ws + (size_t)seq_split_units(tokens, B, p.G, j.R, p.slots) * Hkv * j.R * dh;
     }
-    if (n_pages == 0 || table_width == 0) { rows_form = false; p.slots = 0; }              // nothing to read: zeros
+    const long held = (long)table_width << p.pg.shift;
+    p.most = n_pages == 0 ? 0 : (int)(held < (1l << 30) ? held : 1l << 30);
     hipStream_t st = (hipStream_t)stream;
     if (rows_form) {
         if (dtype == TTSMI_F32) cache_dtype == TTSMI_E4M3 ? pg_rows_launch<float, uint8_t>(p, j, st) : pg_rows_launch<float, float>(p, j, st);

@@ -27,7 +27,7 @@ __global__ __launch_bounds__(256, (DHP <= 128 && sizeof(T) == 2) ? 2 : 1) void s
     const int hk = blockIdx.x % p.Hkv, unit = blockIdx.x / p.Hkv;       // bid % 8 = XCD: the tiles of a key head share few L2s
     SeqUnit un;
     if constexpr (PAGED) {
-        if (p.slots > 0) un = find_unit(p.starts, p.lens, 1, p.B, p.tokens, p.G, 128, p.slots, KT, SEQ_TILE_LEAST, unit, false);
+        if (p.slots > 0) un = find_unit(p.starts, p.lens, 1, p.most, p.B, p.tokens, p.G, 128, p.slots, KT, SEQ_TILE_LEAST, unit, false);
     }
     const bool splits = PAGED && p.slots > 0;
     const SeqTile st = splits ? un.t : find_tile(p.starts, p.B, p.tokens, p.G, ROWS, unit);
@@ -51,6 +51,7 @@ __global__ __launch_bounds__(256, (DHP <= 128 && sizeof(T) == 2) ? 2 : 1) void s
     // the same for the workgroup's last row, and for this wave's: no key behind is fetched / multiplied
     const int last = min(tile * ROWS + ROWS - 1, rows - 1) / p.G;
     int kend = p.causal ? min(max(off + last + 1, 0), len) : len, kbeg = 0;
+    if (PAGED) kend = min(kend, p.most);
     const bool part = splits && un.nsplit > 1;
     if (part) {
         kbeg = min(un.split * un.per, kend);
@@ -97,7 +98,7 @@ __global__ __launch_bounds__(256, (DHP <= 128 && sizeof(T) == 2) ? 2 : 1) void s
 #pragma unroll
             for (int i = 0; i < ITEMS; ++i) {
                 const int at = min(k0 + D::row(i, wave, lane), kend - 1) >> p.pg.shift;
-                pid[i] = at < p.pg.table_width ? trow[at] : -1;
+                pid[i] = trow[at];
             }
         }
     };
@@ -359,8 +360,8 @@ extern "C" int ttsmi_packed_attention_fwd(const void* q, int64_t q_row, int64_t 
     SEQ_CHECK_COMMON("packed_attention_fwd");
     if (tokens == 0) return TTSMI_OK;
     TTSMI_CHECK_ARG(starts, "packed_attention_fwd: null starts");
-    TTSMI_CHECK_ARG(seq_strides_ok(q, q_row, q_head, dtype) && seq_strides_ok(k, k_row, k_head, dtype) && seq_strides_ok(v, v_row, v_head, dtype) &&
-                        seq_strides_ok(out, o_row, o_head, dtype), "packed_attention_fwd: a tensor is null or its rows or heads are not 16-byte aligned");
+    TTSMI_CHECK_ARG(seq_strides_ok(q, q_row, q_head, H / Hkv, dtype) && seq_strides_ok(k, k_row, k_head, 1, dtype) && seq_strides_ok(v, v_row, v_head, 1, dtype) &&
+                        seq_strides_ok(out, o_row, o_head, 0, dtype), "packed_attention_fwd: a tensor is null or its rows or heads are not 16-byte aligned, or too far apart");
     SeqFwdP p = {};
     p.q = q; p.q_row = q_row; p.q_head = q_head; p.k = k; p.k_row = k_row; p.k_head = k_head; p.v = v; p.v_row = v_row; p.v_head = v_head;
     p.o = out; p.zero_rest = zero_rest != 0; p.o_row = o_row; p.o_head = o_head; p.lse = lse; p.starts = starts;

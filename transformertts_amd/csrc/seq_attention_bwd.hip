@@ -200,7 +200,7 @@ __global__ __launch_bounds__(256, (DHP <= 128 && sizeof(T) == 2) ? 2 : 1) void s
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int hk = blockIdx.x % p.Hkv, unit = blockIdx.x / p.Hkv;
     SeqUnit un;
-    if (p.slots > 0) un = find_unit(p.starts, nullptr, p.G, p.B, p.tokens, 1, 128, p.slots, KT, SeqLeast<T>::ROWS, unit, false);
+    if (p.slots > 0) un = find_unit(p.starts, nullptr, p.G, 0x7fffffff, p.B, p.tokens, 1, 128, p.slots, KT, SeqLeast<T>::ROWS, unit, false);
     const SeqTile st = p.slots > 0 ? un.t : find_tile(p.starts, p.B, p.tokens, 1, 128, unit);   // causal: the first keys have the most rows
     if (st.seq < 0) {
         if (p.zero_rest) {
@@ -389,10 +389,10 @@ __global__ __launch_bounds__(256, (DHP <= 128 && sizeof(T) == 2) ? 2 : 1) void s
 template <typename T>
 __global__ __launch_bounds__(256) void seq_dkv_join_kernel(SeqBwdP p) {
     const int hk = blockIdx.x % p.Hkv;
-    const SeqUnit un = find_unit(p.starts, nullptr, p.G, p.B, p.tokens, 1, 128, p.slots, SeqT<T>::KT, SeqLeast<T>::ROWS, blockIdx.x / p.Hkv, true);
+    const SeqUnit un = find_unit(p.starts, nullptr, p.G, 0x7fffffff, p.B, p.tokens, 1, 128, p.slots, SeqT<T>::KT, SeqLeast<T>::ROWS, blockIdx.x / p.Hkv, true);
     if (un.t.seq < 0) return;
     const int key0 = un.t.tile * 128, z0 = (p.causal ? key0 * p.G : 0) / un.per;
-    if (un.nsplit - z0 < 2) return;
+    if (un.nsplit - z0 < 2 || un.first + (long)(un.nsplit - 1) * un.t.ntile >= seq_split_units(p.tokens, p.B, 1, 128, p.slots)) return;   // (the latter: `starts` that overlap)
     const int per = p.dh / 4, keys = min(16, un.t.n - key0 - 16 * (int)blockIdx.y);
     const long step = 2L * 128 * p.dh * p.Hkv * un.t.ntile;
     for (int i = threadIdx.x; i < 2 * keys * per; i += 256) {
@@ -455,10 +455,10 @@ extern "C" int ttsmi_packed_attention_bwd(const void* q, int64_t q_row, int64_t 
     SEQ_CHECK_COMMON("packed_attention_bwd");
     if (tokens == 0) return TTSMI_OK;
     TTSMI_CHECK_ARG(starts && lse, "packed_attention_bwd: null starts or lse");
-    TTSMI_CHECK_ARG(seq_strides_ok(q, q_row, q_head, dtype) && seq_strides_ok(k, k_row, k_head, dtype) && seq_strides_ok(v, v_row, v_head, dtype) &&
-                        seq_strides_ok(out, o_row, o_head, dtype) && seq_strides_ok(dout, d_row, d_head, dtype) &&
-                        seq_strides_ok(dq, dq_row, dq_head, dtype) && seq_strides_ok(dk, dk_row, dk_head, dtype) &&
-                        seq_strides_ok(dv, dv_row, dv_head, dtype), "packed_attention_bwd: a tensor is null or its rows or heads are not 16-byte aligned");
+    TTSMI_CHECK_ARG(seq_strides_ok(q, q_row, q_head, H / Hkv, dtype) && seq_strides_ok(k, k_row, k_head, 1, dtype) && seq_strides_ok(v, v_row, v_head, 1, dtype) &&
+                        seq_strides_ok(out, o_row, o_head, 0, dtype) && seq_strides_ok(dout, d_row, d_head, H / Hkv, dtype) &&
+                        seq_strides_ok(dq, dq_row, dq_head, 0, dtype) && seq_strides_ok(dk, dk_row, dk_head, 0, dtype) &&
+                        seq_strides_ok(dv, dv_row, dv_head, 0, dtype), "packed_attention_bwd: a tensor is null or its rows or heads are not 16-byte aligned, or too far apart");
     const size_t need = ttsmi_packed_attention_bwd_ws_bytes(B, tokens, H, Hkv, dh, causal);
     if (!ws || ws_bytes < need || ((uintptr_t)ws & 15)) {
         ttsmi_set_error("packed_attention_bwd: workspace of %zu bytes, %zu (16-byte aligned) needed", ws_bytes, need);

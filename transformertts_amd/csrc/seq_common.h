@@ -76,6 +76,7 @@ __device__ __forceinline__ int seq_scan_add(int v) {
 __device__ __forceinline__ int seq_wave_total(int v) { return __builtin_amdgcn_readlane(seq_scan_add(v), 63); }
 
 // ---- which tile of which sequence ------------------------------------------------------------------
+#define SEQ_NO_TILE 0x40000000
 struct SeqTile {
     int seq, tile, ntile;         // seq < 0: this workgroup has none
     int s0, n;                    // first token and length of the sequence
@@ -104,6 +105,7 @@ __device__ __forceinline__ SeqTile find_tile(const int* starts, int B, int token
             t.tile = unit - (__builtin_amdgcn_readlane(upto, at) - t.ntile);
             t.s0 = __builtin_amdgcn_readlane(s0, at);
             t.n = __builtin_amdgcn_readlane(n, at);
+            if ((unsigned)t.tile >= (unsigned)t.ntile) { t.seq = -1; t.tile = SEQ_NO_TILE; }   // (`starts` that overlap: the count wrapped)
             return t;
         }
         unit -= __builtin_amdgcn_readlane(upto, 63);
@@ -113,16 +115,16 @@ __device__ __forceinline__ SeqTile find_tile(const int* starts, int B, int token
 }
 // Grid of tiles: at least the sum of the sequences' tiles, and at least one more unit for every tile of rows behind them.
 static inline long seq_units(long tokens, int B, int G, int rows_per_tile) { return tokens * G / rows_per_tile + B + 1; }
-// Zeros into the rows behind the last sequence (tensors that the host mirror has just allocated): unit `past` of the grid past
-// the last tile clears the past-th tile of them, for G heads from head0 on.
+// Zeros into the rows of no sequence - in front of the first and behind the last (tensors that the host mirror has just
+// allocated): unit `past` of the grid past the last tile clears the past-th tile of them, for G heads from head0 on.
 template <typename T>
 __device__ __forceinline__ void seq_zero_rest(T* dst, long row, long head, const int* starts, int B, int tokens, int G, int rows_per_tile,
                                               int head0, int dh, int past) {
-    const int end = min(max(starts[B], 0), tokens), per = dh / 4;
-    const long r0 = (long)past * rows_per_tile, rows = min((long)(tokens - end) * G - r0, (long)rows_per_tile);
+    const int front = min(max(starts[0], 0), tokens), end = min(max(starts[B], front), tokens), per = dh / 4;
+    const long r0 = (long)past * rows_per_tile, rows = min((long)(front + tokens - end) * G - r0, (long)rows_per_tile);
     for (long i = threadIdx.x; i < rows * per; i += blockDim.x) {
-        const long r = r0 + i / per;
-        T* d = dst + (end + r / G) * row + (head0 + r % G) * head + (i % per) * 4;
+        const long r = r0 + i / per, t = r / G;
+        T* d = dst + (t < front ? t : end - front + t) * row + (head0 + r % G) * head + (i % per) * 4;
 #pragma unroll
         for (int e = 0; e < 4; ++e) d[e] = (T)0.f;
     }
@@ -135,18 +137,18 @@ __device__ __forceinline__ void seq_zero_rest(T* dst, long row, long head, const
 // workgroups that run together read the same range, through one L2.
 struct SeqUnit {
     SeqTile t;
-    int len;                      // keys of the sequence
+    int len;                      // cached length of the sequence, as `lens` has it
     int split, nsplit, per;       // key range [split per, (split + 1) per)
     long first;                   // unit number of the tile's first split; its next ones follow at steps of ntile
 };
 static inline __host__ __device__ long seq_split_units(long tokens, int B, int G, int R, int slots) { return tokens * G / R + B + 1 + slots; }
-// Tiles: R rows of G a token.  Keys: lens, or `own` times the sequence's tokens where lens is null (the backward's splits of the
-// rows that a key tile meets).  by_tile: `unit` counts tiles instead (the join).
-__device__ __forceinline__ SeqUnit find_unit(const int* starts, const int* lens, int own, int B, int tokens, int G, int R, int slots,
+// Tiles: R rows of G a token.  Keys: lens, `most` of them at most, or `own` times the sequence's tokens where lens is null (the
+// backward's splits of the rows that a key tile meets).  by_tile: `unit` counts tiles instead (the join).
+__device__ __forceinline__ SeqUnit find_unit(const int* starts, const int* lens, int own, int most, int B, int tokens, int G, int R, int slots,
                                              int quantum, int least, int unit, bool by_tile) {
     const int lane = threadIdx.x & 63;
     float total = 0.f;
-    int s0 = 0, n = 0, len = 0, tiles = 0;
+    int s0 = 0, n = 0, len = 0, keys = 0, tiles = 0;
     auto look = [&](int b) {
         s0 = n = len = 0;
         if (b < B) {
@@ -154,11 +156,12 @@ __device__ __forceinline__ SeqUnit find_unit(const int* starts, const int* lens,
             n = min(max(starts[b + 1], s0), tokens) - s0;
             len = lens ? max(lens[b], 0) : n * own;
         }
+        keys = min(len, most);
         tiles = (int)(((long)n * G + R - 1) / R);
     };
     for (int b0 = 0; b0 < B; b0 += 64) {
         look(b0 + lane);
-        total += (float)tiles * (float)len;
+        total += (float)tiles * (float)keys;
     }
     total = wave_sum_dpp(total) * (1.f + 0x1p-16f);                  // (never short of the true sum: the grid is sized by it)
     long per_l = max((long)(total / (float)slots) + 1, (long)least);
@@ -171,7 +174,7 @@ __device__ __forceinline__ SeqUnit find_unit(const int* starts, const int* lens,
             int units = 0, all = 0;
             for (int b0 = 0; b0 < B; b0 += 64) {
                 if (B > 64) look(b0 + lane);
-                units += tiles * max((int)(((long)len + per - 1) / per), 1);
+                units += tiles * max((int)(((long)keys + per - 1) / per), 1);
                 all += tiles;
             }
             units = seq_wave_total(units);
@@ -187,7 +190,7 @@ __device__ __forceinline__ SeqUnit find_unit(const int* starts, const int* lens,
     long before = 0;
     for (int b0 = 0; b0 < B; b0 += 64) {
         if (B > 64) look(b0 + lane);                               // (the only 64 are still in registers)
-        const int splits = max((int)(((long)len + per - 1) / per), 1), units = tiles * splits, counted = by_tile ? tiles : units;
+        const int splits = max((int)(((long)keys + per - 1) / per), 1), units = tiles * splits, counted = by_tile ? tiles : units;
         const int upto = seq_scan_add(counted), all = by_tile ? seq_scan_add(units) : upto;
         const uint64_t hit = __ballot(upto > unit);
         if (hit) {
@@ -202,6 +205,7 @@ __device__ __forceinline__ SeqUnit find_unit(const int* starts, const int* lens,
             u.split = __builtin_amdgcn_readfirstlane(by_tile ? 0 : rem / u.t.ntile);
             u.t.tile = by_tile ? rem : rem - u.split * u.t.ntile;
             u.first = before + __builtin_amdgcn_readlane(all, at) - __builtin_amdgcn_readlane(units, at) + u.t.tile;
+            if ((unsigned)u.t.tile >= (unsigned)u.t.ntile || u.split >= u.nsplit) { u.t.seq = -1; u.t.tile = SEQ_NO_TILE; }
             return u;
         }
         unit -= __builtin_amdgcn_readlane(upto, 63);
@@ -255,6 +259,7 @@ struct SeqFwdP {
     const int* starts; const int* lens;                   // lens: paged only (tokens in the cache, the new ones among them)
     SeqPages pg;
     int B, tokens, Hkv, G, dh, causal, zero_rest;
+    int most;                                             // positions that the table's pages hold (paged only)
     float c1;                                             // scale log2(e)
     // key splits (slots > 0): partial sums of unit u, key head hk at [(u Hkv + hk)][R rows][dh], their maximum and sum at [..][R][2]
     int slots; float* part_o; float* part_ml;
@@ -411,17 +416,19 @@ __device__ __forceinline__ uint4 seq_dequant_chunk(uint2 w, float scale) {
 }
 
 // ---- argument checks of the entry points -----------------------------------------------------------
-// What every tensor of [tokens, heads, dh] has to be: 16-byte aligned rows and heads, so that 16-byte accesses are whole.
-static inline bool seq_strides_ok(const void* ptr, int64_t row, int64_t head, int dtype) {
+// What every tensor of [tokens, heads, dh] has to be: 16-byte aligned rows and heads, so that 16-byte accesses are whole; and
+// where a kernel stages tiles of it, a tile (128 tokens and a partial one, `group` heads) within 32-bit offsets of its first row.
+static inline bool seq_strides_ok(const void* ptr, int64_t row, int64_t head, int group, int dtype) {
     const int n = dtype == TTSMI_F32 ? 4 : 8;
-    return ptr != nullptr && ((uintptr_t)ptr & 15) == 0 && row % n == 0 && head % n == 0 && row >= 0 && head >= 0;
+    return ptr != nullptr && ((uintptr_t)ptr & 15) == 0 && row % n == 0 && head % n == 0 && row >= 0 && head >= 0 &&
+           (group == 0 || (row < (1l << 25) && head < (1l << 32) && (130 * row + group * head) * (16 / n) < (1l << 32)));
 }
 #define SEQ_CHECK_COMMON(who)                                                                                               \
     TTSMI_CHECK_ARG(dtype == TTSMI_F32 || dtype == TTSMI_BF16_IO, who ": dtype %d (TTSMI_F32 or TTSMI_BF16_IO)", dtype);          \
     TTSMI_CHECK_ARG(B >= 0 && tokens >= 0 && H > 0 && Hkv > 0 && H % Hkv == 0, who ": sequences %d, tokens %d, heads %d / %d", B, tokens, H, Hkv); \
     TTSMI_CHECK_ARG(dh > 0 && dh <= 192 && dh % 8 == 0, who ": head size %d (a multiple of 8 up to 192)", dh);             \
     TTSMI_CHECK_ARG(scale > 0.f && scale < INFINITY, who ": scale must be positive and finite");                          \
-    TTSMI_CHECK_ARG((long)tokens * H + 128L * B * Hkv < (1L << 31), who ": tokens * heads too large");
+    TTSMI_CHECK_ARG((long)tokens * H + 512L * B * Hkv < (1L << 30), who ": tokens * heads too large");
 #define SEQ_CHECK_PAGES(who)                                                                                                      \
     TTSMI_CHECK_ARG(n_pages >= 0 && page_size > 0 && page_size <= 1024 && (page_size & (page_size - 1)) == 0 && table_width >= 0 &&  \
                         (long)n_pages * Hkv < (1L << 31), who ": %d pages of %d rows (a power of two up to 1024)", n_pages, page_size)

@@ -2193,14 +2193,20 @@ def _ints_check(name, what, t, index, dim=1):
     return t if t.is_contiguous() else t.contiguous()
 
 
-def _strided(t, aligned=True):
-    """t, or a contiguous copy of it where its last dimension is not contiguous or (aligned) its rows or heads do not lie on
-    16-byte boundaries."""
+def _strided(t, aligned=True, group=0):
+    """t, or a contiguous copy of it where its last dimension is not contiguous, (aligned) its rows or heads do not lie on
+    16-byte boundaries or (group) a tile of rows and `group` heads spans more than 32-bit offsets."""
     row, head, one = t.stride()
-    if one == 1 and (not aligned or (t.data_ptr() | row * t.element_size() | head * t.element_size()) % 16 == 0):
+    size = t.element_size()
+    if one == 1 and (not aligned or (t.data_ptr() | row * size | head * size) % 16 == 0) and (group == 0 or (130 * row + group * head) * size < 1 << 32):
         return t
     c = torch.empty(t.shape, dtype=t.dtype, device=t.device)
     return c.copy_(t)
+
+
+def _own_rows(t):
+    """Whether every element of t, a destination, has its own memory as far as its strides can tell: none of them is 0."""
+    return all(s > 0 or n < 2 for s, n in zip(t.stride(), t.shape))
 
 
 def _rs(t):
@@ -2281,9 +2287,10 @@ def rotary(q, k, positions, freqs, interleaved=False, scale=1.0, inplace=False):
     if inplace:
         if grad:
             _refuse('rotary: in place on a tensor that wants a gradient')
-        if q.stride(2) != 1 or (k is not None and k.stride(2) != 1):
-            _refuse('rotary: in place needs a contiguous last dimension')
+        if any(t is not None and (t.stride(2) != 1 or not _own_rows(t)) for t in (q, k)):
+            _refuse('rotary: in place needs a contiguous last dimension, and no broadcast one')
         _rotary(q, k, q, k, positions, freqs, interleaved, scale, False)
+        torch.autograd.graph.increment_version([q] if k is None else [q, k])
         return q, k
     q, k = _strided(q, False), None if k is None else _strided(k, False)
     if grad:
@@ -2327,7 +2334,7 @@ class PackedAttentionFn(torch.autograd.Function):
         M, H, dh = q.shape
         l = _lib.lib()
         with pin_stream(ctx.stream_h):
-            dout = _strided(dout)
+            dout = _strided(dout, True, H // k.shape[1])
             dq, dk, dv = torch.empty_like(out), torch.empty(k.shape, dtype=k.dtype, device=k.device), torch.empty(v.shape, dtype=v.dtype, device=v.device)
             ws = _ws(l.ttsmi_packed_attention_bwd_ws_bytes(starts.numel() - 1, M, H, k.shape[1], dh, int(causal)), q.device)
             check(l.ttsmi_packed_attention_bwd(*_rs(q), *_rs(k), *_rs(v), *_rs(out), *_rs(dout), lse.data_ptr(), starts.data_ptr(),
@@ -2340,8 +2347,8 @@ class PackedAttentionFn(torch.autograd.Function):
 def packed_attention(q, k, v, starts, causal=True, scale=None):
     """Attention within each of the packed sequences: q [tokens, H, dh], k and v [tokens, Hkv, dh], H a multiple of Hkv (query
     head h reads key head h // (H // Hkv)), dh a multiple of 8 up to 192; sequence b is tokens starts[b] .. starts[b + 1], over
-    the keys up to the query's own if causal and over all of them otherwise; scale defaults to dh ** -0.5.  Tokens behind
-    starts[-1] get zeros, and zero gradients.  -> [tokens, H, dh].  Tensors whose rows or heads do not lie on 16-byte
+    the keys up to the query's own if causal and over all of them otherwise; scale defaults to dh ** -0.5.  Tokens in
+    front of starts[0] and behind starts[-1] get zeros, and zero gradients.  -> [tokens, H, dh].  Tensors whose rows or heads do not lie on 16-byte
     boundaries are copied first."""
     _seq_check('packed_attention: q', q)
     dev = q.get_device()
@@ -2360,7 +2367,7 @@ def packed_attention(q, k, v, starts, causal=True, scale=None):
     if starts.numel() == 0:
         _refuse('packed_attention: starts holds the end of the last sequence at least')
     scale = _scale_of(scale, dh)
-    q, k, v = _strided(q), _strided(k), _strided(v)
+    q, k, v = _strided(q, True, H // Hkv), _strided(k, True, 1), _strided(v, True, 1)
     if (q.requires_grad or k.requires_grad or v.requires_grad) and torch.is_grad_enabled():
         return PackedAttentionFn.apply(q, k, v, starts, scale, bool(causal))
     return _packed_fwd(q, k, v, starts, scale, causal, False)[0]
@@ -2392,8 +2399,8 @@ class KVCache:
             if t.shape != k.shape[:3] or t.dtype != torch.uint8 or t.device != k.device or not t.is_contiguous():
                 _refuse(f'KVCache: exponents {tuple(t.shape)} {t.dtype} of pages {tuple(k.shape)}')
         _need_gpu(k)
-        if not k.is_contiguous() or not v.is_contiguous() or (k.data_ptr() | v.data_ptr()) % 16:
-            _refuse('KVCache: contiguous, 16-byte aligned pages')
+        if not k.is_contiguous() or not v.is_contiguous() or (k.data_ptr() | v.data_ptr()) % 16 or (k.numel() and k.data_ptr() == v.data_ptr()):
+            _refuse('KVCache: contiguous, 16-byte aligned pages, of keys and of values')
         self.k, self.v, self.k_exp, self.v_exp, self.dtype, self.page_size = k, v, k_exp, v_exp, k.dtype, size
         self.index, self.code = k.get_device(), _CACHE_DTYPES[k.dtype]
         self.args = (k.data_ptr(), v.data_ptr(), _p(k_exp), _p(v_exp), self.code, n, size)
@@ -2446,7 +2453,7 @@ def kv_cache_write(cache, k, v, table, starts, lens):
 def kv_cache_read(cache, table, lens, starts, tokens, dtype=None, out=None):
     """The last starts[b + 1] - starts[b] cached tokens of every sequence (all of them where starts holds the cumulative lens)
     in packed order -> (k, v) [tokens, Hkv, dh].  dtype: the pages' own, or either for float8_e4m3fn pages (default bfloat16).
-    Rows behind starts[-1] are zeros; with out = (k, v) they are left as they were."""
+    Rows of no sequence are zeros; with out = (k, v) they are left as they were."""
     table, starts, lens = _paged_check('kv_cache_read', cache, table, starts, lens)
     if cache.index != _current_device():
         with _OnDevice(cache.k.device):
@@ -2458,7 +2465,7 @@ def kv_cache_read(cache, table, lens, starts, tokens, dtype=None, out=None):
     else:
         k, v = out
     _kv_check('kv_cache_read', cache, k, v)
-    if out is not None and (k.shape[0] != tokens or _strided(k) is not k or _strided(v) is not v):
+    if out is not None and (k.shape[0] != tokens or _strided(k) is not k or _strided(v) is not v or not _own_rows(k) or not _own_rows(v)):
         _refuse(f'kv_cache_read: out of {tokens} tokens on 16-byte boundaries')
     check(_lib.lib().ttsmi_kv_cache_read(*cache.args, table.data_ptr(), table.shape[1], starts.data_ptr(), lens.data_ptr(), lens.numel(),
                                          k.shape[0], cache.heads, cache.dh, *_rs(k), *_rs(v), int(out is None), _SEQ_DTYPES[k.dtype],
@@ -2469,7 +2476,8 @@ def kv_cache_read(cache, table, lens, starts, tokens, dtype=None, out=None):
 def paged_attention(q, cache, table, starts, lens, scale=None, out=None):
     """Attention of packed new tokens q [tokens, H, dh] over the cache, their own keys and values in it already
     (kv_cache_write): token i of the n new ones of sequence b is at position lens[b] - n + i and sees the keys up to it; a
-    token that sees none gets zeros.  Without gradients.  Rows behind starts[-1] are zeros; in `out` they are left as they were."""
+    token that sees none gets zeros.  Positions past the table's pages hold no key.  Without gradients.  Rows of no sequence are
+    zeros; in `out` they are left as they were."""
     _seq_check('paged_attention: q', q)
     table, starts, lens = _paged_check('paged_attention', cache, table, starts, lens)
     M, H, dh = q.shape
@@ -2486,7 +2494,7 @@ def paged_attention(q, cache, table, starts, lens, scale=None, out=None):
     given = out is not None
     if not given:
         out = torch.empty((M, H, dh), dtype=q.dtype, device=q.device)
-    elif out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or _strided(out) is not out:
+    elif out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or _strided(out) is not out or not _own_rows(out):
         _refuse(f'paged_attention: out {tuple(out.shape)} {out.dtype} for q {tuple(q.shape)} {q.dtype}, on 16-byte boundaries')
     l = _lib.lib()
     dtype = _SEQ_DTYPES[q.dtype]
