@@ -276,24 +276,26 @@ __global__ __launch_bounds__((64 * PgCfg<T, CT, DHP>::NW), (PgCfg<T, CT, DHP>::W
     }
 }
 
-// joins the splits of a tile's rows: o = sum_z 2^(m_z - m) o_z / sum_z 2^(m_z - m) l_z, a wave a row (grid y: groups of four rows).  A
-// wave is 64 / LPR groups of LPR lanes; group g takes the splits z = g (mod 64 / LPR), four elements a lane, and the groups are added.
-struct PgJoinP { SeqFwdP f; int R, quantum, least; };
+// Joins: o = sum_z 2^(m_z - m) o_z / sum_z 2^(m_z - m) l_z over the splits z of a row.
+//
+// Few rows of many splits (the rows form): a wave a row (grid y: groups of four rows).  A wave is 64 / LPR groups of LPR lanes;
+// group g takes the splits z = g (mod 64 / LPR), four elements a lane, and the groups are added.
+struct PgJoinP { SeqFwdP f; int quantum, least; };
 template <typename T, int LPR>
 __global__ __launch_bounds__(256) void paged_join_kernel(PgJoinP j) {
     const SeqFwdP& p = j.f;
     constexpr int NG = 64 / LPR;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int hk = blockIdx.x % p.Hkv;
-    const SeqUnit un = find_unit(p.starts, p.lens, 1, p.most, p.B, p.tokens, p.G, j.R, p.slots, j.quantum, j.least, blockIdx.x / p.Hkv, true);
+    const SeqUnit un = find_unit(p.starts, p.lens, 1, p.most, p.B, p.tokens, p.G, 32, p.slots, j.quantum, j.least, blockIdx.x / p.Hkv, true);
     if (un.t.seq < 0 || un.nsplit < 2) return;
-    if (un.first + (long)(un.nsplit - 1) * un.t.ntile >= seq_split_units(p.tokens, p.B, p.G, j.R, p.slots)) return;      // (`starts` that overlap)
-    const int rows = un.t.n * p.G, live = min(j.R, rows - un.t.tile * j.R);
+    if (un.first + (long)(un.nsplit - 1) * un.t.ntile >= seq_split_units(p.tokens, p.B, p.G, 32, p.slots)) return;      // (`starts` that overlap)
+    const int rows = un.t.n * p.G, live = min(32, rows - un.t.tile * 32);
     const int c = (lane % LPR) * 4, g = lane / LPR;
     for (int row = blockIdx.y * 4 + wave; row < live; row += 4 * gridDim.y) {
         float m = -INFINITY, l = 0.f;
         float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-        const long step = (long)p.Hkv * j.R * un.t.ntile, base = (un.first * p.Hkv + hk) * j.R + row;
+        const long step = 32L * p.Hkv * un.t.ntile, base = (un.first * p.Hkv + hk) * 32 + row;
         for (int z0 = 0; z0 < un.nsplit; z0 += 64) {
             float2 ml = make_float2(-INFINITY, 0.f);
             if (z0 + lane < un.nsplit) ml = *reinterpret_cast<const float2*>(p.part_ml + (base + (z0 + lane) * step) * 2);
@@ -326,26 +328,81 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PgJoinP j) {
         }
         if (g != 0 || c >= p.dh) continue;
         const float inv = l == 0.f ? 0.f : 1.f / l;
-        const int rr = un.t.tile * j.R + row, t = rr / p.G;
+        const int rr = un.t.tile * 32 + row, t = rr / p.G;
+        T* dst = (T*)p.o + (long)(un.t.s0 + t) * p.o_row + (long)(hk * p.G + rr - t * p.G) * p.o_head + c;
+        dst[0] = (T)(acc.x * inv); dst[1] = (T)(acc.y * inv); dst[2] = (T)(acc.z * inv); dst[3] = (T)(acc.w * inv);
+    }
+}
+// Many rows of few splits (the tile form): 16 rows a workgroup (grid y), four elements a thread, over the splits in their order,
+// four of them in flight.
+template <typename T>
+__global__ __launch_bounds__(256) void paged_join_tiles_kernel(PgJoinP j) {
+    const SeqFwdP& p = j.f;
+    const int hk = blockIdx.x % p.Hkv;
+    const SeqUnit un = find_unit(p.starts, p.lens, 1, p.most, p.B, p.tokens, p.G, 128, p.slots, j.quantum, j.least, blockIdx.x / p.Hkv, true);
+    if (un.t.seq < 0 || un.nsplit < 2) return;
+    if (un.first + (long)(un.nsplit - 1) * un.t.ntile >= seq_split_units(p.tokens, p.B, p.G, 128, p.slots)) return;      // (`starts` that overlap)
+    const int r0 = un.t.tile * 128 + 16 * blockIdx.y, live = min(16, un.t.n * p.G - r0), per = p.dh / 4;
+    const long step = 128L * p.Hkv * un.t.ntile;
+    for (int i = threadIdx.x; i < live * per; i += 256) {
+        const int row = i / per, c = (i - row * per) * 4;
+        const long base = (un.first * p.Hkv + hk) * 128 + 16 * blockIdx.y + row;
+        float m = -INFINITY, l = 0.f;
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int z0 = 0; z0 < un.nsplit; z0 += 4) {
+            float2 ml[4];
+            float4 b[4];
+#pragma unroll
+            for (int z = 0; z < 4; ++z) {
+                const long at = base + min(z0 + z, un.nsplit - 1) * step;
+                ml[z] = *reinterpret_cast<const float2*>(p.part_ml + 2 * at);
+                b[z] = *reinterpret_cast<const float4*>(p.part_o + at * p.dh + c);
+            }
+            float top = m;
+#pragma unroll
+            for (int z = 0; z < 4; ++z) top = fmaxf(top, ml[z].x);
+            const float ms = top == -INFINITY ? 0.f : top, a = __builtin_amdgcn_exp2f(m - ms);
+            m = top;
+            l *= a;
+            acc.x *= a; acc.y *= a; acc.z *= a; acc.w *= a;
+#pragma unroll
+            for (int z = 0; z < 4; ++z) {
+                if (z0 + z >= un.nsplit || ml[z].y == 0.f) continue;      // (an empty split left its rows unwritten)
+                const float w = __builtin_amdgcn_exp2f(ml[z].x - ms);
+                l += w * ml[z].y;
+                acc.x += w * b[z].x; acc.y += w * b[z].y; acc.z += w * b[z].z; acc.w += w * b[z].w;
+            }
+        }
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+        const int rr = r0 + row, t = rr / p.G;
         T* dst = (T*)p.o + (long)(un.t.s0 + t) * p.o_row + (long)(hk * p.G + rr - t * p.G) * p.o_head + c;
         dst[0] = (T)(acc.x * inv); dst[1] = (T)(acc.y * inv); dst[2] = (T)(acc.z * inv); dst[3] = (T)(acc.w * inv);
     }
 }
 template <typename T>
-static void pg_join_launch(const PgJoinP& j, hipStream_t st) {
+static void pg_join_launch(const PgJoinP& j, bool rows_form, hipStream_t st) {
     const SeqFwdP& p = j.f;
+    if (!rows_form) {
+        hipLaunchKernelGGL((paged_join_tiles_kernel<T>), dim3((unsigned)(seq_units(p.tokens, p.B, p.G, 128) * p.Hkv), 8), dim3(256), 0, st, j);
+        return;
+    }
     const int groups = (int)((p.tokens * (long)p.G + 3) / 4);
-    const dim3 g((unsigned)(seq_units(p.tokens, p.B, p.G, j.R) * p.Hkv), (unsigned)(groups < j.R / 4 ? groups : j.R / 4));
+    const dim3 g((unsigned)(seq_units(p.tokens, p.B, p.G, 32) * p.Hkv), (unsigned)(groups < 8 ? groups : 8));
     if (p.dh <= 64) hipLaunchKernelGGL((paged_join_kernel<T, 16>), g, dim3(256), 0, st, j);
     else if (p.dh <= 128) hipLaunchKernelGGL((paged_join_kernel<T, 32>), g, dim3(256), 0, st, j);
     else hipLaunchKernelGGL((paged_join_kernel<T, 64>), g, dim3(256), 0, st, j);
 }
 
 // ---- launches -----------------------------------------------------------------------------------------
-// The rows form: up to 32 rows a sequence on average, and rows of whole 16-byte pieces.
+// The rows form: rows of whole 16-byte pieces, and up to 16 of them a sequence on average in a bf16 cache (64 sequences of 512
+// keys, 16 heads of 64: 58 us against the tile form's 34 with 8 rows, 71 against 32 with 32; 8 of 4096, 32 / 8 heads of 128: 37
+// against 36 with 8, 41 against 37 with 32, 108 against 61 with 256; one row, 32 ragged ones, 8 heads of 64: 69 against 80), up to
+// 64 elsewhere, where the tile form spends its time on converting and multiplying rows that are not there (e4m3, 64 sequences of
+// 4096 keys, 32 / 8 heads of 128: 139 us against 164 with 32 rows, 148 against 175 with 64, 283 against 183 with 128; fp32, 32
+// ragged ones, 4 heads of 64: 69 against 263 with one row).
 static bool pg_rows_form(int B, int tokens, int G, int dh, int cache_dtype) {
     const int size = cache_dtype == TTSMI_F32 ? 4 : cache_dtype == TTSMI_E4M3 ? 1 : 2;
-    return (long)tokens * G <= 32L * B && dh * size % 16 == 0;
+    return (long)tokens * G <= (size == 2 ? 16L : 64L) * B && dh * size % 16 == 0;
 }
 // Key splits a key head: together as many workgroups as the card holds at once; none where the tiles alone fill it.
 template <typename T, typename CT>
@@ -353,13 +410,16 @@ static int pg_resident(int dh) {
     return 256 * (dh <= 64 ? PgCfg<T, CT, 64>::RESIDENT : dh <= 128 ? PgCfg<T, CT, 128>::RESIDENT : PgCfg<T, CT, 192>::RESIDENT);
 }
 static int pg_slots(int B, int tokens, int Hkv, int G, int dh, bool rows_form, int cache_dtype, int dtype) {
-    int all = 1024;
+    // (the tile form: 8192 keys and 512 new tokens of 32 / 8 heads of 128, 128 tiles: 93 us at 512, 104 at 1024, 111 at 256, 178
+    // unsplit; 16 sequences of 2048 keys and 64 new tokens, 256 tiles: 56 us unsplit, 66 at 512; ragged ones, [300, 200, 100] new
+    // over [400, 300, 20000] of 16 heads of 64: 45 us at 512, 53 at 1024, 369 unsplit)
+    int all = dtype != TTSMI_F32 && dh <= 128 ? 512 : 256;
     if (rows_form) {
         if (dtype == TTSMI_F32) all = cache_dtype == TTSMI_E4M3 ? pg_resident<float, uint8_t>(dh) : pg_resident<float, float>(dh);
         else all = cache_dtype == TTSMI_E4M3 ? pg_resident<__bf16, uint8_t>(dh) : pg_resident<__bf16, __bf16>(dh);
     }
     const int fill = all / Hkv < 1 ? 1 : all / Hkv;
-    return !rows_form && (long)tokens * G / 128 >= fill ? 0 : fill;
+    return !rows_form && ((long)tokens * G / 128 + (B + 1) / 2) * Hkv >= all ? 0 : fill;
 }
 template <typename T, typename CT>
 static void pg_rows_launch(const SeqFwdP& p, PgJoinP& j, hipStream_t st) {
@@ -407,11 +467,12 @@ extern "C" int ttsmi_paged_attention(const void* q, int64_t q_row, int64_t q_hea
     }
     const bool rows_form = pg_rows_form(B, tokens, p.G, dh, cache_dtype);
     PgJoinP j = {};
-    j.R = rows_form ? 32 : 128; j.quantum = dtype == TTSMI_F32 ? 32 : 64; j.least = SEQ_TILE_LEAST;
+    j.quantum = dtype == TTSMI_F32 ? 32 : 64; j.least = SEQ_TILE_LEAST;
     p.slots = pg_slots(B, tokens, Hkv, p.G, dh, rows_form, cache_dtype, dtype);
     if (p.slots > 0) {
+        const int R = rows_form ? 32 : 128;
         p.part_o = (float*)ws;
-        p.part_ml = (float*)ws + (size_t)seq_split_units(tokens, B, p.G, j.R, p.slots) * Hkv * j.R * dh;
+        p.part_ml = (float*)ws + (size_t)seq_split_units(tokens, B, p.G, R, p.slots) * Hkv * R * dh;
     }
     const long held = (long)table_width << p.pg.shift;
     p.most = n_pages == 0 ? 0 : (int)(held < (1l << 30) ? held : 1l << 30);
@@ -426,8 +487,8 @@ extern "C" int ttsmi_paged_attention(const void* q, int64_t q_row, int64_t q_hea
     ttsmi_note_kernel(rows_form ? "paged_rows_kernel" : "seq_attn_fwd_kernel");
     if (p.slots > 0) {
         j.f = p;
-        if (dtype == TTSMI_F32) pg_join_launch<float>(j, st);
-        else pg_join_launch<__bf16>(j, st);
+        if (dtype == TTSMI_F32) pg_join_launch<float>(j, rows_form, st);
+        else pg_join_launch<__bf16>(j, rows_form, st);
     }
     TTSMI_CHECK_LAUNCH("paged_attention");
     return TTSMI_OK;
