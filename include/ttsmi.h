@@ -823,19 +823,22 @@ int ttsmi_rotary(const void* q, int64_t q_row, int64_t q_head, void* qo, int64_t
                  ttsmi_stream_t stream);
 /* out = softmax(scale q k^T) v within each sequence, causal != 0: over the keys up to the query's own.  scale > 0.  The sums
  * are held in fp32; bf16: the probabilities are rounded to bf16 for the product with v.  lse [Hkv, tokens, H / Hkv] fp32
- * (natural log; may be NULL) is what the backward reads.  A masked score never reaches the softmax, whatever k holds.  A NaN
+ * (natural log; may be NULL) is what the backward reads;
+ * out_rest [tokens, H, dh] bf16 (contiguous; may be NULL; not used for fp32) is what the rounding of out to bf16 left, with
+ * which the backward is more exact.  A masked score never reaches the softmax, whatever k holds.  A NaN
  * or infinity in a VALUE row, which the product meets with a zero where it is masked, may reach rows of its own sequence up to
  * 127 tokens in front of it (in the backward: one in q, k, v or dout, gradient rows up to 127 tokens off); never another
  * sequence, nor from tokens of none. */
 int ttsmi_packed_attention_fwd(const void* q, int64_t q_row, int64_t q_head, const void* k, int64_t k_row, int64_t k_head,
                                const void* v, int64_t v_row, int64_t v_head, const int32_t* starts, int B, int tokens, int H,
                                int Hkv, int dh, float scale, int causal, void* out, int64_t o_row, int64_t o_head, float* lse,
-                               int zero_rest, int dtype, ttsmi_stream_t stream);
-/* Gradients of q, k and v (summed over the query heads of a group); deterministic.  out and lse are the forward's. */
+                               void* out_rest, int zero_rest, int dtype, ttsmi_stream_t stream);
+/* Gradients of q, k and v (summed over the query heads of a group); deterministic.  out, out_rest (or
+ * NULL) and lse are the forward's. */
 size_t ttsmi_packed_attention_bwd_ws_bytes(int B, int tokens, int H, int Hkv, int dh, int causal);
 int ttsmi_packed_attention_bwd(const void* q, int64_t q_row, int64_t q_head, const void* k, int64_t k_row, int64_t k_head,
                                const void* v, int64_t v_row, int64_t v_head, const void* out, int64_t o_row, int64_t o_head,
-                               const void* dout, int64_t d_row, int64_t d_head, const float* lse, const int32_t* starts, int B,
+                               const void* out_rest, const void* dout, int64_t d_row, int64_t d_head, const float* lse, const int32_t* starts, int B,
                                int tokens, int H, int Hkv, int dh, float scale, int causal, void* dq, int64_t dq_row,
                                int64_t dq_head, void* dk, int64_t dk_row, int64_t dk_head, void* dv, int64_t dv_row,
                                int64_t dv_head, int zero_rest, void* ws, size_t ws_bytes, int dtype, ttsmi_stream_t stream);

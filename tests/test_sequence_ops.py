@@ -19,11 +19,11 @@ F32, BF16, E4M3 = 0, 2, 4
 
 def _packed(lib, bwd=False, **over):
     a = dict(q=ONE, q_row=256, q_head=64, k=ONE, k_row=128, k_head=64, v=ONE, v_row=128, v_head=64, out=ONE, o_row=256, o_head=64, dout=ONE,
-             d_row=256, d_head=64, lse=ONE, starts=ONE, B=2, tokens=10, H=4, Hkv=2, dh=64, scale=0.125, causal=1, dq=ONE, dq_row=256, dq_head=64,
+             d_row=256, d_head=64, lse=ONE, rest=ONE, starts=ONE, B=2, tokens=10, H=4, Hkv=2, dh=64, scale=0.125, causal=1, dq=ONE, dq_row=256, dq_head=64,
              dk=ONE, dk_row=128, dk_head=64, dv=ONE, dv_row=128, dv_head=64, zero_rest=1, ws=ONE, ws_bytes=1 << 30, dtype=BF16)
     a.update(over)
-    fwd = 'q q_row q_head k k_row k_head v v_row v_head starts B tokens H Hkv dh scale causal out o_row o_head lse zero_rest dtype'
-    back = ('q q_row q_head k k_row k_head v v_row v_head out o_row o_head dout d_row d_head lse starts B tokens H Hkv dh scale causal dq dq_row '
+    fwd = 'q q_row q_head k k_row k_head v v_row v_head starts B tokens H Hkv dh scale causal out o_row o_head lse rest zero_rest dtype'
+    back = ('q q_row q_head k k_row k_head v v_row v_head out o_row o_head rest dout d_row d_head lse starts B tokens H Hkv dh scale causal dq dq_row '
             'dq_head dk dk_row dk_head dv dv_row dv_head zero_rest ws ws_bytes dtype')
     f = lib.ttsmi_packed_attention_bwd if bwd else lib.ttsmi_packed_attention_fwd
     return f(*[a[n] for n in (back if bwd else fwd).split()], None), lib.ttsmi_last_error()
@@ -34,7 +34,7 @@ def _packed(lib, bwd=False, **over):
     (dict(dh=60), -1, b'head size'), (dict(dh=200), -1, b'head size'), (dict(dh=0), -1, b'head size'), (dict(scale=0.0), -1, b'scale'),
     (dict(scale=-1.0), -1, b'scale'), (dict(scale=float('nan')), -1, b'scale'), (dict(scale=float('inf')), -1, b'scale'), (dict(tokens=-1), -1, b'tokens'),
     (dict(B=-1), -1, b'sequences'), (dict(tokens=1 << 30), -1, b'too large'), (dict(starts=None), -1, b'starts'), (dict(q=None), -1, b'null'),
-    (dict(k=ODD), -1, b'aligned'), (dict(v_row=132), -1, b'aligned'), (dict(q_head=60), -1, b'aligned'), (dict(out=None), -1, b'null'), (dict(k_row=-128), -1, b'aligned'),
+    (dict(k=ODD), -1, b'aligned'), (dict(v_row=132), -1, b'aligned'), (dict(q_head=60), -1, b'aligned'), (dict(out=None), -1, b'null'), (dict(rest=ODD), -1, b'aligned'), (dict(k_row=-128), -1, b'aligned'),
     (dict(k_row=1 << 24), -1, b'too far apart'), (dict(q_head=1 << 30), -1, b'too far apart'), (dict(q_row=1 << 40), -1, b'too far apart')])
 @pytest.mark.parametrize('bwd', [False, True])
 def test_packed_attention_refuses(lib, over, code, word, bwd):

@@ -212,7 +212,7 @@ def test_packed_attention_rows_behind_the_last_sequence():
         assert torch.equal(g[:used], w) and not g[used:].any()
     out = torch.full((M, H, dh), 7.0, device=DEV)
     args = [a for t in (q, k, v) for a in (t.data_ptr(), t.stride(0), t.stride(1))]
-    assert _lib.lib().ttsmi_packed_attention_fwd(*args, st.data_ptr(), 2, M, H, Hkv, dh, dh ** -0.5, 1, out.data_ptr(), H * dh, dh, None, 0,
+    assert _lib.lib().ttsmi_packed_attention_fwd(*args, st.data_ptr(), 2, M, H, Hkv, dh, dh ** -0.5, 1, out.data_ptr(), H * dh, dh, None, None, 0,
                                                  _lib.TTSMI_F32, torch.cuda.current_stream().cuda_stream) == 0
     assert torch.equal(out[:used], want[0]) and bool((out[used:] == 7).all())
     none = ops.packed_attention(*(t.detach() for t in xs), torch.zeros(1, dtype=torch.int32, device=DEV))
@@ -292,6 +292,61 @@ def test_packed_attention_on_another_stream_and_twice():
     again = go()
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) and torch.equal(a, c) for a, b, c in zip(want, got, again))
+
+
+def test_packed_attention_keeps_what_the_rounding_left():
+    """The forward's second output is at most half a step of the first, and dq is closer to the formula's with it than without
+    (peaked scores: delta is then half of a small difference; 9 % here by arithmetic, the rounding of the score gradients and of
+    dq itself stay)."""
+    from transformertts_amd import _lib
+    ops = _ops()
+    n, H, dh = 1500, 2, 128
+    q, k, v, d = (_randn((n, H, dh), 70 + i, torch.bfloat16, 1.25 if i < 2 else 1.0) for i in range(4))
+    want, _ = packed_oracle(q, k, v, [n], True, dh ** -0.5, d)
+    q, k, v, d, st = (t.to(DEV) for t in (q, k, v, d, _starts([n])))
+    out, lse, rest = ops._packed_fwd(q, k, v, st, dh ** -0.5, True, True)
+    assert rest.any() and bool((rest.float().abs() <= 2.0 ** -8 * out.float().abs() + 2.0 ** -126).all())
+    off = []
+    for r in (rest.data_ptr(), None):
+        g = [torch.zeros_like(t) for t in (q, k, v)]
+        args = lambda *ts: [a for t in ts for a in (t.data_ptr(), t.stride(0), t.stride(1))]
+        ws = torch.empty(_lib.lib().ttsmi_packed_attention_bwd_ws_bytes(1, n, H, H, dh, 1) + 256, dtype=torch.uint8, device=DEV)
+        assert _lib.lib().ttsmi_packed_attention_bwd(*args(q, k, v, out), r, *args(d), lse.data_ptr(), st.data_ptr(), 1, n, H, H, dh, dh ** -0.5, 1, *args(*g), 1,
+                                                     ws.data_ptr(), ws.numel(), _lib.TTSMI_BF16_IO, torch.cuda.current_stream().cuda_stream) == 0
+        off.append(float((g[0].double().cpu() - want[1]).norm() / want[1].norm()))
+    assert off[0] < 0.98 * off[1] and off[0] < 0.003, off
+
+
+def test_training_steps_of_two_threads_at_once():
+    """Each on its own stream, forward and backward interleaved as they come."""
+    import threading
+    ops = _ops()
+    freqs = torch.rand(32, dtype=torch.float64, device=DEV)
+    jobs = []
+    for i, lens in enumerate(([300, 212, 700], [1024, 33])):
+        M = sum(lens)
+        x = [_randn((M, h, 64), 10 * i + j, torch.bfloat16).to(DEV) for j, h in enumerate((8, 2, 2, 8))]
+        jobs.append((x, _starts(lens).to(DEV), torch.arange(M, dtype=torch.int32, device=DEV)))
+    def step(x, st, pos):
+        y = [t.clone().requires_grad_() for t in x[:3]]
+        q, k = ops.rotary(y[0], y[1], pos, freqs)
+        return _grads(ops.packed_attention(q, k, y[2], st), y, x[3])
+    want = [step(*j) for j in jobs]
+    torch.cuda.synchronize()
+    bad = []
+    def work(n):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(15):
+                got = step(*jobs[n])
+                torch.cuda.current_stream().synchronize()
+                if not all(torch.equal(a, b) for a, b in zip(got, want[n])):
+                    bad.append(n)
+    threads = [threading.Thread(target=work, args=(n,)) for n in (0, 1)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad
 
 
 # ------------------------------------------------------------------------------------------------------------------ rotary

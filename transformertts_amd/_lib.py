@@ -139,9 +139,9 @@ SIGNATURES = {
     'ttsmi_add2_f32': (I, [P, P, P, L, S]),
     'ttsmi_pad_cols_f32': (I, [P, I, P, I, I, S]),
     'ttsmi_rotary': (I, [P, L, L, P, L, L, I, P, L, L, P, L, L, I, P, P, I, I, I, I, F, I, I, S]),
-    'ttsmi_packed_attention_fwd': (I, [P, L, L, P, L, L, P, L, L, P, I, I, I, I, I, F, I, P, L, L, P, I, I, S]),
+    'ttsmi_packed_attention_fwd': (I, [P, L, L, P, L, L, P, L, L, P, I, I, I, I, I, F, I, P, L, L, P, P, I, I, S]),
     'ttsmi_packed_attention_bwd_ws_bytes': (c_size_t, [I, I, I, I, I, I]),
-    'ttsmi_packed_attention_bwd': (I, [P, L, L, P, L, L, P, L, L, P, L, L, P, L, L, P, P, I, I, I, I, I, F, I, P, L,
+    'ttsmi_packed_attention_bwd': (I, [P, L, L, P, L, L, P, L, L, P, L, L, P, P, L, L, P, P, I, I, I, I, I, F, I, P, L,
         L, P, L, L, P, L, L, I, P, c_size_t, I, S]),
     'ttsmi_kv_cache_write': (I, [P, L, L, P, L, L, P, P, P, P, I, I, I, P, I, P, P, I, I, I, I, I, S]),
     'ttsmi_kv_cache_read': (I, [P, P, P, P, I, I, I, P, I, P, P, I, I, I, I, P, L, L, P, L, L, I, I, S]),

@@ -310,6 +310,11 @@ __global__ __launch_bounds__(256, (DHP <= 128 && sizeof(T) == 2) ? 2 : 1) void s
 #pragma unroll
                 for (int e = 0; e < 4; ++e) h[e] = (__bf16)(o[cb][4 * g + e] * inv);
                 *reinterpret_cast<bf16x4*>(orow + c) = h;
+                if (!PAGED && p.rest) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) h[e] = (__bf16)(o[cb][4 * g + e] * inv - (float)h[e]);
+                    *reinterpret_cast<bf16x4*>((T*)p.rest + ((long)(st.s0 + tok) * p.Hkv * p.G + head) * p.dh + c) = h;
+                }
             } else {
                 *reinterpret_cast<float4*>(orow + c) = make_float4(o[cb][4 * g] * inv, o[cb][4 * g + 1] * inv, o[cb][4 * g + 2] * inv, o[cb][4 * g + 3] * inv);
             }
@@ -356,15 +361,16 @@ int seq_paged_tiles(const SeqFwdP& p, int dtype, int cache_dtype, hipStream_t st
 extern "C" int ttsmi_packed_attention_fwd(const void* q, int64_t q_row, int64_t q_head, const void* k, int64_t k_row, int64_t k_head,
                                           const void* v, int64_t v_row, int64_t v_head, const int32_t* starts, int B, int tokens,
                                           int H, int Hkv, int dh, float scale, int causal, void* out, int64_t o_row, int64_t o_head,
-                                          float* lse, int zero_rest, int dtype, ttsmi_stream_t stream) {
+                                          float* lse, void* out_rest, int zero_rest, int dtype, ttsmi_stream_t stream) {
     SEQ_CHECK_COMMON("packed_attention_fwd");
     if (tokens == 0) return TTSMI_OK;
     TTSMI_CHECK_ARG(starts, "packed_attention_fwd: null starts");
     TTSMI_CHECK_ARG(seq_strides_ok(q, q_row, q_head, H / Hkv, dtype) && seq_strides_ok(k, k_row, k_head, 1, dtype) && seq_strides_ok(v, v_row, v_head, 1, dtype) &&
                         seq_strides_ok(out, o_row, o_head, 0, dtype), "packed_attention_fwd: a tensor is null or its rows or heads are not 16-byte aligned, or too far apart");
+    TTSMI_CHECK_ARG(((uintptr_t)out_rest & 15) == 0, "packed_attention_fwd: out_rest is not 16-byte aligned");
     SeqFwdP p = {};
     p.q = q; p.q_row = q_row; p.q_head = q_head; p.k = k; p.k_row = k_row; p.k_head = k_head; p.v = v; p.v_row = v_row; p.v_head = v_head;
-    p.o = out; p.zero_rest = zero_rest != 0; p.o_row = o_row; p.o_head = o_head; p.lse = lse; p.starts = starts;
+    p.o = out; p.rest = dtype == TTSMI_BF16_IO ? out_rest : nullptr; p.zero_rest = zero_rest != 0; p.o_row = o_row; p.o_head = o_head; p.lse = lse; p.starts = starts;
     p.B = B; p.tokens = tokens; p.Hkv = Hkv; p.G = H / Hkv; p.dh = dh; p.causal = causal != 0; p.c1 = scale * SEQ_LOG2E;
     return dtype == TTSMI_F32 ? seq_packed_launch<float>(p, (hipStream_t)stream) : seq_packed_launch<__bf16>(p, (hipStream_t)stream);
 }

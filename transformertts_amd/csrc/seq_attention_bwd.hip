@@ -5,7 +5,9 @@
 //   dq_i = scale sum_j ds_ij k_j      dk_j = scale sum_i ds_ij q_i      dv_j = sum_i p_ij do_i      (i: every query head of the group)
 //
 // dQ:     as the forward - 128 rows a workgroup, 32 a wave, S^T and dP^T per key tile, dQ^T += K^T dS^T.  It also forms delta and
-//         lse in log2 units, once, for the second pass.
+//         lse in log2 units, once, for the second pass.  delta is a small difference's other half where a row has a peak: from the
+//         bf16 output alone its error is a third of dq's (2000 causal tokens, heads of 128, scores of deviation 1.6: dq off by
+//         0.26 % instead of 0.24 %, of which 0.17 % is its own rounding), so the forward leaves what its rounding took (out_rest).
 // dK, dV: 128 keys of one key head a workgroup, 32 a wave; the row tiles of every query head of the group pass through LDS, the
 //         wave forms S and dP with a key per lane, so that P and dS are the B operands of dV^T += dO^T P and dK^T += Q^T dS.
 #include "seq_common.h"
@@ -15,6 +17,7 @@ struct SeqBwdP {
     const void* k; long k_row, k_head;
     const void* v; long v_row, v_head;
     const void* o; long o_row, o_head;
+    const void* rest;                                     // [tokens][H][dh]: what the rounding of o to bf16 left, or null
     const void* d; long d_row, d_head;                    // gradient of the output
     void* dq; long dq_row, dq_head;
     void* dk; long dk_row, dk_head;
@@ -88,6 +91,12 @@ __global__ __launch_bounds__(256, (DHP <= 128 && sizeof(T) == 2) ? 2 : 1) void s
 #pragma unroll
         for (int s = 0; s < NS; ++s) {
             const frag f = seq_load8<T>(orow, 16 * s + 8 * hh, 16 * s + 8 * hh < p.dh);
+            if (sizeof(T) == 2 && p.rest) {
+                const frag x = seq_load8<T>((const T*)p.rest + ((long)(st.s0 + tok) * p.Hkv * p.G + head) * p.dh, 16 * s + 8 * hh, 16 * s + 8 * hh < p.dh);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) delta += ((float)f[e] + (float)x[e]) * (float)df[s][e];
+                continue;
+            }
 #pragma unroll
             for (int e = 0; e < 8; ++e) delta += (float)f[e] * (float)df[s][e];
         }
@@ -448,7 +457,7 @@ extern "C" size_t ttsmi_packed_attention_bwd_ws_bytes(int B, int tokens, int H, 
 }
 extern "C" int ttsmi_packed_attention_bwd(const void* q, int64_t q_row, int64_t q_head, const void* k, int64_t k_row, int64_t k_head,
                                           const void* v, int64_t v_row, int64_t v_head, const void* out, int64_t o_row, int64_t o_head,
-                                          const void* dout, int64_t d_row, int64_t d_head, const float* lse, const int32_t* starts,
+                                          const void* out_rest, const void* dout, int64_t d_row, int64_t d_head, const float* lse, const int32_t* starts,
                                           int B, int tokens, int H, int Hkv, int dh, float scale, int causal, void* dq, int64_t dq_row,
                                           int64_t dq_head, void* dk, int64_t dk_row, int64_t dk_head, void* dv, int64_t dv_row,
                                           int64_t dv_head, int zero_rest, void* ws, size_t ws_bytes, int dtype, ttsmi_stream_t stream) {
@@ -459,6 +468,7 @@ extern "C" int ttsmi_packed_attention_bwd(const void* q, int64_t q_row, int64_t 
                         seq_strides_ok(out, o_row, o_head, 0, dtype) && seq_strides_ok(dout, d_row, d_head, H / Hkv, dtype) &&
                         seq_strides_ok(dq, dq_row, dq_head, 0, dtype) && seq_strides_ok(dk, dk_row, dk_head, 0, dtype) &&
                         seq_strides_ok(dv, dv_row, dv_head, 0, dtype), "packed_attention_bwd: a tensor is null or its rows or heads are not 16-byte aligned, or too far apart");
+    TTSMI_CHECK_ARG(((uintptr_t)out_rest & 15) == 0, "packed_attention_bwd: out_rest is not 16-byte aligned");
     const size_t need = ttsmi_packed_attention_bwd_ws_bytes(B, tokens, H, Hkv, dh, causal);
     if (!ws || ws_bytes < need || ((uintptr_t)ws & 15)) {
         ttsmi_set_error("packed_attention_bwd: workspace of %zu bytes, %zu (16-byte aligned) needed", ws_bytes, need);
@@ -466,7 +476,7 @@ extern "C" int ttsmi_packed_attention_bwd(const void* q, int64_t q_row, int64_t 
     }
     SeqBwdP p = {};
     p.q = q; p.q_row = q_row; p.q_head = q_head; p.k = k; p.k_row = k_row; p.k_head = k_head; p.v = v; p.v_row = v_row; p.v_head = v_head;
-    p.o = out; p.o_row = o_row; p.o_head = o_head; p.d = dout; p.d_row = d_row; p.d_head = d_head;
+    p.o = out; p.rest = dtype == TTSMI_BF16_IO ? out_rest : nullptr; p.o_row = o_row; p.o_head = o_head; p.d = dout; p.d_row = d_row; p.d_head = d_head;
     p.dq = dq; p.dq_row = dq_row; p.dq_head = dq_head; p.dk = dk; p.dk_row = dk_row; p.dk_head = dk_head; p.dv = dv; p.dv_row = dv_row; p.dv_head = dv_head;
     p.lse = lse; p.delta = (float*)ws; p.lse2 = (float*)ws + (size_t)tokens * H; p.starts = starts; p.B = B; p.tokens = tokens; p.Hkv = Hkv; p.G = H / Hkv; p.dh = dh;
     p.causal = causal != 0; p.zero_rest = zero_rest != 0; p.scale = scale; p.c1 = scale * SEQ_LOG2E;

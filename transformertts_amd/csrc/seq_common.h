@@ -277,6 +277,7 @@ struct SeqFwdP {
     const void* v; long v_row, v_head;
     void* o; long o_row, o_head;
     float* lse;                                           // [Hkv][tokens G] natural log, or null
+    void* rest;                                           // [tokens][H][dh]: what the rounding of o to bf16 left, or null
     const int* starts; const int* lens;                   // lens: paged only (tokens in the cache, the new ones among them)
     SeqPages pg;
     int B, tokens, Hkv, G, dh, causal, zero_rest;

@@ -2223,11 +2223,12 @@ def _scale_of(scale, dh):
 
 
 # ---- rotary positions ----------------------------------------------------------------------------------------------
-def _rotary(q, k, qo, ko, positions, freqs, interleaved, scale, inverse):
+def _rotary(q, k, qo, ko, positions, freqs, interleaved, scale, inverse, stream=None):
     none = (None, 0, 0)
     check(_lib.lib().ttsmi_rotary(*_rs(q), *_rs(qo), q.shape[1], *(none if k is None else _rs(k)), *(none if k is None else _rs(ko)),
                                   0 if k is None else k.shape[1], positions.data_ptr(), freqs.data_ptr(), q.shape[0], q.shape[2],
-                                  2 * freqs.numel(), int(interleaved), scale, int(inverse), _SEQ_DTYPES[q.dtype], _seq_stream(q.device.index)), 'rotary')
+                                  2 * freqs.numel(), int(interleaved), scale, int(inverse), _SEQ_DTYPES[q.dtype],
+                                  _seq_stream(q.device.index) if stream is None else stream), 'rotary')
 
 
 class RotaryFn(torch.autograd.Function):
@@ -2250,11 +2251,10 @@ class RotaryFn(torch.autograd.Function):
         grads = [None, None]
         some = [(i, _strided(g, aligned=False)) for i, g in enumerate((dq, dk)) if g is not None and ctx.needs_input_grad[i]]
         if some:
-            with pin_stream(ctx.stream_h):
-                for i, g in some:
-                    grads[i] = torch.empty(g.shape, dtype=g.dtype, device=g.device)
-                (a, ga), (b, gb) = some[0], some[1] if len(some) > 1 else (None, None)
-                _rotary(ga, gb, grads[a], None if b is None else grads[b], positions, freqs, *ctx.cfg, True)
+            for i, g in some:
+                grads[i] = torch.empty(g.shape, dtype=g.dtype, device=g.device)
+            (a, ga), (b, gb) = some[0], some[1] if len(some) > 1 else (None, None)
+            _rotary(ga, gb, grads[a], None if b is None else grads[b], positions, freqs, *ctx.cfg, True, ctx.stream_h)
         return grads[0], grads[1], None, None, None, None
 
 
@@ -2302,15 +2302,16 @@ def rotary(q, k, positions, freqs, interleaved=False, scale=1.0, inplace=False):
 
 
 # ---- attention over packed sequences --------------------------------------------------------------------------------
-def _packed_fwd(q, k, v, starts, scale, causal, want_lse):
+def _packed_fwd(q, k, v, starts, scale, causal, train):
     M, H, dh = q.shape
     Hkv = k.shape[1]
     out = torch.empty((M, H, dh), dtype=q.dtype, device=q.device)
-    lse = torch.empty((Hkv, M, H // Hkv), dtype=torch.float32, device=q.device) if want_lse else None
+    lse = torch.empty((Hkv, M, H // Hkv), dtype=torch.float32, device=q.device) if train else None
+    rest = torch.empty_like(out) if train and q.dtype == torch.bfloat16 else None
     check(_lib.lib().ttsmi_packed_attention_fwd(*_rs(q), *_rs(k), *_rs(v), starts.data_ptr(), starts.numel() - 1, M, H, Hkv, dh, scale,
-                                                int(causal), *_rs(out), _p(lse), 1, _SEQ_DTYPES[q.dtype], _seq_stream(q.device.index)),
+                                                int(causal), *_rs(out), _p(lse), _p(rest), 1, _SEQ_DTYPES[q.dtype], _seq_stream(q.device.index)),
           'packed_attention_fwd')
-    return out, lse
+    return out, lse, rest
 
 
 class PackedAttentionFn(torch.autograd.Function):
@@ -2319,8 +2320,8 @@ class PackedAttentionFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, starts, scale, causal):
         ctx.stream_h = _seq_stream(q.device.index)
-        out, lse = _packed_fwd(q, k, v, starts, scale, causal, True)
-        ctx.save_for_backward(q, k, v, out, lse, starts)
+        out, lse, rest = _packed_fwd(q, k, v, starts, scale, causal, True)
+        ctx.save_for_backward(q, k, v, out, lse, rest, starts)
         ctx.cfg = (scale, causal)
         ctx.set_materialize_grads(False)
         return out
@@ -2329,18 +2330,17 @@ class PackedAttentionFn(torch.autograd.Function):
     def backward(ctx, dout):
         if dout is None:
             return (None,) * 6
-        q, k, v, out, lse, starts = ctx.saved_tensors
+        q, k, v, out, lse, rest, starts = ctx.saved_tensors
         scale, causal = ctx.cfg
         M, H, dh = q.shape
         l = _lib.lib()
-        with pin_stream(ctx.stream_h):
-            dout = _strided(dout, True, H // k.shape[1])
-            dq, dk, dv = torch.empty_like(out), torch.empty(k.shape, dtype=k.dtype, device=k.device), torch.empty(v.shape, dtype=v.dtype, device=v.device)
-            ws = _ws(l.ttsmi_packed_attention_bwd_ws_bytes(starts.numel() - 1, M, H, k.shape[1], dh, int(causal)), q.device)
-            check(l.ttsmi_packed_attention_bwd(*_rs(q), *_rs(k), *_rs(v), *_rs(out), *_rs(dout), lse.data_ptr(), starts.data_ptr(),
-                                               starts.numel() - 1, M, H, k.shape[1], dh, scale, int(causal), *_rs(dq), *_rs(dk),
-                                               *_rs(dv), 1, ws.data_ptr(), ws.numel(), _SEQ_DTYPES[q.dtype], _seq_stream(q.device.index)),
-                  'packed_attention_bwd')
+        B, Hkv = starts.numel() - 1, k.shape[1]
+        dout = _strided(dout, True, H // Hkv)
+        dq, dk, dv = torch.empty_like(out), torch.empty(k.shape, dtype=k.dtype, device=k.device), torch.empty(v.shape, dtype=v.dtype, device=v.device)
+        ws = _ws(l.ttsmi_packed_attention_bwd_ws_bytes(B, M, H, Hkv, dh, int(causal)), q.device)
+        check(l.ttsmi_packed_attention_bwd(*_rs(q), *_rs(k), *_rs(v), *_rs(out), _p(rest), *_rs(dout), lse.data_ptr(), starts.data_ptr(), B, M, H,
+                                           Hkv, dh, scale, int(causal), *_rs(dq), *_rs(dk), *_rs(dv), 1, ws.data_ptr(), ws.numel(),
+                                           _SEQ_DTYPES[q.dtype], ctx.stream_h), 'packed_attention_bwd')
         return dq, dk, dv, None, None, None
 
 
