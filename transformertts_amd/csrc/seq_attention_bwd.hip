@@ -10,6 +10,10 @@
 //         0.26 % instead of 0.24 %, of which 0.17 % is its own rounding), so the forward leaves what its rounding took (out_rest).
 // dK, dV: 128 keys of one key head a workgroup, 32 a wave; the row tiles of every query head of the group pass through LDS, the
 //         wave forms S and dP with a key per lane, so that P and dS are the B operands of dV^T += dO^T P and dK^T += Q^T dS.
+//
+// Bound like the forward, with less softmax and more LDS reads a product.  Measured, causal bf16, 6000 + 1999 + 193 tokens of 16 / 2
+// heads of 128: dQ 265 us (720 TFLOP/s), dK / dV 380 (670) and 22 for the join of its row splits; 32 utterances of 202 .. 900, 4 heads
+// of 64: 35 and 40 us; fp32, 8 utterances of 117 .. 700, 4 / 2 heads of 64: 48, 38 and 5 us.
 #include "seq_common.h"
 
 struct SeqBwdP {
