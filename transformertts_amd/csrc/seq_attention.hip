@@ -16,8 +16,10 @@
 // launch joins them (paged_attention.hip).
 #include "seq_common.h"
 
-// CT: the cache's element type for PAGED (T, or uint8_t = e4m3)
-template <typename T, typename CT, int DHP, bool PAGED, int KS = 1>
+// CT: the cache's element type for PAGED (T, or uint8_t = e4m3).  WIDE: pages of whole load instructions (the RPI rows that one
+// brings), so that an instruction has one page and its address is a scalar base and a constant lane offset; without it every lane
+// looks its rows up, forming 64-bit addresses of its own.
+template <typename T, typename CT, int DHP, bool PAGED, int KS = 1, bool WIDE = false>
 __global__ __launch_bounds__(256, (DHP <= 128 && sizeof(T) == 2) ? 2 : 1) void seq_attn_fwd_kernel(SeqFwdP p) {
     using I = SeqImg<T, DHP>;
     using frag = typename SeqT<T>::frag;
@@ -63,6 +65,8 @@ __global__ __launch_bounds__(256, (DHP <= 128 && sizeof(T) == 2) ? 2 : 1) void s
         kbeg = min(un.split * un.per, kend);
         kend = min(kbeg + un.per, kend);
     }
+    kbeg = __builtin_amdgcn_readfirstlane(kbeg);
+    kend = __builtin_amdgcn_readfirstlane(kend);
     const int wlast = min(wrow + 31, rows - 1) / p.G;
     const int wend = wrow >= rows ? 0 : min(kend, p.causal ? max(off + wlast + 1, 0) : len);
     const int wfull = wrow + 31 < rows ? (p.causal ? off + wrow / p.G + 1 : len) : 0;     // keys that every row of the wave sees
@@ -94,12 +98,18 @@ __global__ __launch_bounds__(256, (DHP <= 128 && sizeof(T) == 2) ? 2 : 1) void s
             vo[i] = D::row(i, wave, lane) * (uint32_t)(p.v_row * (long)sizeof(T)) + D::piece(i, wave, lane, p.dh);
         }
     }
+    constexpr int RPI = 64 / I::CH;
     int pid[PAGED ? ITEMS : 1];                           // page numbers of the next tile's rows, as they come
     uint32_t gone = 0, gone_next = 0;                     // bit i: item i's row of the tile has no page
     uint2 wk[Q8 ? ITEMS : 1], wv[Q8 ? ITEMS : 1];
     uint32_t ek[Q8 ? ITEMS : 1], ev[Q8 ? ITEMS : 1];
     auto look = [&](int k0) {
-        if constexpr (PAGED) {
+        if constexpr (WIDE) {
+            typedef __attribute__((address_space(4))) const int* scalar;                     // (a scalar load: uniform, and not written meanwhile)
+            const scalar trow = (scalar)(p.pg.table + (long)st.seq * p.pg.table_width);
+#pragma unroll
+            for (int i = 0; i < ITEMS; ++i) pid[i] = trow[min(k0 + (wave + 4 * i) * RPI, kend - 1) >> p.pg.shift];
+        } else if constexpr (PAGED) {
             const int* const trow = p.pg.table + (long)st.seq * p.pg.table_width;
 #pragma unroll
             for (int i = 0; i < ITEMS; ++i) {
@@ -110,8 +120,19 @@ __global__ __launch_bounds__(256, (DHP <= 128 && sizeof(T) == 2) ? 2 : 1) void s
     };
     auto fetch = [&](int k0, int buf) {
         unsigned char* const img = sm + buf * 2 * IMG;
-        long at[PAGED ? ITEMS : 1];
-        if constexpr (PAGED) {
+        long at[PAGED ? ITEMS : 1];                       // the lane's row of the pages; WIDE: the instruction's first row
+        uint32_t in[WIDE ? ITEMS : 1];                    // WIDE: the lane's row behind it
+        if constexpr (WIDE) {
+            gone_next = 0;
+#pragma unroll
+            for (int i = 0; i < ITEMS; ++i) {
+                const int first = min(k0 + (wave + 4 * i) * RPI, kend - 1);
+                const bool ok = (unsigned)pid[i] < (unsigned)p.pg.n_pages;
+                if (!ok) gone_next |= 1u << i;
+                at[i] = (((long)(ok ? pid[i] : 0) * p.pg.heads + hk) << p.pg.shift) + (first & ((1 << p.pg.shift) - 1));
+                in[i] = min(lane / I::CH, kend - 1 - first);
+            }
+        } else if constexpr (PAGED) {
 #pragma unroll
             for (int i = 0; i < ITEMS; ++i) asm volatile("" : "+v"(pid[i]));                  // all of them, in front of the first load below
             gone_next = 0;
@@ -130,8 +151,9 @@ __global__ __launch_bounds__(256, (DHP <= 128 && sizeof(T) == 2) ? 2 : 1) void s
                 wk[i] = wv[i] = make_uint2(0u, 0u);
                 ek[i] = ev[i] = 127;
                 if ((gone_next >> i) & 1) continue;
-                const uint8_t* const a = (const uint8_t*)p.pg.k + at[i] * p.dh + c;
-                const uint8_t* const b = (const uint8_t*)p.pg.v + at[i] * p.dh + c;
+                const uint32_t off = (WIDE ? in[i] * (uint32_t)p.dh : 0) + c;
+                const uint8_t* const a = (const uint8_t*)p.pg.k + at[i] * p.dh + off;
+                const uint8_t* const b = (const uint8_t*)p.pg.v + at[i] * p.dh + off;
                 if constexpr (sizeof(T) == 2) {
                     wk[i] = *reinterpret_cast<const uint2*>(a);
                     wv[i] = *reinterpret_cast<const uint2*>(b);
@@ -139,8 +161,16 @@ __global__ __launch_bounds__(256, (DHP <= 128 && sizeof(T) == 2) ? 2 : 1) void s
                     wk[i].x = *reinterpret_cast<const uint32_t*>(a);
                     wv[i].x = *reinterpret_cast<const uint32_t*>(b);
                 }
-                ek[i] = p.pg.ke[at[i]];
-                ev[i] = p.pg.ve[at[i]];
+                ek[i] = p.pg.ke[at[i] + (WIDE ? in[i] : 0)];
+                ev[i] = p.pg.ve[at[i] + (WIDE ? in[i] : 0)];
+            }
+        } else if constexpr (WIDE) {
+            const uint32_t rb = (uint32_t)p.dh * (uint32_t)sizeof(T);
+#pragma unroll
+            for (int i = 0; i < ITEMS; ++i) {
+                const uint32_t off = in[i] * rb + D::piece(i, wave, lane, p.dh);
+                seq_dma16((const char*)p.pg.k + at[i] * rb, off, seq_lds(img + (wave + 4 * i) * 1024));
+                seq_dma16((const char*)p.pg.v + at[i] * rb, off, seq_lds(img + IMG + (wave + 4 * i) * 1024));
             }
         } else if constexpr (PAGED) {
 #pragma unroll
@@ -329,9 +359,9 @@ __global__ __launch_bounds__(256, (DHP <= 128 && sizeof(T) == 2) ? 2 : 1) void s
 
 // ---- launches -----------------------------------------------------------------------------------------
 
-template <typename T, typename CT, int DHP, bool PAGED, int KS>
+template <typename T, typename CT, int DHP, bool PAGED, int KS, bool WIDE = false>
 static void seq_fwd_go(const SeqFwdP& p, long units, hipStream_t st) {
-    hipLaunchKernelGGL((seq_attn_fwd_kernel<T, CT, DHP, PAGED, KS>), dim3((unsigned)(units * p.Hkv)), dim3(256), 0, st, p);
+    hipLaunchKernelGGL((seq_attn_fwd_kernel<T, CT, DHP, PAGED, KS, WIDE>), dim3((unsigned)(units * p.Hkv)), dim3(256), 0, st, p);
 }
 template <typename T>
 static int seq_packed_launch(const SeqFwdP& p, hipStream_t st) {
@@ -351,7 +381,11 @@ static int seq_packed_launch(const SeqFwdP& p, hipStream_t st) {
 template <typename T, typename CT>
 static int seq_paged_launch(const SeqFwdP& p, hipStream_t st) {
     const long units = p.slots > 0 ? seq_split_units(p.tokens, p.B, p.G, 128, p.slots) : seq_units(p.tokens, p.B, p.G, 128);
-    if (p.dh <= 64) seq_fwd_go<T, CT, 64, true, 1>(p, units, st);
+    // pages of 8 rows or more hold whole instructions of heads up to 128 (RPI 2 .. 8); an image row of 192 is no whole part of one
+    const bool wide = p.pg.shift >= 3;
+    if (p.dh <= 64 && wide) seq_fwd_go<T, CT, 64, true, 1, true>(p, units, st);
+    else if (p.dh <= 64) seq_fwd_go<T, CT, 64, true, 1>(p, units, st);
+    else if (p.dh <= 128 && wide) seq_fwd_go<T, CT, 128, true, 1, true>(p, units, st);
     else if (p.dh <= 128) seq_fwd_go<T, CT, 128, true, 1>(p, units, st);
     else seq_fwd_go<T, CT, 192, true, 1>(p, units, st);
     TTSMI_CHECK_LAUNCH("paged_attention");
