@@ -52,6 +52,9 @@ template <typename T, typename CT, int DHP> struct PgCfg {
     static constexpr int BY_LDS = 163840 / LDS, BY_WAVES = 4 * WPS / NW, RESIDENT = BY_LDS < BY_WAVES ? BY_LDS : BY_WAVES;   // workgroups a compute unit
 };
 
+// keys of a split and wave at least: two blocks (8 single tokens over 200 .. 1500 keys: 19 us; 22 with four)
+#define PG_LEAST 64
+
 template <typename T, typename CT, int DHP>
 __global__ __launch_bounds__((64 * PgCfg<T, CT, DHP>::NW), (PgCfg<T, CT, DHP>::WPS)) void paged_rows_kernel(SeqFwdP p) {
     using C = PgCfg<T, CT, DHP>;
@@ -71,7 +74,7 @@ __global__ __launch_bounds__((64 * PgCfg<T, CT, DHP>::NW), (PgCfg<T, CT, DHP>::W
     float* const mls = reinterpret_cast<float*>(sm + MAIN + (Q8 ? 2 : 1) * SIDE);           // [NW][32][2]
 
     const int hk = blockIdx.x % p.Hkv;
-    const SeqUnit un = find_unit(p.starts, p.lens, 1, p.most, p.B, p.tokens, p.G, 32, p.slots, 32 * NW, 64 * NW, blockIdx.x / p.Hkv, false);
+    const SeqUnit un = find_unit(p.starts, p.lens, 1, p.most, p.B, p.tokens, p.G, 32, p.slots, 32 * NW, PG_LEAST * NW, blockIdx.x / p.Hkv, false);
     if (un.t.seq < 0) {
         if (p.zero_rest) seq_zero_rest<T>((T*)p.o, p.o_row, p.o_head, p.starts, p.B, p.tokens, p.G, 32, hk * p.G, p.dh, un.t.tile);
         return;
@@ -414,9 +417,9 @@ static int pg_resident(int dh) {
     return 256 * (dh <= 64 ? PgCfg<T, CT, 64>::RESIDENT : dh <= 128 ? PgCfg<T, CT, 128>::RESIDENT : PgCfg<T, CT, 192>::RESIDENT);
 }
 static int pg_slots(int B, int tokens, int Hkv, int G, int dh, bool rows_form, int cache_dtype, int dtype) {
-    // (the tile form: 8192 keys and 512 new tokens of 32 / 8 heads of 128, 128 tiles: 93 us at 512, 104 at 1024, 111 at 256, 178
-    // unsplit; 16 sequences of 2048 keys and 64 new tokens, 256 tiles: 56 us unsplit, 66 at 512; ragged ones, [300, 200, 100] new
-    // over [400, 300, 20000] of 16 heads of 64: 45 us at 512, 53 at 1024, 369 unsplit)
+    // (the tile form, before its page lookups became scalars: 8192 keys and 512 new tokens of 32 / 8 heads of 128, 128 tiles: 93 us at
+    // 512, 104 at 1024, 111 at 256, 178 unsplit - 83 at 512 since; 16 sequences of 2048 keys and 64 new tokens, 256 tiles: 56 us
+    // unsplit, 66 at 512; [300, 200, 100] new over [400, 300, 20000] of 16 heads of 64: 45 us at 512, 53 at 1024, 369 unsplit)
     int all = dtype != TTSMI_F32 && dh <= 128 ? 512 : 256;
     if (rows_form) {
         if (dtype == TTSMI_F32) all = cache_dtype == TTSMI_E4M3 ? pg_resident<float, uint8_t>(dh) : pg_resident<float, float>(dh);
@@ -431,7 +434,7 @@ static void pg_rows_launch(const SeqFwdP& p, PgJoinP& j, hipStream_t st) {
 #define PG_GO(D)                                                                                                           \
     do {                                                                                                                   \
         constexpr int NW = PgCfg<T, CT, D>::NW;                                                                               \
-        j.quantum = 32 * NW; j.least = 64 * NW;                                                                            \
+        j.quantum = 32 * NW; j.least = PG_LEAST * NW;                                                                         \
         hipLaunchKernelGGL((paged_rows_kernel<T, CT, D>), g, dim3(64 * NW), 0, st, p);                                     \
     } while (0)
     if (p.dh <= 64) PG_GO(64);

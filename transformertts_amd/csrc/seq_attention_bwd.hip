@@ -33,7 +33,9 @@ struct SeqBwdP {
     // row splits of the dK / dV pass (slots > 0): sums of unit u, key head hk at [(u Hkv + hk)][dK, dV][128 keys][dh], fp32
     int slots; float* part;
 };
-// rows of a split at least: eight tiles of work against the traffic of its partial sums (bf16); the fp32 products are slower
+// rows of a split at least: eight tiles of work against the traffic of its partial sums (bf16: a training step of 8 x 512 tokens, 16 / 4
+// heads of 128, 128 us at 512, 144 at 256, 132 at 1024); the fp32 products are slower (8 utterances of 117 .. 700, 4 / 2 heads of 64:
+// 133 us at 192, 140 at 96, 160 at 384)
 template <typename T> struct SeqLeast { static constexpr int ROWS = sizeof(T) == 2 ? 512 : 192; };
 
 // four accumulator registers -> four consecutive elements of a gradient row
@@ -426,7 +428,8 @@ __global__ __launch_bounds__(256) void seq_dkv_join_kernel(SeqBwdP p) {
 
 // Row splits a key head, for all key heads together: enough for two workgroups a compute unit; three times that where causal, whose
 // splits are empty to a half and uneven at the ends (8192 tokens of three sequences, 16 / 2 heads of 128: dK / dV pass 384 us at
-// 1536, 450 us at 1024, 410 us at 2048).  None where the key tiles alone are that many.
+// 1536, 450 us at 1024, 410 us at 2048; not causal, one sequence of 8192, a training step 2178 us at 512, 2345 at 256, 2206 at 768).  None
+// where the key tiles alone are that many.
 static int seq_bwd_slots(int tokens, int Hkv, int causal) {
     const int all = causal ? 1536 : 512, fill = all / Hkv < 1 ? 1 : all / Hkv;
     return tokens / 128 >= fill ? 0 : fill;
