@@ -132,6 +132,24 @@ def test_packed_attention_many_tiles(dtype, lens, H, Hkv, dh, causal):
         _within(g, w, b, name)
 
 
+@pytest.mark.parametrize('dtype,lens,H,Hkv,dh,causal,parts', [
+    (torch.bfloat16, [1000, 333], 4, 2, 128, True, 'four'), (torch.bfloat16, [700, 90, 400], 8, 8, 64, False, 'four'), (torch.bfloat16, [1999], 6, 2, 40, True, 'four'),
+    (torch.float32, [515, 300], 2, 1, 64, True, 'four'), (torch.float32, [129, 600], 3, 3, 24, False, 'four'), (torch.bfloat16, [900, 7], 8, 8, 128, True, 'four'), (torch.bfloat16, [1500], 8, 8, 128, True, 'two'),
+    (torch.float32, [450, 450], 4, 4, 128, False, 'two'), (torch.bfloat16, [333, 500], 4, 2, 192, True, 'two'), (torch.float32, [60] * 20, 4, 4, 64, True, 'two')])
+def test_packed_attention_keys_in_parts(dtype, lens, H, Hkv, dh, causal, parts):
+    """Few tiles: two or four waves share a row block, the keys between them - parts that have none, or end inside a run, among them."""
+    from transformertts_amd import _lib
+    ops = _ops()
+    M = sum(lens)
+    q, k, v, d = (_randn((M, h, dh), 60 + i, dtype) for i, h in enumerate((H, Hkv, Hkv, H)))
+    want, bound = packed_oracle(q, k, v, lens, causal, dh ** -0.5, d)
+    xs = [x.to(DEV).requires_grad_() for x in (q, k, v)]
+    out = ops.packed_attention(*xs, _starts(lens).to(DEV), causal=causal)
+    assert _lib.lib().ttsmi_last_kernel() == b'seq_attn_fwd_kernel, keys in ' + parts.encode()
+    for name, g, w, b in zip(('out', 'dq', 'dk', 'dv'), _grads(out, xs, d.to(DEV)), want, bound):
+        _within(g, w, b, name)
+
+
 def test_packed_attention_scale_and_peaked_scores():
     """Scores of some hundreds: the running maximum carries them, forward and backward stay finite and right."""
     ops = _ops()
@@ -202,8 +220,8 @@ def test_packed_attention_rows_behind_the_last_sequence():
     H, Hkv, dh, M, used = 4, 2, 64, 700, 133
     st = torch.tensor([0, 100, used], dtype=torch.int32, device=DEV)
     q, k, v, d = (_randn((M, h, dh), i).to(DEV) for i, h in enumerate((H, Hkv, Hkv, H)))
-    clean = [t[:used].clone().requires_grad_() for t in (q, k, v)]
-    want = _grads(ops.packed_attention(*clean, st), clean, d[:used].clone())
+    clean = [t.clone().requires_grad_() for t in (q, k, v)]       # (as many tokens: their number decides how the keys are shared out)
+    want = [t[:used] for t in _grads(ops.packed_attention(*clean, st), clean, d.clone())]
     for t in (q, k, v, d):
         t[used:] = float('nan')
     xs = [t.requires_grad_() for t in (q, k, v)]

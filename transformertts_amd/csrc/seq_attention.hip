@@ -51,7 +51,8 @@ __global__ __launch_bounds__(256, (DHP <= 128 && sizeof(T) == 2) ? 2 : 1) void s
         off = len - st.n;                                 // position of the first new token
     }
     // this lane's row and the number of keys it sees
-    const int half = KS == 2 ? wave >> 1 : 0, wrow = tile * ROWS + (KS == 2 ? wave & 1 : wave) * 32;
+    constexpr int RW = 4 / KS;                            // row blocks of the workgroup; wave: row block wave % RW, part wave / RW
+    const int kpart = wave / RW, wrow = tile * ROWS + wave % RW * 32;
     const int r = wrow + l31;
     const bool rok = r < rows;
     const int tok = r / p.G, head = hk * p.G + r - tok * p.G;
@@ -225,7 +226,7 @@ __global__ __launch_bounds__(256, (DHP <= 128 && sizeof(T) == 2) ? 2 : 1) void s
         if (kbeg + KT < kend) look(kbeg + KT);
     }
     using A = SeqLane<T, DHP>;
-    const uint32_t kbase = A::rows(sm, lane) + half * KW * I::ROWB, vbase = A::cols(sm + IMG, lane) + half * KW * I::ROWB;
+    const uint32_t kbase = A::rows(sm, lane) + kpart * KW * I::ROWB, vbase = A::cols(sm + IMG, lane) + kpart * KW * I::ROWB;
     int buf = 0;
     for (int k0 = kbeg; k0 < kend; k0 += KT, buf ^= 1) {
         land(buf);
@@ -233,7 +234,7 @@ __global__ __launch_bounds__(256, (DHP <= 128 && sizeof(T) == 2) ? 2 : 1) void s
             fetch(k0 + KT, buf ^ 1);
             look(k0 + 2 * KT);
         }
-        const int kw = k0 + half * KW;                    // this wave's keys of the tile
+        const int kw = k0 + kpart * KW;                   // this wave's keys of the tile
         if (kw >= wend) continue;
         const uint32_t ka = kbase + buf * 2 * IMG, va = vbase + buf * 2 * IMG;
         f32x16 s[NKB];
@@ -290,11 +291,12 @@ __global__ __launch_bounds__(256, (DHP <= 128 && sizeof(T) == 2) ? 2 : 1) void s
             }
     }
     l = seq_half_sum(l);
-    if constexpr (KS == 2) {                              // the two halves of the keys: the second wave of a row block hands over
-        constexpr int LDO = DHP + 4;
-        float* const mo = reinterpret_cast<float*>(sm) + (wave & 1) * 32 * (LDO + 2) + l31 * (LDO + 2);
+    if constexpr (KS > 1) {                               // the parts of the keys: a row block's first wave takes over the others' sums
+        constexpr int LDO = DHP + 4, PART = RW * 32 * (LDO + 2);
+        float* mo = reinterpret_cast<float*>(sm) + (wave % RW * 32 + l31) * (LDO + 2);
         seq_dma_barrier();
-        if (half == 1) {
+        if (kpart > 0) {
+            mo += (kpart - 1) * PART;
             if (hh == 0) *reinterpret_cast<float2*>(mo + LDO) = make_float2(m, l);
 #pragma unroll
             for (int cb = 0; cb < NCB; ++cb)
@@ -305,16 +307,19 @@ __global__ __launch_bounds__(256, (DHP <= 128 && sizeof(T) == 2) ? 2 : 1) void s
                         *reinterpret_cast<float2*>(mo + cb * 32 + 8 * g + 4 * hh + 2 * e) = make_float2(o[cb][4 * g + 2 * e], o[cb][4 * g + 2 * e + 1]);
         }
         __syncthreads();
-        if (half == 1) return;
-        const float2 other = *reinterpret_cast<const float2*>(mo + LDO);
-        const float mn = fmaxf(m, other.x), ms = mn == -INFINITY ? 0.f : mn;
-        const float a = __builtin_amdgcn_exp2f(m - ms), b = __builtin_amdgcn_exp2f(other.x - ms);
-        m = mn;
-        l = l * a + other.y * b;
+        if (kpart > 0) return;
 #pragma unroll
-        for (int cb = 0; cb < NCB; ++cb)
+        for (int x = 1; x < KS; ++x, mo += PART) {
+            const float2 other = *reinterpret_cast<const float2*>(mo + LDO);
+            const float mn = fmaxf(m, other.x), ms = mn == -INFINITY ? 0.f : mn;
+            const float a = __builtin_amdgcn_exp2f(m - ms), b = __builtin_amdgcn_exp2f(other.x - ms);
+            m = mn;
+            l = l * a + other.y * b;
 #pragma unroll
-            for (int i = 0; i < 16; ++i) o[cb][i] = o[cb][i] * a + mo[cb * 32 + 8 * (i >> 2) + 4 * hh + (i & 3)] * b;
+            for (int cb = 0; cb < NCB; ++cb)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) o[cb][i] = o[cb][i] * a + mo[cb * 32 + 8 * (i >> 2) + 4 * hh + (i & 3)] * b;
+        }
     }
     if (!rok) return;
     const long slot = (long)hk * p.tokens * p.G + (long)st.s0 * p.G + r;
@@ -365,16 +370,19 @@ static void seq_fwd_go(const SeqFwdP& p, long units, hipStream_t st) {
 }
 template <typename T>
 static int seq_packed_launch(const SeqFwdP& p, hipStream_t st) {
-    const bool two = seq_two_halves(p.tokens, p.B, p.G, p.Hkv, p.dh, sizeof(T) == 4);
-    const long units = seq_units(p.tokens, p.B, p.G, two ? 64 : 128);
-    if (two) {
+    const int parts = seq_key_parts(p.tokens, p.B, p.G, p.Hkv, p.dh, sizeof(T) == 4, p.causal);
+    const long units = seq_units(p.tokens, p.B, p.G, 128 / parts);
+    if (parts == 4) {
+        if (p.dh <= 64) seq_fwd_go<T, T, 64, false, 4>(p, units, st);
+        else if constexpr (sizeof(T) == 2) seq_fwd_go<T, T, 128, false, 4>(p, units, st);
+    } else if (parts == 2) {
         if (p.dh <= 64) seq_fwd_go<T, T, 64, false, 2>(p, units, st);
         else if (p.dh <= 128) seq_fwd_go<T, T, 128, false, 2>(p, units, st);
         else if constexpr (sizeof(T) == 2) seq_fwd_go<T, T, 192, false, 2>(p, units, st);
     } else if (p.dh <= 64) seq_fwd_go<T, T, 64, false, 1>(p, units, st);
     else if (p.dh <= 128) seq_fwd_go<T, T, 128, false, 1>(p, units, st);
     else seq_fwd_go<T, T, 192, false, 1>(p, units, st);
-    ttsmi_note_kernel(two ? "seq_attn_fwd_kernel, two halves" : "seq_attn_fwd_kernel");
+    ttsmi_note_kernel(parts == 4 ? "seq_attn_fwd_kernel, keys in four" : parts == 2 ? "seq_attn_fwd_kernel, keys in two" : "seq_attn_fwd_kernel");
     TTSMI_CHECK_LAUNCH("packed_attention_fwd");
     return TTSMI_OK;
 }

@@ -68,7 +68,8 @@ __global__ __launch_bounds__(256, (DHP <= 128 && sizeof(T) == 2) ? 2 : 1) void s
         return;
     }
     const int tile = st.ntile - 1 - st.tile, rows = st.n * p.G, len = st.n;
-    const int half = KS == 2 ? wave >> 1 : 0, wrow = tile * ROWS + (KS == 2 ? wave & 1 : wave) * 32;
+    constexpr int RW = 4 / KS;                                         // as in the forward
+    const int kpart = wave / RW, wrow = tile * ROWS + wave % RW * 32;
     const int r = wrow + l31;
     const bool rok = r < rows;
     const int tok = r / p.G, head = hk * p.G + r - tok * p.G;
@@ -108,7 +109,7 @@ __global__ __launch_bounds__(256, (DHP <= 128 && sizeof(T) == 2) ? 2 : 1) void s
         }
     }
     delta = seq_half_sum(delta);
-    if (rok && hh == 0 && half == 0) {
+    if (rok && hh == 0 && kpart == 0) {
         p.delta[slot] = delta;
         p.lse2[slot] = lse2;
     }
@@ -141,12 +142,12 @@ __global__ __launch_bounds__(256, (DHP <= 128 && sizeof(T) == 2) ? 2 : 1) void s
     };
     fetch(0, 0);
     using A = SeqLane<T, DHP>;
-    const uint32_t kbase = A::rows(sm, lane) + half * KW * I::ROWB, tbase = A::cols(sm, lane) + half * KW * I::ROWB;
+    const uint32_t kbase = A::rows(sm, lane) + kpart * KW * I::ROWB, tbase = A::cols(sm, lane) + kpart * KW * I::ROWB;
     int buf = 0;
     for (int k0 = 0; k0 < kend; k0 += KT, buf ^= 1) {
         seq_dma_barrier();
         if (k0 + KT < kend) fetch(k0 + KT, buf ^ 1);
-        const int kw = k0 + half * KW;                                 // this wave's keys of the tile
+        const int kw = k0 + kpart * KW;                                // this wave's keys of the tile
         if (kw >= wend) continue;
         const uint32_t ka = kbase + buf * 2 * IMG, ta = tbase + buf * 2 * IMG;
         const bool edge = kw + KW > wfull;
@@ -178,21 +179,25 @@ __global__ __launch_bounds__(256, (DHP <= 128 && sizeof(T) == 2) ? 2 : 1) void s
             }
         }
     }
-    if constexpr (KS == 2) {
-        float* const mo = reinterpret_cast<float*>(sm) + ((wave & 1) * 32 + l31) * (DHP + 4) + 4 * hh;
+    if constexpr (KS > 1) {
+        constexpr int PART = RW * 32 * (DHP + 4);
+        float* mo = reinterpret_cast<float*>(sm) + (wave % RW * 32 + l31) * (DHP + 4) + 4 * hh;
         seq_dma_barrier();
-        if (half == 1) {
+        if (kpart > 0) {
+            mo += (kpart - 1) * PART;
 #pragma unroll
             for (int cb = 0; cb < NCB; ++cb)
 #pragma unroll
                 for (int g = 0; g < 4; ++g) seq_store4<float>(mo + cb * 32 + 8 * g, acc[cb], g, 1.f);
         }
         __syncthreads();
-        if (half == 1) return;
+        if (kpart > 0) return;
 #pragma unroll
-        for (int cb = 0; cb < NCB; ++cb)
+        for (int x = 1; x < KS; ++x, mo += PART)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) acc[cb][i] += mo[cb * 32 + 8 * (i >> 2) + (i & 3)];
+            for (int cb = 0; cb < NCB; ++cb)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) acc[cb][i] += mo[cb * 32 + 8 * (i >> 2) + (i & 3)];
     }
     if (!rok) return;
     T* dst = (T*)p.dq + (long)(st.s0 + tok) * p.dq_row + (long)head * p.dq_head;
@@ -438,12 +443,15 @@ static int seq_bwd_slots(int tokens, int Hkv, int causal) {
 template <typename T, int DHP>
 static void seq_bwd_launch(const SeqBwdP& p, hipStream_t st) {
     // the dQ pass divides its tiles as the forward does
-    const bool two = seq_two_halves(p.tokens, p.B, p.G, p.Hkv, p.dh, sizeof(T) == 4);
-    const dim3 g((unsigned)(seq_units(p.tokens, p.B, p.G, two ? 64 : 128) * p.Hkv));
-    if constexpr (sizeof(T) == 2 || DHP <= 128) {
-        if (two) hipLaunchKernelGGL((seq_attn_dq_kernel<T, DHP, 2>), g, dim3(256), 0, st, p);
+    const int parts = seq_key_parts(p.tokens, p.B, p.G, p.Hkv, p.dh, sizeof(T) == 4, p.causal);
+    const dim3 g((unsigned)(seq_units(p.tokens, p.B, p.G, 128 / parts) * p.Hkv));
+    if constexpr (DHP <= (sizeof(T) == 4 ? 64 : 128)) {
+        if (parts == 4) hipLaunchKernelGGL((seq_attn_dq_kernel<T, DHP, 4>), g, dim3(256), 0, st, p);
     }
-    if (!two) hipLaunchKernelGGL((seq_attn_dq_kernel<T, DHP, 1>), g, dim3(256), 0, st, p);
+    if constexpr (sizeof(T) == 2 || DHP <= 128) {
+        if (parts == 2) hipLaunchKernelGGL((seq_attn_dq_kernel<T, DHP, 2>), g, dim3(256), 0, st, p);
+    }
+    if (parts == 1) hipLaunchKernelGGL((seq_attn_dq_kernel<T, DHP, 1>), g, dim3(256), 0, st, p);
     hipLaunchKernelGGL((seq_attn_dkv_kernel<T, DHP>), dim3((unsigned)((p.slots > 0 ? seq_split_units(p.tokens, p.B, 1, 128, p.slots) : seq_units(p.tokens, p.B, 1, 128)) * p.Hkv)), dim3(256), 0, st, p);
     if (p.slots > 0) hipLaunchKernelGGL((seq_dkv_join_kernel<T>), dim3((unsigned)(seq_units(p.tokens, p.B, 1, 128) * p.Hkv), 8), dim3(256), 0, st, p);
 }

@@ -254,19 +254,26 @@ struct SeqPages {
 // 2^(e - 127) of a stored exponent byte (0 and 255 are not written by the cache kernels)
 __device__ __forceinline__ float seq_scale_of(uint32_t e) { return __builtin_bit_cast(float, e << 23); }
 
-// ---- few tiles: two halves of the keys --------------------------------------------------------------
+// ---- few tiles: the keys in parts --------------------------------------------------------------------
 // With 128 rows a workgroup, 32 a wave, a small batch leaves most of the card idle and its time is one wave's walk over a whole
-// sequence.  Then (KS = 2) a workgroup takes 64 rows, and two waves share a row block: each meets every other KW keys of the tiles,
-// and their sums are joined through LDS at the end.  KW: keys of a wave's step; a stage of KS KW keys has to fit twice.
+// sequence.  Then a workgroup takes 128 / KS rows and KS = 2 or 4 waves share a row block: each meets every KS-th run of KW keys, and
+// their sums are joined through LDS at the end.  KW: keys of a wave's step; a stage of KS KW keys has to fit twice.
 template <typename T, int DHP, int KS> struct SeqKeys {
-    static constexpr int KW = KS == 2 && DHP > 128 ? 32 : SeqT<T>::KT;
+    static constexpr int KW = KS == 4 || (KS == 2 && DHP > 128) ? 32 : SeqT<T>::KT;
 };
-// where the tiles of 128 rows are fewer than the compute units (fp32 heads above 128 have no room for it).  Causal, sequences of
-// 2048, bf16, 16 / 4 heads of 128: 24 us against 29 at 128 tiles, 44 against 49 at 256, 84 against 71 at 384; of 512: 18 against 20
-// at 128, 27 against 22 at 256; fp32, 4 heads of 64, of 2048: 102 against 178 at 128, 157 against 179 at 256.
-static inline bool seq_two_halves(long tokens, int B, int G, int Hkv, int dh, bool f32) {
-    const long tiles = (tokens * G / 128 + (B + 1) / 2) * Hkv;
-    return tiles < 256 && !(f32 && dh > 128);
+// Parts where the workgroups - half a tile more than whole ones a sequence - are about one a compute unit, as far as LDS has room.
+// A causal batch of long sequences is uneven enough for twice as many.  Forward and backward in us with the keys in 1 / 2 / 4:
+//   8 heads of 64, bf16, causal: 1 x 512 tokens 50 / 44 / 41, 3 x 512 52 / 46 / 48, 1 x 2048 107 / 81 / 74, 1 x 3072 146 / 112 / 109, 20 x 102 38 / 41 / 51
+//   16 / 4 heads of 128, bf16, causal: 1 x 512 79 / 71 / 67, 1 x 1024 110 / 94 / 104, 3 x 512 87 / 97 / 118, 1 x 2048 198 / 186 / 244, 10 x 102 57 / 72 / 90
+//   4 heads of 128, bf16, full: 4 x 512 73 / 64 / 64, 8 x 512 77 / 73 / 93, 12 x 512 82 / 105 / 126, 3 x 2048 197 / 243 / 273
+//   4 heads of 64, fp32, causal: 4 x 512 159 / 113 / 89, 6 x 512 185 / 137 / 139, 2 x 2048 576 / 387 / 320, 20 x 102 72 / 60 / 77, 40 x 102 92 / 92 / 118
+static inline int seq_key_parts(long tokens, int B, int G, int Hkv, int dh, bool f32, int causal) {
+    const long mean = tokens / (B > 0 ? B : 1);
+    const bool uneven = causal && mean >= 1024;
+    auto workgroups = [&](int parts) { return (tokens * G * parts / 128 + (B + 1) / 2) * Hkv; };
+    if (dh <= (f32 ? 64 : 128) && mean >= 256 && workgroups(4) <= (uneven && dh <= 64 ? 528 : 320)) return 4;
+    if (!(f32 && dh > 128) && workgroups(2) <= (uneven ? 528 : mean >= 256 ? 288 : 256)) return 2;
+    return 1;
 }
 
 // ---- what a forward launch takes ----
