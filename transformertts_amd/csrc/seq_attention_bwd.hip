@@ -13,7 +13,7 @@
 //
 // Bound like the forward, with less softmax and more LDS reads a product.  Measured, causal bf16, 6000 + 1999 + 193 tokens of 16 / 2
 // heads of 128: dQ 265 us (720 TFLOP/s), dK / dV 380 (670) and 22 for the join of its row splits; 32 utterances of 202 .. 900, 4 heads
-// of 64: 35 and 40 us; fp32, 8 utterances of 117 .. 700, 4 / 2 heads of 64: 48, 38 and 5 us.
+// of 64: 35 and 40 us; fp32, 8 utterances of 117 .. 700, 4 / 2 heads of 64: 32 (48 with two waves a row block), 38 and 5 us.
 #include "seq_common.h"
 
 struct SeqBwdP {

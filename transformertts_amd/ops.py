@@ -10,6 +10,7 @@ for that parameter."""
 from __future__ import annotations
 
 import ctypes
+import functools
 import os
 from typing import Optional
 
@@ -2309,9 +2310,20 @@ def _packed_fwd(q, k, v, starts, scale, causal, train):
     lse = torch.empty((Hkv, M, H // Hkv), dtype=torch.float32, device=q.device) if train else None
     rest = torch.empty_like(out) if train and q.dtype == torch.bfloat16 else None
     check(_lib.lib().ttsmi_packed_attention_fwd(*_rs(q), *_rs(k), *_rs(v), starts.data_ptr(), starts.numel() - 1, M, H, Hkv, dh, scale,
-                                                int(causal), *_rs(out), _p(lse), _p(rest), 1, _SEQ_DTYPES[q.dtype], _seq_stream(q.device.index)),
+                                                int(causal), out.data_ptr(), H * dh, dh, _p(lse), _p(rest), 1, _SEQ_DTYPES[q.dtype],
+                                                _seq_stream(q.device.index)),
           'packed_attention_fwd')
     return out, lse, rest
+
+
+@functools.lru_cache(maxsize=1024)
+def _packed_bwd_ws(*sizes):
+    return _lib.lib().ttsmi_packed_attention_bwd_ws_bytes(*sizes)
+
+
+@functools.lru_cache(maxsize=1024)
+def _paged_ws(*sizes):
+    return _lib.lib().ttsmi_paged_attention_ws_bytes(*sizes)
 
 
 class PackedAttentionFn(torch.autograd.Function):
@@ -2333,14 +2345,15 @@ class PackedAttentionFn(torch.autograd.Function):
         q, k, v, out, lse, rest, starts = ctx.saved_tensors
         scale, causal = ctx.cfg
         M, H, dh = q.shape
-        l = _lib.lib()
         B, Hkv = starts.numel() - 1, k.shape[1]
         dout = _strided(dout, True, H // Hkv)
         dq, dk, dv = torch.empty_like(out), torch.empty(k.shape, dtype=k.dtype, device=k.device), torch.empty(v.shape, dtype=v.dtype, device=v.device)
-        ws = _ws(l.ttsmi_packed_attention_bwd_ws_bytes(B, M, H, Hkv, dh, int(causal)), q.device)
-        check(l.ttsmi_packed_attention_bwd(*_rs(q), *_rs(k), *_rs(v), *_rs(out), _p(rest), *_rs(dout), lse.data_ptr(), starts.data_ptr(), B, M, H,
-                                           Hkv, dh, scale, int(causal), *_rs(dq), *_rs(dk), *_rs(dv), 1, ws.data_ptr(), ws.numel(),
-                                           _SEQ_DTYPES[q.dtype], ctx.stream_h), 'packed_attention_bwd')
+        ws = _ws(_packed_bwd_ws(B, M, H, Hkv, dh, int(causal)), q.device)
+        row, krow = H * dh, Hkv * dh
+        check(_lib.lib().ttsmi_packed_attention_bwd(*_rs(q), *_rs(k), *_rs(v), out.data_ptr(), row, dh, _p(rest), *_rs(dout), lse.data_ptr(),
+                                                    starts.data_ptr(), B, M, H, Hkv, dh, scale, int(causal), dq.data_ptr(), row, dh,
+                                                    dk.data_ptr(), krow, dh, dv.data_ptr(), krow, dh, 1, ws.data_ptr(), ws.numel(),
+                                                    _SEQ_DTYPES[q.dtype], ctx.stream_h), 'packed_attention_bwd')
         return dq, dk, dv, None, None, None
 
 
@@ -2496,11 +2509,10 @@ def paged_attention(q, cache, table, starts, lens, scale=None, out=None):
         out = torch.empty((M, H, dh), dtype=q.dtype, device=q.device)
     elif out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or _strided(out) is not out or not _own_rows(out):
         _refuse(f'paged_attention: out {tuple(out.shape)} {out.dtype} for q {tuple(q.shape)} {q.dtype}, on 16-byte boundaries')
-    l = _lib.lib()
     dtype = _SEQ_DTYPES[q.dtype]
-    need = l.ttsmi_paged_attention_ws_bytes(lens.numel(), M, H, Hkv, dh, cache.code, dtype)
+    need = _paged_ws(lens.numel(), M, H, Hkv, dh, cache.code, dtype)
     ws = _ws(need, q.device) if need else None
-    check(l.ttsmi_paged_attention(*_rs(q), *cache.args, table.data_ptr(), table.shape[1], starts.data_ptr(), lens.data_ptr(), lens.numel(), M, H,
-                                  Hkv, dh, scale, *_rs(out), int(not given), _p(ws), 0 if ws is None else ws.numel(), dtype,
-                                  _seq_stream(cache.index)), 'paged_attention')
+    check(_lib.lib().ttsmi_paged_attention(*_rs(q), *cache.args, table.data_ptr(), table.shape[1], starts.data_ptr(), lens.data_ptr(),
+                                           lens.numel(), M, H, Hkv, dh, scale, *_rs(out), int(not given), _p(ws),
+                                           0 if ws is None else ws.numel(), dtype, _seq_stream(cache.index)), 'paged_attention')
     return out
