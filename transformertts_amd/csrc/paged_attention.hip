@@ -14,7 +14,7 @@
 //
 // Measured: 32 single tokens over 262 .. 8192 keys, 16 / 4 heads of 128, bf16 pages of 16: 42 us, 5.5 TB/s, and 6.7 us for the join;
 // two over 131072 and 70001 keys, 32 / 8 heads, e4m3 pages of 64: 78 us, 5.3 TB/s, and 11 us.  The tile form, chunks of 512 + 384 +
-// 97 + 1 tokens over 16384 .. 97 keys, 16 / 4 heads: 141 us and 15 us for its join (670 TFLOP/s together).
+// 97 + 1 tokens over 16384 .. 97 keys, 16 / 4 heads: 133 us with its join of 15 (720 TFLOP/s).
 #include "seq_common.h"
 
 template <int N> __device__ __forceinline__ void pg_wait() {

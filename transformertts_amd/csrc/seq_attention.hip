@@ -6,11 +6,12 @@
 // sequence and key head (seq_common.h: rows are (token, query head of the group) pairs), 32 rows a wave.  The wave forms the
 // TRANSPOSED score tile S^T = K Q^T, so that a lane holds one row's scores for 16 keys: the softmax is in-lane plus one exchange
 // of the two half-waves, and the accumulator registers, rounded, ARE the B operand of O^T += V^T P^T.
-// Each product of a wave's 32 rows reads a fragment of 1 KB from LDS: at the matrix pipes' full rate the four of them would ask for
-// 128 bytes a clock, all that LDS delivers.  So LDS reads, issue and the matrix pipe bound the kernel about equally (of 342 us a
-// pass, taking away the reads of fragments saves 96, either product 80 .. 90, the loads 42, the exponentials 29).  Measured: prompts of 8192 + 3001 + 513 + 1 tokens,
-// 16 / 8 heads of 128, causal, bf16: 318 us, 980 TFLOP/s where a large library product reaches 1330; 6000 + 1999 + 193 of 16 / 2 heads:
-// 193 us, 660 (two rounds of uneven tiles); 32 utterances of 202 .. 900, 4 heads of 64: 26 us; fp32, 8 utterances, 4 / 2 heads of 64:
+// Bound by the matrix and the vector pipes together: the matrix pipes are busy half of the time, a wave's vector instructions (the
+// softmax, 16 clocks an exponential) take as long as its products, and the two waves that the registers leave a SIMD overlap
+// only in part.  LDS is busy a third of the time, without bank conflicts.  (Of 342 us a pass, taking away the reads of fragments saved 96,
+// either product 80 .. 90, the loads 42, the exponentials 29.)  Measured: prompts of 8192 + 3001 + 513 + 1 tokens,
+// 16 / 8 heads of 128, causal, bf16: 313 us, 1000 TFLOP/s where a large library product reaches 1330; 6000 + 1999 + 193 of 16 / 2 heads:
+// 175 us, 730 (two rounds of uneven tiles); 32 utterances of 202 .. 900, 4 heads of 64: 26 us; fp32, 8 utterances, 4 / 2 heads of 64:
 // 26 us, the walk of four waves over the longest (38 of two).
 // Where tiles are few, two or four waves share a row block and the keys (seq_key_parts).
 // Over a cache the keys can be split over workgroups (find_unit): each leaves its maximum, sum and unnormalised output, and a second
@@ -39,7 +40,7 @@ __global__ __launch_bounds__(256, (DHP <= 128 && sizeof(T) == 2) ? 2 : 1) void s
         if (p.slots > 0) un = find_unit(p.starts, p.lens, 1, p.most, p.B, p.tokens, p.G, 128, p.slots, KT, SEQ_TILE_LEAST, unit, false);
     }
     const bool splits = PAGED && p.slots > 0;
-    const SeqTile st = splits ? un.t : find_tile(p.starts, p.B, p.tokens, p.G, ROWS, unit);
+    const SeqTile st = splits ? un.t : find_tile(p.starts, p.B, p.tokens, p.G, ROWS, unit, !PAGED && p.causal);
     if (st.seq < 0) {
         if (p.zero_rest) seq_zero_rest<T>((T*)p.o, p.o_row, p.o_head, p.starts, p.B, p.tokens, p.G, ROWS, hk * p.G, p.dh, st.tile);
         return;
@@ -246,6 +247,10 @@ __global__ __launch_bounds__(256, (DHP <= 128 && sizeof(T) == 2) ? 2 : 1) void s
 #pragma unroll
             for (int t = 0; t < NS; ++t) s[kb] = seq_mma(A::row(ka, kb * 32, t), qf[t], s[kb]);
         }
+        // The two waves of a SIMD are better off apart - one at its scores' product while the other is past it - so a wave that has its
+        // scores goes first (8192 tokens, 16 / 8 heads of 128, causal: 306 -> 278 us; full, 2 x 4096: 287 -> 279).  The backward
+        // passes do not gain by it.
+        __builtin_amdgcn_s_setprio(1);
         if (kw + KW > wfull || kw + KW > kend) {
             const int seen = seq_rare(min(lim, kend) - kw);
 #pragma unroll
@@ -290,6 +295,7 @@ __global__ __launch_bounds__(256, (DHP <= 128 && sizeof(T) == 2) ? 2 : 1) void s
 #pragma unroll
                 for (int cb = 0; cb < NCB; ++cb) o[cb] = seq_mma(A::col(va, kb * 32, t, cb), pf, o[cb]);
             }
+        __builtin_amdgcn_s_setprio(0);
     }
     l = seq_half_sum(l);
     if constexpr (KS > 1) {                               // the parts of the keys: a row block's first wave takes over the others' sums

@@ -11,8 +11,9 @@
 // dK, dV: 128 keys of one key head a workgroup, 32 a wave; the row tiles of every query head of the group pass through LDS, the
 //         wave forms S and dP with a key per lane, so that P and dS are the B operands of dV^T += dO^T P and dK^T += Q^T dS.
 //
-// Bound like the forward, with less softmax and more LDS reads a product.  Measured, causal bf16, 6000 + 1999 + 193 tokens of 16 / 2
-// heads of 128: dQ 265 us (720 TFLOP/s), dK / dV 380 (670) and 22 for the join of its row splits; 32 utterances of 202 .. 900, 4 heads
+// Bound like the forward (matrix pipes busy 52 %, LDS 26 - 33 %); the causal dK / dV pass leaves a quarter of the card idle at its ends.
+// Measured, causal bf16, 6000 + 1999 + 193 tokens of 16 / 2
+// heads of 128: dQ 251 us (760 TFLOP/s), dK / dV 385 (660) and 23 for the join of its row splits; 32 utterances of 202 .. 900, 4 heads
 // of 64: 35 and 40 us; fp32, 8 utterances of 117 .. 700, 4 / 2 heads of 64: 32 (48 with two waves a row block), 38 and 5 us.
 #include "seq_common.h"
 
@@ -62,7 +63,7 @@ __global__ __launch_bounds__(256, (DHP <= 128 && sizeof(T) == 2) ? 2 : 1) void s
     const int tid = threadIdx.x, lane = tid & 63, l31 = lane & 31, hh = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int hk = blockIdx.x % p.Hkv, unit = blockIdx.x / p.Hkv;
-    const SeqTile st = find_tile(p.starts, p.B, p.tokens, p.G, ROWS, unit);
+    const SeqTile st = find_tile(p.starts, p.B, p.tokens, p.G, ROWS, unit, p.causal);
     if (st.seq < 0) {
         if (p.zero_rest) seq_zero_rest<T>((T*)p.dq, p.dq_row, p.dq_head, p.starts, p.B, p.tokens, p.G, ROWS, hk * p.G, p.dh, st.tile);
         return;

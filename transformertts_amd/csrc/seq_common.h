@@ -98,7 +98,12 @@ __device__ __forceinline__ void seq_longest_first(int count, int& seq, int& s0, 
 // Tile `unit` of the sequences' tiles laid end to end; `tokens` rows of the packed tensors bound every length, so a `starts`
 // that is not ascending or points outside gives wrong rows but no access out of range.  Every lane of the wave calls it; 64
 // sequences are looked at at a time.
-__device__ __forceinline__ SeqTile find_tile(const int* starts, int B, int tokens, int G, int rows_per_tile, int unit) {
+// `falling`: a tile's work grows with its place in the sequence (causal), and there is more than one round of workgroups: the tiles
+// of 64 sequences in falling order of that place, all sequences mixed, so that the last ones to start are the smallest.  Level s is
+// the tiles in place s - 1; N(s) = sum max(0, tiles - s + 1) of them lie at level s or above, and the level of a unit is found by
+// halving.  (t.tile counts from the tile with the most work.)  Forward of 8 x 2048 tokens, 8 heads of 64: 70 -> 51 us; of 6000 + 1999 +
+// 193, 16 / 2 heads of 128: 193 -> 175, the priority below among them.
+__device__ __forceinline__ SeqTile find_tile(const int* starts, int B, int tokens, int G, int rows_per_tile, int unit, bool falling = false) {
     const int lane = threadIdx.x & 63;
     SeqTile t;
     t.seq = -1; t.tile = t.ntile = t.s0 = t.n = 0;
@@ -108,9 +113,28 @@ __device__ __forceinline__ SeqTile find_tile(const int* starts, int B, int token
             s0 = min(max(starts[b], 0), tokens);
             n = min(max(starts[b + 1], s0), tokens) - s0;
         }
-        if (B > 1 && gridDim.x > 256) seq_longest_first(min(B - b0, 64), b, s0, n);
+        if (B > 1 && gridDim.x > 256 && !falling) seq_longest_first(min(B - b0, 64), b, s0, n);
         const int tiles = (int)(((long)n * G + rows_per_tile - 1) / rows_per_tile);
         const int upto = seq_scan_add(tiles);
+        if (falling && B > 1 && gridDim.x > 256 && unit < __builtin_amdgcn_readlane(upto, 63)) {
+            int low = 1, high = __builtin_amdgcn_readlane(upto, 63) + 1, above = 0;             // N(low) > unit >= N(high) = above
+            while (high - low > 1) {
+                const int mid = low + (high - low) / 2, count = seq_wave_total(max(tiles - mid + 1, 0));
+                if (count > unit) low = mid;
+                else { high = mid; above = count; }
+            }
+            const uint64_t there = __ballot(tiles >= low);
+            const int before = __builtin_amdgcn_mbcnt_hi((uint32_t)(there >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)there, 0));
+            const uint64_t mine = __ballot(tiles >= low && before == unit - above);
+            if (!mine) { t.tile = SEQ_NO_TILE; return t; }          // (`starts` that overlap: the count wrapped)
+            const int at = __builtin_amdgcn_readfirstlane(__builtin_ctzll(mine));
+            t.seq = b0 + at;
+            t.ntile = __builtin_amdgcn_readlane(tiles, at);
+            t.tile = t.ntile - low;
+            t.s0 = __builtin_amdgcn_readlane(s0, at);
+            t.n = __builtin_amdgcn_readlane(n, at);
+            return t;
+        }
         const uint64_t hit = __ballot(upto > unit);
         if (hit) {
             const int at = __builtin_amdgcn_readfirstlane(__builtin_ctzll(hit));
