@@ -287,7 +287,7 @@ template <typename T, int DHP, int KS> struct SeqKeys {
 };
 // Parts where the workgroups - half a tile more than whole ones a sequence - are about one a compute unit, as far as LDS has room.
 // A causal batch of long sequences is uneven enough for twice as many.  Forward and backward in us with the keys in 1 / 2 / 4:
-//   8 heads of 64, bf16, causal: 1 x 512 tokens 50 / 44 / 41, 3 x 512 52 / 46 / 48, 1 x 2048 107 / 81 / 74, 1 x 3072 146 / 112 / 109, 20 x 102 38 / 41 / 51
+//   8 heads of 64, bf16, causal: 1 x 512 tokens 50 / 44 / 41, 3 x 512 52 / 46 / 48, 1 x 2048 107 / 81 / 74, 20 x 102 38 / 41 / 51
 //   16 / 4 heads of 128, bf16, causal: 1 x 512 79 / 71 / 67, 1 x 1024 110 / 94 / 104, 3 x 512 87 / 97 / 118, 1 x 2048 198 / 186 / 244, 10 x 102 57 / 72 / 90
 //   4 heads of 128, bf16, full: 4 x 512 73 / 64 / 64, 8 x 512 77 / 73 / 93, 12 x 512 82 / 105 / 126, 3 x 2048 197 / 243 / 273
 //   4 heads of 64, fp32, causal: 4 x 512 159 / 113 / 89, 6 x 512 185 / 137 / 139, 2 x 2048 576 / 387 / 320, 20 x 102 72 / 60 / 77, 40 x 102 92 / 92 / 118
