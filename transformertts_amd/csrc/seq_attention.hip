@@ -11,7 +11,7 @@
 // only in part.  LDS is busy a third of the time, without bank conflicts.  (Of 342 us a pass, taking away the reads of fragments saved 96,
 // either product 80 .. 90, the loads 42, the exponentials 29.)  Measured: prompts of 8192 + 3001 + 513 + 1 tokens,
 // 16 / 8 heads of 128, causal, bf16: 313 us, 1000 TFLOP/s where a large library product reaches 1330; 6000 + 1999 + 193 of 16 / 2 heads:
-// 175 us, 730 (two rounds of uneven tiles); 32 utterances of 202 .. 900, 4 heads of 64: 26 us; fp32, 8 utterances, 4 / 2 heads of 64:
+// 175 us, 730 (two rounds of uneven tiles); 32 utterances of 202 .. 900, 4 heads of 64, training: 29 us; fp32, 8 utterances, 4 / 2 heads of 64:
 // 26 us, the walk of four waves over the longest (38 of two).
 // Where tiles are few, two or four waves share a row block and the keys (seq_key_parts).
 // Over a cache the keys can be split over workgroups (find_unit): each leaves its maximum, sum and unnormalised output, and a second

@@ -14,7 +14,7 @@
 // Bound like the forward (matrix pipes busy 52 %, LDS 26 - 33 %); the causal dK / dV pass leaves a quarter of the card idle at its ends.
 // Measured, causal bf16, 6000 + 1999 + 193 tokens of 16 / 2
 // heads of 128: dQ 251 us (760 TFLOP/s), dK / dV 385 (660) and 23 for the join of its row splits; 32 utterances of 202 .. 900, 4 heads
-// of 64: 35 and 40 us; fp32, 8 utterances of 117 .. 700, 4 / 2 heads of 64: 32 (48 with two waves a row block), 38 and 5 us.
+// of 64: 38 and 40 us; fp32, 8 utterances of 117 .. 700, 4 / 2 heads of 64: 32 (48 with two waves a row block), 38 and 5 us.
 #include "seq_common.h"
 
 struct SeqBwdP {

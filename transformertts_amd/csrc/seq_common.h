@@ -83,7 +83,7 @@ struct SeqTile {
 };
 // The sequences of 64 lanes in falling order of their lengths: with more workgroups than compute units the long ones start
 // first and the short ones fill up behind them (a training step over 32 utterances of 202 .. 900 in any order, 4 heads of 64, 592
-// tiles: 119 -> 102 us of kernels; over 16 causal sequences of 20 .. 2000, 8 / 2 heads of 128: 358 -> 343, 16 heads of 64: 330 ->
+// tiles: 119 -> 102 us of kernels, 107 with out_rest; over 16 causal sequences of 20 .. 2000, 8 / 2 heads of 128: 358 -> 343, 16 heads of 64: 330 ->
 // 307).  A lane's rank is the number of keys above its own - lengths, made distinct by the lane - and every lane sends its sequence
 // to the lane of its rank.
 __device__ __forceinline__ void seq_longest_first(int count, int& seq, int& s0, int& n) {
