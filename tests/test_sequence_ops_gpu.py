@@ -132,6 +132,20 @@ def test_packed_attention_many_tiles(dtype, lens, H, Hkv, dh, causal):
         _within(g, w, b, name)
 
 
+@pytest.mark.parametrize('dtype,causal', [(torch.bfloat16, True), (torch.bfloat16, False), (torch.float32, True)])
+def test_packed_attention_more_sequences_than_lanes(dtype, causal):
+    """Seventy and more sequences, several rounds of workgroups: tiles start in the order of their work, 64 sequences at a time, and
+    every one of them starts once."""
+    ops = _ops()
+    lens, H, Hkv, dh = [37] * 40 + [500, 0, 1, 129] + [37] * 30 + [900, 0, 130, 64], 8, 8, 64
+    M = sum(lens)
+    q, k, v, d = (_randn((M, h, dh), 80 + i, dtype) for i, h in enumerate((H, Hkv, Hkv, H)))
+    want, bound = packed_oracle(q, k, v, lens, causal, dh ** -0.5, d)
+    xs = [x.to(DEV).requires_grad_() for x in (q, k, v)]
+    for name, g, w, b in zip(('out', 'dq', 'dk', 'dv'), _grads(ops.packed_attention(*xs, _starts(lens).to(DEV), causal=causal), xs, d.to(DEV)), want, bound):
+        _within(g, w, b, name)
+
+
 @pytest.mark.parametrize('dtype,lens,H,Hkv,dh,causal,parts', [
     (torch.bfloat16, [1000, 333], 4, 2, 128, True, 'four'), (torch.bfloat16, [700, 90, 400], 8, 8, 64, False, 'four'), (torch.bfloat16, [1999], 6, 2, 40, True, 'four'),
     (torch.float32, [515, 300], 2, 1, 64, True, 'four'), (torch.float32, [129, 600], 3, 3, 24, False, 'four'), (torch.bfloat16, [900, 7], 8, 8, 128, True, 'four'), (torch.bfloat16, [1500], 8, 8, 128, True, 'two'),
