@@ -1,0 +1,140 @@
+"""CPU-side checks of what the host mirror of the sequence operators does around its launches: the stream that they go to, what
+autograd is told, and which calls it refuses.  A recorder stands in for the library, and CPU tensors say that they are on a GPU:
+nothing is launched."""
+import threading
+
+import pytest
+import torch
+
+
+class OnGpu(torch.Tensor):
+    is_cuda = True
+
+    def get_device(self):
+        return 0
+
+
+def _t(*shape, dtype=torch.float32, fill=1.0, grad=False):
+    return torch.full(shape, fill, dtype=dtype).as_subclass(OnGpu).requires_grad_(grad)
+
+
+def _ints(*values):
+    return torch.tensor(values, dtype=torch.int32).as_subclass(OnGpu)
+
+
+class Recorder:
+    def __init__(self):
+        self.calls = []
+
+    def __getattr__(self, name):
+        if name.endswith('_ws_bytes'):
+            return lambda *a: 256
+
+        def call(*a):
+            self.calls.append((name, a))
+            return 0
+        return call
+
+
+@pytest.fixture
+def world(monkeypatch):
+    """(ops, the recorder): the current device is 0, and every thread's current stream is its own number."""
+    from transformertts_amd import _lib, ops
+    rec = Recorder()
+    monkeypatch.setattr(_lib, 'lib', lambda: rec)
+    monkeypatch.setattr(ops, '_current_device', lambda: 0)
+    monkeypatch.setattr(ops, '_raw_stream', lambda index: threading.get_ident())
+    yield ops, rec
+    ops._packed_bwd_ws.cache_clear()                       # (the recorder's sizes)
+    ops._paged_ws.cache_clear()
+
+
+def _every_call(ops):
+    """One call of each entry point, by name."""
+    q, k, v, cache = _t(3, 2, 8), _t(3, 1, 8), _t(3, 1, 8), _cache(ops)
+    st, ln, table, pos, freqs = _ints(0, 3), _ints(3), _ints(0).view(1, 1), _ints(0, 1, 2), _t(4, dtype=torch.float64)
+
+    def training_step():
+        x = [t.detach().requires_grad_() for t in (q, k, v)]
+        a, b = (t.as_subclass(OnGpu) for t in ops.rotary(x[0], x[1], pos, freqs))
+        torch.autograd.grad(ops.packed_attention(a, b, x[2], st), x, torch.ones(3, 2, 8))
+    return {'rotary': lambda: ops.rotary(q, k, pos, freqs), 'rotary in place': lambda: ops.rotary(q, k, pos, freqs, inplace=True),
+            'packed_attention': lambda: ops.packed_attention(q, k, v, st), 'training step': training_step,
+            'kv_cache_write': lambda: ops.kv_cache_write(cache, k, v, table, st, ln),
+            'kv_cache_read': lambda: ops.kv_cache_read(cache, table, ln, st, 3, out=(_t(3, 1, 8), _t(3, 1, 8))),
+            'paged_attention': lambda: ops.paged_attention(q, cache, table, st, ln)}
+
+
+def _cache(ops, dtype=torch.float32):
+    exp = () if dtype != torch.float8_e4m3fn else (_t(2, 1, 4, dtype=torch.uint8), _t(2, 1, 4, dtype=torch.uint8))
+    pages = [torch.zeros(2, 1, 4, 8, dtype=torch.uint8).view(dtype) if exp else torch.zeros(2, 1, 4, 8, dtype=dtype) for _ in 'kv']
+    return ops.KVCache(*(t.as_subclass(OnGpu) for t in pages), *exp)
+
+
+class _InAnotherThread:
+    """`with _InAnotherThread(context):` - the context is entered by another thread and left by it at the end."""
+
+    def __init__(self, context):
+        self.context, self.inside, self.leave = context, threading.Event(), threading.Event()
+
+    def _run(self):
+        with self.context:
+            self.inside.set()
+            self.leave.wait(60)
+
+    def __enter__(self):
+        self.thread = threading.Thread(target=self._run)
+        self.thread.start()
+        assert self.inside.wait(60)
+        return self
+
+    def __exit__(self, *exc):
+        self.leave.set()
+        self.thread.join()
+        return False
+
+
+NAMES = ['rotary', 'rotary in place', 'packed_attention', 'training step', 'kv_cache_write', 'kv_cache_read', 'paged_attention']
+
+
+@pytest.mark.parametrize('name', NAMES)
+def test_launches_go_to_the_calling_threads_stream(world, name):
+    """A training step of another thread pins ITS stream for as long as it takes; a call made meanwhile stays on its own."""
+    ops, rec = world
+    with _InAnotherThread(ops.pin_stream(99)):
+        _every_call(ops)[name]()
+    assert len(rec.calls) == (4 if name == 'training step' else 1) and all(a[-1] == threading.get_ident() for _, a in rec.calls)
+
+
+@pytest.mark.parametrize('name', NAMES)
+def test_a_call_on_another_device_leaves_another_threads_pin_alone(world, monkeypatch, name):
+    """The step of the other thread keeps its pinned stream during the call, and no stream of an ended step is put back after it."""
+    ops, rec = world
+    import contextlib
+    step = _InAnotherThread(ops.pin_stream(99))
+    here, seen = [1], []
+
+    @contextlib.contextmanager
+    def device(d):
+        here[0] = 0
+        seen.append(ops._PINNED_STREAM)
+        yield
+        if step.thread.is_alive():                         # the step ends while the call runs
+            step.__exit__()
+        here[0] = 1
+    monkeypatch.setattr(torch.cuda, 'device', device)
+    monkeypatch.setattr(ops, '_current_device', lambda: here[0])
+    launch = rec.__class__.__getattr__
+
+    def watched(self, n):
+        f = launch(self, n)
+
+        def call(*a):
+            seen.append(ops._PINNED_STREAM)
+            return f(*a)
+        return call
+    monkeypatch.setattr(Recorder, '__getattr__', watched)
+    with step:
+        _every_call(ops)[name]()
+    assert rec.calls and seen[0] == 99 and (name == 'training step' or set(seen) == {99})
+    assert ops._PINNED_STREAM is None

@@ -1,0 +1,90 @@
+"""-m gpu tests of the sequence operators' calls beside other work of the process: steps of other threads, autograd, caches whose
+tensors change."""
+import threading
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+DEV = 'cuda:0'
+
+
+def _ops():
+    from transformertts_amd import ops
+    return ops
+
+
+def _randn(shape, seed, dtype=torch.float32):
+    return torch.randn(shape, generator=torch.Generator().manual_seed(seed)).to(dtype).to(DEV)
+
+
+def _ints(values):
+    return torch.tensor(values, dtype=torch.int32, device=DEV)
+
+
+def _calls(ops, x):
+    """Every entry point on x = (q, k, v, dout), results in one list."""
+    q, k, v, d = x
+    n = len(q)
+    st, ln, table, pos = _ints([0, n]), _ints([n]), _ints([[1, 0]]), torch.arange(n, dtype=torch.int32, device=DEV)
+    freqs = torch.linspace(1.0, 0.1, 32, dtype=torch.float64).to(DEV)
+    cache = ops.KVCache.zeros(2, 64, k.shape[1], 64, torch.bfloat16, DEV)
+
+    def run():
+        y = [t.detach().requires_grad_() for t in (q, k, v)]
+        a, b = ops.rotary(y[0], y[1], pos, freqs)
+        out = ops.packed_attention(a, b, y[2], st)
+        grads = torch.autograd.grad(out, y, d)
+        with torch.no_grad():
+            ops.kv_cache_write(cache, b, v, table, st, ln)
+            return [a, b, out, *grads, ops.paged_attention(a, cache, table, st, ln), *ops.kv_cache_read(cache, table, ln, st, n)]
+    return run
+
+
+def test_a_pinned_step_of_another_thread_is_not_followed():
+    """While another thread pins a stream of its own, a capture here holds every launch of the calls made here: its replays
+    give what new inputs ask for."""
+    ops = _ops()
+    x = [_randn((100, h, 64), i, torch.bfloat16) for i, h in enumerate((4, 2, 2, 4))]
+    run = _calls(ops, x)
+    side, other = torch.cuda.Stream(), torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        run()
+    torch.cuda.synchronize()
+    inside, leave = threading.Event(), threading.Event()
+
+    def step():
+        with torch.cuda.stream(other), ops.pinned_stream():
+            inside.set()
+            leave.wait(60)
+    thread = threading.Thread(target=step)
+    thread.start()
+    try:
+        assert inside.wait(60)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            res = run()
+    finally:
+        leave.set()
+        thread.join()
+    for seed in (10, 20, 30):
+        for i, t in enumerate(x):
+            t.copy_(_randn(t.shape, seed + i, torch.bfloat16))
+        graph.replay()
+        want = run()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(res, want))
+
+
+def test_calls_on_a_device_that_is_not_the_current_one(monkeypatch):
+    """The way through a change of the device (to the same one here: that is all a test machine has), forward and backward."""
+    ops = _ops()
+    run = _calls(ops, [_randn((100, h, 64), i, torch.bfloat16) for i, h in enumerate((4, 2, 2, 4))])
+    want, asked = run(), []
+
+    def current():
+        asked.append(1)
+        return -1 if len(asked) % 2 else 0
+    monkeypatch.setattr(ops, '_current_device', current)
+    got = run()
+    assert len(asked) == 10 and all(torch.equal(a, b) for a, b in zip(got, want))

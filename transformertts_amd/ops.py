@@ -2153,28 +2153,13 @@ _current_device = torch._C._cuda_getDevice
 
 
 def _seq_stream(device_index):
-    return _PINNED_STREAM if _PINNED_STREAM is not None else _raw_stream(device_index)
+    """The calling thread's current stream of that device.  Not _PINNED_STREAM: a step pins it for every thread of the process,
+    and what another thread calls meanwhile belongs on that thread's own stream."""
+    return _raw_stream(device_index)
 
 
 def _refuse(message):
     raise _lib.TtsmiError(message)
-
-
-class _OnDevice:
-    """Another GPU than the current one: launches inside go to that GPU's current stream."""
-
-    def __init__(self, device):
-        self.device = torch.cuda.device(device)
-
-    def __enter__(self):
-        self.device.__enter__()
-        self.pin = pin_stream(None)
-        self.pin.__enter__()
-        return self
-
-    def __exit__(self, *exc):
-        self.pin.__exit__(*exc)
-        return self.device.__exit__(*exc)
 
 
 def _seq_check(name, t, like=None):
@@ -2224,12 +2209,12 @@ def _scale_of(scale, dh):
 
 
 # ---- rotary positions ----------------------------------------------------------------------------------------------
-def _rotary(q, k, qo, ko, positions, freqs, interleaved, scale, inverse, stream=None):
+def _rotary(q, k, qo, ko, positions, freqs, interleaved, scale, inverse):
     none = (None, 0, 0)
     check(_lib.lib().ttsmi_rotary(*_rs(q), *_rs(qo), q.shape[1], *(none if k is None else _rs(k)), *(none if k is None else _rs(ko)),
                                   0 if k is None else k.shape[1], positions.data_ptr(), freqs.data_ptr(), q.shape[0], q.shape[2],
                                   2 * freqs.numel(), int(interleaved), scale, int(inverse), _SEQ_DTYPES[q.dtype],
-                                  _seq_stream(q.device.index) if stream is None else stream), 'rotary')
+                                  _seq_stream(q.device.index)), 'rotary')
 
 
 class RotaryFn(torch.autograd.Function):
@@ -2237,7 +2222,6 @@ class RotaryFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, q, k, positions, freqs, interleaved, scale):
-        ctx.stream_h = _seq_stream(q.device.index)
         ctx.save_for_backward(positions, freqs)
         ctx.cfg = (interleaved, scale)
         ctx.set_materialize_grads(False)
@@ -2255,7 +2239,7 @@ class RotaryFn(torch.autograd.Function):
             for i, g in some:
                 grads[i] = torch.empty(g.shape, dtype=g.dtype, device=g.device)
             (a, ga), (b, gb) = some[0], some[1] if len(some) > 1 else (None, None)
-            _rotary(ga, gb, grads[a], None if b is None else grads[b], positions, freqs, *ctx.cfg, True, ctx.stream_h)
+            _rotary(ga, gb, grads[a], None if b is None else grads[b], positions, freqs, *ctx.cfg, True)
         return grads[0], grads[1], None, None, None, None
 
 
@@ -2267,7 +2251,7 @@ def rotary(q, k, positions, freqs, interleaved=False, scale=1.0, inplace=False):
     _seq_check('rotary: q', q)
     dev = q.get_device()
     if dev != _current_device():
-        with _OnDevice(q.device):
+        with torch.cuda.device(q.device):
             return rotary(q, k, positions, freqs, interleaved, scale, inplace)
     pairs, M, dh = freqs.numel(), q.shape[0], q.shape[2]
     if freqs.dtype != torch.float64 or freqs.dim() != 1 or not freqs.is_cuda or freqs.get_device() != dev:
@@ -2331,7 +2315,6 @@ class PackedAttentionFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, q, k, v, starts, scale, causal):
-        ctx.stream_h = _seq_stream(q.device.index)
         out, lse, rest = _packed_fwd(q, k, v, starts, scale, causal, True)
         ctx.save_for_backward(q, k, v, out, lse, rest, starts)
         ctx.cfg = (scale, causal)
@@ -2353,7 +2336,7 @@ class PackedAttentionFn(torch.autograd.Function):
         check(_lib.lib().ttsmi_packed_attention_bwd(*_rs(q), *_rs(k), *_rs(v), out.data_ptr(), row, dh, _p(rest), *_rs(dout), lse.data_ptr(),
                                                     starts.data_ptr(), B, M, H, Hkv, dh, scale, int(causal), dq.data_ptr(), row, dh,
                                                     dk.data_ptr(), krow, dh, dv.data_ptr(), krow, dh, 1, ws.data_ptr(), ws.numel(),
-                                                    _SEQ_DTYPES[q.dtype], ctx.stream_h), 'packed_attention_bwd')
+                                                    _SEQ_DTYPES[q.dtype], _seq_stream(q.device.index)), 'packed_attention_bwd')
         return dq, dk, dv, None, None, None
 
 
@@ -2366,7 +2349,7 @@ def packed_attention(q, k, v, starts, causal=True, scale=None):
     _seq_check('packed_attention: q', q)
     dev = q.get_device()
     if dev != _current_device():
-        with _OnDevice(q.device):
+        with torch.cuda.device(q.device):
             return packed_attention(q, k, v, starts, causal, scale)
     _seq_check('packed_attention: k', k, q)
     _seq_check('packed_attention: v', v, q)
@@ -2455,7 +2438,7 @@ def kv_cache_write(cache, k, v, table, starts, lens):
     table, starts, lens = _paged_check('kv_cache_write', cache, table, starts, lens)
     _kv_check('kv_cache_write', cache, k, v)
     if cache.index != _current_device():
-        with _OnDevice(k.device):
+        with torch.cuda.device(k.device):
             return kv_cache_write(cache, k, v, table, starts, lens)
     k, v = _strided(k), _strided(v)
     check(_lib.lib().ttsmi_kv_cache_write(*_rs(k), *_rs(v), *cache.args, table.data_ptr(), table.shape[1], starts.data_ptr(), lens.data_ptr(),
@@ -2469,7 +2452,7 @@ def kv_cache_read(cache, table, lens, starts, tokens, dtype=None, out=None):
     Rows of no sequence are zeros; with out = (k, v) they are left as they were."""
     table, starts, lens = _paged_check('kv_cache_read', cache, table, starts, lens)
     if cache.index != _current_device():
-        with _OnDevice(cache.k.device):
+        with torch.cuda.device(cache.k.device):
             return kv_cache_read(cache, table, lens, starts, tokens, dtype, out)
     if out is None:
         dtype = dtype or (torch.bfloat16 if cache.dtype == torch.float8_e4m3fn else cache.dtype)
@@ -2500,7 +2483,7 @@ def paged_attention(q, cache, table, starts, lens, scale=None, out=None):
     if q.requires_grad and torch.is_grad_enabled():
         _refuse('paged_attention: has no gradient')
     if cache.index != _current_device():
-        with _OnDevice(q.device):
+        with torch.cuda.device(q.device):
             return paged_attention(q, cache, table, starts, lens, scale, out)
     scale = _scale_of(scale, dh)
     q = _strided(q)
