@@ -138,3 +138,25 @@ def test_a_call_on_another_device_leaves_another_threads_pin_alone(world, monkey
         _every_call(ops)[name]()
     assert rec.calls and seen[0] == 99 and (name == 'training step' or set(seen) == {99})
     assert ops._PINNED_STREAM is None
+
+
+def _versions(*ts):
+    return [t._version for t in ts]
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.float8_e4m3fn])
+def test_autograd_is_told_of_every_tensor_written(world, dtype):
+    ops, _ = world
+    cache = _cache(ops, dtype)
+    q, k, v = _t(3, 2, 8), _t(3, 1, 8), _t(3, 1, 8)
+    st, ln, table = _ints(0, 3), _ints(3), _ints(0).view(1, 1)
+    written = [t for t in (cache.k, cache.v, cache.k_exp, cache.v_exp) if t is not None]
+    before = _versions(*written)
+    ops.kv_cache_write(cache, k, v, table, st, ln)
+    assert all(a < b for a, b in zip(before, _versions(*written)))
+    before, outs = _versions(*written), (_t(3, 1, 8), _t(3, 1, 8), _t(3, 2, 8))
+    ops.kv_cache_read(cache, table, ln, st, 3, out=outs[:2])
+    ops.paged_attention(q, cache, table, st, ln, out=outs[2])
+    assert all(n > 0 for n in _versions(*outs)) and _versions(*written) == before and _versions(q, k, v) == [0, 0, 0]
+    with torch.inference_mode():                           # (tensors of no version take the same way)
+        ops.paged_attention(q, cache, table, st, ln, out=_t(3, 2, 8))

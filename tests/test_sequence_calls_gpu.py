@@ -88,3 +88,20 @@ def test_calls_on_a_device_that_is_not_the_current_one(monkeypatch):
     monkeypatch.setattr(ops, '_current_device', current)
     got = run()
     assert len(asked) == 10 and all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_a_saved_tensor_that_was_written_is_refused_not_used():
+    """A tensor that a product keeps for its gradient, then handed to an operator as its output: the gradient is refused."""
+    ops = _ops()
+    cache = ops.KVCache.zeros(2, 16, 2, 64, torch.float32, DEV)
+    st, ln, table = _ints([0, 3]), _ints([3]), _ints([[0]])
+    q, k = _randn((3, 4, 64), 1), _randn((3, 2, 64), 2)
+    w = torch.ones((64, 8), device=DEV, requires_grad=True)
+    for out, write in ((torch.zeros_like(q), lambda t: ops.paged_attention(q, cache, table, st, ln, out=t)),
+                       (torch.zeros_like(k), lambda t: ops.kv_cache_read(cache, table, ln, st, 3, out=(t, torch.zeros_like(k)))),
+                       (torch.zeros_like(k), lambda t: ops.kv_cache_read(cache, table, ln, st, 3, out=(torch.zeros_like(k), t))),
+                       (cache.k, lambda t: ops.kv_cache_write(cache, k, k, table, st, ln)), (cache.v, lambda t: ops.kv_cache_write(cache, k, k, table, st, ln))):
+        y = (out @ w).sum()
+        write(out)
+        with pytest.raises(RuntimeError, match='modified by an inplace operation'):
+            y.backward()

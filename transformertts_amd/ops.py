@@ -2208,6 +2208,11 @@ def _scale_of(scale, dh):
     return scale
 
 
+# The kernels write through raw pointers: autograd is told, so that a product that kept one of these tensors for its gradient
+# refuses it instead of using what stands there now.
+_written = torch.autograd.graph.increment_version
+
+
 # ---- rotary positions ----------------------------------------------------------------------------------------------
 def _rotary(q, k, qo, ko, positions, freqs, interleaved, scale, inverse):
     none = (None, 0, 0)
@@ -2275,7 +2280,7 @@ def rotary(q, k, positions, freqs, interleaved=False, scale=1.0, inplace=False):
         if any(t is not None and (t.stride(2) != 1 or not _own_rows(t)) for t in (q, k)):
             _refuse('rotary: in place needs a contiguous last dimension, and no broadcast one')
         _rotary(q, k, q, k, positions, freqs, interleaved, scale, False)
-        torch.autograd.graph.increment_version([q] if k is None else [q, k])
+        _written([q] if k is None else [q, k])
         return q, k
     q, k = _strided(q, False), None if k is None else _strided(k, False)
     if grad:
@@ -2444,6 +2449,7 @@ def kv_cache_write(cache, k, v, table, starts, lens):
     check(_lib.lib().ttsmi_kv_cache_write(*_rs(k), *_rs(v), *cache.args, table.data_ptr(), table.shape[1], starts.data_ptr(), lens.data_ptr(),
                                           lens.numel(), k.shape[0], cache.heads, cache.dh, _SEQ_DTYPES[k.dtype], _seq_stream(cache.index)),
           'kv_cache_write')
+    _written([cache.k, cache.v] if cache.k_exp is None else [cache.k, cache.v, cache.k_exp, cache.v_exp])
 
 
 def kv_cache_read(cache, table, lens, starts, tokens, dtype=None, out=None):
@@ -2466,6 +2472,8 @@ def kv_cache_read(cache, table, lens, starts, tokens, dtype=None, out=None):
     check(_lib.lib().ttsmi_kv_cache_read(*cache.args, table.data_ptr(), table.shape[1], starts.data_ptr(), lens.data_ptr(), lens.numel(),
                                          k.shape[0], cache.heads, cache.dh, *_rs(k), *_rs(v), int(out is None), _SEQ_DTYPES[k.dtype],
                                          _seq_stream(cache.index)), 'kv_cache_read')
+    if out is not None:
+        _written([k, v])
     return k, v
 
 
@@ -2498,4 +2506,6 @@ def paged_attention(q, cache, table, starts, lens, scale=None, out=None):
     check(_lib.lib().ttsmi_paged_attention(*_rs(q), *cache.args, table.data_ptr(), table.shape[1], starts.data_ptr(), lens.data_ptr(),
                                            lens.numel(), M, H, Hkv, dh, scale, *_rs(out), int(not given), _p(ws),
                                            0 if ws is None else ws.numel(), dtype, _seq_stream(cache.index)), 'paged_attention')
+    if given:
+        _written([out])
     return out
