@@ -41,7 +41,7 @@ def _calls(ops, x):
     return run
 
 
-def test_a_pinned_step_of_another_thread_is_not_followed():
+def test_a_pinned_step_of_another_thread_beside_a_graph():
     """While another thread pins a stream of its own, a capture here holds every launch of the calls made here: its replays
     give what new inputs ask for."""
     ops = _ops()
