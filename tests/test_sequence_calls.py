@@ -160,3 +160,27 @@ def test_autograd_is_told_of_every_tensor_written(world, dtype):
     assert all(n > 0 for n in _versions(*outs)) and _versions(*written) == before and _versions(q, k, v) == [0, 0, 0]
     with torch.inference_mode():                           # (tensors of no version take the same way)
         ops.paged_attention(q, cache, table, st, ln, out=_t(3, 2, 8))
+
+
+def test_gradients_that_would_be_dropped_are_refused(world):
+    """Keys, pages, outputs and frequencies that want a gradient no operator gives; without grad mode the calls go through."""
+    from transformertts_amd import _lib
+    ops, rec = world
+    q, k, v = _t(3, 2, 8), _t(3, 1, 8), _t(3, 1, 8)
+    st, ln, table, pos, freqs = _ints(0, 3), _ints(3), _ints(0).view(1, 1), _ints(0, 1, 2), _t(4, dtype=torch.float64)
+    cache, learned = _cache(ops), ops.KVCache(*(torch.zeros(2, 1, 4, 8).as_subclass(OnGpu).requires_grad_() for _ in 'kv'))
+    g = dict(q=_t(3, 2, 8, grad=True), k=_t(3, 1, 8, grad=True), freqs=_t(4, dtype=torch.float64, grad=True))
+    calls = [lambda: ops.kv_cache_write(cache, g['k'], v, table, st, ln), lambda: ops.kv_cache_write(cache, k, g['k'], table, st, ln),
+             lambda: ops.kv_cache_write(learned, k, v, table, st, ln), lambda: ops.kv_cache_read(learned, table, ln, st, 3, out=(_t(3, 1, 8), _t(3, 1, 8))),
+             lambda: ops.kv_cache_read(cache, table, ln, st, 3, out=(g['k'], _t(3, 1, 8))), lambda: ops.kv_cache_read(cache, table, ln, st, 3, out=(_t(3, 1, 8), g['k'])),
+             lambda: ops.paged_attention(g['q'], cache, table, st, ln), lambda: ops.paged_attention(q, learned, table, st, ln),
+             lambda: ops.paged_attention(q, cache, table, st, ln, out=g['q']), lambda: ops.rotary(q, k, pos, g['freqs']),
+             lambda: ops.rotary(q, k, pos, g['freqs'], inplace=True), lambda: ops.rotary(g['q'], k, pos, g['freqs'])]
+    for call in calls:
+        with pytest.raises(_lib.TtsmiError, match='gradient'):
+            call()
+    assert not rec.calls
+    with torch.no_grad():
+        for call in calls:
+            call()
+    assert len(rec.calls) == len(calls)

@@ -2208,6 +2208,14 @@ def _scale_of(scale, dh):
     return scale
 
 
+def _no_gradient(name, *tensors):
+    """Refuses tensors that want a gradient which the call does not give."""
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                _refuse(f'{name}: has no gradient for a tensor of {tuple(t.shape)} that wants one (detach it, or call it under torch.no_grad)')
+
+
 # The kernels write through raw pointers: autograd is told, so that a product that kept one of these tensors for its gradient
 # refuses it instead of using what stands there now.
 _written = torch.autograd.graph.increment_version
@@ -2250,7 +2258,7 @@ class RotaryFn(torch.autograd.Function):
 
 def rotary(q, k, positions, freqs, interleaved=False, scale=1.0, inplace=False):
     """The first 2 * len(freqs) elements of every head of q [tokens, H, dh] and k [tokens, Hkv, dh] (or None) turned by
-    positions [tokens] int32 times freqs (float64 radians per position, model.transformer_utils.rotary_frequencies), pairs
+    positions [tokens] int32 times freqs (float64 radians per position, model.transformer_utils.rotary_frequencies; no gradient), pairs
     (2 i, 2 i + 1) if interleaved and (i, i + len(freqs)) otherwise, times scale; the rest passes through.  -> (q, k).
     inplace: q and k themselves, without gradients."""
     _seq_check('rotary: q', q)
@@ -2263,6 +2271,7 @@ def rotary(q, k, positions, freqs, interleaved=False, scale=1.0, inplace=False):
         _refuse(f'rotary: freqs: 1-d float64 on {q.device}')
     if 2 * pairs > dh or dh % 2 or pairs > 256:
         _refuse(f'rotary: {pairs} pairs in a head of {dh} elements (even; at most 256 pairs)')
+    _no_gradient('rotary: freqs', freqs)
     positions = _ints_check('rotary', 'positions', positions, dev)
     if positions.numel() != M:
         _refuse(f'rotary: {positions.numel()} positions for {M} tokens')
@@ -2439,9 +2448,11 @@ def _kv_check(name, cache, k, v):
 def kv_cache_write(cache, k, v, table, starts, lens):
     """The packed new tokens' keys and values [tokens, Hkv, dh] into their pages, quantised if the pages are float8_e4m3fn.
     table [B, n] int32: the pages of every sequence in order; starts [B + 1] int32: its new tokens; lens [B] int32: its cached
-    length with them, which are the last ones.  A page number outside the cache, or a token without a position, is not written."""
+    length with them, which are the last ones.  A page number outside the cache, or a token without a position, is not written.
+    Without gradients."""
     table, starts, lens = _paged_check('kv_cache_write', cache, table, starts, lens)
     _kv_check('kv_cache_write', cache, k, v)
+    _no_gradient('kv_cache_write', k, v, cache.k, cache.v)
     if cache.index != _current_device():
         with torch.cuda.device(k.device):
             return kv_cache_write(cache, k, v, table, starts, lens)
@@ -2455,7 +2466,7 @@ def kv_cache_write(cache, k, v, table, starts, lens):
 def kv_cache_read(cache, table, lens, starts, tokens, dtype=None, out=None):
     """The last starts[b + 1] - starts[b] cached tokens of every sequence (all of them where starts holds the cumulative lens)
     in packed order -> (k, v) [tokens, Hkv, dh].  dtype: the pages' own, or either for float8_e4m3fn pages (default bfloat16).
-    Rows of no sequence are zeros; with out = (k, v) they are left as they were."""
+    Rows of no sequence are zeros; with out = (k, v) they are left as they were.  Without gradients."""
     table, starts, lens = _paged_check('kv_cache_read', cache, table, starts, lens)
     if cache.index != _current_device():
         with torch.cuda.device(cache.k.device):
@@ -2467,6 +2478,7 @@ def kv_cache_read(cache, table, lens, starts, tokens, dtype=None, out=None):
     else:
         k, v = out
     _kv_check('kv_cache_read', cache, k, v)
+    _no_gradient('kv_cache_read', cache.k, cache.v, k, v)
     if out is not None and (k.shape[0] != tokens or _strided(k) is not k or _strided(v) is not v or not _own_rows(k) or not _own_rows(v)):
         _refuse(f'kv_cache_read: out of {tokens} tokens on 16-byte boundaries')
     check(_lib.lib().ttsmi_kv_cache_read(*cache.args, table.data_ptr(), table.shape[1], starts.data_ptr(), lens.data_ptr(), lens.numel(),
@@ -2488,8 +2500,7 @@ def paged_attention(q, cache, table, starts, lens, scale=None, out=None):
     Hkv = cache.heads
     if dh != cache.dh or H == 0 or H % Hkv or q.get_device() != cache.index or (cache.dtype != q.dtype and cache.dtype != torch.float8_e4m3fn):
         _refuse(f'paged_attention: q {tuple(q.shape)} {q.dtype} on {q.device}; pages {tuple(cache.k.shape)} {cache.dtype} on {cache.k.device}')
-    if q.requires_grad and torch.is_grad_enabled():
-        _refuse('paged_attention: has no gradient')
+    _no_gradient('paged_attention', q, cache.k, cache.v, out)
     if cache.index != _current_device():
         with torch.cuda.device(q.device):
             return paged_attention(q, cache, table, starts, lens, scale, out)
