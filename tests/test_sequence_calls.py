@@ -184,3 +184,29 @@ def test_gradients_that_would_be_dropped_are_refused(world):
         for call in calls:
             call()
     assert len(rec.calls) == len(calls)
+
+
+def test_second_derivatives_of_attention_are_refused(world):
+    """A penalty on a gradient is refused, not given without a term - however the gradient is asked for, and also where the loss is
+    linear in the output; create_graph alone is not."""
+    from transformertts_amd import _lib
+    ops, _ = world
+    for power in (1, 2):
+        for grad in (lambda loss, x: torch.autograd.grad(loss, x), lambda loss, x: loss.backward()):
+            x = [_t(3, h, 8, grad=True) for h in (2, 1, 1)]
+            loss = (ops.packed_attention(*x, _ints(0, 3)) ** power).sum()
+            grads = torch.autograd.grad(loss, x, create_graph=True)
+            torch.autograd.grad(loss, x, retain_graph=True)
+            with pytest.raises(_lib.TtsmiError, match='second derivatives'):
+                grad(loss + sum((g ** 2).sum() for g in grads), x)
+
+
+def test_second_derivatives_of_rotary_are_turns(world):
+    """The gradient's own gradient is asked of the kernel, turned the other way again."""
+    ops, rec = world
+    q, k, dq, dk = (_t(3, h, 8, grad=True) for h in (2, 1, 2, 1))
+    out = ops.rotary(q, k, _ints(0, 1, 2), _t(4, dtype=torch.float64), scale=0.5)
+    grads = torch.autograd.grad(out, (q, k), (dq, dk), create_graph=True)
+    again = torch.autograd.grad(grads, (dq, dk), (torch.ones(3, 2, 8), torch.ones(3, 1, 8)))
+    assert [tuple(g.shape) for g in again] == [(3, 2, 8), (3, 1, 8)]
+    assert [a[-3] for _, a in rec.calls] == [0, 1, 0] and [a[-4] for _, a in rec.calls] == [0.5] * 3

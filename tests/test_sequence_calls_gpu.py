@@ -105,3 +105,32 @@ def test_a_saved_tensor_that_was_written_is_refused_not_used():
         write(out)
         with pytest.raises(RuntimeError, match='modified by an inplace operation'):
             y.backward()
+
+
+def test_rotary_differentiated_twice():
+    """The gradient is linear in the incoming one: its own gradient is the turn itself, to the same bits."""
+    ops = _ops()
+    q, k, dq, dk, wq, wk = (_randn((37, h, 64), i, torch.bfloat16) for i, h in enumerate((4, 2) * 3))
+    pos, freqs = torch.arange(37, dtype=torch.int32, device=DEV), torch.linspace(1.0, 0.1, 16, dtype=torch.float64).to(DEV)
+    for t in (q, k, dq, dk):
+        t.requires_grad_()
+    out = ops.rotary(q, k, pos, freqs, scale=1.5)
+    grads = torch.autograd.grad(out, (q, k), (dq, dk), create_graph=True)
+    once = torch.autograd.grad(out, (q, k), (dq, dk), retain_graph=True)
+    again = torch.autograd.grad(grads, (dq, dk), (wq, wk), retain_graph=True)
+    want = ops.rotary(wq, wk, pos, freqs, scale=1.5)
+    assert all(torch.equal(a, b) for a, b in zip([*grads, *again], [*once, *want]))
+    only, = torch.autograd.grad(grads[1], dk, wk)
+    assert torch.equal(only, want[1])
+
+
+def test_attention_differentiated_twice_is_refused():
+    from transformertts_amd import _lib
+    ops = _ops()
+    x = [_randn((37, h, 64), i, torch.bfloat16).requires_grad_() for i, h in enumerate((4, 2, 2))]
+    out = ops.packed_attention(*x, _ints([0, 30, 37]))
+    grads = torch.autograd.grad(out.sum(), x, create_graph=True)
+    once = torch.autograd.grad(out.sum(), x)
+    assert all(torch.equal(a, b) for a, b in zip(grads, once))
+    with pytest.raises(_lib.TtsmiError, match='second derivatives'):
+        torch.autograd.grad(sum((g.float() ** 2).sum() for g in grads), x)

@@ -2230,30 +2230,34 @@ def _rotary(q, k, qo, ko, positions, freqs, interleaved, scale, inverse):
                                   _seq_stream(q.device.index)), 'rotary')
 
 
+def _turned(q, k, positions, freqs, interleaved, scale, inverse):
+    qo, ko = q.new_empty(q.shape), None if k is None else k.new_empty(k.shape)
+    _rotary(q, k, qo, ko, positions, freqs, interleaved, scale, inverse)
+    return qo, ko
+
+
 class RotaryFn(torch.autograd.Function):
     """Queries and keys turned by their positions; the gradients are turned back (ttsmi_rotary)."""
 
     @staticmethod
-    def forward(ctx, q, k, positions, freqs, interleaved, scale):
+    def forward(ctx, q, k, positions, freqs, interleaved, scale, inverse):
         ctx.save_for_backward(positions, freqs)
-        ctx.cfg = (interleaved, scale)
+        ctx.cfg = (interleaved, scale, not inverse)
         ctx.set_materialize_grads(False)
-        qo = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        ko = None if k is None else torch.empty(k.shape, dtype=k.dtype, device=k.device)
-        _rotary(q, k, qo, ko, positions, freqs, interleaved, scale, False)
-        return qo, ko
+        return _turned(q, k, positions, freqs, interleaved, scale, inverse)
 
     @staticmethod
     def backward(ctx, dq, dk):
-        positions, freqs = ctx.saved_tensors
         grads = [None, None]
         some = [(i, _strided(g, aligned=False)) for i, g in enumerate((dq, dk)) if g is not None and ctx.needs_input_grad[i]]
         if some:
-            for i, g in some:
-                grads[i] = torch.empty(g.shape, dtype=g.dtype, device=g.device)
             (a, ga), (b, gb) = some[0], some[1] if len(some) > 1 else (None, None)
-            _rotary(ga, gb, grads[a], None if b is None else grads[b], positions, freqs, *ctx.cfg, True)
-        return grads[0], grads[1], None, None, None, None
+            # the turn is linear: with create_graph its gradient is a turn that has one too
+            turn = RotaryFn.apply if torch.is_grad_enabled() else _turned
+            grads[a], other = turn(ga, gb, *ctx.saved_tensors, *ctx.cfg)
+            if b is not None:
+                grads[b] = other
+        return grads[0], grads[1], None, None, None, None, None
 
 
 def rotary(q, k, positions, freqs, interleaved=False, scale=1.0, inplace=False):
@@ -2293,11 +2297,8 @@ def rotary(q, k, positions, freqs, interleaved=False, scale=1.0, inplace=False):
         return q, k
     q, k = _strided(q, False), None if k is None else _strided(k, False)
     if grad:
-        return RotaryFn.apply(q, k, positions, freqs, bool(interleaved), scale)
-    qo = q.new_empty(q.shape)
-    ko = None if k is None else k.new_empty(k.shape)
-    _rotary(q, k, qo, ko, positions, freqs, interleaved, scale, False)
-    return qo, ko
+        return RotaryFn.apply(q, k, positions, freqs, bool(interleaved), scale, False)
+    return _turned(q, k, positions, freqs, interleaved, scale, False)
 
 
 # ---- attention over packed sequences --------------------------------------------------------------------------------
@@ -2324,6 +2325,19 @@ def _paged_ws(*sizes):
     return _lib.lib().ttsmi_paged_attention_ws_bytes(*sizes)
 
 
+class _OnceFn(torch.autograd.Function):
+    """The first n of the tensors, gradients of a pass that has no derivative, tied to what they were computed from (the others):
+    differentiating them is refused.  (torch's once_differentiable ties them to nothing: autograd.grad passes by its error.)"""
+
+    @staticmethod
+    def forward(ctx, n, *tensors):
+        return tuple(t.view_as(t) for t in tensors[:n])
+
+    @staticmethod
+    def backward(ctx, *grads):
+        _refuse('packed_attention: has no second derivatives')
+
+
 class PackedAttentionFn(torch.autograd.Function):
     """softmax(scale q k^T) v within packed sequences, grouped heads (ttsmi_packed_attention_fwd / _bwd)."""
 
@@ -2343,7 +2357,7 @@ class PackedAttentionFn(torch.autograd.Function):
         scale, causal = ctx.cfg
         M, H, dh = q.shape
         B, Hkv = starts.numel() - 1, k.shape[1]
-        dout = _strided(dout, True, H // Hkv)
+        given, dout = dout, _strided(dout, True, H // Hkv)
         dq, dk, dv = torch.empty_like(out), torch.empty(k.shape, dtype=k.dtype, device=k.device), torch.empty(v.shape, dtype=v.dtype, device=v.device)
         ws = _ws(_packed_bwd_ws(B, M, H, Hkv, dh, int(causal)), q.device)
         row, krow = H * dh, Hkv * dh
@@ -2351,14 +2365,16 @@ class PackedAttentionFn(torch.autograd.Function):
                                                     starts.data_ptr(), B, M, H, Hkv, dh, scale, int(causal), dq.data_ptr(), row, dh,
                                                     dk.data_ptr(), krow, dh, dv.data_ptr(), krow, dh, 1, ws.data_ptr(), ws.numel(),
                                                     _SEQ_DTYPES[q.dtype], _seq_stream(q.device.index)), 'packed_attention_bwd')
+        if torch.is_grad_enabled():                        # create_graph
+            dq, dk, dv = _OnceFn.apply(3, dq, dk, dv, q, k, v, given)
         return dq, dk, dv, None, None, None
 
 
 def packed_attention(q, k, v, starts, causal=True, scale=None):
     """Attention within each of the packed sequences: q [tokens, H, dh], k and v [tokens, Hkv, dh], H a multiple of Hkv (query
     head h reads key head h // (H // Hkv)), dh a multiple of 8 up to 192; sequence b is tokens starts[b] .. starts[b + 1], over
-    the keys up to the query's own if causal and over all of them otherwise; scale defaults to dh ** -0.5.  Tokens in
-    front of starts[0] and behind starts[-1] get zeros, and zero gradients.  -> [tokens, H, dh].  Tensors whose rows or heads do not lie on 16-byte
+    the keys up to the query's own if causal and over all of them otherwise; scale defaults to dh ** -0.5.  Gradients, but no
+    second derivatives.  Tokens in front of starts[0] and behind starts[-1] get zeros, and zero gradients.  -> [tokens, H, dh].  Tensors whose rows or heads do not lie on 16-byte
     boundaries are copied first."""
     _seq_check('packed_attention: q', q)
     dev = q.get_device()
