@@ -210,3 +210,29 @@ def test_second_derivatives_of_rotary_are_turns(world):
     again = torch.autograd.grad(grads, (dq, dk), (torch.ones(3, 2, 8), torch.ones(3, 1, 8)))
     assert [tuple(g.shape) for g in again] == [(3, 2, 8), (3, 1, 8)]
     assert [a[-3] for _, a in rec.calls] == [0, 1, 0] and [a[-4] for _, a in rec.calls] == [0.5] * 3
+
+
+def test_forward_mode_tangents_are_refused(world):
+    """A dual tensor wants no gradient and has a pointer: its tangent would be dropped."""
+    from transformertts_amd import _lib
+    import torch.autograd.forward_ad as fwd
+    ops, rec = world
+    q, k, v, freqs = _t(3, 2, 8), _t(3, 1, 8), _t(3, 1, 8), _t(4, dtype=torch.float64)
+    st, ln, table, pos, cache = _ints(0, 3), _ints(3), _ints(0).view(1, 1), _ints(0, 1, 2), _cache(ops)
+    with fwd.dual_level():
+        def dual(t):
+            return fwd.make_dual(t, torch.ones(t.shape, dtype=t.dtype)).as_subclass(OnGpu)
+        a, b, f = dual(q), dual(k), dual(freqs)
+        learned = ops.KVCache(dual(torch.zeros(2, 1, 4, 8)), torch.zeros(2, 1, 4, 8).as_subclass(OnGpu))
+        for call in (lambda: ops.rotary(a, k, pos, freqs), lambda: ops.rotary(q, b, pos, freqs), lambda: ops.rotary(a, None, pos, freqs, inplace=True),
+                     lambda: ops.rotary(q, k, pos, f), lambda: ops.packed_attention(a, k, v, st), lambda: ops.packed_attention(q, b, v, st),
+                     lambda: ops.packed_attention(q, k, b, st), lambda: ops.packed_attention(a.detach().requires_grad_(), b, v, st),
+                     lambda: ops.kv_cache_write(cache, b, v, table, st, ln), lambda: ops.kv_cache_write(cache, k, b, table, st, ln),
+                     lambda: ops.kv_cache_read(learned, table, ln, st, 3, out=(_t(3, 1, 8), _t(3, 1, 8))), lambda: ops.paged_attention(a, cache, table, st, ln),
+                     lambda: ops.paged_attention(q, learned, table, st, ln), lambda: ops.paged_attention(q, cache, table, st, ln, out=dual(_t(3, 2, 8)))):
+            with pytest.raises(_lib.TtsmiError, match='tangent'):
+                call()
+        assert not rec.calls
+        ops.packed_attention(q, k, v, st)                  # tensors of no tangent go through
+        ops.paged_attention(q, cache, table, st, ln)
+    assert len(rec.calls) == 2

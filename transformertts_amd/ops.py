@@ -15,6 +15,7 @@ import os
 from typing import Optional
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from ._lib import TTSMI_F32, check
@@ -2208,8 +2209,17 @@ def _scale_of(scale, dh):
     return scale
 
 
+def _no_tangent(name, *tensors):
+    """Refuses the dual tensors of forward-mode differentiation: no operator here gives tangents."""
+    if forward_ad._current_level >= 0:
+        for t in tensors:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                _refuse(f'{name}: has no forward-mode derivative for a tensor of {tuple(t.shape)} with a tangent')
+
+
 def _no_gradient(name, *tensors):
     """Refuses tensors that want a gradient which the call does not give."""
+    _no_tangent(name, *tensors)
     if torch.is_grad_enabled():
         for t in tensors:
             if t is not None and t.requires_grad:
@@ -2286,6 +2296,7 @@ def rotary(q, k, positions, freqs, interleaved=False, scale=1.0, inplace=False):
             _refuse(f'rotary: {M} queries and {k.shape[0]} keys')
         grad = grad or k.requires_grad
     grad = grad and torch.is_grad_enabled()
+    _no_tangent('rotary', q, k)
     freqs, scale = _c(freqs), float(scale)
     if inplace:
         if grad:
@@ -2392,6 +2403,7 @@ def packed_attention(q, k, v, starts, causal=True, scale=None):
     starts = _ints_check('packed_attention', 'starts', starts, dev)
     if starts.numel() == 0:
         _refuse('packed_attention: starts holds the end of the last sequence at least')
+    _no_tangent('packed_attention', q, k, v)
     scale = _scale_of(scale, dh)
     q, k, v = _strided(q, True, H // Hkv), _strided(k, True, 1), _strided(v, True, 1)
     if (q.requires_grad or k.requires_grad or v.requires_grad) and torch.is_grad_enabled():
