@@ -236,3 +236,37 @@ def test_forward_mode_tangents_are_refused(world):
         ops.packed_attention(q, k, v, st)                  # tensors of no tangent go through
         ops.paged_attention(q, cache, table, st, ln)
     assert len(rec.calls) == 2
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.float8_e4m3fn])
+def test_a_cache_holds_the_tensors_it_was_made_of(world, dtype):
+    """Its tensors cannot be exchanged under the pointers that the calls use: assigning is an error, and a tensor whose memory has
+    moved is noticed before anything is launched."""
+    from transformertts_amd import _lib
+    ops, rec = world
+    q, k, v = _t(3, 2, 8), _t(3, 1, 8), _t(3, 1, 8)
+    st, ln, table = _ints(0, 3), _ints(3), _ints(0).view(1, 1)
+    cache = _cache(ops, dtype)
+    names = ['k', 'v'] + ['k_exp', 'v_exp'] * (cache.k_exp is not None)
+    for name in names + ['args', 'heads', 'dh', 'page_size', 'dtype', 'code', 'index']:
+        old = getattr(cache, name)
+        with pytest.raises(AttributeError):
+            setattr(cache, name, old)
+        with pytest.raises(AttributeError):
+            delattr(cache, name)
+        assert getattr(cache, name) is old
+    for name in names:
+        cache = _cache(ops, dtype)
+        t = getattr(cache, name)
+        kept = t.data                                      # (the old memory stays where it is)
+        t.data = torch.zeros((64,) + t.shape[1:], dtype=torch.uint8).view(t.dtype) if t.element_size() == 1 else torch.zeros((64,) + t.shape[1:])
+        for call in (lambda: ops.kv_cache_write(cache, k, v, table, st, ln), lambda: ops.paged_attention(q, cache, table, st, ln),
+                     lambda: ops.kv_cache_read(cache, table, ln, st, 3, out=(_t(3, 1, 8), _t(3, 1, 8)))):
+            with pytest.raises(_lib.TtsmiError, match='moved'):
+                call()
+        t.data = kept
+        ops.kv_cache_write(cache, k, v, table, st, ln)
+    assert len(rec.calls) == len(names)
+    import copy
+    other = copy.copy(cache)
+    assert other.args == cache.args and other.k is cache.k and other.heads == cache.heads

@@ -134,3 +134,26 @@ def test_attention_differentiated_twice_is_refused():
     assert all(torch.equal(a, b) for a, b in zip(grads, once))
     with pytest.raises(_lib.TtsmiError, match='second derivatives'):
         torch.autograd.grad(sum((g.float() ** 2).sum() for g in grads), x)
+
+
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float8_e4m3fn])
+def test_growing_a_cache(dtype):
+    """Larger pages are a new cache: the old rows copied, both read as before; the tensors of a cache are not exchanged."""
+    ops = _ops()
+    old = ops.KVCache.zeros(2, 16, 2, 64, dtype, DEV)
+    st, ln, table = _ints([0, 20]), _ints([20]), _ints([[1, 0]])
+    q, k, v = (_randn((20, h, 64), i, torch.bfloat16) for i, h in enumerate((4, 2, 2)))
+    ops.kv_cache_write(old, k, v, table, st, ln)
+    want = ops.paged_attention(q, old, table, st, ln)
+    with pytest.raises(AttributeError):
+        old.k = torch.zeros_like(old.k)
+    grown = ops.KVCache.zeros(5, 16, 2, 64, dtype, DEV)
+    for name in ('k', 'v', 'k_exp', 'v_exp'):
+        a, b = getattr(old, name), getattr(grown, name)
+        if a is not None:
+            b.view(torch.uint8)[:2].copy_(a.view(torch.uint8))
+    import copy
+    twin = copy.deepcopy(old)
+    assert twin.k.data_ptr() != old.k.data_ptr() == old.args[0]
+    for cache in (grown, old, twin):
+        assert torch.equal(ops.paged_attention(q, cache, table, st, ln), want)

@@ -2418,18 +2418,27 @@ _CACHE_DTYPES = {torch.float32: TTSMI_F32, torch.bfloat16: _lib.TTSMI_BF16_IO, t
 class KVCache:
     """The pages of a key / value cache: k and v [pages, Hkv, page size, dh] of float32, bfloat16 or float8_e4m3fn, the page size
     a power of two up to 1024; float8_e4m3fn pages with k_exp and v_exp [pages, Hkv, page size] uint8, the biased exponent of
-    each row's power-of-two scale (value = e4m3 * 2 ** (exp - 127)).  It holds the tensors it is given; which pages belong to
-    which sequence is the caller's (`table`)."""
+    each row's power-of-two scale (value = e4m3 * 2 ** (exp - 127)).  It holds the tensors it is given, for good: a cache of other
+    or larger tensors is a new KVCache.  Which pages belong to which sequence is the caller's (`table`)."""
     __slots__ = ('k', 'v', 'k_exp', 'v_exp', 'args', 'heads', 'dh', 'page_size', 'dtype', 'code', 'index')
+
+    def __setattr__(self, name, value):                    # (the calls pass the pointers in `args`)
+        raise AttributeError(f'KVCache.{name} is read-only: make a KVCache of other tensors')
+
+    def __delattr__(self, name):
+        self.__setattr__(name, None)
+
+    def __reduce__(self):                                  # a copy is a cache of the copied tensors
+        return type(self), (self.k, self.v, self.k_exp, self.v_exp)
 
     def __init__(self, k, v, k_exp=None, v_exp=None):
         if k.dim() != 4 or k.shape != v.shape or k.dtype != v.dtype or k.device != v.device or k.dtype not in _CACHE_DTYPES:
             _refuse(f'KVCache: pages {tuple(k.shape)} {k.dtype} and {tuple(v.shape)} {v.dtype}')
-        n, self.heads, size, self.dh = k.shape
-        if not 0 < size <= 1024 or size & (size - 1) or self.heads == 0:
+        n, heads, size, dh = k.shape
+        if not 0 < size <= 1024 or size & (size - 1) or heads == 0:
             _refuse(f'KVCache: pages of {size} rows (a power of two up to 1024)')
-        if self.dh % 8 or not 0 < self.dh <= 192:
-            _refuse(f'KVCache: head size {self.dh} (a multiple of 8 up to 192)')
+        if dh % 8 or not 0 < dh <= 192:
+            _refuse(f'KVCache: head size {dh} (a multiple of 8 up to 192)')
         quantised = k.dtype == torch.float8_e4m3fn
         if (k_exp is None or v_exp is None) if quantised else (k_exp is not None or v_exp is not None):
             _refuse('KVCache: float8_e4m3fn pages, and only they, have exponents')
@@ -2439,9 +2448,10 @@ class KVCache:
         _need_gpu(k)
         if not k.is_contiguous() or not v.is_contiguous() or (k.data_ptr() | v.data_ptr()) % 16 or (k.numel() and k.data_ptr() == v.data_ptr()):
             _refuse('KVCache: contiguous, 16-byte aligned pages, of keys and of values')
-        self.k, self.v, self.k_exp, self.v_exp, self.dtype, self.page_size = k, v, k_exp, v_exp, k.dtype, size
-        self.index, self.code = k.get_device(), _CACHE_DTYPES[k.dtype]
-        self.args = (k.data_ptr(), v.data_ptr(), _p(k_exp), _p(v_exp), self.code, n, size)
+        code = _CACHE_DTYPES[k.dtype]
+        args = (k.data_ptr(), v.data_ptr(), _p(k_exp), _p(v_exp), code, n, size)
+        for name, value in zip(self.__slots__, (k, v, k_exp, v_exp, args, heads, dh, size, k.dtype, code, k.get_device())):
+            object.__setattr__(self, name, value)
 
     @classmethod
     def zeros(cls, pages, page_size, heads, dh, dtype=torch.bfloat16, device='cuda'):
@@ -2457,6 +2467,9 @@ class KVCache:
 def _paged_check(name, cache, table, starts, lens):
     if not isinstance(cache, KVCache):
         _refuse(f'{name}: a KVCache')
+    k, v, ke, ve = cache.args[:4]
+    if cache.k.data_ptr() != k or cache.v.data_ptr() != v or (ke is not None and (cache.k_exp.data_ptr() != ke or cache.v_exp.data_ptr() != ve)):
+        _refuse(f'{name}: a tensor of the cache has moved to other memory (resize_, set_, .data): make a KVCache of it')
     dev = cache.index
     table, starts, lens = _ints_check(name, 'table', table, dev, 2), _ints_check(name, 'starts', starts, dev), _ints_check(name, 'lens', lens, dev)
     if starts.numel() != lens.numel() + 1 or table.shape[0] != lens.numel():
