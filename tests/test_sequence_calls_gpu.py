@@ -157,3 +157,29 @@ def test_growing_a_cache(dtype):
     assert twin.k.data_ptr() != old.k.data_ptr() == old.args[0]
     for cache in (grown, old, twin):
         assert torch.equal(ops.paged_attention(q, cache, table, st, ln), want)
+
+
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize('causal', [True, False])
+@pytest.mark.parametrize('lens,H,Hkv', [([61], 2, 2), ([193], 1, 1), ([200], 2, 1), ([61], 16, 1), ([130, 0, 400, 1], 8, 2), ([129] * 7, 16, 4), ([1500], 4, 1), ([5, 700, 3], 32, 2)])
+def test_backward_stays_in_its_workspace(lens, H, Hkv, causal, dtype):
+    """No byte behind the size asked for, with splits and without; the gradients are the ones that a far larger batch's workspace
+    gives (which division of the rows is made goes by the tokens, not by the workspace)."""
+    from transformertts_amd import _lib
+    ops, dh = _ops(), 64
+    M, B = sum(lens), len(lens)
+    q, k, v, d = (_randn((M, h, dh), i, dtype) for i, h in enumerate((H, Hkv, Hkv, H)))
+    st = _ints([0] + torch.tensor(lens).cumsum(0).tolist())
+    out, lse, rest = ops._packed_fwd(q, k, v, st, 0.125, causal, True)
+    need = _lib.lib().ttsmi_packed_attention_bwd_ws_bytes(B, M, H, Hkv, dh, int(causal))
+    args = lambda *ts: [a for t in ts for a in (t.data_ptr(), t.stride(0), t.stride(1))]
+    want = None
+    for ws_bytes, fill in ((need, 0x7f), (need, 0xff), (need + (1 << 20), 0x55)):
+        ws = torch.full((ws_bytes + 4096,), fill, dtype=torch.uint8, device=DEV)
+        g = [torch.full_like(t, float('nan')) for t in (q, k, v)]
+        assert _lib.lib().ttsmi_packed_attention_bwd(*args(q, k, v, out), None if rest is None else rest.data_ptr(), *args(d), lse.data_ptr(), st.data_ptr(), B, M, H, Hkv,
+                                                     dh, 0.125, int(causal), *args(*g), 1, ws.data_ptr(), ws_bytes, ops._SEQ_DTYPES[dtype],
+                                                     torch.cuda.current_stream().cuda_stream) == 0
+        assert bool((ws[need:] == fill).all()) and all(bool(torch.isfinite(t).all()) for t in g)
+        want = want or g
+        assert all(torch.equal(a, b) for a, b in zip(g, want))

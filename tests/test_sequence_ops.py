@@ -133,3 +133,17 @@ def test_rotary_frequencies():
     for bad in (dict(dim=7), dict(dim=0), dict(dim=8, scaling='ntk'), dict(dim=8, factor=0.0), dict(dim=8, scaling='bands', slow_turns=4.0, fast_turns=4.0)):
         with pytest.raises(ValueError):
             rotary_frequencies(**bad)
+
+
+def test_packed_attention_bwd_workspace_follows_the_tokens(lib):
+    """delta and lse2, and partial sums for no more row splits than the tokens allow: a split has 192 rows at least, a sequence of
+    no more than that (61 tokens, one or two heads a key head) none."""
+    need = lib.ttsmi_packed_attention_bwd_ws_bytes
+    for B, tokens, H, Hkv, dh in ((1, 61, 2, 2, 192), (1, 61, 4, 2, 64), (3, 190, 8, 8, 128), (0, 96, 4, 2, 64), (40, 96, 32, 16, 192)):
+        for causal in (0, 1):
+            assert need(B, tokens, H, Hkv, dh, causal) == (2 * tokens * H * 4 + 255) // 256 * 256
+    tile = 2 * 128 * 64 * 4                                              # dK and dV of 128 keys of 64
+    assert need(1, 61, 16, 1, 64, 1) == (2 * 61 * 16 * 4 + 255) // 256 * 256 + (1 + 1 + 5) * tile                 # 976 rows, one key tile: 5 splits behind the first
+    for causal, slots in ((0, 512), (1, 1536)):                          # long ones: what the card holds, as before
+        assert need(1, 6000, 16, 2, 128, causal) == 2 * 6000 * 16 * 4 + (6000 // 128 + 2 + slots // 2) * 2 * 2 * tile
+        assert need(1, 6000, 2, 1, 64, causal) == 2 * 6000 * 2 * 4 + (6000 // 128 + 2 + slots) * tile

@@ -17,6 +17,8 @@
 // of 64: 38 and 40 us; fp32, 8 utterances of 117 .. 700, 4 / 2 heads of 64: 32 (48 with two waves a row block), 38 and 5 us.
 #include "seq_common.h"
 
+#include <algorithm>
+
 struct SeqBwdP {
     const void* q; long q_row, q_head;
     const void* k; long k_row, k_head;
@@ -31,8 +33,9 @@ struct SeqBwdP {
     const int* starts;
     int B, tokens, Hkv, G, dh, causal, zero_rest;
     float scale, c1;
-    // row splits of the dK / dV pass (slots > 0): sums of unit u, key head hk at [(u Hkv + hk)][dK, dV][128 keys][dh], fp32
-    int slots; float* part;
+    // row splits of the dK / dV pass (slots > 0): sums of unit u, key head hk at [(u Hkv + hk)][dK, dV][128 keys][dh], fp32.
+    // extra: how many splits there can be behind their tiles' first ones, the slots or fewer (seq_bwd_extra)
+    int slots; long extra; float* part;
 };
 // rows of a split at least: eight tiles of work against the traffic of its partial sums (bf16: a training step of 8 x 512 tokens, 16 / 4
 // heads of 128, 128 us at 512, 144 at 256, 132 at 1024); the fp32 products are slower (8 utterances of 117 .. 700, 4 / 2 heads of 64:
@@ -413,7 +416,7 @@ __global__ __launch_bounds__(256) void seq_dkv_join_kernel(SeqBwdP p) {
     const SeqUnit un = find_unit(p.starts, nullptr, p.G, 0x7fffffff, p.B, p.tokens, 1, 128, p.slots, SeqT<T>::KT, SeqLeast<T>::ROWS, blockIdx.x / p.Hkv, true);
     if (un.t.seq < 0) return;
     const int key0 = un.t.tile * 128, z0 = (p.causal ? key0 * p.G : 0) / un.per;
-    if (un.nsplit - z0 < 2 || un.first + (long)(un.nsplit - 1) * un.t.ntile >= seq_split_units(p.tokens, p.B, 1, 128, p.slots)) return;   // (the latter: `starts` that overlap)
+    if (un.nsplit - z0 < 2 || un.first + (long)(un.nsplit - 1) * un.t.ntile >= seq_split_units(p.tokens, p.B, 1, 128, p.extra)) return;   // (the latter: `starts` that overlap)
     const int per = p.dh / 4, keys = min(16, un.t.n - key0 - 16 * (int)blockIdx.y);
     const long step = 2L * 128 * p.dh * p.Hkv * un.t.ntile;
     for (int i = threadIdx.x; i < 2 * keys * per; i += 256) {
@@ -440,6 +443,12 @@ static int seq_bwd_slots(int tokens, int Hkv, int causal) {
     const int all = causal ? 1536 : 512, fill = all / Hkv < 1 ? 1 : all / Hkv;
     return tokens / 128 >= fill ? 0 : fill;
 }
+// Splits that there can be behind their tiles' first ones, sum_b tiles_b (splits_b - 1), a split having `least` rows or more: the
+// slots, or fewer where the tokens do not allow that many - most where one sequence has them all.  None: no sequence is split, and
+// nothing is joined.  (The partial sums of one utterance of 61 tokens, 2 heads of 192: none, where 1536 slots took 303 MB.)
+static long seq_bwd_extra(int tokens, int G, int slots, int least) {
+    return std::min((long)slots, ((long)tokens + 127) / 128 * (((long)tokens * G - 1) / least));
+}
 
 template <typename T, int DHP>
 static void seq_bwd_launch(const SeqBwdP& p, hipStream_t st) {
@@ -453,7 +462,7 @@ static void seq_bwd_launch(const SeqBwdP& p, hipStream_t st) {
         if (parts == 2) hipLaunchKernelGGL((seq_attn_dq_kernel<T, DHP, 2>), g, dim3(256), 0, st, p);
     }
     if (parts == 1) hipLaunchKernelGGL((seq_attn_dq_kernel<T, DHP, 1>), g, dim3(256), 0, st, p);
-    hipLaunchKernelGGL((seq_attn_dkv_kernel<T, DHP>), dim3((unsigned)((p.slots > 0 ? seq_split_units(p.tokens, p.B, 1, 128, p.slots) : seq_units(p.tokens, p.B, 1, 128)) * p.Hkv)), dim3(256), 0, st, p);
+    hipLaunchKernelGGL((seq_attn_dkv_kernel<T, DHP>), dim3((unsigned)((p.slots > 0 ? seq_split_units(p.tokens, p.B, 1, 128, p.extra) : seq_units(p.tokens, p.B, 1, 128)) * p.Hkv)), dim3(256), 0, st, p);
     if (p.slots > 0) hipLaunchKernelGGL((seq_dkv_join_kernel<T>), dim3((unsigned)(seq_units(p.tokens, p.B, 1, 128) * p.Hkv), 8), dim3(256), 0, st, p);
 }
 template <typename T>
@@ -468,8 +477,8 @@ static int seq_bwd_route(const SeqBwdP& p, hipStream_t st) {
 static size_t seq_delta_bytes(int tokens, int H) { return (2 * (size_t)tokens * H * sizeof(float) + 255) / 256 * 256; }     // delta and lse2
 extern "C" size_t ttsmi_packed_attention_bwd_ws_bytes(int B, int tokens, int H, int Hkv, int dh, int causal) {
     if (B < 0 || tokens <= 0 || H <= 0 || Hkv <= 0 || dh <= 0) return 0;
-    const int slots = seq_bwd_slots(tokens, Hkv, causal);
-    return seq_delta_bytes(tokens, H) + (slots ? (size_t)seq_split_units(tokens, B, 1, 128, slots) * Hkv * 2 * 128 * dh * sizeof(float) : 0);
+    const long extra = seq_bwd_extra(tokens, H / Hkv, seq_bwd_slots(tokens, Hkv, causal), std::min(SeqLeast<float>::ROWS, SeqLeast<__bf16>::ROWS));
+    return seq_delta_bytes(tokens, H) + (extra ? (size_t)seq_split_units(tokens, B, 1, 128, extra) * Hkv * 2 * 128 * dh * sizeof(float) : 0);
 }
 extern "C" int ttsmi_packed_attention_bwd(const void* q, int64_t q_row, int64_t q_head, const void* k, int64_t k_row, int64_t k_head,
                                           const void* v, int64_t v_row, int64_t v_head, const void* out, int64_t o_row, int64_t o_head,
@@ -497,6 +506,8 @@ extern "C" int ttsmi_packed_attention_bwd(const void* q, int64_t q_row, int64_t 
     p.lse = lse; p.delta = (float*)ws; p.lse2 = (float*)ws + (size_t)tokens * H; p.starts = starts; p.B = B; p.tokens = tokens; p.Hkv = Hkv; p.G = H / Hkv; p.dh = dh;
     p.causal = causal != 0; p.zero_rest = zero_rest != 0; p.scale = scale; p.c1 = scale * SEQ_LOG2E;
     p.slots = seq_bwd_slots(tokens, Hkv, causal);
+    p.extra = seq_bwd_extra(tokens, p.G, p.slots, dtype == TTSMI_F32 ? SeqLeast<float>::ROWS : SeqLeast<__bf16>::ROWS);
+    if (p.extra == 0) p.slots = 0;
     p.part = (float*)((char*)ws + seq_delta_bytes(tokens, H));
     return dtype == TTSMI_F32 ? seq_bwd_route<float>(p, (hipStream_t)stream) : seq_bwd_route<__bf16>(p, (hipStream_t)stream);
 }

@@ -179,7 +179,7 @@ struct SeqUnit {
     int split, nsplit, per;       // key range [split per, (split + 1) per)
     long first;                   // unit number of the tile's first split; its next ones follow at steps of ntile
 };
-static inline __host__ __device__ long seq_split_units(long tokens, int B, int G, int R, int slots) { return tokens * G / R + B + 1 + slots; }
+static inline __host__ __device__ long seq_split_units(long tokens, int B, int G, int R, long slots) { return tokens * G / R + B + 1 + slots; }
 // Tiles: R rows of G a token.  Keys: lens, `most` of them at most, or `own` times the sequence's tokens where lens is null (the
 // backward's splits of the rows that a key tile meets).  by_tile: `unit` counts tiles instead (the join).
 __device__ __forceinline__ SeqUnit find_unit(const int* starts, const int* lens, int own, int most, int B, int tokens, int G, int R, int slots,
