@@ -815,7 +815,7 @@ int ttsmi_pad_cols_f32(const float* src, int C, float* dst, int Cp, int M, ttsmi
 /* The first rot elements of every head turned by position: pair (2i, 2i + 1) (interleaved != 0) or (i, i + rot / 2) of a
  * token at positions[t] by the angle positions[t] * freqs[i] (freqs: rot / 2 doubles, radians per position; the angle is
  * reduced in 64 bits), times scale; inverse != 0 turns back (the gradient).  Elements from rot on are copied.  q and k in
- * one launch; either may be absent (heads 0).  In place (output = input, same strides) is allowed.  dh even, rot even and at
+ * one launch; either may be absent (heads 0).  In place (output = input, same strides) is allowed where q and k share no memory.  dh even, rot even and at
  * most 512; no other alignment is needed. */
 int ttsmi_rotary(const void* q, int64_t q_row, int64_t q_head, void* qo, int64_t qo_row, int64_t qo_head, int H, const void* k,
                  int64_t k_row, int64_t k_head, void* ko, int64_t ko_row, int64_t ko_head, int Hkv, const int32_t* positions,
@@ -848,7 +848,8 @@ int ttsmi_packed_attention_bwd(const void* q, int64_t q_row, int64_t q_head, con
  * sequence b INCLUDING its starts[b + 1] - starts[b] new tokens, which are the last ones.  A page number outside
  * [0, n_pages) is never written and reads as zeros; a new token without a position (lens too small, or past the table) is not
  * written.
- * A page may stand in several tables for reading; a call that writes one row twice leaves either.
+ * A page may stand in several tables for reading; a row that one call writes twice may hold parts of both (and, e4m3, the scale
+ * of the other).  k and v are not rows of the pages.
  * e4m3: the smallest power-of-two scale that brings the row's largest finite magnitude to 448 at most, each value rounded to
  * nearest even; NaN and infinity become NaN. */
 int ttsmi_kv_cache_write(const void* k, int64_t k_row, int64_t k_head, const void* v, int64_t v_row, int64_t v_head, void* k_pages,
@@ -863,7 +864,7 @@ int ttsmi_kv_cache_read(const void* k_pages, const void* v_pages, const uint8_t*
                         int64_t v_row, int64_t v_head, int zero_rest, int dtype, ttsmi_stream_t stream);
 /* Attention of the packed new tokens over the cache (their own keys and values written before): token i of sequence b, n of
  * them, is at position lens[b] - n + i and sees the keys up to it.  A token that sees none gets zeros; positions past the
- * table's pages (or 2^30) hold no key.  The keys are split over workgroups by the lengths found on the device; the sums of the
+ * table's pages (or 2^30) hold no key.  out may be q (with its strides).  The keys are split over workgroups by the lengths found on the device; the sums of the
  * splits pass through ws. */
 size_t ttsmi_paged_attention_ws_bytes(int B, int tokens, int H, int Hkv, int dh, int cache_dtype, int dtype);
 int ttsmi_paged_attention(const void* q, int64_t q_row, int64_t q_head, const void* k_pages, const void* v_pages,

@@ -270,3 +270,64 @@ def test_a_cache_holds_the_tensors_it_was_made_of(world, dtype):
     import copy
     other = copy.copy(cache)
     assert other.args == cache.args and other.k is cache.k and other.heads == cache.heads
+
+
+def test_the_overlap_of_views_is_found(world):
+    """ops._share against the elements' own addresses, over views of one buffer in every order that a layer makes."""
+    import random
+    ops, _ = world
+    rng, found = random.Random(3), [0, 0]
+    base = torch.zeros(6000)
+
+    def addresses(t):
+        return {t.storage_offset() + i * t.stride(0) + j * t.stride(1) + c for i in range(t.shape[0]) for j in range(t.shape[1]) for c in range(t.shape[2])}
+    for n in range(4000):
+        M, dh = rng.choice([1, 2, 3, 7]), rng.choice([2, 4, 8])
+        views = []
+        layout, W = rng.choice(['rows', 'heads', 'parts']), rng.choice([2, 3, 6])
+        for _ in 'ab':
+            if layout == 'rows':                           # parts of a fused projection
+                x, lo = base[:M * W * dh].view(M, W, dh), rng.randrange(W)
+                views.append(x[:, lo:lo + rng.randint(1, W)] if rng.random() < 0.8 else x[:, lo::2])
+            elif layout == 'heads':                        # [heads, tokens, dh]
+                x, lo = base[:W * M * dh].view(W, M, dh), rng.randrange(W)
+                views.append(x[lo:lo + rng.randint(1, W)].transpose(0, 1))
+            else:                                          # [tokens, heads, parts, dh]
+                x = base[:M * W * 3 * dh].view(M, W, 3, dh)
+                views.append(x[:, :, rng.randrange(3)])
+        if rng.random() < 0.3:
+            shift = rng.randrange(1, 3 * dh)
+            views[1] = torch.as_strided(base, views[1].shape, views[1].stride(), views[1].storage_offset() + shift)
+        common = bool(addresses(views[0]) & addresses(views[1]))
+        found[common] += 1
+        assert ops._share(*views) == common, (n, layout, [(tuple(v.shape), v.stride(), v.storage_offset()) for v in views])
+    assert min(found) > 500
+    assert not ops._share(base[:0].view(0, 1, 2), base[:2].view(1, 1, 2)) and not ops._share(base[:4].view(2, 1, 2), torch.zeros(2, 1, 2))
+
+
+def test_destinations_that_share_memory_are_refused(world):
+    """Keys and queries turned in place, rows read back and attention's output would be written over each other or while they are
+    read; an output that is the queries themselves is not among them."""
+    from transformertts_amd import _lib
+    ops, rec = world
+    x = torch.ones(3, 6, 8).as_subclass(OnGpu)
+    st, ln, table, pos, freqs, cache = _ints(0, 3), _ints(3), _ints(0).view(1, 1), _ints(0, 1, 2), _t(4, dtype=torch.float64), _cache(ops)
+    pages = torch.zeros(3, 1, 4, 8).as_subclass(OnGpu)
+    bytes_ = torch.zeros(256, dtype=torch.uint8)
+    e4m3 = [bytes_[n:n + 64].view(torch.float8_e4m3fn).view(2, 1, 4, 8).as_subclass(OnGpu) for n in (0, 64)]
+    exps = [bytes_[n:n + 8].view(2, 1, 4).as_subclass(OnGpu) for n in (128, 136, 132, 60)]
+    for call in (lambda: ops.rotary(x[:, :4], x[:, :4], pos, freqs, inplace=True), lambda: ops.rotary(x[:, :4], x[:, 3:5], pos, freqs, inplace=True),
+                 lambda: ops.kv_cache_read(cache, table, ln, st, 3, out=(x[:, :1], x[:, :1])),
+                 lambda: ops.paged_attention(x[:, :4], cache, table, st, ln, out=x[:, 1:5]),
+                 lambda: ops.KVCache(pages[:2], pages[1:]), lambda: ops.KVCache(*e4m3, exps[0], exps[2]), lambda: ops.KVCache(*e4m3, exps[0], exps[0]),
+                 lambda: ops.KVCache(*e4m3, exps[3], exps[1])):
+        with pytest.raises(_lib.TtsmiError, match='memory'):
+            call()
+    assert not rec.calls
+    ops.rotary(x[:, :4], x[:, 4:6], pos, freqs, inplace=True)
+    ops.rotary(x[:, :4], x[:, 3:5], pos, freqs)
+    ops.kv_cache_read(cache, table, ln, st, 3, out=(x[:, :1], x[:, 1:2]))
+    ops.paged_attention(x[:, :4], cache, table, st, ln, out=x[:, :4])
+    ops.KVCache(pages[:1], pages[1:2])
+    ops.KVCache(*e4m3, exps[0], exps[1])
+    assert len(rec.calls) == 4

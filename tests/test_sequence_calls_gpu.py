@@ -183,3 +183,26 @@ def test_backward_stays_in_its_workspace(lens, H, Hkv, causal, dtype):
         assert bool((ws[need:] == fill).all()) and all(bool(torch.isfinite(t).all()) for t in g)
         want = want or g
         assert all(torch.equal(a, b) for a, b in zip(g, want))
+
+
+@pytest.mark.parametrize('new,lens,H,Hkv,page', [([1] * 3, [900, 33, 4000], 8, 2, 16), ([200, 5], [2000, 5], 16, 2, 8), ([70], [70], 4, 4, 64), ([300], [3000], 8, 1, 4)])
+@pytest.mark.parametrize('dtype,stored', [(torch.bfloat16, torch.bfloat16), (torch.bfloat16, torch.float8_e4m3fn), (torch.float32, torch.float32)])
+def test_attention_into_its_own_queries(new, lens, H, Hkv, page, dtype, stored):
+    """out = q, split keys and whole ones: the same bits as into a tensor of its own, rows of no sequence left as they were."""
+    ops, dh = _ops(), 64
+    counts = [-(-n // page) for n in lens]
+    cache = ops.KVCache.zeros(sum(counts), page, Hkv, dh, stored, DEV)
+    order = torch.randperm(sum(counts), generator=torch.Generator().manual_seed(1)).to(torch.int32)
+    table, at = torch.full((len(lens), max(counts)), -1, dtype=torch.int32), 0
+    for b, c in enumerate(counts):
+        table[b, :c] = order[at:at + c]
+        at += c
+    table, ln, total = table.to(DEV), _ints(lens), sum(lens)
+    ops.kv_cache_write(cache, *(_randn((total, Hkv, dh), i, dtype) for i in (1, 2)), table, _ints([0] + torch.tensor(lens).cumsum(0).tolist()), ln)
+    st = _ints([0] + torch.tensor(new).cumsum(0).tolist())
+    fused = _randn((sum(new) + 3, H + 2, dh), 3, dtype)
+    q = fused[:, 1:H + 1]
+    before, want = fused.clone(), ops.paged_attention(q, cache, table, st, ln)
+    assert ops.paged_attention(q, cache, table, st, ln, out=q) is q
+    assert torch.equal(q[:sum(new)], want[:sum(new)]) and torch.equal(q[sum(new):], before[sum(new):, 1:H + 1])
+    assert torch.equal(fused[:, 0], before[:, 0]) and torch.equal(fused[:, -1], before[:, -1])

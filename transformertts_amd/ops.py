@@ -2196,6 +2196,36 @@ def _own_rows(t):
     return all(s > 0 or n < 2 for s, n in zip(t.stride(), t.shape))
 
 
+def _meet(a, b):
+    """Whether the address ranges of two tensors meet."""
+    def ends(t):
+        return t.data_ptr(), t.data_ptr() + (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size()
+    if not a.numel() or not b.numel():
+        return False
+    (a0, a1), (b0, b1) = ends(a), ends(b)
+    return a0 < b1 and b0 < a1
+
+
+def _share(a, b):
+    """Whether two tensors [tokens, heads, dh] of as many tokens have an element's memory in common."""
+    if not _meet(a, b):
+        return False
+    (M, H, dh), (row, head, _), (row2, head2, _) = a.shape, a.stride(), b.stride()
+    if M > 1 and row != row2:
+        return True                                        # (orders as different as that in one buffer: not looked into)
+    at = (b.data_ptr() - a.data_ptr()) // a.element_size()
+    first, last = (a, b) if at >= 0 else (b, a)            # the parts of a fused projection lie one behind the other within a row
+    if (first.shape[1] - 1) * first.stride(1) + dh <= abs(at) and abs(at) + (last.shape[1] - 1) * last.stride(1) + dh <= row:
+        return False
+    for i in range(H):
+        for j in range(b.shape[1]):                        # heads i and j, b's a number of rows behind a's
+            d = at + j * head2 - i * head
+            rows = (0,) if M == 1 else (d // row, d // row + 1)
+            if any(abs(d - n * row) < dh and abs(n) < M for n in rows):
+                return True
+    return False
+
+
 def _rs(t):
     """(pointer, row stride, head stride)"""
     row, head, _ = t.stride()
@@ -2274,7 +2304,7 @@ def rotary(q, k, positions, freqs, interleaved=False, scale=1.0, inplace=False):
     """The first 2 * len(freqs) elements of every head of q [tokens, H, dh] and k [tokens, Hkv, dh] (or None) turned by
     positions [tokens] int32 times freqs (float64 radians per position, model.transformer_utils.rotary_frequencies; no gradient), pairs
     (2 i, 2 i + 1) if interleaved and (i, i + len(freqs)) otherwise, times scale; the rest passes through.  -> (q, k).
-    inplace: q and k themselves, without gradients."""
+    inplace: q and k themselves, which share no memory, without gradients."""
     _seq_check('rotary: q', q)
     dev = q.get_device()
     if dev != _current_device():
@@ -2303,6 +2333,8 @@ def rotary(q, k, positions, freqs, interleaved=False, scale=1.0, inplace=False):
             _refuse('rotary: in place on a tensor that wants a gradient')
         if any(t is not None and (t.stride(2) != 1 or not _own_rows(t)) for t in (q, k)):
             _refuse('rotary: in place needs a contiguous last dimension, and no broadcast one')
+        if k is not None and _share(q, k):
+            _refuse('rotary: in place on queries and keys that share memory')
         _rotary(q, k, q, k, positions, freqs, interleaved, scale, False)
         _written([q] if k is None else [q, k])
         return q, k
@@ -2446,8 +2478,11 @@ class KVCache:
             if t.shape != k.shape[:3] or t.dtype != torch.uint8 or t.device != k.device or not t.is_contiguous():
                 _refuse(f'KVCache: exponents {tuple(t.shape)} {t.dtype} of pages {tuple(k.shape)}')
         _need_gpu(k)
-        if not k.is_contiguous() or not v.is_contiguous() or (k.data_ptr() | v.data_ptr()) % 16 or (k.numel() and k.data_ptr() == v.data_ptr()):
-            _refuse('KVCache: contiguous, 16-byte aligned pages, of keys and of values')
+        if not k.is_contiguous() or not v.is_contiguous() or (k.data_ptr() | v.data_ptr()) % 16:
+            _refuse('KVCache: contiguous, 16-byte aligned pages')
+        spans = sorted((t.data_ptr(), t.nbytes) for t in ((k, v, k_exp, v_exp) if quantised else (k, v)))
+        if n and any(a + held > b for (a, held), (b, _) in zip(spans, spans[1:])):
+            _refuse('KVCache: pages and exponents of keys and values that share memory')
         code = _CACHE_DTYPES[k.dtype]
         args = (k.data_ptr(), v.data_ptr(), _p(k_exp), _p(v_exp), code, n, size)
         for name, value in zip(self.__slots__, (k, v, k_exp, v_exp, args, heads, dh, size, k.dtype, code, k.get_device())):
@@ -2489,8 +2524,8 @@ def _kv_check(name, cache, k, v):
 def kv_cache_write(cache, k, v, table, starts, lens):
     """The packed new tokens' keys and values [tokens, Hkv, dh] into their pages, quantised if the pages are float8_e4m3fn.
     table [B, n] int32: the pages of every sequence in order; starts [B + 1] int32: its new tokens; lens [B] int32: its cached
-    length with them, which are the last ones.  A page number outside the cache, or a token without a position, is not written.
-    Without gradients."""
+    length with them, which are the last ones.  A page number outside the cache, or a token without a position, is not written; a
+    row that one call writes twice may hold parts of both.  k and v are not views of the pages.  Without gradients."""
     table, starts, lens = _paged_check('kv_cache_write', cache, table, starts, lens)
     _kv_check('kv_cache_write', cache, k, v)
     _no_gradient('kv_cache_write', k, v, cache.k, cache.v)
@@ -2522,6 +2557,8 @@ def kv_cache_read(cache, table, lens, starts, tokens, dtype=None, out=None):
     _no_gradient('kv_cache_read', cache.k, cache.v, k, v)
     if out is not None and (k.shape[0] != tokens or _strided(k) is not k or _strided(v) is not v or not _own_rows(k) or not _own_rows(v)):
         _refuse(f'kv_cache_read: out of {tokens} tokens on 16-byte boundaries')
+    if out is not None and _share(k, v):
+        _refuse('kv_cache_read: out of keys and values that share memory')
     check(_lib.lib().ttsmi_kv_cache_read(*cache.args, table.data_ptr(), table.shape[1], starts.data_ptr(), lens.data_ptr(), lens.numel(),
                                          k.shape[0], cache.heads, cache.dh, *_rs(k), *_rs(v), int(out is None), _SEQ_DTYPES[k.dtype],
                                          _seq_stream(cache.index)), 'kv_cache_read')
@@ -2534,7 +2571,7 @@ def paged_attention(q, cache, table, starts, lens, scale=None, out=None):
     """Attention of packed new tokens q [tokens, H, dh] over the cache, their own keys and values in it already
     (kv_cache_write): token i of the n new ones of sequence b is at position lens[b] - n + i and sees the keys up to it; a
     token that sees none gets zeros.  Positions past the table's pages hold no key.  Without gradients.  Rows of no sequence are
-    zeros; in `out` they are left as they were."""
+    zeros; in `out`, which may be q itself, they are left as they were."""
     _seq_check('paged_attention: q', q)
     table, starts, lens = _paged_check('paged_attention', cache, table, starts, lens)
     M, H, dh = q.shape
@@ -2552,6 +2589,8 @@ def paged_attention(q, cache, table, starts, lens, scale=None, out=None):
         out = torch.empty((M, H, dh), dtype=q.dtype, device=q.device)
     elif out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or _strided(out) is not out or not _own_rows(out):
         _refuse(f'paged_attention: out {tuple(out.shape)} {out.dtype} for q {tuple(q.shape)} {q.dtype}, on 16-byte boundaries')
+    elif _rs(out) != _rs(q) and _share(out, q):            # (q itself may be the output: a row is written when its last reader is done)
+        _refuse('paged_attention: out shares memory with q, and is not q')
     dtype = _SEQ_DTYPES[q.dtype]
     need = _paged_ws(lens.numel(), M, H, Hkv, dh, cache.code, dtype)
     ws = _ws(need, q.device) if need else None
