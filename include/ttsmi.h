@@ -822,7 +822,7 @@ int ttsmi_rotary(const void* q, int64_t q_row, int64_t q_head, void* qo, int64_t
                  const double* freqs, int tokens, int dh, int rot, int interleaved, float scale, int inverse, int dtype,
                  ttsmi_stream_t stream);
 /* out = softmax(scale q k^T) v within each sequence, causal != 0: over the keys up to the query's own.  scale > 0.  The sums
- * are held in fp32; bf16: the probabilities are rounded to bf16 for the product with v.  lse [Hkv, tokens, H / Hkv] fp32
+ * are held in fp32; bf16: the probabilities are rounded to bf16 for the product with v (batches of short sequences: to two parts).  lse [Hkv, tokens, H / Hkv] fp32
  * (natural log; may be NULL) is what the backward reads;
  * out_rest [tokens, H, dh] bf16 (contiguous; may be NULL; not used for fp32) is what the rounding of out to bf16 left, with
  * which the backward is more exact.  A masked score never reaches the softmax, whatever k holds.  A NaN

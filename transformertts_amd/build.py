@@ -17,11 +17,12 @@ OBJDIR = os.path.join(HERE, 'build')
 LIB = os.path.join(LIBDIR, 'libttsmi.so')
 SOURCES = ['api.cpp', 'gemm.hip', 'gemm_bf16.hip', 'attention.hip', 'attention_bf16.hip', 'layernorm.hip',
            'elementwise.hip', 'lenreg.hip', 'stft_mel.hip', 'dense_block.hip', 'rowgemm.hip', 'gemm_k256.hip', 'chain.hip', 'train_step.hip', 'griffinlim.hip', 'nnls.hip', 'collective.cpp',
-           'rotary.hip', 'kvcache.hip', 'seq_attention.hip', 'seq_attention_bwd.hip', 'paged_attention.hip']
+           'rotary.hip', 'kvcache.hip', 'seq_attention.hip', 'seq_attention_bwd.hip', 'seq_attention_bwd_two.hip', 'paged_attention.hip']
 FLAGS = ['--offload-arch=gfx950', '-O3', '-std=c++17', '-fPIC', '-Wno-unused-result']
 # The sources built without packed fp32 arithmetic (v_pk_add / mul / fma_f32): some of its forms have given wrong results on
 # this card now and then, with no error.
-UNPACKED = {'rotary.hip', 'kvcache.hip', 'seq_attention.hip', 'seq_attention_bwd.hip', 'paged_attention.hip'}
+UNPACKED = {'rotary.hip', 'kvcache.hip', 'seq_attention.hip', 'seq_attention_bwd.hip', 'seq_attention_bwd_two.hip',
+            'paged_attention.hip'}
 UNPACKED_FLAGS = ['-Xclang', '-target-feature', '-Xclang', '-packed-fp32-ops']
 # measurement builds only, e.g. TTSMI_EXTRA_HIPCC_FLAGS=-DTTSMI_ABLATION_BUILD (stage-ablation knobs, csrc/common.h)
 FLAGS += os.environ.get('TTSMI_EXTRA_HIPCC_FLAGS', '').split()

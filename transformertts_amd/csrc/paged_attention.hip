@@ -55,7 +55,8 @@ template <typename T, typename CT, int DHP> struct PgCfg {
 // keys of a split and wave at least: two blocks (8 single tokens over 200 .. 1500 keys: 19 us; 22 with four)
 #define PG_LEAST 64
 
-template <typename T, typename CT, int DHP>
+// TWO: probabilities in two parts (pg_two_parts).
+template <typename T, typename CT, int DHP, bool TWO>
 __global__ __launch_bounds__((64 * PgCfg<T, CT, DHP>::NW), (PgCfg<T, CT, DHP>::WPS)) void paged_rows_kernel(SeqFwdP p) {
     using C = PgCfg<T, CT, DHP>;
     using frag = typename SeqT<T>::frag;
@@ -201,21 +202,23 @@ __global__ __launch_bounds__((64 * PgCfg<T, CT, DHP>::NW), (PgCfg<T, CT, DHP>::W
             }
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
-                frag pf;
+                frag pf, pr;
                 seq_to_frag(s, t, pf);
+                if constexpr (TWO) seq_to_rest(s, t, pf, pr);
 #pragma unroll
                 for (int cb = 0; cb < NCB; ++cb) {
+                    frag f;
                     if constexpr (Q8) {
                         typedef int pg_v2i __attribute__((ext_vector_type(2)));
                         typedef __attribute__((address_space(3))) pg_v2i* lds_ptr;
                         const int j = lane & 15, e = j >> 1, row = 16 * t + 8 * (e >> 2) + 4 * hh + (e & 3), ch = cb * 2 + ((lane >> 4) & 1);
                         const pg_v2i w = __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_ptr)(Vs + I::at(row, ch) + 8 * (j & 1)));
-                        frag f;
                         pg_cvt8(make_uint2((uint32_t)w[0], (uint32_t)w[1]), 1.f, f);
-                        o[cb] = seq_mma(f, pf, o[cb]);
                     } else {
-                        o[cb] = seq_mma(A::col(A::cols(Vs, lane), 0, t, cb), pf, o[cb]);
+                        f = A::col(A::cols(Vs, lane), 0, t, cb);
                     }
+                    o[cb] = seq_mma(f, pf, o[cb]);
+                    if constexpr (TWO) o[cb] = seq_mma(f, pr, o[cb]);
                 }
             }
         };
@@ -428,6 +431,11 @@ static int pg_slots(int B, int tokens, int Hkv, int G, int dh, bool rows_form, i
     const int fill = all / Hkv < 1 ? 1 : all / Hkv;
     return !rows_form && ((long)tokens * G / 128 + (B + 1) / 2) * Hkv >= all ? 0 : fill;
 }
+// Probabilities of bf16 queries as operands of two parts (seq_to_rest) where a sequence has one tile of rows on average: the kernel
+// waits for memory, the second part costs 1 - 2 % (32 single tokens over 100 .. 8192 keys, 16 / 4 heads of 128, with the join: bf16
+// 51.8 -> 52.5 us, e4m3 36.3 -> 36.9; 32 rows each of 64 sequences of 4096 e4m3 keys, 32 / 8 heads: 137 -> 140), and the error of one part, up to
+// 1.6 times the output's own rounding in single tokens, is gone.  With two tiles it does not wait: 64 rows each, 155 -> 179 us.
+static bool pg_two_parts(const SeqFwdP& p) { return (long)p.tokens * p.G <= 32L * p.B; }
 template <typename T, typename CT>
 static void pg_rows_launch(const SeqFwdP& p, PgJoinP& j, hipStream_t st) {
     const dim3 g((unsigned)(seq_split_units(p.tokens, p.B, p.G, 32, p.slots) * p.Hkv));
@@ -435,7 +443,15 @@ static void pg_rows_launch(const SeqFwdP& p, PgJoinP& j, hipStream_t st) {
     do {                                                                                                                   \
         constexpr int NW = PgCfg<T, CT, D>::NW;                                                                               \
         j.quantum = 32 * NW; j.least = PG_LEAST * NW;                                                                         \
-        hipLaunchKernelGGL((paged_rows_kernel<T, CT, D>), g, dim3(64 * NW), 0, st, p);                                     \
+        if constexpr (sizeof(T) == 2) {                                                                                    \
+            if (pg_two_parts(p)) {                                                                                         \
+                hipLaunchKernelGGL((paged_rows_kernel<T, CT, D, true>), g, dim3(64 * NW), 0, st, p);                       \
+                break;                                                                                                     \
+            }                                                                                                              \
+        }                                                                                                                  \
+        /* (over a bf16 cache this form has 16 rows a sequence at most, pg_rows_form: two parts always) */                 \
+        if constexpr (sizeof(T) == 4 || sizeof(CT) == 1)                                                                   \
+            hipLaunchKernelGGL((paged_rows_kernel<T, CT, D, false>), g, dim3(64 * NW), 0, st, p);                          \
     } while (0)
     if (p.dh <= 64) PG_GO(64);
     else if (p.dh <= 128) PG_GO(128);

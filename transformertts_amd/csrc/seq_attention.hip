@@ -21,7 +21,8 @@
 // CT: the cache's element type for PAGED (T, or uint8_t = e4m3).  WIDE: pages of whole load instructions (the RPI rows that one
 // brings), so that an instruction has one page and its address is a scalar base and a constant lane offset; without it every lane
 // looks its rows up, forming 64-bit addresses of its own.
-template <typename T, typename CT, int DHP, bool PAGED, int KS = 1, bool WIDE = false>
+// TWO: probabilities in two parts (seq_two_parts).
+template <typename T, typename CT, int DHP, bool PAGED, int KS = 1, bool WIDE = false, bool TWO = false>
 __global__ __launch_bounds__(256, (DHP <= 128 && sizeof(T) == 2) ? 2 : 1) void seq_attn_fwd_kernel(SeqFwdP p) {
     using I = SeqImg<T, DHP>;
     using frag = typename SeqT<T>::frag;
@@ -292,8 +293,18 @@ __global__ __launch_bounds__(256, (DHP <= 128 && sizeof(T) == 2) ? 2 : 1) void s
             for (int t = 0; t < 2; ++t) {
                 frag pf;
                 seq_to_frag(s[kb], t, pf);
+                if constexpr (TWO) {
+                    frag pr;
+                    seq_to_rest(s[kb], t, pf, pr);
 #pragma unroll
-                for (int cb = 0; cb < NCB; ++cb) o[cb] = seq_mma(A::col(va, kb * 32, t, cb), pf, o[cb]);
+                    for (int cb = 0; cb < NCB; ++cb) {
+                        const frag vf = A::col(va, kb * 32, t, cb);
+                        o[cb] = seq_mma(vf, pr, seq_mma(vf, pf, o[cb]));
+                    }
+                } else {
+#pragma unroll
+                    for (int cb = 0; cb < NCB; ++cb) o[cb] = seq_mma(A::col(va, kb * 32, t, cb), pf, o[cb]);
+                }
             }
         __builtin_amdgcn_s_setprio(0);
     }
@@ -371,14 +382,24 @@ __global__ __launch_bounds__(256, (DHP <= 128 && sizeof(T) == 2) ? 2 : 1) void s
 
 // ---- launches -----------------------------------------------------------------------------------------
 
-template <typename T, typename CT, int DHP, bool PAGED, int KS, bool WIDE = false>
+template <typename T, typename CT, int DHP, bool PAGED, int KS, bool WIDE = false, bool TWO = false>
 static void seq_fwd_go(const SeqFwdP& p, long units, hipStream_t st) {
-    hipLaunchKernelGGL((seq_attn_fwd_kernel<T, CT, DHP, PAGED, KS, WIDE>), dim3((unsigned)(units * p.Hkv)), dim3(256), 0, st, p);
+    hipLaunchKernelGGL((seq_attn_fwd_kernel<T, CT, DHP, PAGED, KS, WIDE, TWO>), dim3((unsigned)(units * p.Hkv)), dim3(256), 0, st, p);
 }
 template <typename T>
 static int seq_packed_launch(const SeqFwdP& p, hipStream_t st) {
     const int parts = seq_key_parts(p.tokens, p.B, p.G, p.Hkv, p.dh, sizeof(T) == 4, p.causal);
     const long units = seq_units(p.tokens, p.B, p.G, 128 / parts);
+    if constexpr (sizeof(T) == 2) {
+        if (seq_two_parts(p.tokens, p.B, parts, false)) {
+            if (p.dh <= 64) seq_fwd_go<T, T, 64, false, 2, false, true>(p, units, st);
+            else if (p.dh <= 128) seq_fwd_go<T, T, 128, false, 2, false, true>(p, units, st);
+            else seq_fwd_go<T, T, 192, false, 2, false, true>(p, units, st);
+            ttsmi_note_kernel("seq_attn_fwd_kernel, keys in two");
+            TTSMI_CHECK_LAUNCH("packed_attention_fwd");
+            return TTSMI_OK;
+        }
+    }
     if (parts == 4) {
         if (p.dh <= 64) seq_fwd_go<T, T, 64, false, 4>(p, units, st);
         else if constexpr (sizeof(T) == 2) seq_fwd_go<T, T, 128, false, 4>(p, units, st);

@@ -50,6 +50,12 @@ __device__ __forceinline__ void seq_to_frag(const f32x16& p, int t, f32x8& f) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) f[e] = p[8 * t + e];
 }
+// What that rounding took, as a second operand of the same product: together they are the fp32 value to 2^-16 (taken where
+// seq_two_parts and, over a cache, pg_two_parts say).
+__device__ __forceinline__ void seq_to_rest(const f32x16& p, int t, const bf16x8& f, bf16x8& g) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) g[e] = (__bf16)(p[8 * t + e] - (float)f[e]);
+}
 
 // lanes l and l ^ 32 combined (both get the same bits); inline asm because the builtin's two results are folded into one
 __device__ __forceinline__ float seq_half_max(float v) {
@@ -299,6 +305,13 @@ static inline int seq_key_parts(long tokens, int B, int G, int Hkv, int dh, bool
     if (!(f32 && dh > 128) && workgroups(2) <= (uneven ? 528 : mean >= 256 ? 288 : 256)) return 2;
     return 1;
 }
+
+// Probabilities and score gradients of bf16 tensors as operands of two parts (seq_to_rest): batches of short sequences with few
+// tiles.  Nothing averages the rounding of one part over a few keys - dq and dk of two keys were up to 2.1 times as far from the
+// formula as their own rounding puts them, of 100 keys 1.5 times, and 1.0 with two parts - while the matrix pipes of a small launch
+// have the time.  Forward and backward in us with one part / two: 61 tokens, 2 heads of 192, 38 / 37; 20 x 102, 8 heads of 64, 37 / 37;
+// 10 x 102, 16 / 4 heads of 128, 56 / 57; longer ones pay more for less: 1 x 512, 8 heads of 64, 41 / 47, 1 x 2048, 16 / 4 of 128, 185 / 232.
+static inline bool seq_two_parts(long tokens, int B, int parts, bool f32) { return !f32 && parts == 2 && tokens / (B > 0 ? B : 1) < 256; }
 
 // ---- what a forward launch takes ----
 // keys of a split, tile form: at least four tiles (200 new tokens over 2000 keys, 4 heads of 128: 24 us; 25 at 128, 28 at 512)
