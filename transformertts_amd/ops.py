@@ -2196,29 +2196,20 @@ def _own_rows(t):
     return all(s > 0 or n < 2 for s, n in zip(t.stride(), t.shape))
 
 
-def _meet(a, b):
-    """Whether the address ranges of two tensors meet."""
-    def ends(t):
-        return t.data_ptr(), t.data_ptr() + (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size()
-    if not a.numel() or not b.numel():
-        return False
-    (a0, a1), (b0, b1) = ends(a), ends(b)
-    return a0 < b1 and b0 < a1
-
-
 def _share(a, b):
-    """Whether two tensors [tokens, heads, dh] of as many tokens have an element's memory in common."""
-    if not _meet(a, b):
+    """Whether two tensors [tokens, heads, dh] of as many tokens, the last dimension contiguous, have an element's memory in common."""
+    (M, H, dh), H2 = a.shape, b.shape[1]
+    (row, head, _), (row2, head2, _) = a.stride(), b.stride()
+    at = (b.data_ptr() - a.data_ptr()) // a.element_size()
+    if at >= (M - 1) * row + (H - 1) * head + dh or -at >= (M - 1) * row2 + (H2 - 1) * head2 + dh or not M * H * H2:
         return False
-    (M, H, dh), (row, head, _), (row2, head2, _) = a.shape, a.stride(), b.stride()
     if M > 1 and row != row2:
         return True                                        # (orders as different as that in one buffer: not looked into)
-    at = (b.data_ptr() - a.data_ptr()) // a.element_size()
-    first, last = (a, b) if at >= 0 else (b, a)            # the parts of a fused projection lie one behind the other within a row
-    if (first.shape[1] - 1) * first.stride(1) + dh <= abs(at) and abs(at) + (last.shape[1] - 1) * last.stride(1) + dh <= row:
+    # the parts of a fused projection lie one behind the other within a row
+    if (H - 1) * head + dh <= at <= row - (H2 - 1) * head2 - dh or (H2 - 1) * head2 + dh <= -at <= row - (H - 1) * head - dh:
         return False
     for i in range(H):
-        for j in range(b.shape[1]):                        # heads i and j, b's a number of rows behind a's
+        for j in range(H2):                                # heads i and j, b's a number of rows behind a's
             d = at + j * head2 - i * head
             rows = (0,) if M == 1 else (d // row, d // row + 1)
             if any(abs(d - n * row) < dh and abs(n) < M for n in rows):
@@ -2241,15 +2232,15 @@ def _scale_of(scale, dh):
 
 def _no_tangent(name, *tensors):
     """Refuses the dual tensors of forward-mode differentiation: no operator here gives tangents."""
-    if forward_ad._current_level >= 0:
-        for t in tensors:
-            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
-                _refuse(f'{name}: has no forward-mode derivative for a tensor of {tuple(t.shape)} with a tangent')
+    for t in tensors:
+        if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+            _refuse(f'{name}: has no forward-mode derivative for a tensor of {tuple(t.shape)} with a tangent')
 
 
 def _no_gradient(name, *tensors):
-    """Refuses tensors that want a gradient which the call does not give."""
-    _no_tangent(name, *tensors)
+    """Refuses tensors that want a gradient, or have a tangent, which the call does not give."""
+    if forward_ad._current_level >= 0:
+        _no_tangent(name, *tensors)
     if torch.is_grad_enabled():
         for t in tensors:
             if t is not None and t.requires_grad:
@@ -2258,7 +2249,7 @@ def _no_gradient(name, *tensors):
 
 # The kernels write through raw pointers: autograd is told, so that a product that kept one of these tensors for its gradient
 # refuses it instead of using what stands there now.
-_written = torch.autograd.graph.increment_version
+_written = torch._C._increment_version
 
 
 # ---- rotary positions ----------------------------------------------------------------------------------------------
@@ -2326,7 +2317,8 @@ def rotary(q, k, positions, freqs, interleaved=False, scale=1.0, inplace=False):
             _refuse(f'rotary: {M} queries and {k.shape[0]} keys')
         grad = grad or k.requires_grad
     grad = grad and torch.is_grad_enabled()
-    _no_tangent('rotary', q, k)
+    if forward_ad._current_level >= 0:
+        _no_tangent('rotary', q, k)
     freqs, scale = _c(freqs), float(scale)
     if inplace:
         if grad:
@@ -2435,7 +2427,8 @@ def packed_attention(q, k, v, starts, causal=True, scale=None):
     starts = _ints_check('packed_attention', 'starts', starts, dev)
     if starts.numel() == 0:
         _refuse('packed_attention: starts holds the end of the last sequence at least')
-    _no_tangent('packed_attention', q, k, v)
+    if forward_ad._current_level >= 0:
+        _no_tangent('packed_attention', q, k, v)
     scale = _scale_of(scale, dh)
     q, k, v = _strided(q, True, H // Hkv), _strided(k, True, 1), _strided(v, True, 1)
     if (q.requires_grad or k.requires_grad or v.requires_grad) and torch.is_grad_enabled():
@@ -2478,15 +2471,24 @@ class KVCache:
             if t.shape != k.shape[:3] or t.dtype != torch.uint8 or t.device != k.device or not t.is_contiguous():
                 _refuse(f'KVCache: exponents {tuple(t.shape)} {t.dtype} of pages {tuple(k.shape)}')
         _need_gpu(k)
-        if not k.is_contiguous() or not v.is_contiguous() or (k.data_ptr() | v.data_ptr()) % 16:
+        pk, pv, pke, pve = k.data_ptr(), v.data_ptr(), _p(k_exp), _p(v_exp)
+        if not k.is_contiguous() or not v.is_contiguous() or (pk | pv) % 16:
             _refuse('KVCache: contiguous, 16-byte aligned pages')
-        spans = sorted((t.data_ptr(), t.nbytes) for t in ((k, v, k_exp, v_exp) if quantised else (k, v)))
+        spans = sorted(((pk, k.nbytes), (pv, k.nbytes), (pke, k_exp.nbytes), (pve, k_exp.nbytes))) if quantised else ((min(pk, pv), k.nbytes), (max(pk, pv), 0))
         if n and any(a + held > b for (a, held), (b, _) in zip(spans, spans[1:])):
             _refuse('KVCache: pages and exponents of keys and values that share memory')
-        code = _CACHE_DTYPES[k.dtype]
-        args = (k.data_ptr(), v.data_ptr(), _p(k_exp), _p(v_exp), code, n, size)
-        for name, value in zip(self.__slots__, (k, v, k_exp, v_exp, args, heads, dh, size, k.dtype, code, k.get_device())):
-            object.__setattr__(self, name, value)
+        code, put = _CACHE_DTYPES[k.dtype], object.__setattr__
+        put(self, 'k', k)
+        put(self, 'v', v)
+        put(self, 'k_exp', k_exp)
+        put(self, 'v_exp', v_exp)
+        put(self, 'args', (pk, pv, pke, pve, code, n, size))
+        put(self, 'heads', heads)
+        put(self, 'dh', dh)
+        put(self, 'page_size', size)
+        put(self, 'dtype', k.dtype)
+        put(self, 'code', code)
+        put(self, 'index', k.get_device())
 
     @classmethod
     def zeros(cls, pages, page_size, heads, dh, dtype=torch.bfloat16, device='cuda'):
