@@ -7,8 +7,9 @@
 // infinity are stored as NaN: e4m3 has no infinity.
 //
 // Bound by memory: a wave owns a token, finds its sequence among `starts` (64 at a time) and moves the rows of all key heads, K
-// and V, 8 elements a lane.  Measured: 12620 tokens of 8 heads of 128, bf16 into e4m3 pages 16.5 us and back 14.5 us, 155 MB in
-// all or 5.0 TB/s, the rate of a copy; 64 single tokens into bf16 pages: 3.5 us, a launch.
+// and V, 8 elements a lane.  Measured: 12620 tokens of 8 heads of 128, bf16 into e4m3 pages 16.7 us and back 14.5 us, 155 MB in
+// all or 5.0 TB/s, the rate of a copy; into bf16 pages and back, a replayed call each, 22 and 22 us (104 MB), fp32 38 and 37 (207 MB); 64
+// single tokens into bf16 pages: 3.5 us, a launch.
 #include "seq_common.h"
 
 struct KvP {

@@ -12,9 +12,14 @@
 // e4m3 values stay bytes in LDS.  K fragments are converted with the row's scale (a lane is a key); V fragments come through the
 // transposing 8-bit LDS read, and the value scales multiply the probabilities instead (both exact: powers of two).
 //
-// Measured: 32 single tokens over 262 .. 8192 keys, 16 / 4 heads of 128, bf16 pages of 16: 42 us, 5.5 TB/s, and 6.7 us for the join;
-// two over 131072 and 70001 keys, 32 / 8 heads, e4m3 pages of 64: 78 us, 5.3 TB/s, and 11 us.  The tile form, chunks of 512 + 384 +
-// 97 + 1 tokens over 16384 .. 97 keys, 16 / 4 heads: 133 us with its join of 15 (720 TFLOP/s).
+// Measured (average of 150 launches under the profiler, the least in brackets): 32 single tokens over 262 .. 8192 keys, 16 / 4 heads of 128,
+// bf16 pages of 16: 42 us (41), 5.5 TB/s, and 6.4 for the join; two over 131072 and 70001 keys, 32 / 8 heads, e4m3 pages of 64: 81 us (75),
+// 5.1 TB/s, and 13.  The tile form, chunks of 512 + 384 + 97 + 1 tokens over 16384 .. 97 keys, 16 / 4 heads: 131 us (122), 730 TFLOP/s, and
+// 15 for the join.
+// Other types, a replayed call with its join, beside the time of its bytes at 6.5 TB/s or of its products: fp32, 32 single tokens over
+// 100 .. 8192 keys, 16 / 4 heads of 128, 174 us (71: LDS holds two waves of two blocks a compute unit), of 64, 65 (36), 8 / 2 heads of 192,
+// 259 (53: one such wave, and 88 registers spilled inside the counted loop, whose reloads wait for the blocks in flight); over e4m3 pages
+// 98 (18), and of 192, which spills none, 83 (13).  The chunks above in fp32 1276 (624), over e4m3 pages 176 (72), fp32 over e4m3 1478 (624).
 #include "seq_common.h"
 
 template <int N> __device__ __forceinline__ void pg_wait() {

@@ -6,13 +6,16 @@
 // sequence and key head (seq_common.h: rows are (token, query head of the group) pairs), 32 rows a wave.  The wave forms the
 // TRANSPOSED score tile S^T = K Q^T, so that a lane holds one row's scores for 16 keys: the softmax is in-lane plus one exchange
 // of the two half-waves, and the accumulator registers, rounded, ARE the B operand of O^T += V^T P^T.
-// Bound by the matrix and the vector pipes together: the matrix pipes are busy half of the time, a wave's vector instructions (the
-// softmax, 16 clocks an exponential) take as long as its products, and the two waves that the registers leave a SIMD overlap
-// only in part.  LDS is busy a third of the time, without bank conflicts.  (Of 342 us a pass, taking away the reads of fragments saved 96,
-// either product 80 .. 90, the loads 42, the exponentials 29.)  Measured: prompts of 8192 + 3001 + 513 + 1 tokens,
-// 16 / 8 heads of 128, causal, bf16: 313 us, 1000 TFLOP/s where a large library product reaches 1330; 6000 + 1999 + 193 of 16 / 2 heads:
-// 175 us, 730 (two rounds of uneven tiles); 32 utterances of 202 .. 900, 4 heads of 64, training: 29 us; fp32, 8 utterances, 4 / 2 heads of 64:
-// 26 us, the walk of four waves over the longest (38 of two).
+// Long prompts are bound by the matrix and the vector pipes together: the matrix pipes are busy half of the time, a wave's vector
+// instructions (the softmax, 16 clocks an exponential) take as long as its products, and the two waves that the registers leave a
+// SIMD overlap only in part.  LDS is busy a third of the time, without bank conflicts.  (Of 342 us a pass, taking away the reads of
+// fragments saved 96, either product 80 .. 90, the loads 42, the exponentials 29.)  Batches of utterances are bound by balance - with all
+// workgroups resident the slowest compute unit's three whole walks are the time -, the small fp32 batch by waits: 128 KB of LDS leave one
+// wave a SIMD, and 60 of its 316 workgroups run in a second round.  One short utterance is a chain: starts, then Q, then K and V.
+// Measured (average of 150 launches under the profiler, the least in brackets): prompts of 8192 + 3001 + 513 + 1 tokens, 16 / 8 heads of
+// 128, causal, bf16: 329 us (309), 950 TFLOP/s (1010) where a large library product reaches 1330; 6000 + 1999 + 193 of 16 / 2 heads: 180 us
+// (174), 910 TFLOP/s; 32 utterances of 202 .. 900, 4 heads of 64: 28 us; fp32, 8 utterances, 4 / 2 heads of 64: 26 us (38 with two waves a
+// row block); 61 tokens of 2 heads of 192: 9 us.
 // Where tiles are few, two or four waves share a row block and the keys (seq_key_parts).
 // Over a cache the keys can be split over workgroups (find_unit): each leaves its maximum, sum and unnormalised output, and a second
 // launch joins them (paged_attention.hip).

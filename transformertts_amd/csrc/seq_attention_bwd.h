@@ -11,10 +11,14 @@
 // dK, dV: 128 keys of one key head a workgroup, 32 a wave; the row tiles of every query head of the group pass through LDS, the
 //         wave forms S and dP with a key per lane, so that P and dS are the B operands of dV^T += dO^T P and dK^T += Q^T dS.
 //
-// Bound like the forward (matrix pipes busy 52 %, LDS 26 - 33 %); the causal dK / dV pass leaves a quarter of the card idle at its ends.
-// Measured, causal bf16, 6000 + 1999 + 193 tokens of 16 / 2
-// heads of 128: dQ 251 us (760 TFLOP/s), dK / dV 385 (660) and 23 for the join of its row splits; 32 utterances of 202 .. 900, 4 heads
-// of 64: 38 and 40 us; fp32, 8 utterances of 117 .. 700, 4 / 2 heads of 64: 32 (48 with two waves a row block), 38 and 5 us.
+// Bound like the forward (long batches: matrix pipes busy 52 %, LDS 26 - 33 %); the causal dK / dV pass leaves a quarter of the card idle
+// at its ends.  The scores and dP are formed in both passes: seven products where five would do.
+// Measured as in the forward, causal bf16, 6000 + 1999 + 193 tokens of 16 / 2 heads of 128: dQ 245 us (238), 1000 TFLOP/s of its three
+// products, dK / dV 369 (353), 890 of its four, and 23 for the join of its row splits; 32 utterances of 202 .. 900, 4 heads of 64: 37 and
+// 38 us; fp32, 8 utterances of 117 .. 700, 4 / 2 heads of 64: 32 (48 with two waves a row block), 38 and 6 us.
+// fp32 heads of 129 .. 192 do not fit the registers: 258 of the dK / dV pass and 17 of dQ are spilled (756 bytes of scratch a lane in the
+// former; of heads of 65 .. 128 it spills 10), whose reloads wait for the tile in flight behind them.  2048 causal tokens, 4 / 2 heads,
+// forward / with the backward: 414 / 1346 us for heads of 192, 160 / 580 for heads of 128.
 #pragma once
 #include "seq_common.h"
 
@@ -36,9 +40,11 @@ struct SeqBwdP {
     // extra: how many splits there can be behind their tiles' first ones, the slots or fewer (seq_bwd_extra)
     int slots; long extra; float* part;
 };
-// rows of a split at least: eight tiles of work against the traffic of its partial sums (bf16: a training step of 8 x 512 tokens, 16 / 4
-// heads of 128, 128 us at 512, 144 at 256, 132 at 1024); the fp32 products are slower (8 utterances of 117 .. 700, 4 / 2 heads of 64:
-// 133 us at 192, 140 at 96, 160 at 384)
+// Rows of a split at least: eight tiles of work against the traffic of its partial sums; fp32 products are slower.  Backward in us:
+//   bf16, at 256 / 512 / 1024 / 2048 rows: causal 8 x 512 tokens, 16 / 4 heads of 128, 106 / 92 / 94 / 118; 3 x 1024, 8 heads of 64,
+//   53 / 55 / 57 / 56; 2048, 8 / 2 of 64, 66 / 59 / 64 / 85; 4096, 4 of 128, 169 / 168 / 160 / 173; full, 8 of 264 .. 900, 4 of 64, 56 / 57 / 60 / 60
+//   fp32, at 96 / 192 / 384 / 768: causal 8 of 117 .. 700, 4 / 2 heads of 64, 111 / 104 / 123 / 176; 2048, 4 of 64, 177 / 164 / 154 / 194;
+//   1000 + 500, 4 / 2 of 128, 208 / 193 / 241 / 343; full, 3 x 800, 8 of 64, 209 / 206 / 233 / 236; 1500, 4 / 1 of 64, 136 / 141 / 128 / 179
 template <typename T> struct SeqLeast { static constexpr int ROWS = sizeof(T) == 2 ? 512 : 192; };
 
 // four accumulator registers -> four consecutive elements of a gradient row

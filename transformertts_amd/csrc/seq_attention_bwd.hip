@@ -7,9 +7,13 @@
 void seq_bwd_two(const SeqBwdP& p, dim3 g, dim3 gk, hipStream_t st);                          // seq_attention_bwd_two.hip
 
 // Row splits a key head, for all key heads together: enough for two workgroups a compute unit; three times that where causal, whose
-// splits are empty to a half and uneven at the ends (8192 tokens of three sequences, 16 / 2 heads of 128: dK / dV pass 384 us at
-// 1536, 450 us at 1024, 410 us at 2048; not causal, one sequence of 8192, a training step 2178 us at 512, 2345 at 256, 2206 at 768).  None
-// where the key tiles alone are that many.
+// splits are empty to a half and uneven at the ends: long sequences gain up to a fifth, short ones lose 6 % at most.  None where the
+// key tiles alone are that many.  Backward in us:
+//   causal, at 512 / 1024 / 1536 / 2048: 6000 + 1999 + 193 tokens, 16 / 2 heads of 128, 711 / 669 / 621 / 627; 16384, 8 / 2 of 64,
+//   1382 / 1104 / 1089 / 1046; 8192, 16 / 4 of 80, 1111 / 966 / 921 / 908; 2 x 2048, 16 / 4 of 128, 201 / 205 / 207 / 218; 8 x 512, the same heads,
+//   95 / 91 / 91 / 93; 4096, 8 / 1 of 64, 130 / 131 / 131 / 137; fp32, 2 x 2048, 8 / 2 of 64, 495 / 518 / 523 / 538; 1000 + 700 + 300, 4 / 2 of 128, 196 / 197 / 197 / 197
+//   full, at 256 / 512 / 768 / 1024: 8192, 16 / 2 of 128, 1830 / 1691 / 1708 / 1705; 2 x 2048, 16 / 4 of 128, 265 / 256 / 267 / 275; 4096, 8 / 1 of 64,
+//   193 / 171 / 168 / 183; 700 + 3000 + 200, 8 / 2 of 64, 129 / 123 / 135 / 130; fp32, 2 x 2048, 8 / 2 of 64, 555 / 567 / 578 / 597
 static int seq_bwd_slots(int tokens, int Hkv, int causal) {
     const int all = causal ? 1536 : 512, fill = all / Hkv < 1 ? 1 : all / Hkv;
     return tokens / 128 >= fill ? 0 : fill;
