@@ -284,7 +284,7 @@ def test_the_overlap_of_views_is_found(world):
     for n in range(4000):
         M, dh = rng.choice([1, 2, 3, 7]), rng.choice([2, 4, 8])
         views = []
-        layout, W = rng.choice(['rows', 'heads', 'parts']), rng.choice([2, 3, 6])
+        layout, W = rng.choice(['rows', 'heads', 'parts', 'blocks']), rng.choice([2, 3, 6])
         for _ in 'ab':
             if layout == 'rows':                           # parts of a fused projection
                 x, lo = base[:M * W * dh].view(M, W, dh), rng.randrange(W)
@@ -292,6 +292,9 @@ def test_the_overlap_of_views_is_found(world):
             elif layout == 'heads':                        # [heads, tokens, dh]
                 x, lo = base[:W * M * dh].view(W, M, dh), rng.randrange(W)
                 views.append(x[lo:lo + rng.randint(1, W)].transpose(0, 1))
+            elif layout == 'blocks':                       # [heads, parts, tokens, dh]
+                x, lo = base[:M * W * 3 * dh].view(W, 3, M, dh), rng.randrange(W)
+                views.append(x[lo:lo + rng.randint(1, W), rng.randrange(3)].transpose(0, 1))
             else:                                          # [tokens, heads, parts, dh]
                 x = base[:M * W * 3 * dh].view(M, W, 3, dh)
                 views.append(x[:, :, rng.randrange(3)])

@@ -2205,11 +2205,15 @@ def _share(a, b):
         return False
     if M > 1 and row != row2:
         return True                                        # (orders as different as that in one buffer: not looked into)
-    # the parts of a fused projection lie one behind the other within a row
+    # the parts of a fused projection: one behind the other within a row, or within a head
     if (H - 1) * head + dh <= at <= row - (H2 - 1) * head2 - dh or (H2 - 1) * head2 + dh <= -at <= row - (H - 1) * head - dh:
         return False
-    for i in range(H):
-        for j in range(H2):                                # heads i and j, b's a number of rows behind a's
+    if head == head2 and head > 0:
+        inner = dh if M == 1 or row % head == 0 else (M - 1) * row + dh
+        if inner <= at % head <= head - inner:
+            return False
+    for i in range(H if head != head2 else 1):
+        for j in range(H2) if head != head2 else range(1 - H, H2):      # head j of b a number of rows behind head i of a (equal strides: heads apart)
             d = at + j * head2 - i * head
             rows = (0,) if M == 1 else (d // row, d // row + 1)
             if any(abs(d - n * row) < dh and abs(n) < M for n in rows):
